@@ -92,6 +92,39 @@ class QadGroup(ctypes.Structure):
 
 SIGNATURES["hi2x_assemble_batch"] = [_P, _I64, _P, _P]
 
+
+class Packed(ctypes.Structure):
+    """hi2x_packed (include/hi2x.h): tensors laid out for products."""
+
+    _fields_ = [("codes", _P), ("params", _P), ("rows", _P), ("segments", _P),
+                ("experts", _I64), ("n", _I64), ("k", _I64), ("kp", _I64), ("frags", _I64),
+                ("max_frags", _I64), ("max_tiles", _I64 * 3)]
+
+
+class ActivationsDesc(ctypes.Structure):
+    """hi2x_activations (include/hi2x.h): activations in the stored basis."""
+
+    _fields_ = [("planes", _P), ("scale", _P), ("rows", _I64), ("kp", _I64),
+                ("nplanes", ctypes.c_int32), ("pad_", ctypes.c_int32)]
+
+
+class Epilogue(ctypes.Structure):
+    """hi2x_epilogue (include/hi2x.h): what follows a product."""
+
+    _fields_ = [("bias", _P), ("mul", _P), ("residual", _P), ("out", _P), ("ld_mul", _I64),
+                ("ld_residual", _I64), ("ld_out", _I64), ("dt_bias", ctypes.c_int32),
+                ("dt_mul", ctypes.c_int32), ("dt_residual", ctypes.c_int32),
+                ("dt_out", ctypes.c_int32), ("act", ctypes.c_int32), ("pad_", ctypes.c_int32)]
+
+
+SIGNATURES["hi2x_packed_layout"] = [_P, _P, _P, _P, _P, _P, _P]
+SIGNATURES["hi2x_packed_activations"] = [_P, _I, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _P, _P]
+SIGNATURES["hi2x_packed_linear"] = [_P, _P, _P, _P, _I64, _P, _P]
+SIGNATURES["hi2x_route"] = [_P, _I, _I64, _I64, _I64, _I64, _I, _P, _I64, _I64, _I, _F, _P, _P,
+                            _P, _P, _P, _P, _I64, _P]
+SIGNATURES["hi2x_route_backward"] = [_P, _I, _I64, _I64, _I64, _I64, _I, _I, _F, _P, _P, _P, _P]
+SIGNATURES["hi2x_moe_combine"] = [_P, _I, _I64, _I64, _P, _P, _I64, _I64, _P, _I, _P, _I, _P]
+
 # workspace sizes (int64 bytes, -1 for bad arguments): name -> argtypes
 SIZES = {
     "hi2x_hessian_workspace_bytes": [_I, _I64, _I64],
@@ -101,6 +134,7 @@ SIZES = {
     "hi2x_chol_batched_workspace_bytes": [_I64, _I64],
     "hi2x_refine_workspace_bytes": [_I64, _I64, _I64],
     "hi2x_colstats_workspace_bytes": [_I64, _I64],
+    "hi2x_route_workspace_bytes": [_I64, _I64],
 }
 
 

@@ -1,0 +1,265 @@
+// Packed tensors laid out for products, and the activations' transform in front of them.
+#include "packed.h"
+
+namespace hi2x {
+namespace {
+
+// ---- layout ------------------------------------------------------------------------------
+// One thread per (fragment, chunk, lane): the 32 codes a lane feeds to the chunk's four
+// MFMA steps are 32 neighbours of its row, nbits whole words.  In each laid-out dword the
+// pair p of codes (2p, 2p + 1) sits at bits nbits * p and 16 + nbits * p, so that one mask
+// takes a pair out as two halves.  At nbits 8 a lane's 32 bytes go as two 16-byte pieces,
+// 64 lanes of each next to each other.
+__global__ __launch_bounds__(256) void layout_codes_kernel(hi2x_packed w,
+                                                           const int32_t* __restrict__ codes,
+                                                           const int64_t* __restrict__ code_off) {
+  const hi2x_packed_segment sg = w.segments[blockIdx.y];
+  const int64_t e = blockIdx.y / PK_SEGS;
+  const int64_t nch = w.kp / PK_CHUNK;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= sg.frags * nch * 64) return;
+  const int lane = (int)(i & 63);
+  const int64_t c = (i >> 6) % nch, f = (i >> 6) / nch;
+  const int nbits = sg.nbits, per = 32 / nbits;
+  const int row = w.rows[(sg.frag0 + f) * 16 + (lane & 15)];
+  const int64_t k0 = c * PK_CHUNK + 32 * (lane >> 4);
+  const int64_t left = w.k - k0;  // columns there are, a multiple of 16
+  const int words = row < 0 || left <= 0 ? 0 : (int)(left >= 32 ? nbits : left * nbits / 32);
+  const int32_t* src = row < 0 ? codes : codes + code_off[e * w.n + row] + k0 * nbits / 32;
+  uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<char*>(w.codes) + sg.codes +
+                                              (f * nch + c) * 256 * nbits);
+  for (int q = 0; q < nbits; ++q) {
+    uint32_t v = q < words ? (uint32_t)src[q] : 0u, o = 0;
+    const uint32_t m = (1u << nbits) - 1u;
+    for (int j = 0; j < per; ++j)
+      o |= ((v >> (nbits * j)) & m) << (nbits * (j >> 1) + 16 * (j & 1));
+    const int at = nbits == 8 ? (q >> 2) * 256 + lane * 4 + (q & 3) : lane * nbits + q;
+    dst[at] = o;
+  }
+}
+
+// One thread per (fragment, block, row): the block's fp16 lo and step (hi2/format.py:45-60:
+// lo = fp16(f32(f64(u) lo_scale + lo_min)); the product of a byte and an fp16 is exact in
+// f32, so one f32 fma rounds as the f64 sum does).
+__global__ __launch_bounds__(256) void layout_params_kernel(
+    hi2x_packed w, const uint8_t* __restrict__ params, const int64_t* __restrict__ param_off,
+    const uint16_t* __restrict__ consts) {
+  const hi2x_packed_segment sg = w.segments[blockIdx.y];
+  if (sg.frags == 0) return;
+  const int64_t e = blockIdx.y / PK_SEGS;
+  const int64_t nblk = w.kp / sg.block;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= sg.frags * nblk * 16) return;
+  const int64_t b = (i >> 4) % nblk, f = (i >> 4) / nblk;
+  const int row = w.rows[(sg.frag0 + f) * 16 + (i & 15)];
+  uint32_t v = 0;
+  if (row >= 0 && b < w.k / sg.block) {
+    const int64_t r = e * w.n + row;
+    const uint8_t* p = params + 2 * (param_off[r] + b);
+    const float lo = __builtin_fmaf((float)p[0], f16_from_bits(consts[3 * r + 1]),
+                                    f16_from_bits(consts[3 * r]));
+    const float st = (float)p[1] * f16_from_bits(consts[3 * r + 2]);
+    v = (uint32_t)f16_bits(lo) | (uint32_t)f16_bits(st) << 16;
+  }
+  reinterpret_cast<uint32_t*>(static_cast<char*>(w.params) + sg.params)[i] = v;
+}
+
+// ---- activations -------------------------------------------------------------------------
+template <int DT>
+__device__ __forceinline__ void load16(const void* x, int64_t at, float (&v)[16]) {
+  if constexpr (DT == 0) {
+    const float* p = static_cast<const float*>(x) + at;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = p[i];
+  } else {
+    const uint16_t* p = static_cast<const uint16_t*>(x) + at;
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      v[i] = DT == 1 ? f16_from_bits(p[i]) : __uint_as_float((uint32_t)p[i] << 16);
+  }
+}
+
+// A workgroup transforms one row.  First pass: the largest finite |x / s|; the rotation can
+// grow it fourfold at most, so 2^(13 - exponent) brings every value to at most 2^15, with
+// nothing of the row below fp16's normal range unless it is 2^-27 of the largest.  Second
+// pass: scaled (exact), rotated by butterflies in f32, rounded to fp16.  That rounding
+// (2^-12 of each value, independent) is below the output's own for bf16 and as large as
+// fp16's; nplanes 2 keeps the rest of it in a second plane.
+template <int DT>
+__global__ __launch_bounds__(256) void activations_kernel(
+    const void* __restrict__ x, int64_t ldx, int64_t x_rows, int64_t k,
+    const int64_t* __restrict__ src, const uint8_t* __restrict__ had,
+    const uint16_t* __restrict__ cs, const int64_t* __restrict__ offs, int experts,
+    hi2x_activations out) {
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x;
+  const int64_t from = src ? src[row] : row;
+  const bool bad = from < 0 || from >= x_rows;
+  const int64_t base = bad ? 0 : from * ldx;
+  if (offs) {
+    int lo = 0, hi = experts - 1;  // the expert whose range holds the row
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (offs[mid + 1] > row)
+        hi = mid;
+      else
+        lo = mid + 1;
+    }
+    had += (int64_t)lo * (k / 16);
+    if (cs) cs += (int64_t)lo * k;
+  }
+  const int groups = (int)(k / 16), all = (int)(out.kp / 16);
+  float m = 0.0f;
+  if (!bad) {
+    for (int g = tid; g < groups; g += 256) {
+      float v[16];
+      load16<DT>(x, base + 16 * (int64_t)g, v);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float a = v[i];
+        if (cs) a = a / f16_from_bits(cs[16 * g + i]);
+        a = fabsf(a);
+        m = fmaxf(m, a < __builtin_inff() ? a : 0.0f);
+      }
+    }
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+  __shared__ float red[4];
+  if ((tid & 63) == 0) red[tid >> 6] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  int ex = 0;
+  if (m > 0.0f) (void)frexpf(m, &ex);
+  // the exponent stays where both 2^e and 2^-e are normal
+  const int e = 13 - ex > 126 ? 126 : (13 - ex < -126 ? -126 : 13 - ex);
+  const float sc = ldexpf(1.0f, e);
+  if (tid == 0) out.scale[row] = bad ? __builtin_nanf("") : ldexpf(1.0f, -e);
+  uint16_t* dst = out.planes + row * out.kp;
+  const int64_t plane = out.rows * out.kp;
+  for (int g = tid; g < all; g += 256) {
+    float v[16];
+    if (bad || g >= groups) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = 0.0f;
+    } else {
+      load16<DT>(x, base + 16 * (int64_t)g, v);
+      if (cs) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = v[i] / f16_from_bits(cs[16 * g + i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] *= sc;
+      if (had[g]) {
+#pragma unroll
+        for (int d = 1; d < 16; d <<= 1)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (!(i & d)) {
+              const float a = v[i], b = v[i | d];
+              v[i] = a + b;
+              v[i | d] = a - b;
+            }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] *= 0.25f;
+      }
+    }
+    uint32_t h[8], l[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint16_t a = f16_bits(v[2 * i]), b = f16_bits(v[2 * i + 1]);
+      h[i] = (uint32_t)a | (uint32_t)b << 16;
+      l[i] = (uint32_t)f16_bits(v[2 * i] - f16_from_bits(a)) |
+             (uint32_t)f16_bits(v[2 * i + 1] - f16_from_bits(b)) << 16;
+    }
+    u32x4* d = reinterpret_cast<u32x4*>(dst + 16 * (int64_t)g);
+    d[0] = u32x4{h[0], h[1], h[2], h[3]};
+    d[1] = u32x4{h[4], h[5], h[6], h[7]};
+    if (out.nplanes == 2) {
+      d = reinterpret_cast<u32x4*>(dst + plane + 16 * (int64_t)g);
+      d[0] = u32x4{l[0], l[1], l[2], l[3]};
+      d[1] = u32x4{l[4], l[5], l[6], l[7]};
+    }
+  }
+}
+
+}  // namespace
+}  // namespace hi2x
+
+using namespace hi2x;
+
+namespace {
+int check_packed(const hi2x_packed* w, const char* what) {
+  HI2X_REQUIRE(w, "%s: null tensor", what);
+  HI2X_REQUIRE(w->experts >= 1 && w->n >= 1 && w->k >= 16 && w->k % 16 == 0,
+               "%s: bad shape (%lld experts of %lld x %lld; columns a multiple of 16)", what,
+               (long long)w->experts, (long long)w->n, (long long)w->k);
+  HI2X_REQUIRE(w->kp % PK_CHUNK == 0 && w->kp >= w->k && w->kp < w->k + PK_CHUNK,
+               "%s: %lld padded columns for %lld", what, (long long)w->kp, (long long)w->k);
+  HI2X_REQUIRE(w->n < (1ll << 31) && w->k < (1ll << 24) && w->frags < (1ll << 27) &&
+                   w->experts <= 7000,
+               "%s: tensor too large", what);
+  HI2X_REQUIRE(w->codes && w->params && w->rows && w->segments, "%s: null buffer", what);
+  HI2X_REQUIRE((((uintptr_t)w->codes | (uintptr_t)w->params) & 255) == 0,
+               "%s: layout not 256-byte aligned", what);
+  return HI2X_OK;
+}
+}  // namespace
+
+extern "C" int hi2x_packed_layout(const hi2x_packed* w, const int32_t* codes,
+                                  const int64_t* code_off, const uint8_t* blk_params,
+                                  const int64_t* param_off, const uint16_t* row_consts,
+                                  void* stream) {
+  clear_error();
+  if (int rc = check_packed(w, "packed_layout")) return rc;
+  HI2X_REQUIRE(codes && code_off && blk_params && param_off && row_consts,
+               "packed_layout: null buffer");
+  const hipStream_t s = as_stream(stream);
+  const int64_t segs = w->experts * PK_SEGS;
+  // the largest segment has at most max_frags fragments; smaller ones leave workgroups idle
+  const int64_t nc = (w->max_frags * (w->kp / PK_CHUNK) * 64 + 255) / 256;
+  const int64_t np = (w->max_frags * (w->kp / 16) * 16 + 255) / 256;
+  HI2X_REQUIRE(segs <= 65535 && nc < (1ll << 31) && np < (1ll << 31),
+               "packed_layout: tensor too large");
+  layout_codes_kernel<<<dim3((unsigned)nc, (unsigned)segs), 256, 0, s>>>(*w, codes, code_off);
+  layout_params_kernel<<<dim3((unsigned)np, (unsigned)segs), 256, 0, s>>>(*w, blk_params,
+                                                                          param_off, row_consts);
+  return launch_status("packed_layout");
+}
+
+extern "C" int hi2x_packed_activations(const void* x, int dtype, int64_t ldx, int64_t x_rows,
+                                       int64_t k, const int64_t* src, const uint8_t* had,
+                                       const uint16_t* col_scale, const int64_t* offs,
+                                       int64_t experts, const hi2x_activations* out,
+                                       void* stream) {
+  clear_error();
+  HI2X_REQUIRE(out, "packed_activations: null output");
+  HI2X_REQUIRE(dtype >= 0 && dtype <= 2, "packed_activations: dtype %d", dtype);
+  HI2X_REQUIRE(k >= 16 && k % 16 == 0 && out->kp % PK_CHUNK == 0 && out->kp >= k &&
+                   out->kp < k + PK_CHUNK,
+               "packed_activations: %lld columns (a multiple of 16), %lld padded", (long long)k,
+               (long long)out->kp);
+  HI2X_REQUIRE(out->nplanes == 1 || out->nplanes == 2, "packed_activations: %d planes",
+               out->nplanes);
+  HI2X_REQUIRE(x_rows >= 0 && out->rows >= 0 && out->rows < (1ll << 31) && ldx >= k,
+               "packed_activations: bad shape");
+  HI2X_REQUIRE(!offs || experts >= 1, "packed_activations: ranges without experts");
+  if (out->rows == 0) return HI2X_OK;
+  HI2X_REQUIRE((x || x_rows == 0) && had && out->planes && out->scale,
+               "packed_activations: null buffer");
+  HI2X_REQUIRE(src || out->rows <= x_rows, "packed_activations: %lld rows of %lld",
+               (long long)out->rows, (long long)x_rows);
+  HI2X_REQUIRE(((uintptr_t)out->planes & 255) == 0, "packed_activations: planes not aligned");
+  const hipStream_t s = as_stream(stream);
+  const dim3 grid((unsigned)out->rows);
+  if (dtype == 0)
+    activations_kernel<0><<<grid, 256, 0, s>>>(x, ldx, x_rows, k, src, had, col_scale, offs,
+                                               (int)experts, *out);
+  else if (dtype == 1)
+    activations_kernel<1><<<grid, 256, 0, s>>>(x, ldx, x_rows, k, src, had, col_scale, offs,
+                                               (int)experts, *out);
+  else
+    activations_kernel<2><<<grid, 256, 0, s>>>(x, ldx, x_rows, k, src, had, col_scale, offs,
+                                               (int)experts, *out);
+  return launch_status("packed_activations");
+}

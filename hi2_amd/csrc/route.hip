@@ -1,0 +1,626 @@
+// The router of an MoE layer: scores, top-k, weights and the experts' slot order, its
+// gradient, and the weighted sum of the experts' outputs.
+//
+// 16 lanes hold one token's E scores (expert 16 i + lane in register i), so four tokens
+// share a wave and every reduction over the experts is four DPP steps without LDS.  The
+// passes read a few MB at most: what bounds them is launches and the latency of the top-k
+// loop, so a workgroup does 64 tokens from logits to indices, and up to 64 tokens in all
+// the slot order too.  That order needs no sort: a token chooses an expert at most once,
+// so 64 tokens' choices of an expert are one 64-bit mask, a choice's rank is the number of
+// lower bits, and the stable order follows from the masks' popcounts.
+#include "packed.h"
+
+namespace hi2x {
+namespace {
+
+constexpr int RT = 64;      // tokens per workgroup (half as many above 256 experts, where a
+                            // token's registers leave room for half the waves)
+constexpr int RK = 32;      // most choices
+constexpr int RE = 512;     // most experts
+constexpr int RG = 64;      // most groups
+constexpr int SCAN_OVER = 512;  // workgroups from which the counts get a scan of their own
+
+template <int CTRL>
+__device__ __forceinline__ int dpp(int x) {
+  return __builtin_amdgcn_update_dpp(x, x, CTRL, 0xf, 0xf, false);
+}
+// Reductions over each row of 16 lanes: neighbours, pairs, halves mirrored, row mirrored.
+#define HI2X_ROW16(x, OP)   \
+  x = OP(x, dpp<0xB1>(x));  \
+  x = OP(x, dpp<0x4E>(x));  \
+  x = OP(x, dpp<0x141>(x)); \
+  x = OP(x, dpp<0x140>(x));
+
+__device__ __forceinline__ int umax_(int a, int b) {
+  return (int)((uint32_t)a > (uint32_t)b ? (uint32_t)a : (uint32_t)b);
+}
+__device__ __forceinline__ int umin_(int a, int b) {
+  return (int)((uint32_t)a < (uint32_t)b ? (uint32_t)a : (uint32_t)b);
+}
+__device__ __forceinline__ int or_(int a, int b) { return a | b; }
+__device__ __forceinline__ uint32_t row_umax(uint32_t v) {
+  int x = (int)v;
+  HI2X_ROW16(x, umax_)
+  return (uint32_t)x;
+}
+__device__ __forceinline__ uint32_t row_umin(uint32_t v) {
+  int x = (int)v;
+  HI2X_ROW16(x, umin_)
+  return (uint32_t)x;
+}
+__device__ __forceinline__ uint32_t row_or(uint32_t v) {
+  int x = (int)v;
+  HI2X_ROW16(x, or_)
+  return (uint32_t)x;
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp_d(double v) {
+  const long long b = __builtin_bit_cast(long long, v);
+  const uint32_t lo = (uint32_t)dpp<CTRL>((int)b), hi = (uint32_t)dpp<CTRL>((int)(b >> 32));
+  return __builtin_bit_cast(double, (long long)((unsigned long long)hi << 32 | lo));
+}
+__device__ __forceinline__ double row_sum(double v) {
+  v += dpp_d<0xB1>(v);
+  v += dpp_d<0x4E>(v);
+  v += dpp_d<0x141>(v);
+  v += dpp_d<0x140>(v);
+  return v;
+}
+
+// An order of u32 that is the floats' (no NaN here; -0 counts as 0); above 0 always.
+__device__ __forceinline__ uint32_t order_key(float v) {
+  const uint32_t b = __float_as_uint(v + 0.0f);
+  return (b & 0x80000000u) ? ~b : b | 0x80000000u;
+}
+
+// One token's logits (-inf where there is no expert, or for NaN) and scores.  The softmax's
+// sum is taken in f64 and rounded once, so that scores do not depend on the order of its
+// terms: experts ranked by score + bias come out the same however the sum is formed.
+template <int EPL>
+__device__ __forceinline__ void token_scores(const void* logits, int dtype, int64_t at, int e,
+                                             int scoring, int l16, float (&v)[EPL],
+                                             float (&p)[EPL]) {
+  const float ninf = -__builtin_inff();
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) {
+    const int x = 16 * i + l16;
+    float a = x < e ? load_as_f32(logits, at + x, dtype) : ninf;
+    v[i] = a == a ? a : ninf;
+  }
+  if (scoring == 1) {
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) p[i] = 1.0f / (1.0f + expf(-v[i]));
+    return;
+  }
+  uint32_t mk = 0;
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) {
+    const uint32_t k = order_key(v[i]);
+    mk = k > mk ? k : mk;
+  }
+  mk = row_umax(mk);
+  const float m = __uint_as_float((mk & 0x80000000u) ? mk & 0x7fffffffu : ~mk);
+  double sum = 0.0;
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) {
+    p[i] = v[i] > ninf ? expf(v[i] - m) : 0.0f;
+    sum += (double)p[i];
+  }
+  const float s = (float)row_sum(sum);
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) p[i] = s > 0.0f ? p[i] / s : (s == s ? 0.0f : s);
+}
+
+struct RouteArgs {
+  const void* logits;
+  int dtype;
+  int64_t ld, t;
+  int e, k, scoring;
+  const float* bias;
+  int groups, top_groups, renorm;
+  float scale;
+  int64_t* index;
+  float* weights;
+  int64_t* rows;
+  int64_t* offs;
+  int64_t* slots;
+  uint8_t* hist;    // [workgroups][e] tokens per expert
+  int32_t* prefix;  // [workgroups][e] tokens of earlier workgroups, or null
+};
+
+// cnt[0..e) -> exclusive prefix in place, by a workgroup of at least e threads.
+__device__ __forceinline__ void scan_experts(int* cnt, int e) {
+  const int tid = threadIdx.x;
+  for (int d = 1; d < e; d <<= 1) {
+    int a = 0;
+    if (tid < e && tid >= d) a = cnt[tid - d];
+    __syncthreads();
+    if (tid < e) cnt[tid] += a;
+    __syncthreads();
+  }
+}
+
+template <int EPL, int NT>
+__global__ __launch_bounds__(NT) void route_kernel(RouteArgs a) {
+  constexpr int RT = NT / 16;
+  __shared__ int sel_e[RT][RK];
+  __shared__ float sel_p[RT][RK];
+  __shared__ uint32_t mask[RE][2];
+  __shared__ int cnt[RE];
+  extern __shared__ float keys[];  // with groups: [RT][e + groups]
+  const int tid = threadIdx.x, tok = tid >> 4, l16 = tid & 15;
+  const int64_t t0 = (int64_t)blockIdx.x * RT, t = t0 + tok;
+  const bool live = t < a.t;
+  const int e = a.e, k = a.k;
+  for (int i = tid; i < e; i += NT) mask[i][0] = mask[i][1] = 0;
+  float v[EPL], p[EPL];
+  token_scores<EPL>(a.logits, a.dtype, (live ? t : a.t - 1) * a.ld, e, a.scoring, l16, v, p);
+  // the keys the experts are ranked by; 0: taken, or not taking part
+  const float ninf = -__builtin_inff();
+  uint32_t key[EPL];
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) {
+    const int x = 16 * i + l16;
+    if (a.bias && v[i] > ninf) {
+      const float c = p[i] + (x < e ? a.bias[x] : 0.0f);
+      v[i] = c == c ? c : ninf;
+    }
+    key[i] = x < e ? order_key(v[i]) : 0u;
+  }
+  if (a.top_groups < a.groups) {
+    const int gs = e / a.groups, pitch = e + a.groups;
+    const float inv = 1.0f / (float)gs;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) {
+      const int x = 16 * i + l16;
+      if (x < e) keys[tok * pitch + x + (int)(((float)x + 0.5f) * inv)] = v[i];
+    }
+    __syncthreads();
+    uint32_t gk[RG / 16];
+#pragma unroll
+    for (int i = 0; i < RG / 16; ++i) {
+      const int g = 16 * i + l16;
+      gk[i] = 0;
+      if (g < a.groups) {
+        float b1 = ninf, b2 = ninf;
+        for (int x = 0; x < gs; ++x) {
+          const float c = keys[tok * pitch + g * (gs + 1) + x];
+          b2 = c > b1 ? b1 : (c > b2 ? c : b2);
+          b1 = c > b1 ? c : b1;
+        }
+        const float s = a.bias && gs > 1 ? b1 + b2 : b1;
+        gk[i] = order_key(s == s ? s : ninf);
+      }
+    }
+    uint32_t keep0 = 0, keep1 = 0;
+    for (int j = 0; j < a.top_groups; ++j) {
+      uint32_t bk = 0;
+      int bg = RG;
+#pragma unroll
+      for (int i = 0; i < RG / 16; ++i)
+        if (gk[i] > bk) {
+          bk = gk[i];
+          bg = 16 * i + l16;
+        }
+      const uint32_t m = row_umax(bk);
+      const int w = (int)row_umin(bk == m ? (uint32_t)bg : 0xffffu);
+#pragma unroll
+      for (int i = 0; i < RG / 16; ++i)
+        if (16 * i + l16 == w) gk[i] = 0;
+      keep0 |= w < 32 ? 1u << (w & 31) : 0u;
+      keep1 |= w >= 32 ? 1u << (w & 31) : 0u;
+    }
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) {
+      const int x = 16 * i + l16;
+      const int g = (int)(((float)x + 0.5f) * inv);
+      if (!(((g < 32 ? keep0 : keep1) >> (g & 31)) & 1u)) key[i] = 0;
+    }
+  }
+  for (int j = 0; j < k; ++j) {
+    uint32_t bk = 0;
+    int be = RE;
+    float bp = 0.0f;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i)
+      if (key[i] > bk) {
+        bk = key[i];
+        be = 16 * i + l16;
+        bp = p[i];
+      }
+    const uint32_t m = row_umax(bk);
+    const int w = (int)row_umin(bk == m ? (uint32_t)be : 0xffffu);
+    if (be == w) {
+      sel_e[tok][j] = w;
+      sel_p[tok][j] = bp;
+#pragma unroll
+      for (int i = 0; i < EPL; ++i)
+        if (16 * i + l16 == w) key[i] = 0;
+    }
+  }
+  __syncthreads();
+  float sum = 0.0f;
+  for (int j = 0; j < k; ++j) sum += sel_p[tok][j];
+  for (int j = l16; j < k; j += 16) {
+    if (!live) break;
+    const int x = sel_e[tok][j];
+    float w = sel_p[tok][j];
+    if (a.renorm) w = sum == 0.0f ? 0.0f : w / sum;
+    a.index[t * k + j] = x;
+    a.weights[t * k + j] = w * a.scale;
+    atomicOr(&mask[x][tok >> 5], 1u << (tok & 31));
+  }
+  __syncthreads();
+  if (a.hist) {
+    for (int i = tid; i < e; i += NT)
+      a.hist[(int64_t)blockIdx.x * e + i] =
+          (uint8_t)(__builtin_popcount(mask[i][0]) + __builtin_popcount(mask[i][1]));
+    return;
+  }
+  // one workgroup in all: the slot order at once
+  if (tid < e) cnt[tid] = __builtin_popcount(mask[tid][0]) + __builtin_popcount(mask[tid][1]);
+  __syncthreads();
+  scan_experts(cnt, e);
+  if (tid < e) a.offs[tid + 1] = cnt[tid];
+  if (tid == 0) a.offs[0] = 0;
+  for (int j = l16; j < k; j += 16) {
+    if (!live) break;
+    const int x = sel_e[tok][j];
+    const uint32_t m0 = mask[x][0], m1 = mask[x][1];
+    const int all = __builtin_popcount(m0) + __builtin_popcount(m1);
+    const uint32_t below = (1u << (tok & 31)) - 1u;
+    const int rank = tok < 32 ? __builtin_popcount(m0 & below)
+                              : __builtin_popcount(m0) + __builtin_popcount(m1 & below);
+    const int64_t at = cnt[x] - all + rank;
+    a.rows[at] = t;
+    a.slots[t * k + j] = at;
+  }
+}
+
+// prefix[b][x] = sum of hist[b'][x] over b' < b; a workgroup takes 64 experts, 16 runs of
+// workgroups side by side.
+__global__ __launch_bounds__(1024) void route_scan_kernel(const uint8_t* __restrict__ hist,
+                                                          int nb, int e,
+                                                          int32_t* __restrict__ prefix) {
+  __shared__ int part[16][64];
+  const int x = blockIdx.x * 64 + (threadIdx.x & 63), r = threadIdx.x >> 6;
+  const int run = (nb + 15) / 16, b0 = r * run, b1 = b0 + run < nb ? b0 + run : nb;
+  int s = 0;
+  if (x < e)
+    for (int b = b0; b < b1; ++b) s += hist[(int64_t)b * e + x];
+  part[r][threadIdx.x & 63] = s;
+  __syncthreads();
+  s = 0;
+  for (int i = 0; i < r; ++i) s += part[i][threadIdx.x & 63];
+  if (x < e)
+    for (int b = b0; b < b1; ++b) {
+      prefix[(int64_t)b * e + x] = s;
+      s += hist[(int64_t)b * e + x];
+    }
+}
+
+// The slot order of workgroup b's tokens, given every workgroup's counts.
+__global__ __launch_bounds__(1024) void route_order_kernel(RouteArgs a, int nb, int rt) {
+  __shared__ uint32_t mask[RE][2];
+  __shared__ int cnt[RE];   // tokens per expert, then their running sum
+  __shared__ int base[RE];  // tokens of earlier workgroups
+  const int tid = threadIdx.x, tok = tid >> 4, l16 = tid & 15;
+  const int b = blockIdx.x, e = a.e, k = a.k;
+  const int64_t t = (int64_t)b * rt + tok;
+  const bool live = tok < rt && t < a.t;
+  for (int i = tid; i < e; i += 1024) {
+    mask[i][0] = mask[i][1] = 0;
+    cnt[i] = base[i] = 0;
+  }
+  __syncthreads();
+  if (live)
+    for (int j = l16; j < k; j += 16)
+      atomicOr(&mask[(int)a.index[t * k + j]][tok >> 5], 1u << (tok & 31));
+  if (a.prefix) {
+    for (int x = tid; x < e; x += 1024) {
+      base[x] = a.prefix[(int64_t)b * e + x];
+      cnt[x] = a.prefix[(int64_t)(nb - 1) * e + x] + a.hist[(int64_t)(nb - 1) * e + x];
+    }
+  } else {
+    const int ep = e <= 64 ? 64 : (e <= 128 ? 128 : (e <= 256 ? 256 : 512));
+    const int x = tid & (ep - 1), parts = 1024 / ep;
+    if (x < e) {
+      int all = 0, pre = 0;
+      for (int i = tid / ep; i < nb; i += parts) {
+        const int h = a.hist[(int64_t)i * e + x];
+        all += h;
+        pre += i < b ? h : 0;
+      }
+      atomicAdd(&cnt[x], all);
+      atomicAdd(&base[x], pre);
+    }
+  }
+  __syncthreads();
+  scan_experts(cnt, e);
+  if (b == 0) {
+    for (int x = tid; x < e; x += 1024) a.offs[x + 1] = cnt[x];
+    if (tid == 0) a.offs[0] = 0;
+  }
+  if (!live) return;
+  for (int j = l16; j < k; j += 16) {
+    const int x = (int)a.index[t * k + j];
+    const uint32_t m0 = mask[x][0], m1 = mask[x][1];
+    const uint32_t below = (1u << (tok & 31)) - 1u;
+    const int rank = tok < 32 ? __builtin_popcount(m0 & below)
+                              : __builtin_popcount(m0) + __builtin_popcount(m1 & below);
+    const int64_t at = (int64_t)(x ? cnt[x - 1] : 0) + base[x] + rank;
+    a.rows[at] = t;
+    a.slots[t * k + j] = at;
+  }
+}
+
+// The gradient: with dp the gradient at the scores (zero for experts not chosen),
+//   weights = c p              dp_j = c g_j
+//   weights = c p / S          dp_j = c (g_j - sum_i g_i p_i / S) / S
+// and through the scores dl = dp p (1 - p) (sigmoid) or p (dp - sum dp p) (softmax; that sum
+// is zero where the weights are renormalised, and not formed).
+template <int EPL>
+__global__ __launch_bounds__(256) void route_backward_kernel(
+    const void* __restrict__ logits, int dtype, int64_t ld, int64_t n_tok, int e, int k,
+    int scoring, int renorm, float scale, const int64_t* __restrict__ index,
+    const float* __restrict__ grad, void* __restrict__ dlogits) {
+  const int l16 = threadIdx.x & 15;
+  const int64_t tt = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
+  const bool live = tt < n_tok;
+  const int64_t t = live ? tt : n_tok - 1;
+  float v[EPL], p[EPL], d[EPL];
+  bool chosen[EPL];
+  token_scores<EPL>(logits, dtype, t * ld, e, scoring, l16, v, p);
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) {
+    d[i] = 0.0f;
+    chosen[i] = false;
+  }
+  for (int j = 0; j < k; ++j) {
+    const int64_t x = index[t * k + j];
+    const float g = grad[t * k + j];
+#pragma unroll
+    for (int i = 0; i < EPL; ++i)
+      if (x == 16 * i + l16) {
+        d[i] += g;
+        chosen[i] = true;
+      }
+  }
+  double sp = 0.0, sgp = 0.0;
+#pragma unroll
+  for (int i = 0; i < EPL; ++i)
+    if (chosen[i]) {
+      sp += (double)p[i];
+      sgp += (double)(d[i] * p[i]);
+    }
+  sp = row_sum(sp);
+  sgp = row_sum(sgp);
+  const float total = (float)sp;
+  const float mean = total == 0.0f ? 0.0f : (float)(sgp / sp);
+  const float dot = scale * (float)sgp;
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) {
+    float dp = 0.0f;
+    if (chosen[i]) {
+      if (renorm)
+        dp = total == 0.0f ? 0.0f : scale * (d[i] - mean) / total;
+      else
+        dp = scale * d[i];
+    }
+    float dl;
+    if (scoring == 1)
+      dl = dp * p[i] * (1.0f - p[i]);
+    else
+      dl = p[i] * (renorm ? dp : dp - dot);
+    const int x = 16 * i + l16;
+    if (live && x < e) store_from_f32(dlogits, t * e + x, dtype, dl);
+  }
+}
+
+// out[t] = residual[t] + sum_j w[t][j] y[slots[t][j]]: a workgroup per token, four columns
+// per thread and step.  Bound by reading y once.
+template <int DT>
+__device__ __forceinline__ f32x4v load4(const void* p, int64_t at) {
+  if constexpr (DT == 0) {
+    return *reinterpret_cast<const f32x4v*>(static_cast<const float*>(p) + at);
+  } else {
+    const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + at);
+    const uint16_t h[4] = {(uint16_t)u.x, (uint16_t)(u.x >> 16), (uint16_t)u.y,
+                           (uint16_t)(u.y >> 16)};
+    f32x4v r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      r[i] = DT == 1 ? f16_from_bits(h[i]) : __uint_as_float((uint32_t)h[i] << 16);
+    return r;
+  }
+}
+
+template <int DT, int V>
+__global__ __launch_bounds__(256) void combine_kernel(
+    const void* __restrict__ y, int64_t y_rows, int64_t n, const int64_t* __restrict__ slots,
+    const float* __restrict__ weights, int k, const void* __restrict__ residual, int dt_res,
+    void* __restrict__ out, int dt_out) {
+  const int64_t t = blockIdx.x;
+  for (int64_t c = ((int64_t)blockIdx.y * 256 + threadIdx.x) * V; c < n;
+       c += (int64_t)gridDim.y * 256 * V) {
+    float acc[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      acc[i] = residual ? load_as_f32(residual, t * n + c + i, dt_res) : 0.0f;
+    for (int j = 0; j < k; ++j) {
+      const int64_t s = slots[t * k + j];
+      const float w = weights[t * k + j];
+      if (s < 0 || s >= y_rows) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[i] = __builtin_nanf("");
+        continue;
+      }
+      if constexpr (V == 4) {
+        const f32x4v r = load4<DT>(y, s * n + c);
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[i] = __builtin_fmaf(w, r[i], acc[i]);
+      } else {
+        acc[0] = __builtin_fmaf(w, load_as_f32(y, s * n + c, DT), acc[0]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) store_from_f32(out, t * n + c + i, dt_out, acc[i]);
+  }
+}
+
+int check_route(const char* what, const void* logits, int dtype, int64_t ld, int64_t t,
+                int64_t e, int64_t k, int scoring) {
+  HI2X_REQUIRE(dtype >= 0 && dtype <= 2, "%s: dtype %d", what, dtype);
+  HI2X_REQUIRE(e >= 1 && e <= RE, "%s: %lld experts (1 to %d)", what, (long long)e, RE);
+  HI2X_REQUIRE(k >= 1 && k <= RK && k <= e, "%s: %lld choices of %lld experts (at most %d)",
+               what, (long long)k, (long long)e, RK);
+  HI2X_REQUIRE(t >= 0 && t < (1ll << 31) / RK && ld >= e, "%s: bad shape", what);
+  HI2X_REQUIRE(scoring == 0 || scoring == 1, "%s: scoring %d", what, scoring);
+  HI2X_REQUIRE(logits || t == 0, "%s: null logits", what);
+  return HI2X_OK;
+}
+
+int route_tokens(int64_t e) { return e <= 256 ? RT : RT / 2; }
+
+// Clears offs where there are no tokens.
+__global__ void zero_i64_kernel(int64_t* p, int64_t n) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i < n) p[i] = 0;
+}
+
+}  // namespace
+}  // namespace hi2x
+
+using namespace hi2x;
+
+extern "C" int64_t hi2x_route_workspace_bytes(int64_t t, int64_t e) {
+  if (t < 0 || e < 1 || e > RE) return -1;
+  const int64_t nb = (t + route_tokens(e) - 1) / route_tokens(e);
+  if (nb <= 1) return 0;
+  const int64_t hist = (nb * e + 255) / 256 * 256;
+  return hist + (nb > SCAN_OVER ? nb * e * 4 : 0);
+}
+
+extern "C" int hi2x_route(const void* logits, int dtype, int64_t ld, int64_t t, int64_t e,
+                          int64_t top_k, int scoring, const float* bias, int64_t groups,
+                          int64_t top_groups, int renormalise, float scale, int64_t* index,
+                          float* weights, int64_t* rows, int64_t* offs, int64_t* slots, void* ws,
+                          int64_t ws_bytes, void* stream) {
+  clear_error();
+  if (int rc = check_route("route", logits, dtype, ld, t, e, top_k, scoring)) return rc;
+  HI2X_REQUIRE(groups >= 1 && groups <= RG && e % groups == 0,
+               "route: %lld experts in %lld groups (equal ones, at most %d)", (long long)e,
+               (long long)groups, RG);
+  HI2X_REQUIRE(top_groups >= 1 && top_groups <= groups && top_k <= e / groups * top_groups,
+               "route: %lld choices from %lld of %lld groups", (long long)top_k,
+               (long long)top_groups, (long long)groups);
+  HI2X_REQUIRE(offs && (t == 0 || (index && weights && rows && slots)), "route: null output");
+  const hipStream_t s = as_stream(stream);
+  if (t == 0) {
+    zero_i64_kernel<<<dim3((unsigned)(e / 256 + 1)), 256, 0, s>>>(offs, e + 1);
+    return launch_status("route");
+  }
+  const int rt = route_tokens(e);
+  const int64_t nb = (t + rt - 1) / rt;
+  Workspace w;
+  const int64_t need = hi2x_route_workspace_bytes(t, e);
+  if (int rc = take_workspace(w, ws, ws_bytes, (size_t)need, s, "route")) return rc;
+  RouteArgs a{logits, dtype,  ld,      t,     (int)e, (int)top_k, scoring, bias,
+              (int)groups, (int)top_groups, renormalise, scale, index, weights, rows, offs,
+              slots, nullptr, nullptr};
+  if (nb > 1) {
+    a.hist = reinterpret_cast<uint8_t*>(w.p);
+    if (nb > SCAN_OVER)
+      a.prefix = reinterpret_cast<int32_t*>(w.p + (nb * e + 255) / 256 * 256);
+  }
+  const size_t dyn = top_groups < groups ? (size_t)rt * (e + groups) * 4 : 0;
+  const dim3 grid((unsigned)nb);
+#define HI2X_ROUTE(EPL, NT)                                                                    \
+  {                                                                                            \
+    if (dyn > 32768)                                                                           \
+      HI2X_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(route_kernel<EPL, NT>),       \
+                                   hipFuncAttributeMaxDynamicSharedMemorySize, (int)dyn));     \
+    route_kernel<EPL, NT><<<grid, NT, dyn, s>>>(a);                                            \
+  }
+  if (e <= 64)
+    HI2X_ROUTE(4, 1024)
+  else if (e <= 128)
+    HI2X_ROUTE(8, 1024)
+  else if (e <= 256)
+    HI2X_ROUTE(16, 1024)
+  else
+    HI2X_ROUTE(32, 512)
+#undef HI2X_ROUTE
+  if (nb > 1) {
+    if (a.prefix)
+      route_scan_kernel<<<dim3((unsigned)((e + 63) / 64)), 1024, 0, s>>>(a.hist, (int)nb, (int)e,
+                                                                        a.prefix);
+    route_order_kernel<<<grid, 1024, 0, s>>>(a, (int)nb, rt);
+  }
+  return launch_status("route");
+}
+
+extern "C" int hi2x_route_backward(const void* logits, int dtype, int64_t ld, int64_t t,
+                                   int64_t e, int64_t top_k, int scoring, int renormalise,
+                                   float scale, const int64_t* index, const float* grad,
+                                   void* dlogits, void* stream) {
+  clear_error();
+  if (int rc = check_route("route_backward", logits, dtype, ld, t, e, top_k, scoring)) return rc;
+  if (t == 0) return HI2X_OK;
+  HI2X_REQUIRE(index && grad && dlogits, "route_backward: null buffer");
+  const hipStream_t s = as_stream(stream);
+  const dim3 grid((unsigned)((t + 15) / 16));
+#define HI2X_ROUTE(EPL)                                                                     \
+  route_backward_kernel<EPL><<<grid, 256, 0, s>>>(logits, dtype, ld, t, (int)e, (int)top_k, \
+                                                  scoring, renormalise, scale, index, grad, \
+                                                  dlogits)
+  if (e <= 64)
+    HI2X_ROUTE(4);
+  else if (e <= 128)
+    HI2X_ROUTE(8);
+  else if (e <= 256)
+    HI2X_ROUTE(16);
+  else
+    HI2X_ROUTE(32);
+#undef HI2X_ROUTE
+  return launch_status("route_backward");
+}
+
+extern "C" int hi2x_moe_combine(const void* y, int dt_y, int64_t y_rows, int64_t n,
+                                const int64_t* slots, const float* weights, int64_t t,
+                                int64_t top_k, const void* residual, int dt_residual, void* out,
+                                int dt_out, void* stream) {
+  clear_error();
+  for (int d : {dt_y, dt_residual, dt_out})
+    HI2X_REQUIRE(d >= 0 && d <= 2, "moe_combine: dtype %d", d);
+  HI2X_REQUIRE(t >= 0 && t < (1ll << 31) && n >= 1 && top_k >= 1 && top_k < (1 << 20) &&
+                   y_rows >= 0,
+               "moe_combine: bad shape");
+  if (t == 0) return HI2X_OK;
+  HI2X_REQUIRE((y || y_rows == 0) && slots && weights && out, "moe_combine: null buffer");
+  const hipStream_t s = as_stream(stream);
+  const bool vec = n % 4 == 0 && (uintptr_t)y % 16 == 0;
+  const int64_t cols = (n + (vec ? 1023 : 255)) / (vec ? 1024 : 256);
+  const dim3 grid((unsigned)t, (unsigned)(cols < 64 ? cols : 64));
+#define HI2X_COMBINE(DT, V)                                                                  \
+  combine_kernel<DT, V><<<grid, 256, 0, s>>>(y, y_rows, n, slots, weights, (int)top_k,       \
+                                             residual, dt_residual, out, dt_out)
+  if (dt_y == 0) {
+    if (vec)
+      HI2X_COMBINE(0, 4);
+    else
+      HI2X_COMBINE(0, 1);
+  } else if (dt_y == 1) {
+    if (vec)
+      HI2X_COMBINE(1, 4);
+    else
+      HI2X_COMBINE(1, 1);
+  } else {
+    if (vec)
+      HI2X_COMBINE(2, 4);
+    else
+      HI2X_COMBINE(2, 1);
+  }
+#undef HI2X_COMBINE
+  return launch_status("moe_combine");
+}

@@ -25,14 +25,109 @@ Hessian GEMM's tolerance, everything after it bit for bit with this package's
 per-expert entry points.
 """
 
+from dataclasses import dataclass
+
 import torch
 
 from . import _lib
 from .format import GROUP
 from .hessian import inverse_factors_batched, inverse_factors_batched_async
 
-__all__ = ["ExpertHessians", "route_order", "inverse_factors_batched",
+__all__ = ["ExpertHessians", "Routing", "route", "route_order", "inverse_factors_batched",
            "inverse_factors_batched_async"]
+
+SCORING = {"softmax": 0, "sigmoid": 1}
+_FLOATS = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+@dataclass
+class Routing:
+    """A routed batch (:func:`route`): ``index`` (int64) and ``weights`` (float32) ``[T, k]``,
+    and the expert order of its ``T * k`` slots: ``rows[j]`` the token of slot j, ``offs``
+    ``[E + 1]`` the experts' slot ranges, ``slots [T, k]`` the slot of each choice."""
+
+    index: torch.Tensor
+    weights: torch.Tensor
+    rows: torch.Tensor
+    offs: torch.Tensor
+    slots: torch.Tensor
+
+
+class _Weights(torch.autograd.Function):
+    """The weights' gradient to the logits (``hi2x_route_backward``)."""
+
+    @staticmethod
+    def forward(ctx, logits, out, scoring, renormalise, scale):
+        ctx.save_for_backward(logits, out[0])
+        ctx.args = (scoring, renormalise, scale)
+        return out[1]
+
+    @staticmethod
+    def backward(ctx, grad):
+        logits, index = ctx.saved_tensors
+        scoring, renormalise, scale = ctx.args
+        t, e = logits.shape
+        d = torch.empty(t, e, dtype=logits.dtype, device=logits.device)
+        grad = grad.to(torch.float32).contiguous()
+        if t:
+            _lib.call("hi2x_route_backward", logits.device, _lib.ptr(logits),
+                      _FLOATS[logits.dtype], logits.stride(0) if t > 1 else e, t, e,
+                      index.shape[1], scoring, renormalise, scale, _lib.ptr(index),
+                      _lib.ptr(grad), _lib.ptr(d))
+        return d, None, None, None, None
+
+
+def route(logits: torch.Tensor, top_k: int, scoring: str = "softmax", bias=None,
+          groups: int = 1, top_groups: int | None = None, renormalise: bool = True,
+          scale: float = 1.0) -> Routing:
+    """The router in front of ``hi2/moe.py:83-100``: the ``top_k`` experts of every row of
+    ``logits [T, E]`` (float32, float16 or bfloat16), their weights, and the slot order that
+    :meth:`ExpertHessians.update_routed` and :func:`hi2_amd.packed.experts_linear` take.
+
+    Scores are the softmax or the sigmoid of the logits in float32.  Experts are ranked by
+    score + ``bias`` (float32 ``[E]``, for the balance of their load; it does not enter the
+    weights), without a bias by the logits; ties go to the lowest index, and a logit of -inf
+    or NaN has score 0 and ranks last.  With ``top_groups`` < ``groups`` only the experts of
+    the best groups (``E / groups`` neighbours each) take part, a group counting as its best
+    expert, with a bias as the sum of its best two.  The weights are ``scale`` times the
+    chosen scores, divided by their sum if ``renormalise`` (0 where the sum is 0); where
+    ``logits`` requires a gradient they have one (the choice has none).
+
+    Limits: 512 experts, 32 choices, 64 groups.  One launch for up to 64 tokens (32 above
+    256 experts), two above; the host never waits."""
+    dev = _lib.require_gpu(logits, bias)
+    if logits.dim() != 2:
+        raise ValueError(f"logits has shape {tuple(logits.shape)}, expected [T, E]")
+    if logits.dtype not in _FLOATS:
+        raise ValueError(f"logits is {logits.dtype} (float32, float16 or bfloat16)")
+    if scoring not in SCORING:
+        raise ValueError(f"scoring {scoring!r} (softmax or sigmoid)")
+    t, e = logits.shape
+    top_groups = groups if top_groups is None else top_groups
+    if bias is not None and bias.numel() != e:
+        raise ValueError(f"bias has {bias.numel()} entries, expected {e}")
+    b = None if bias is None else bias.detach().reshape(-1).to(torch.float32).contiguous()
+    x = logits.detach()
+    if (e > 1 and x.stride(1) != 1) or (t > 1 and x.stride(0) < e):
+        x = x.contiguous()
+    # one allocation: int64 index, rows, slots and offs, then the weights
+    k = max(top_k, 0)
+    n = t * k
+    i64 = torch.empty(3 * n + e + 1, dtype=torch.int64, device=dev)
+    weights = torch.empty(t, k, dtype=torch.float32, device=dev)
+    index, slots = i64[:n].view(t, k), i64[n:2 * n].view(t, k)
+    rows, offs = i64[2 * n:3 * n], i64[3 * n:]
+    size = _lib.lib().hi2x_route_workspace_bytes(t, e)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size > 0 else None
+    _lib.call("hi2x_route", dev, _lib.ptr(x), _FLOATS[x.dtype], x.stride(0) if t > 1 else e, t,
+              e, top_k, SCORING[scoring], _lib.ptr(b), groups, top_groups, int(renormalise),
+              float(scale), _lib.ptr(index), _lib.ptr(weights), _lib.ptr(rows), _lib.ptr(offs),
+              _lib.ptr(slots), _lib.ptr(ws), max(size, 0))
+    if logits.requires_grad and torch.is_grad_enabled():
+        weights = _Weights.apply(logits if x.data_ptr() == logits.data_ptr() else
+                                 logits.contiguous(), (index, weights), SCORING[scoring],
+                                 int(renormalise), float(scale))
+    return Routing(index, weights, rows, offs, slots)
 
 
 def route_order(top_k_index: torch.Tensor, n_experts: int):

@@ -1,0 +1,431 @@
+"""Running an encoded model on the MI355X: products by packed tensors.
+
+``hi2.format.reference_linear`` (``hi2/format.py:195-249``) defines what a packed tensor
+computes: ``y = T(x) Wq^T`` with ``Wq = fp16(lo + code * step)`` per ladder block and ``T``
+the smoothing and rotation of the activations (``H16(x / col_scale)`` on the flagged
+16-column groups).  Here the packed rows are never unpacked to memory: the codes are laid
+out once per tensor in the order the matrix instructions take them and decoded in
+registers on the way.
+
+* :class:`PackedLinear`: one tensor, laid out.  :func:`packed_linear` multiplies by it with
+  bias, activation, factor and residual in the epilogue, from one token to long prompts.
+* :class:`PackedExperts`: the experts of one projection of an MoE layer.
+  :func:`experts_linear` multiplies every expert's routed slots in one launch, in the order
+  :func:`hi2_amd.moe.route` gives; :func:`combine` is the weighted sum over each token's
+  experts; :func:`moe_mlp` runs a gated MLP of them.
+* :func:`activations`: the transformed activations, for tensors that share their input
+  (q, k, v; gate, up) to be multiplied one after the other.
+
+Inputs are float32, float16 or bfloat16; products are summed in float32 and rounded once,
+to ``out_dtype``.  Nothing here has a gradient (the codes are integers; inputs that
+require one are refused while gradients are recorded).
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from dataclasses import dataclass
+
+import numpy as np
+import torch
+
+from . import _lib
+from .format import GROUP, HI2Tensor
+
+__all__ = ["PackedLinear", "PackedExperts", "Activations", "activations", "packed_linear",
+           "experts_linear", "combine", "moe_mlp"]
+
+CHUNK = 128  # columns are padded to whole chunks
+FRAG = 16  # rows of one matrix-instruction fragment
+CLASSES = [(nb, b) for nb in (2, 4, 8) for b in (16, 32, 64)]
+DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
+
+_SEGMENT = np.dtype([("codes", np.int64), ("params", np.int64), ("frag0", np.int32),
+                     ("frags", np.int32), ("nbits", np.int32), ("block", np.int32)])
+
+
+def _classes_of(t: HI2Tensor, what: str) -> np.ndarray:
+    """The class index of each row of ``t``, checked against its shape and offsets."""
+    r, k = t.shape
+    if k % GROUP or k < GROUP or r < 1:
+        raise ValueError(f"{what}: shape {tuple(t.shape)} (columns a multiple of {GROUP})")
+    nb = t.row_nbits.cpu().numpy().astype(np.int64)
+    blk = t.row_block.cpu().numpy().astype(np.int64)
+    if nb.shape != (r,) or blk.shape != (r,):
+        raise ValueError(f"{what}: {nb.size} row widths and {blk.size} blocks for {r} rows")
+    cls = np.full(r, -1, np.int64)
+    for i, (b, w) in enumerate(CLASSES):
+        cls[(nb == b) & (blk == w)] = i
+    if (cls < 0).any():
+        at = int(np.argmax(cls < 0))
+        raise ValueError(f"{what}: row {at} is INT{nb[at]} in blocks of {blk[at]}")
+    if (k % blk).any():
+        raise ValueError(f"{what}: K={k} is not a multiple of every row's block")
+    code_off = np.concatenate([[0], np.cumsum(k * nb // 32)])
+    param_off = np.concatenate([[0], np.cumsum(k // blk)])
+    if t.code_off.numel() != r + 1 or t.param_off.numel() != r + 1 or \
+            not np.array_equal(t.code_off.cpu().numpy(), code_off) or \
+            not np.array_equal(t.param_off.cpu().numpy(), param_off):
+        raise ValueError(f"{what}: offsets do not follow from the rows' widths and blocks")
+    if t.codes.numel() != code_off[-1] or t.blk_params.numel() != 2 * param_off[-1] or \
+            t.row_consts.shape != (r, 3):
+        raise ValueError(f"{what}: buffers do not match the offsets")
+    if t.codes.dtype != torch.int32 or t.blk_params.dtype != torch.uint8 or \
+            t.row_consts.dtype != torch.float16:
+        raise ValueError(f"{what}: codes int32, blk_params uint8 and row_consts float16 expected")
+    if t.had.numel() != k // GROUP:
+        raise ValueError(f"{what}: had has {t.had.numel()} entries, expected {k // GROUP}")
+    if t.col_scale is not None and t.col_scale.numel() != k:
+        raise ValueError(f"{what}: col_scale has {t.col_scale.numel()} entries, expected {k}")
+    return cls
+
+
+class _Packed:
+    """One or more tensors of one shape, laid out on the device (``hi2x_packed_layout``)."""
+
+    def __init__(self, tensors: list[HI2Tensor], device="cuda"):
+        dev = torch.device(device)
+        if dev.type != "cuda":
+            raise RuntimeError(f"hi2_amd.packed runs on the MI355X; got device {dev}")
+        if dev.index is None:
+            dev = torch.device("cuda", torch.cuda.current_device())
+        tensors = list(tensors)
+        if not tensors:
+            raise ValueError("no tensor to lay out")
+        n, k = (int(v) for v in tensors[0].shape)
+        for i, t in enumerate(tensors):
+            if tuple(t.shape) != (n, k):
+                raise ValueError(f"expert {i} has shape {tuple(t.shape)}, expected {(n, k)}")
+        e = len(tensors)
+        if e > 7000:
+            raise ValueError(f"{e} experts (at most 7000)")
+        kp = -(-k // CHUNK) * CHUNK
+        self.device, self.n, self.k, self.kp, self.experts = dev, n, k, kp, e
+        segs = np.zeros((e, len(CLASSES)), _SEGMENT)
+        slot_rows = []
+        codes_at = params_at = frag = 0
+        most, tiles = 0, np.zeros(3, np.int64)
+        for i, t in enumerate(tensors):
+            cls = _classes_of(t, "tensor" if e == 1 else f"expert {i}")
+            first = frag
+            cut = np.zeros(3, np.int64)
+            for c in np.unique(cls):
+                nb, blk = CLASSES[c]
+                rows = np.flatnonzero(cls == c).astype(np.int32)
+                f = -(-rows.size // FRAG)
+                slot_rows += [rows, np.full(f * FRAG - rows.size, -1, np.int32)]
+                segs[i, c] = (codes_at, params_at, frag, f, nb, blk)
+                codes_at += f * (kp // CHUNK) * 256 * nb
+                params_at += -(-(f * (kp // blk) * 64) // 256) * 256
+                frag += f
+                cut += [-(-f // 4), -(-f // 8), -(-f // 16)]
+            most = max(most, frag - first)
+            tiles = np.maximum(tiles, cut)
+        self._codes = torch.empty(codes_at, dtype=torch.uint8, device=dev)
+        self._params = torch.empty(params_at, dtype=torch.uint8, device=dev)
+        self._rows = _lib.h2d(torch.from_numpy(np.concatenate(slot_rows)), dev)
+        self._segments = _lib.h2d(torch.from_numpy(segs.reshape(-1).view(np.uint8)), dev)
+        self.desc = _lib.Packed(self._codes.data_ptr(), self._params.data_ptr(),
+                                self._rows.data_ptr(), self._segments.data_ptr(), e, n, k, kp,
+                                frag, most, (ctypes.c_int64 * 3)(*(int(v) for v in tiles)))
+
+        def flat(parts, dtype):
+            parts = [_lib.to_device(p.reshape(-1), dev, dtype) for p in parts]
+            return (parts[0] if len(parts) == 1 else torch.cat(parts)).contiguous()
+
+        words = flat([t.codes for t in tensors], torch.int32)
+        bytes_ = flat([t.blk_params for t in tensors], torch.uint8)
+        consts = flat([t.row_consts for t in tensors], torch.float16)
+        co = np.concatenate([[0], np.cumsum([t.codes.numel() for t in tensors])])
+        po = np.concatenate([[0], np.cumsum([t.blk_params.numel() // 2 for t in tensors])])
+        offs = np.stack([
+            np.concatenate([t.code_off.cpu().numpy()[:-1].astype(np.int64) + a
+                            for t, a in zip(tensors, co)]),
+            np.concatenate([t.param_off.cpu().numpy()[:-1].astype(np.int64) + a
+                            for t, a in zip(tensors, po)])])
+        offs = _lib.h2d(torch.from_numpy(offs), dev)
+        _lib.call("hi2x_packed_layout", dev, ctypes.byref(self.desc), _lib.ptr(words),
+                  _lib.ptr(offs[0]), _lib.ptr(bytes_), _lib.ptr(offs[1]), _lib.ptr(consts))
+        # the transform: one for all where every expert has the same
+        had = [t.had.reshape(-1).cpu().to(torch.uint8).numpy() for t in tensors]
+        cs = [None if t.col_scale is None else
+              t.col_scale.reshape(-1).cpu().to(torch.float16).numpy() for t in tensors]
+        if any(c is None for c in cs) and not all(c is None for c in cs):
+            cs = [np.ones(k, np.float16) if c is None else c for c in cs]
+        keys = [(h.astype(bool).tobytes(), b"" if c is None else c.tobytes())
+                for h, c in zip(had, cs)]
+        #: the transform all tensors share, None where experts have their own
+        self.transform = keys[0] if all(x == keys[0] for x in keys) else None
+        own = 1 if self.transform is not None else e
+        self._had = _lib.h2d(torch.from_numpy(np.stack(had[:own])), dev)
+        self._scale = None if cs[0] is None else \
+            _lib.h2d(torch.from_numpy(np.stack(cs[:own])), dev)
+
+    @property
+    def nbytes(self) -> int:
+        """Device bytes of the laid-out codes and ladder parameters."""
+        return self._codes.numel() + self._params.numel()
+
+
+class PackedLinear(_Packed):
+    """A packed tensor (``HI2Tensor``, host or device buffers) laid out for
+    :func:`packed_linear`.  The layout is made once; the tensor is not needed after it."""
+
+    def __init__(self, tensor: HI2Tensor, device="cuda"):
+        super().__init__([tensor], device)
+
+
+class PackedExperts(_Packed):
+    """The experts of one projection, one ``HI2Tensor`` each, all of one shape (each with
+    its own rows' widths and its own transform)."""
+
+
+@dataclass
+class Activations:
+    """Transformed activations (:func:`activations`): usable with every tensor whose
+    transform is ``transform``."""
+
+    planes: torch.Tensor  # float16 [nplanes, rows, kp]
+    scale: torch.Tensor  # float32 [rows]
+    k: int
+    dtype: torch.dtype  # of the activations they were made from
+    transform: tuple | None
+    desc: object
+
+
+def _no_grad_inputs(what, *tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad() or detach "
+                           "its inputs")
+
+
+def _dtype(t: torch.Tensor | torch.dtype, what: str) -> int:
+    d = t if isinstance(t, torch.dtype) else t.dtype
+    if d not in DTYPES:
+        raise ValueError(f"{what} is {d} (float32, float16 or bfloat16)")
+    return DTYPES[d]
+
+
+def _rows_of(x: torch.Tensor, k: int, what: str) -> torch.Tensor:
+    """``x`` as [rows, k] with unit column stride, without a copy where its strides allow."""
+    if x.dim() < 1 or x.shape[-1] != k:
+        raise ValueError(f"{what} has shape {tuple(x.shape)}, expected {k} columns")
+    x = x.reshape(-1, k) if x.dim() != 2 else x
+    if x.shape[0] > 1 and x.stride(0) < k or k > 1 and x.stride(1) != 1:
+        x = x.contiguous()
+    return x
+
+
+def _pitch(x: torch.Tensor) -> int:
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
+def _planes(dtype: torch.dtype) -> int:
+    # bf16 and fp16 activations are rounded to one fp16 plane behind the transform; fp32
+    # ones keep 22 bits in two
+    return 2 if dtype == torch.float32 else 1
+
+
+def _transformed(x: torch.Tensor, w: _Packed, src=None, offs=None, rows=None, npl=None
+                 ) -> Activations:
+    dev = w.device
+    dt = _dtype(x, "x")
+    x = _rows_of(x, w.k, "x")
+    rows = x.shape[0] if rows is None else rows
+    npl = npl or _planes(x.dtype)
+    planes = torch.empty(npl, rows, w.kp, dtype=torch.float16, device=dev)
+    scale = torch.empty(rows, dtype=torch.float32, device=dev)
+    desc = _lib.ActivationsDesc(planes.data_ptr(), scale.data_ptr(), rows, w.kp, npl, 0)
+    _lib.call("hi2x_packed_activations", dev, _lib.ptr(x), dt, _pitch(x), x.shape[0], w.k,
+              _lib.ptr(src), _lib.ptr(w._had), _lib.ptr(w._scale), _lib.ptr(offs),
+              w.experts, ctypes.byref(desc))
+    return Activations(planes, scale, w.k, x.dtype, w.transform, desc)
+
+
+def activations(x: torch.Tensor, w: PackedLinear | PackedExperts) -> Activations:
+    """``T(x)`` for ``w`` and every tensor with the same transform, to be handed to
+    :func:`packed_linear` or :func:`experts_linear` in the place of ``x [..., K]``.  The
+    product then has one row per row of ``x``."""
+    if _lib.require_gpu(x) != w.device:
+        raise RuntimeError(f"x is on {x.device}, the weights on {w.device}")
+    _no_grad_inputs("activations", x)
+    if w.transform is None:
+        raise ValueError("the experts have transforms of their own: give experts_linear x itself")
+    return _transformed(x, w)
+
+
+def _epilogue(w, slots, bias, activation, mul, residual, out, what):
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation {activation!r} ({', '.join(ACTIVATIONS)})")
+    e = _lib.Epilogue()
+    e.act = ACTIVATIONS[activation]
+    keep = []
+    if bias is not None:
+        if bias.numel() != w.n:
+            raise ValueError(f"bias has {bias.numel()} entries, expected {w.n}")
+        bias = bias.reshape(-1).contiguous()
+        e.bias, e.dt_bias = bias.data_ptr(), _dtype(bias, "bias")
+        keep.append(bias)
+    for name, t in (("mul", mul), ("residual", residual)):
+        if t is None:
+            continue
+        if t.numel() != slots * w.n:
+            raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {slots} rows of {w.n}")
+        dt = _dtype(t, name)
+        t = _rows_of(t, w.n, name)
+        keep.append(t)
+        setattr(e, name, t.data_ptr())
+        setattr(e, "ld_" + name, _pitch(t))
+        setattr(e, "dt_" + name, dt)
+    e.out, e.ld_out, e.dt_out = out.data_ptr(), w.n, _dtype(out, "out_dtype")
+    return e, keep
+
+
+def _product(w, x, act, src, offs, slots, bias, activation, mul, residual, out_dtype, what):
+    dev = w.device
+    if _lib.require_gpu(x if isinstance(x, torch.Tensor) else x.planes, bias, mul,
+                        residual, src, offs) != dev:
+        raise RuntimeError(f"{what}: inputs are not on the weights' device {dev}")
+    out = torch.empty(slots, w.n, dtype=out_dtype, device=dev)
+    epi, keep = _epilogue(w, slots, bias, activation, mul, residual, out, what)
+    if slots:
+        _lib.call("hi2x_packed_linear", dev, ctypes.byref(w.desc), ctypes.byref(act.desc),
+                  _lib.ptr(src), _lib.ptr(offs), slots, ctypes.byref(epi))
+    return out
+
+
+def _check_activations(x: Activations, w):
+    if x.k != w.k or x.transform is None or x.transform != w.transform:
+        raise ValueError("activations of another transform than the weights'")
+
+
+def packed_linear(x: torch.Tensor | Activations, w: PackedLinear, bias=None,
+                  activation: str = "none", mul=None, residual=None, out_dtype=None
+                  ) -> torch.Tensor:
+    """``activation(T(x) Wq^T + bias) * mul + residual`` for ``x [..., K]`` (or its
+    :func:`activations`), as ``[..., N]`` in ``out_dtype`` (default: x's): summed in float32,
+    rounded once.  ``bias [N]``, ``mul`` and ``residual`` (one row per row of x; rows may be
+    strided) in any of the float types; activation one of none, relu, silu, gelu (erf) and
+    gelu_tanh."""
+    if not isinstance(w, PackedLinear):
+        raise TypeError(f"packed_linear takes a PackedLinear, got {type(w).__name__}")
+    if isinstance(x, Activations):
+        _check_activations(x, w)
+        lead, act, dtype = (x.scale.numel(),), x, x.dtype
+        _no_grad_inputs("packed_linear", bias, mul, residual)
+    else:
+        if _lib.require_gpu(x) != w.device:
+            raise RuntimeError(f"x is on {x.device}, the weights on {w.device}")
+        _no_grad_inputs("packed_linear", x, bias, mul, residual)
+        lead, dtype = tuple(x.shape[:-1]), x.dtype
+        act = _transformed(x, w)
+    slots = act.scale.numel()
+    y = _product(w, x, act, None, None, slots, bias, activation, mul, residual,
+                 out_dtype or dtype, "packed_linear")
+    return y.reshape(*lead, w.n)
+
+
+def _routed(offs, rows, w, what):
+    if offs.dtype != torch.int64 or offs.numel() != w.experts + 1:
+        raise ValueError(f"{what}: offs is {offs.dtype} of {offs.numel()} entries, expected "
+                         f"int64 of {w.experts + 1}")
+    if rows is not None and rows.dtype != torch.int64:
+        raise ValueError(f"{what}: rows is {rows.dtype}, expected int64")
+    return offs.contiguous(), None if rows is None else rows.reshape(-1).contiguous()
+
+
+def experts_linear(x: torch.Tensor | Activations, w: PackedExperts, offs: torch.Tensor,
+                   rows: torch.Tensor | None = None, activation: str = "none", mul=None,
+                   residual=None, out_dtype=None, *, _planes=None) -> torch.Tensor:
+    """``[S, N]``: row j is expert e's product for the routed slot j of its range
+    ``offs[e]:offs[e + 1]``, which reads row ``rows[j]`` of ``x`` (row j itself without
+    ``rows``), with the epilogue of :func:`packed_linear`.  ``offs`` (device int64, E + 1
+    entries, 0 to S) and ``rows`` (device int64; an index outside x gives a row of NaN) are
+    those of :func:`hi2_amd.moe.route` and are never read by the host; the ranges must cover
+    all S slots, rows outside them are left unwritten."""
+    if not isinstance(w, PackedExperts):
+        raise TypeError(f"experts_linear takes PackedExperts, got {type(w).__name__}")
+    given = isinstance(x, Activations)
+    if _lib.require_gpu(offs, rows, x.planes if given else x) != w.device:
+        raise RuntimeError(f"experts_linear: inputs are not on the weights' device {w.device}")
+    offs, rows = _routed(offs, rows, w, "experts_linear")
+    _no_grad_inputs("experts_linear", None if given else x, mul, residual)
+    if given:
+        _check_activations(x, w)
+        act, dtype = x, x.dtype
+    else:
+        dtype = x.dtype
+        if w.transform is not None:
+            act = _transformed(x, w, npl=_planes)
+        else:  # every slot through its own expert's transform
+            n = rows.numel() if rows is not None else _rows_of(x, w.k, "x").shape[0]
+            act, rows = _transformed(x, w, src=rows, offs=offs, rows=n, npl=_planes), None
+    slots = rows.numel() if rows is not None else act.scale.numel()
+    return _product(w, x, act, rows, offs, slots, None, activation, mul, residual,
+                    out_dtype or dtype, "experts_linear")
+
+
+def combine(y: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor, residual=None,
+            out_dtype=None) -> torch.Tensor:
+    """``out[t] = residual[t] + sum_j weights[t, j] * y[slots[t, j]]`` over ``y [S, N]``, with
+    ``slots`` (int64) and ``weights`` (float32) ``[T, k]`` of :func:`hi2_amd.moe.route`: summed
+    in float32 in the order of j, rounded once to ``out_dtype`` (default: residual's, else
+    y's)."""
+    dev = _lib.require_gpu(y, slots, weights, residual)
+    _no_grad_inputs("combine", y, weights, residual)
+    if y.dim() != 2:
+        raise ValueError(f"y has shape {tuple(y.shape)}, expected [S, N]")
+    if slots.dim() != 2 or weights.shape != slots.shape or slots.shape[1] < 1:
+        raise ValueError(f"slots {tuple(slots.shape)} and weights {tuple(weights.shape)}: one "
+                         "shape [T, k] expected")
+    if slots.dtype != torch.int64 or weights.dtype != torch.float32:
+        raise ValueError(f"slots {slots.dtype} and weights {weights.dtype}: int64 and float32 "
+                         "expected")
+    t, n = slots.shape[0], y.shape[1]
+    if residual is not None and residual.numel() != t * n:
+        raise ValueError(f"residual has shape {tuple(residual.shape)}, expected {(t, n)}")
+    y, slots, weights = y.contiguous(), slots.contiguous(), weights.contiguous()
+    res = None if residual is None else residual.contiguous()
+    out_dtype = out_dtype or (y.dtype if res is None else res.dtype)
+    out = torch.empty(t, n, dtype=out_dtype, device=dev)
+    if t and n:
+        _lib.call("hi2x_moe_combine", dev, _lib.ptr(y), _dtype(y, "y"), y.shape[0], n,
+                  _lib.ptr(slots), _lib.ptr(weights), t, slots.shape[1], _lib.ptr(res),
+                  0 if res is None else _dtype(res, "residual"), _lib.ptr(out),
+                  _dtype(out_dtype, "out_dtype"))
+    return out
+
+
+def moe_mlp(x: torch.Tensor, routing, gate: PackedExperts, up: PackedExperts,
+            down: PackedExperts, activation: str = "silu", residual=None) -> torch.Tensor:
+    """The gated MLP of packed experts over routed tokens:
+    ``residual + sum_j w_j down(activation(gate(x)) * up(x))`` for ``x [..., K]`` and the
+    :class:`hi2_amd.moe.Routing` of its tokens, as x's shape and type.  What the experts
+    hand on stays in float32; the rounding to x's type is one, at the end."""
+    for name, p in (("gate", gate), ("up", up), ("down", down)):
+        if not isinstance(p, PackedExperts):
+            raise TypeError(f"{name} is {type(p).__name__}, expected PackedExperts")
+    if (gate.n, gate.k, gate.experts) != (up.n, up.k, up.experts) or \
+            (down.k, down.n, down.experts) != (gate.n, gate.k, gate.experts):
+        raise ValueError("gate and up [I, K] and down [K, I] of the same experts expected")
+    if _lib.require_gpu(x) != gate.device:
+        raise RuntimeError(f"x is on {x.device}, the experts on {gate.device}")
+    _no_grad_inputs("moe_mlp", x, routing.weights, residual)
+    flat = _rows_of(x, gate.k, "x")
+    if routing.index.shape[0] != flat.shape[0]:
+        raise ValueError(f"routing of {routing.index.shape[0]} tokens for {flat.shape[0]}")
+    shared = gate.transform is not None and gate.transform == up.transform
+    inp = activations(flat, gate) if shared else flat
+    offs, rows = routing.offs, routing.rows
+    g = experts_linear(inp, gate, offs, rows, activation=activation, out_dtype=torch.float32)
+    h = experts_linear(inp, up, offs, rows, mul=g, out_dtype=torch.float32)
+    del g
+    # one fp16 plane of the hidden values is well below a bf16 result's own rounding, and
+    # half the products; next to an fp16 result it would show
+    y = experts_linear(h, down, offs, out_dtype=torch.float32,
+                       _planes=1 if x.dtype == torch.bfloat16 else 2)
+    res = None if residual is None else residual.reshape(flat.shape)
+    out = combine(y, routing.slots, routing.weights, residual=res, out_dtype=x.dtype)
+    return out.reshape(x.shape)

@@ -513,6 +513,130 @@ int hi2x_qad_weights_bwd(const float* grad, const float* latent, const float* un
 int hi2x_qad_wht_scale(const float* x, int64_t n_rows, int64_t k, const uint8_t* flags,
                        const uint16_t* scale, int pre_div, float* out, void* stream);
 
+/* ---- products by packed tensors ------------------------------------------------------------ */
+
+/* What hi2's consumers compute from a packed tensor (hi2/format.py:195-249,
+ * `dequantize_stored` and `reference_linear`): y = T(x) Wq^T with Wq the decoded ladders,
+ * fp16(lo + code * step), and T the smoothing and rotation of the activations.
+ *
+ * Layout.  hi2x_packed_layout turns the flat buffers of one tensor (or of the experts of
+ * one projection, one after the other) into the order in which the products read them,
+ * once per tensor.  The rows of an expert are grouped into segments of one (nbits, block)
+ * each, in row order, and cut into fragments of 16 slots; the last fragment of a segment
+ * may hold empty slots (rows[slot] = -1).  Columns are padded to kp, a multiple of 128,
+ * with weights of zero. */
+#define HI2X_PACKED_SEGMENTS 9 /* per expert: nbits 2, 4, 8 x block 16, 32, 64 */
+
+typedef struct {
+  int64_t codes;  /* byte offset of the segment's codes: frags x kp / 128 x 256 nbits */
+  int64_t params; /* byte offset of its (lo, step) pairs: frags x kp / block x 16 x 4 */
+  int32_t frag0;  /* first fragment (over all experts) */
+  int32_t frags;  /* 0: segment unused */
+  int32_t nbits;
+  int32_t block;
+} hi2x_packed_segment;
+
+typedef struct {
+  void* codes;                         /* laid-out codes, 256-byte aligned */
+  void* params;                        /* laid-out fp16 (lo, step) pairs, 256-byte aligned */
+  const int32_t* rows;                 /* [16 * frags] row of each slot, -1: empty */
+  const hi2x_packed_segment* segments; /* [experts][HI2X_PACKED_SEGMENTS] */
+  int64_t experts;
+  int64_t n, k, kp;                    /* rows of one expert, columns, padded columns */
+  int64_t frags;                       /* fragments of all experts */
+  int64_t max_frags;                   /* most fragments of one expert */
+  int64_t max_tiles[3];                /* most tiles of one expert, of 4, 8 and 16 fragments */
+} hi2x_packed;
+
+/* Fills w->codes and w->params.  codes i32 words, blk_params u8 pairs, row_consts fp16
+ * [experts * n, 3] and the offsets of hi2/format.py:97-124 over all experts' rows:
+ * code_off (words) and param_off (blocks) [experts * n] i64. */
+int hi2x_packed_layout(const hi2x_packed* w, const int32_t* codes, const int64_t* code_off,
+                       const uint8_t* blk_params, const int64_t* param_off,
+                       const uint16_t* row_consts, void* stream);
+
+/* Activations in the stored basis: T(x) of every row in fp16, each row times a power of
+ * two that puts its values in fp16's range, and that factor's inverse in scale.  With
+ * nplanes 2 a second plane holds what the first one's rounding left (together 22 bits). */
+typedef struct {
+  uint16_t* planes; /* [nplanes][rows][kp] fp16, 256-byte aligned, columns from k on zero */
+  float* scale;     /* [rows] */
+  int64_t rows;
+  int64_t kp;
+  int32_t nplanes;
+  int32_t pad_;
+} hi2x_activations;
+
+/* T(x) = H16(x / col_scale) on the flagged 16-column groups, x / col_scale elsewhere.
+ * x [.., k] f32 (dtype 0), fp16 (1) or bf16 (2), rows ldx elements apart; row i of the
+ * result is row src[i] of x (src NULL: row i; an index outside [0, x_rows): a row of NaN).
+ * had [k / 16] u8 and col_scale [k] fp16 or NULL.  With offs (experts + 1 row ranges on
+ * the device) row i belongs to the expert whose range holds it and uses that expert's
+ * had [experts][k / 16] and col_scale [experts][k]. */
+int hi2x_packed_activations(const void* x, int dtype, int64_t ldx, int64_t x_rows, int64_t k,
+                            const int64_t* src, const uint8_t* had, const uint16_t* col_scale,
+                            const int64_t* offs, int64_t experts, const hi2x_activations* out,
+                            void* stream);
+
+#define HI2X_ACT_NONE 0
+#define HI2X_ACT_RELU 1
+#define HI2X_ACT_SILU 2
+#define HI2X_ACT_GELU 3      /* 0.5 y (1 + erf(y / sqrt 2)) */
+#define HI2X_ACT_GELU_TANH 4 /* 0.5 y (1 + tanh(sqrt(2 / pi) (y + 0.044715 y^3))) */
+
+/* out = act(y + bias) * mul + residual, in f32 with one rounding at the end; bias [n],
+ * mul, residual and out [slots][n] with rows ld elements apart, absent operands NULL,
+ * dtypes 0 f32, 1 fp16, 2 bf16. */
+typedef struct {
+  const void* bias;
+  const void* mul;
+  const void* residual;
+  void* out;
+  int64_t ld_mul, ld_residual, ld_out;
+  int32_t dt_bias, dt_mul, dt_residual, dt_out;
+  int32_t act;
+  int32_t pad_;
+} hi2x_epilogue;
+
+/* out[slot] = epilogue(T(x)[src[slot]] Wq^T) for every slot (src NULL: the slot itself).
+ * With several experts offs [experts + 1] gives each one's slot range and must cover all
+ * slots; offs NULL: one expert. */
+int hi2x_packed_linear(const hi2x_packed* w, const hi2x_activations* x, const int64_t* src,
+                       const int64_t* offs, int64_t slots, const hi2x_epilogue* epi,
+                       void* stream);
+
+/* ---- routing ------------------------------------------------------------------------------ */
+
+/* The router in front of hi2/moe.py:83-100.  logits [t][e] (rows ld apart; dtype 0 f32,
+ * 1 fp16, 2 bf16), e <= 512, top_k <= 32, groups <= 64.  scores = softmax (scoring 0) or
+ * sigmoid (1) of the logits in f32.  Experts are ranked by score + bias, without bias
+ * (NULL, else f32 [e]) by the logits; ties go to the lowest index; a logit of -inf or NaN
+ * has score 0 and ranks below all others.  With top_groups < groups only the experts of
+ * the top_groups best groups (e / groups neighbours each) take part: a group counts as its
+ * best expert, with a bias as the sum of its best two.  weights = scale * score, with
+ * renormalise scale * score / sum over the chosen ones (0 where that sum is 0).
+ * index i64 and weights f32 [t][top_k]; the expert order of the t * top_k slots: rows i64
+ * (the token of each), offs i64 [e + 1], slots i64 [t][top_k] (the slot of each choice),
+ * token order kept inside an expert.  Workspace: hi2x_route_workspace_bytes. */
+int hi2x_route(const void* logits, int dtype, int64_t ld, int64_t t, int64_t e, int64_t top_k,
+               int scoring, const float* bias, int64_t groups, int64_t top_groups,
+               int renormalise, float scale, int64_t* index, float* weights, int64_t* rows,
+               int64_t* offs, int64_t* slots, void* ws, int64_t ws_bytes, void* stream);
+int64_t hi2x_route_workspace_bytes(int64_t t, int64_t e);
+
+/* The gradient of hi2x_route's weights to its logits: grad f32 [t][top_k] -> dlogits
+ * [t][e] contiguous, in the logits' dtype.  The choice itself has no gradient. */
+int hi2x_route_backward(const void* logits, int dtype, int64_t ld, int64_t t, int64_t e,
+                        int64_t top_k, int scoring, int renormalise, float scale,
+                        const int64_t* index, const float* grad, void* dlogits, void* stream);
+
+/* out[t] = residual[t] + sum_j weights[t][j] * y[slots[t][j]] in f32, one rounding; y
+ * [y_rows][n] contiguous, residual (or NULL) and out contiguous [t][n]; a slot outside
+ * [0, y_rows) gives a row of NaN. */
+int hi2x_moe_combine(const void* y, int dt_y, int64_t y_rows, int64_t n, const int64_t* slots,
+                     const float* weights, int64_t t, int64_t top_k, const void* residual,
+                     int dt_residual, void* out, int dt_out, void* stream);
+
 /* ---- streams ---------------------------------------------------------------------------- */
 
 /* Background hint for a stream.  No counterpart in the reference (its encode runs one
