@@ -120,6 +120,8 @@ class Epilogue(ctypes.Structure):
 SIGNATURES["hi2x_packed_layout"] = [_P, _P, _P, _P, _P, _P, _P]
 SIGNATURES["hi2x_packed_activations"] = [_P, _I, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _P, _P]
 SIGNATURES["hi2x_packed_linear"] = [_P, _P, _P, _P, _I64, _P, _P]
+SIGNATURES["hi2x_packed_linear_few"] = [_P, _P, _I, _I64, _I64, _I, _P, _P, _I, _P, _P, _I64,
+                                        _P, _P]
 SIGNATURES["hi2x_route"] = [_P, _I, _I64, _I64, _I64, _I64, _I, _P, _I64, _I64, _I, _F, _P, _P,
                             _P, _P, _P, _P, _I64, _P]
 SIGNATURES["hi2x_route_backward"] = [_P, _I, _I64, _I64, _I64, _I64, _I, _I, _F, _P, _P, _P, _P]
@@ -134,6 +136,7 @@ SIZES = {
     "hi2x_chol_batched_workspace_bytes": [_I64, _I64],
     "hi2x_refine_workspace_bytes": [_I64, _I64, _I64],
     "hi2x_colstats_workspace_bytes": [_I64, _I64],
+    "hi2x_packed_few_rows": [_I64, _I],
     "hi2x_route_workspace_bytes": [_I64, _I64],
 }
 

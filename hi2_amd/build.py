@@ -16,7 +16,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libhi2x.so")
 SOURCES = ["api.hip", "gptq.hip", "ladder.hip", "format.hip", "hessian.hip", "chol.hip",
-           "refine.hip", "stats.hip", "qad.hip", "packed.hip", "packed_gemm.hip", "route.hip"]
+           "refine.hip", "stats.hip", "qad.hip", "packed.hip", "packed_few.hip",
+           "packed_gemm.hip", "route.hip"]
 ARCH = "gfx950"
 
 OBJDIR = os.path.join(os.path.dirname(HERE), "_build")

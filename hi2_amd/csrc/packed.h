@@ -96,13 +96,6 @@ __device__ __forceinline__ h16x8 decode_step(const uint32_t (&cw)[BITS], int s, 
   return out;
 }
 
-// A fragment of 16 slots (rows in layout order): where a lane's codes and ladder
-// parameters are.
-struct PkFrag {
-  const uint8_t* codes;    // chunk c at + c * 256 * BITS
-  const uint32_t* params;  // block b of the lane's row at [16 * b]
-};
-
 // The expert and token tile a workgroup row works on: tile `want` in the order of the
 // experts' ceil(n_e / tile) tiles.  Every wave computes it for itself; e < 0 past the end.
 struct PkWork {
@@ -150,6 +143,149 @@ __device__ __forceinline__ PkWork find_work(const int64_t* offs, int experts, in
     before += __shfl(inc, 63);
   }
   return w;
+}
+
+struct GemmArgs {
+  hi2x_packed w;
+  hi2x_activations x;
+  const int64_t* src;
+  const int64_t* offs;
+  int64_t slots;
+  hi2x_epilogue epi;
+};
+
+// Loads go through buffer resources: a lane's offset is one 32-bit register, the walk along
+// the columns is a scalar offset, and what lies past the resource reads as zero.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void* base, int64_t bytes) {
+  const int64_t most = 0xffffffffll;
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0,
+                                           (int)(uint32_t)(bytes < most ? bytes : most),
+                                           0x00020000);
+}
+
+// A tile of up to `per` fragments of one segment.
+struct Tile {
+  hi2x_packed_segment sg;
+  int first;  // fragment in the segment
+  int count;
+};
+
+__device__ __forceinline__ bool find_tile(const hi2x_packed& w, int e, int t, int per,
+                                          Tile& out) {
+  for (int i = 0; i < PK_SEGS; ++i) {
+    const hi2x_packed_segment sg = w.segments[e * PK_SEGS + i];
+    const int n = (sg.frags + per - 1) / per;
+    if (t < n) {
+      out.sg = sg;
+      out.first = t * per;
+      out.count = sg.frags - out.first < per ? sg.frags - out.first : per;
+      return true;
+    }
+    t -= n;
+  }
+  return false;
+}
+
+template <int BITS>
+__device__ __forceinline__ void load_codes(__amdgpu_buffer_rsrc_t rs, int lane, uint32_t soff,
+                                           uint32_t (&cw)[BITS]) {
+  if constexpr (BITS == 2) {
+    const auto v = __builtin_amdgcn_raw_buffer_load_b64(rs, 8 * lane, (int)soff, 0);
+    cw[0] = v[0];
+    cw[1] = v[1];
+  } else {
+#pragma unroll
+    for (int h = 0; h < BITS / 4; ++h) {
+      const auto v =
+          __builtin_amdgcn_raw_buffer_load_b128(rs, 16 * lane + 1024 * h, (int)soff, 0);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) cw[4 * h + i] = v[i];
+    }
+  }
+}
+
+// What a product becomes: out[o][n] from its sum y (bias already looked up).
+__device__ __forceinline__ void finish(const hi2x_epilogue& E, float y, float bias, int64_t o,
+                                       int64_t n) {
+  y = activate(y + bias, E.act);
+  if (E.mul) y = y * load_as_f32(E.mul, o * E.ld_mul + n, E.dt_mul);
+  if (E.residual) y = y + load_as_f32(E.residual, o * E.ld_residual + n, E.dt_residual);
+  store_from_f32(E.out, o * E.ld_out + n, E.dt_out, y);
+}
+
+// 16 neighbouring activations, 16-byte aligned.
+__device__ __forceinline__ void load16(const void* x, int64_t at, int dtype, float (&v)[16]) {
+  if (dtype == 0) {
+    const f32x4v* p = reinterpret_cast<const f32x4v*>(static_cast<const float*>(x) + at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f32x4v u = p[i];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[4 * i + j] = u[j];
+    }
+    return;
+  }
+  const u32x4* p = reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(x) + at);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const u32x4 u = p[i];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[8 * i + 2 * j] =
+          dtype == 1 ? f16_from_bits((uint16_t)u[j]) : __uint_as_float(u[j] << 16);
+      v[8 * i + 2 * j + 1] =
+          dtype == 1 ? f16_from_bits((uint16_t)(u[j] >> 16)) : __uint_as_float(u[j] & 0xffff0000u);
+    }
+  }
+}
+
+// Few rows: the epilogue's arguments as for hi2x_packed_linear (packed_few.hip).
+int packed_few(const GemmArgs& g, hipStream_t s);
+
+inline int check_packed(const hi2x_packed* w, const char* what) {
+  HI2X_REQUIRE(w, "%s: null tensor", what);
+  HI2X_REQUIRE(w->experts >= 1 && w->n >= 1 && w->k >= 16 && w->k % 16 == 0,
+               "%s: bad shape (%lld experts of %lld x %lld; columns a multiple of 16)", what,
+               (long long)w->experts, (long long)w->n, (long long)w->k);
+  HI2X_REQUIRE(w->kp % PK_CHUNK == 0 && w->kp >= w->k && w->kp < w->k + PK_CHUNK,
+               "%s: %lld padded columns for %lld", what, (long long)w->kp, (long long)w->k);
+  // a tile's 16 fragments stay below 4 GiB of codes (32-bit offsets)
+  HI2X_REQUIRE(w->n < (1ll << 31) && w->k < (1ll << 20) && w->frags < (1ll << 27) &&
+                   w->experts <= 7000,
+               "%s: tensor too large", what);
+  HI2X_REQUIRE(w->codes && w->params && w->rows && w->segments, "%s: null buffer", what);
+  HI2X_REQUIRE((((uintptr_t)w->codes | (uintptr_t)w->params) & 255) == 0,
+               "%s: layout not 256-byte aligned", what);
+  return HI2X_OK;
+}
+
+inline int check_x(const void* x, int dtype, int64_t ldx, int64_t x_rows, int64_t k,
+                   const char* what) {
+  HI2X_REQUIRE(dtype >= 0 && dtype <= 2, "%s: dtype %d", what, dtype);
+  HI2X_REQUIRE(x_rows >= 0 && ldx >= k, "%s: bad shape", what);
+  HI2X_REQUIRE(x || x_rows == 0, "%s: null activations", what);
+  HI2X_REQUIRE(((uintptr_t)x & 15) == 0 && ldx % (dtype == 0 ? 4 : 8) == 0,
+               "%s: activations not aligned to 16 bytes", what);
+  return HI2X_OK;
+}
+
+inline int check_product(const hi2x_packed* w, const int64_t* src, const int64_t* offs,
+                         int64_t slots, int64_t x_rows, const hi2x_epilogue* epi,
+                         const char* what) {
+  HI2X_REQUIRE(offs || w->experts == 1, "%s: %lld experts without ranges", what,
+               (long long)w->experts);
+  HI2X_REQUIRE(slots >= 0 && slots < (1ll << 31) && x_rows >= 0, "%s: bad rows", what);
+  HI2X_REQUIRE(src || slots <= x_rows, "%s: %lld rows of %lld", what, (long long)slots,
+               (long long)x_rows);
+  HI2X_REQUIRE(epi->act >= HI2X_ACT_NONE && epi->act <= HI2X_ACT_GELU_TANH, "%s: activation %d",
+               what, epi->act);
+  for (int32_t d : {epi->dt_bias, epi->dt_mul, epi->dt_residual, epi->dt_out})
+    HI2X_REQUIRE(d >= 0 && d <= 2, "%s: dtype %d", what, d);
+  HI2X_REQUIRE(slots == 0 || epi->out, "%s: null output", what);
+  HI2X_REQUIRE(epi->ld_out >= w->n && (!epi->mul || epi->ld_mul >= w->n) &&
+                   (!epi->residual || epi->ld_residual >= w->n),
+               "%s: rows overlap", what);
+  return HI2X_OK;
 }
 
 }  // namespace hi2x

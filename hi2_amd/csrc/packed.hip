@@ -65,20 +65,6 @@ __global__ __launch_bounds__(256) void layout_params_kernel(
 }
 
 // ---- activations -------------------------------------------------------------------------
-template <int DT>
-__device__ __forceinline__ void load16(const void* x, int64_t at, float (&v)[16]) {
-  if constexpr (DT == 0) {
-    const float* p = static_cast<const float*>(x) + at;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = p[i];
-  } else {
-    const uint16_t* p = static_cast<const uint16_t*>(x) + at;
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-      v[i] = DT == 1 ? f16_from_bits(p[i]) : __uint_as_float((uint32_t)p[i] << 16);
-  }
-}
-
 // A workgroup transforms one row.  First pass: the largest finite |x / s|; the rotation can
 // grow it fourfold at most, so 2^(13 - exponent) brings every value to at most 2^15, with
 // nothing of the row below fp16's normal range unless it is 2^-27 of the largest.  Second
@@ -113,7 +99,7 @@ __global__ __launch_bounds__(256) void activations_kernel(
   if (!bad) {
     for (int g = tid; g < groups; g += 256) {
       float v[16];
-      load16<DT>(x, base + 16 * (int64_t)g, v);
+      load16(x, base + 16 * (int64_t)g, DT, v);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         float a = v[i];
@@ -143,7 +129,7 @@ __global__ __launch_bounds__(256) void activations_kernel(
 #pragma unroll
       for (int i = 0; i < 16; ++i) v[i] = 0.0f;
     } else {
-      load16<DT>(x, base + 16 * (int64_t)g, v);
+      load16(x, base + 16 * (int64_t)g, DT, v);
       if (cs) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) v[i] = v[i] / f16_from_bits(cs[16 * g + i]);
@@ -188,24 +174,6 @@ __global__ __launch_bounds__(256) void activations_kernel(
 
 using namespace hi2x;
 
-namespace {
-int check_packed(const hi2x_packed* w, const char* what) {
-  HI2X_REQUIRE(w, "%s: null tensor", what);
-  HI2X_REQUIRE(w->experts >= 1 && w->n >= 1 && w->k >= 16 && w->k % 16 == 0,
-               "%s: bad shape (%lld experts of %lld x %lld; columns a multiple of 16)", what,
-               (long long)w->experts, (long long)w->n, (long long)w->k);
-  HI2X_REQUIRE(w->kp % PK_CHUNK == 0 && w->kp >= w->k && w->kp < w->k + PK_CHUNK,
-               "%s: %lld padded columns for %lld", what, (long long)w->kp, (long long)w->k);
-  HI2X_REQUIRE(w->n < (1ll << 31) && w->k < (1ll << 24) && w->frags < (1ll << 27) &&
-                   w->experts <= 7000,
-               "%s: tensor too large", what);
-  HI2X_REQUIRE(w->codes && w->params && w->rows && w->segments, "%s: null buffer", what);
-  HI2X_REQUIRE((((uintptr_t)w->codes | (uintptr_t)w->params) & 255) == 0,
-               "%s: layout not 256-byte aligned", what);
-  return HI2X_OK;
-}
-}  // namespace
-
 extern "C" int hi2x_packed_layout(const hi2x_packed* w, const int32_t* codes,
                                   const int64_t* code_off, const uint8_t* blk_params,
                                   const int64_t* param_off, const uint16_t* row_consts,
@@ -234,18 +202,17 @@ extern "C" int hi2x_packed_activations(const void* x, int dtype, int64_t ldx, in
                                        void* stream) {
   clear_error();
   HI2X_REQUIRE(out, "packed_activations: null output");
-  HI2X_REQUIRE(dtype >= 0 && dtype <= 2, "packed_activations: dtype %d", dtype);
+  if (int rc = check_x(x, dtype, ldx, x_rows, k, "packed_activations")) return rc;
   HI2X_REQUIRE(k >= 16 && k % 16 == 0 && out->kp % PK_CHUNK == 0 && out->kp >= k &&
                    out->kp < k + PK_CHUNK,
                "packed_activations: %lld columns (a multiple of 16), %lld padded", (long long)k,
                (long long)out->kp);
   HI2X_REQUIRE(out->nplanes == 1 || out->nplanes == 2, "packed_activations: %d planes",
                out->nplanes);
-  HI2X_REQUIRE(x_rows >= 0 && out->rows >= 0 && out->rows < (1ll << 31) && ldx >= k,
-               "packed_activations: bad shape");
+  HI2X_REQUIRE(out->rows >= 0 && out->rows < (1ll << 31), "packed_activations: bad shape");
   HI2X_REQUIRE(!offs || experts >= 1, "packed_activations: ranges without experts");
   if (out->rows == 0) return HI2X_OK;
-  HI2X_REQUIRE((x || x_rows == 0) && had && out->planes && out->scale,
+  HI2X_REQUIRE(had && out->planes && out->scale,
                "packed_activations: null buffer");
   HI2X_REQUIRE(src || out->rows <= x_rows, "packed_activations: %lld rows of %lld",
                (long long)out->rows, (long long)x_rows);

@@ -5,24 +5,6 @@
 namespace hi2x {
 namespace {
 
-struct GemmArgs {
-  hi2x_packed w;
-  hi2x_activations x;
-  const int64_t* src;
-  const int64_t* offs;
-  int64_t slots;
-  hi2x_epilogue epi;
-};
-
-// Loads go through buffer resources: a lane's offset is one 32-bit register, the walk along
-// the columns is a scalar offset, and what lies past the resource reads as zero.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void* base, int64_t bytes) {
-  const int64_t most = 0xffffffffll;
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0,
-                                           (int)(uint32_t)(bytes < most ? bytes : most),
-                                           0x00020000);
-}
-
 // 64 lanes x 16 bytes from global memory straight into LDS at `lds` (+ 16 lane).  As inline
 // assembly: the compiler would otherwise take the asynchronous write for an alias of every
 // later LDS read and wait for all loads in flight before each one.
@@ -41,47 +23,6 @@ __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rs, uint32_t voff, 
 
 constexpr int waitcnt(int vm, int lgkm) {
   return (vm & 15) | ((vm >> 4) << 14) | (7 << 4) | (lgkm << 8);
-}
-
-// A tile of up to 4 * NF fragments of one segment.
-struct Tile {
-  hi2x_packed_segment sg;
-  int first;  // fragment in the segment
-  int count;
-};
-
-template <int NF>
-__device__ __forceinline__ bool find_tile(const hi2x_packed& w, int e, int t, Tile& out) {
-  for (int i = 0; i < PK_SEGS; ++i) {
-    const hi2x_packed_segment sg = w.segments[e * PK_SEGS + i];
-    const int n = (sg.frags + 4 * NF - 1) / (4 * NF);
-    if (t < n) {
-      out.sg = sg;
-      out.first = t * 4 * NF;
-      out.count = sg.frags - out.first < 4 * NF ? sg.frags - out.first : 4 * NF;
-      return true;
-    }
-    t -= n;
-  }
-  return false;
-}
-
-template <int BITS>
-__device__ __forceinline__ void load_codes(__amdgpu_buffer_rsrc_t rs, int lane, uint32_t soff,
-                                           uint32_t (&cw)[BITS]) {
-  if constexpr (BITS == 2) {
-    const auto v = __builtin_amdgcn_raw_buffer_load_b64(rs, 8 * lane, (int)soff, 0);
-    cw[0] = v[0];
-    cw[1] = v[1];
-  } else {
-#pragma unroll
-    for (int h = 0; h < BITS / 4; ++h) {
-      const auto v =
-          __builtin_amdgcn_raw_buffer_load_b128(rs, 16 * lane + 1024 * h, (int)soff, 0);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) cw[4 * h + i] = v[i];
-    }
-  }
 }
 
 // The main loop of one tile: 4 waves of NF fragments x 16 MF slots each, all reading the
@@ -186,7 +127,7 @@ __global__ __launch_bounds__(256, 2) void packed_gemm_kernel(GemmArgs g) {
   const int e = __builtin_amdgcn_readfirstlane(wk.e);
   if (e < 0) return;
   Tile tile;
-  if (!find_tile<NF>(g.w, e, blockIdx.x, tile)) return;
+  if (!find_tile(g.w, e, blockIdx.x, 4 * NF, tile)) return;
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
   const int64_t first = __builtin_amdgcn_readfirstlane((int)wk.first);  // slots < 2^31
   const int64_t left = __builtin_amdgcn_readfirstlane((int)wk.end) - first;
@@ -261,10 +202,7 @@ __global__ __launch_bounds__(256, 2) void packed_gemm_kernel(GemmArgs g) {
         int64_t r = g.src ? g.src[o] : o;
         float sc = __builtin_nanf("");
         if (r >= 0 && r < g.x.rows) sc = g.x.scale[r];
-        float y = activate(ep[t * NS + slot] * sc + bias, E.act);
-        if (E.mul) y = y * load_as_f32(E.mul, o * E.ld_mul + n, E.dt_mul);
-        if (E.residual) y = y + load_as_f32(E.residual, o * E.ld_residual + n, E.dt_residual);
-        store_from_f32(E.out, o * E.ld_out + n, E.dt_out, y);
+        finish(E, ep[t * NS + slot] * sc, bias, o, n);
       }
     }
   }
@@ -293,30 +231,17 @@ extern "C" int hi2x_packed_linear(const hi2x_packed* w, const hi2x_activations* 
                                   const hi2x_epilogue* epi, void* stream) {
   clear_error();
   HI2X_REQUIRE(w && x && epi, "packed_linear: null argument");
-  HI2X_REQUIRE(w->experts >= 1 && w->n >= 1 && w->k >= 16 && w->kp % PK_CHUNK == 0 &&
-                   w->kp >= w->k && w->kp < w->k + PK_CHUNK,
-               "packed_linear: bad tensor shape");
-  HI2X_REQUIRE(w->codes && w->params && w->rows && w->segments, "packed_linear: null tensor");
+  if (int rc = check_packed(w, "packed_linear")) return rc;
+  if (int rc = check_product(w, src, offs, slots, x->rows, epi, "packed_linear")) return rc;
   HI2X_REQUIRE(x->kp == w->kp, "packed_linear: activations of %lld padded columns, %lld needed",
                (long long)x->kp, (long long)w->kp);
   HI2X_REQUIRE(x->nplanes == 1 || x->nplanes == 2, "packed_linear: %d planes", x->nplanes);
-  HI2X_REQUIRE(offs || w->experts == 1, "packed_linear: %lld experts without ranges",
-               (long long)w->experts);
-  HI2X_REQUIRE(slots >= 0 && slots < (1ll << 31) && x->rows >= 0, "packed_linear: bad rows");
   HI2X_REQUIRE(!src || x->rows * x->kp * 2 < (1ll << 32) - 1,
                "packed_linear: 4 GiB of activations or more cannot be taken by index");
-  HI2X_REQUIRE(src || slots <= x->rows, "packed_linear: %lld rows of %lld", (long long)slots,
-               (long long)x->rows);
-  HI2X_REQUIRE(epi->act >= HI2X_ACT_NONE && epi->act <= HI2X_ACT_GELU_TANH,
-               "packed_linear: activation %d", epi->act);
-  for (int32_t d : {epi->dt_bias, epi->dt_mul, epi->dt_residual, epi->dt_out})
-    HI2X_REQUIRE(d >= 0 && d <= 2, "packed_linear: dtype %d", d);
   if (slots == 0) return HI2X_OK;
-  HI2X_REQUIRE(x->rows > 0 && x->planes && x->scale && epi->out, "packed_linear: null buffer");
-  HI2X_REQUIRE(epi->ld_out >= w->n && (!epi->mul || epi->ld_mul >= w->n) &&
-                   (!epi->residual || epi->ld_residual >= w->n),
-               "packed_linear: rows overlap");
+  HI2X_REQUIRE(x->rows > 0 && x->planes && x->scale, "packed_linear: null activations");
   const GemmArgs g{*w, *x, src, offs, slots, *epi};
   const hipStream_t s = as_stream(stream);
+  if (slots <= 64 || (offs && slots <= 16 * w->experts)) return packed_few(g, s);
   return launch_gemm<4, 8>(g, s);
 }

@@ -127,6 +127,7 @@ class _Packed:
         self._params = torch.empty(params_at, dtype=torch.uint8, device=dev)
         self._rows = _lib.h2d(torch.from_numpy(np.concatenate(slot_rows)), dev)
         self._segments = _lib.h2d(torch.from_numpy(segs.reshape(-1).view(np.uint8)), dev)
+        self._few = [int(_lib.lib().hi2x_packed_few_rows(k, p)) for p in (1, 2)]
         self.desc = _lib.Packed(self._codes.data_ptr(), self._params.data_ptr(),
                                 self._rows.data_ptr(), self._segments.data_ptr(), e, n, k, kp,
                                 frag, most, (ctypes.c_int64 * 3)(*(int(v) for v in tiles)))
@@ -158,6 +159,8 @@ class _Packed:
                 for h, c in zip(had, cs)]
         #: the transform all tensors share, None where experts have their own
         self.transform = keys[0] if all(x == keys[0] for x in keys) else None
+        #: no rotation and no smoothing at all
+        self.plain = all(c is None for c in cs) and not any(h.any() for h in had)
         own = 1 if self.transform is not None else e
         self._had = _lib.h2d(torch.from_numpy(np.stack(had[:own])), dev)
         self._scale = None if cs[0] is None else \
@@ -222,10 +225,18 @@ def _pitch(x: torch.Tensor) -> int:
     return x.stride(0) if x.shape[0] > 1 else x.shape[1]
 
 
-def _planes(dtype: torch.dtype) -> int:
-    # bf16 and fp16 activations are rounded to one fp16 plane behind the transform; fp32
-    # ones keep 22 bits in two
-    return 2 if dtype == torch.float32 else 1
+def _planes(dtype: torch.dtype, w: _Packed) -> int:
+    """fp16 planes of the transformed activations.  One plane rounds each value by up to
+    2^-11, which a bf16 result's own rounding hides, but not an fp16 or fp32 one's: those
+    take two (22 bits), except fp16 values that the transform leaves as they are."""
+    return 1 if dtype == torch.bfloat16 or dtype == torch.float16 and w.plain else 2
+
+
+def _aligned(x: torch.Tensor) -> torch.Tensor:
+    """Rows that begin at multiples of 16 bytes, as the kernels read them."""
+    if _pitch(x) * x.element_size() % 16:
+        x = x.contiguous()
+    return x.clone() if x.data_ptr() % 16 else x
 
 
 def _transformed(x: torch.Tensor, w: _Packed, src=None, offs=None, rows=None, npl=None
@@ -234,7 +245,8 @@ def _transformed(x: torch.Tensor, w: _Packed, src=None, offs=None, rows=None, np
     dt = _dtype(x, "x")
     x = _rows_of(x, w.k, "x")
     rows = x.shape[0] if rows is None else rows
-    npl = npl or _planes(x.dtype)
+    x = _aligned(x)
+    npl = npl or _planes(x.dtype, w)
     planes = torch.empty(npl, rows, w.kp, dtype=torch.float16, device=dev)
     scale = torch.empty(rows, dtype=torch.float32, device=dev)
     desc = _lib.ActivationsDesc(planes.data_ptr(), scale.data_ptr(), rows, w.kp, npl, 0)
@@ -283,16 +295,40 @@ def _epilogue(w, slots, bias, activation, mul, residual, out, what):
     return e, keep
 
 
-def _product(w, x, act, src, offs, slots, bias, activation, mul, residual, out_dtype, what):
+def _few(x, w, npl, slots, offs):
+    """Whether a product takes its activations as they are and transforms them inside: the
+    rows fit one workgroup tile (of each expert on average at most two)."""
+    fit = w._few[npl - 1]
+    return fit >= 1 and (slots <= fit if offs is None else slots <= min(2, fit) * w.experts)
+
+
+def _product(w, x, src, offs, slots, bias, activation, mul, residual, out_dtype, what, npl=None):
     dev = w.device
     if _lib.require_gpu(x if isinstance(x, torch.Tensor) else x.planes, bias, mul,
                         residual, src, offs) != dev:
         raise RuntimeError(f"{what}: inputs are not on the weights' device {dev}")
     out = torch.empty(slots, w.n, dtype=out_dtype, device=dev)
     epi, keep = _epilogue(w, slots, bias, activation, mul, residual, out, what)
-    if slots:
-        _lib.call("hi2x_packed_linear", dev, ctypes.byref(w.desc), ctypes.byref(act.desc),
-                  _lib.ptr(src), _lib.ptr(offs), slots, ctypes.byref(epi))
+    if not slots:
+        return out
+    if isinstance(x, torch.Tensor):
+        dt = _dtype(x, "x")
+        npl = npl or _planes(x.dtype, w)
+        if _few(x, w, npl, slots, offs):
+            x = _aligned(_rows_of(x, w.k, "x"))
+            _lib.call("hi2x_packed_linear_few", dev, ctypes.byref(w.desc), _lib.ptr(x), dt,
+                      _pitch(x), x.shape[0], npl, _lib.ptr(w._had), _lib.ptr(w._scale),
+                      int(w.transform is None), _lib.ptr(src), _lib.ptr(offs), slots,
+                      ctypes.byref(epi))
+            return out
+        if w.transform is not None:
+            act = _transformed(x, w, npl=npl)
+        else:  # every slot through its own expert's transform
+            act, src = _transformed(x, w, src=src, offs=offs, rows=slots, npl=npl), None
+    else:
+        act = x
+    _lib.call("hi2x_packed_linear", dev, ctypes.byref(w.desc), ctypes.byref(act.desc),
+              _lib.ptr(src), _lib.ptr(offs), slots, ctypes.byref(epi))
     return out
 
 
@@ -313,16 +349,16 @@ def packed_linear(x: torch.Tensor | Activations, w: PackedLinear, bias=None,
         raise TypeError(f"packed_linear takes a PackedLinear, got {type(w).__name__}")
     if isinstance(x, Activations):
         _check_activations(x, w)
-        lead, act, dtype = (x.scale.numel(),), x, x.dtype
+        lead, slots, dtype = (x.scale.numel(),), x.scale.numel(), x.dtype
         _no_grad_inputs("packed_linear", bias, mul, residual)
     else:
         if _lib.require_gpu(x) != w.device:
             raise RuntimeError(f"x is on {x.device}, the weights on {w.device}")
         _no_grad_inputs("packed_linear", x, bias, mul, residual)
         lead, dtype = tuple(x.shape[:-1]), x.dtype
-        act = _transformed(x, w)
-    slots = act.scale.numel()
-    y = _product(w, x, act, None, None, slots, bias, activation, mul, residual,
+        x = _rows_of(x, w.k, "x")
+        slots = x.shape[0]
+    y = _product(w, x, None, None, slots, bias, activation, mul, residual,
                  out_dtype or dtype, "packed_linear")
     return y.reshape(*lead, w.n)
 
@@ -338,7 +374,7 @@ def _routed(offs, rows, w, what):
 
 def experts_linear(x: torch.Tensor | Activations, w: PackedExperts, offs: torch.Tensor,
                    rows: torch.Tensor | None = None, activation: str = "none", mul=None,
-                   residual=None, out_dtype=None, *, _planes=None) -> torch.Tensor:
+                   residual=None, out_dtype=None, *, _npl=None) -> torch.Tensor:
     """``[S, N]``: row j is expert e's product for the routed slot j of its range
     ``offs[e]:offs[e + 1]``, which reads row ``rows[j]`` of ``x`` (row j itself without
     ``rows``), with the epilogue of :func:`packed_linear`.  ``offs`` (device int64, E + 1
@@ -354,17 +390,11 @@ def experts_linear(x: torch.Tensor | Activations, w: PackedExperts, offs: torch.
     _no_grad_inputs("experts_linear", None if given else x, mul, residual)
     if given:
         _check_activations(x, w)
-        act, dtype = x, x.dtype
     else:
-        dtype = x.dtype
-        if w.transform is not None:
-            act = _transformed(x, w, npl=_planes)
-        else:  # every slot through its own expert's transform
-            n = rows.numel() if rows is not None else _rows_of(x, w.k, "x").shape[0]
-            act, rows = _transformed(x, w, src=rows, offs=offs, rows=n, npl=_planes), None
-    slots = rows.numel() if rows is not None else act.scale.numel()
-    return _product(w, x, act, rows, offs, slots, None, activation, mul, residual,
-                    out_dtype or dtype, "experts_linear")
+        x = _rows_of(x, w.k, "x")
+    slots = rows.numel() if rows is not None else (x.scale.numel() if given else x.shape[0])
+    return _product(w, x, rows, offs, slots, None, activation, mul, residual,
+                    out_dtype or x.dtype, "experts_linear", _npl)
 
 
 def combine(y: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor, residual=None,
@@ -417,15 +447,16 @@ def moe_mlp(x: torch.Tensor, routing, gate: PackedExperts, up: PackedExperts,
     if routing.index.shape[0] != flat.shape[0]:
         raise ValueError(f"routing of {routing.index.shape[0]} tokens for {flat.shape[0]}")
     shared = gate.transform is not None and gate.transform == up.transform
-    inp = activations(flat, gate) if shared else flat
     offs, rows = routing.offs, routing.rows
+    few = _few(flat, gate, _planes(x.dtype, gate), rows.numel(), offs)
+    inp = activations(flat, gate) if shared and not few else flat
     g = experts_linear(inp, gate, offs, rows, activation=activation, out_dtype=torch.float32)
     h = experts_linear(inp, up, offs, rows, mul=g, out_dtype=torch.float32)
     del g
     # one fp16 plane of the hidden values is well below a bf16 result's own rounding, and
     # half the products; next to an fp16 result it would show
     y = experts_linear(h, down, offs, out_dtype=torch.float32,
-                       _planes=1 if x.dtype == torch.bfloat16 else 2)
+                       _npl=1 if x.dtype == torch.bfloat16 else 2)
     res = None if residual is None else residual.reshape(flat.shape)
     out = combine(y, routing.slots, routing.weights, residual=res, out_dtype=x.dtype)
     return out.reshape(x.shape)

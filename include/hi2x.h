@@ -568,7 +568,8 @@ typedef struct {
 } hi2x_activations;
 
 /* T(x) = H16(x / col_scale) on the flagged 16-column groups, x / col_scale elsewhere.
- * x [.., k] f32 (dtype 0), fp16 (1) or bf16 (2), rows ldx elements apart; row i of the
+ * x [.., k] f32 (dtype 0), fp16 (1) or bf16 (2), rows ldx elements apart, each at a
+ * multiple of 16 bytes; row i of the
  * result is row src[i] of x (src NULL: row i; an index outside [0, x_rows): a row of NaN).
  * had [k / 16] u8 and col_scale [k] fp16 or NULL.  With offs (experts + 1 row ranges on
  * the device) row i belongs to the expert whose range holds it and uses that expert's
@@ -604,6 +605,18 @@ typedef struct {
 int hi2x_packed_linear(const hi2x_packed* w, const hi2x_activations* x, const int64_t* src,
                        const int64_t* offs, int64_t slots, const hi2x_epilogue* epi,
                        void* stream);
+
+/* hi2x_packed_linear for few rows, with the transform of hi2x_packed_activations inside:
+ * x, had, col_scale and src as there (per_expert: one transform per expert), nplanes 1 or
+ * 2 the planes the transformed rows are held in.  One launch; meant for up to
+ * hi2x_packed_few_rows(k, nplanes) rows (per expert: more are taken in several tiles, each
+ * reading the weights again), which is 0 where k columns do not fit. */
+int hi2x_packed_linear_few(const hi2x_packed* w, const void* x, int dtype, int64_t ldx,
+                           int64_t x_rows, int nplanes, const uint8_t* had,
+                           const uint16_t* col_scale, int per_expert, const int64_t* src,
+                           const int64_t* offs, int64_t slots, const hi2x_epilogue* epi,
+                           void* stream);
+int64_t hi2x_packed_few_rows(int64_t k, int nplanes);
 
 /* ---- routing ------------------------------------------------------------------------------ */
 
