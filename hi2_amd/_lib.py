@@ -93,12 +93,20 @@ class QadGroup(ctypes.Structure):
 SIGNATURES["hi2x_assemble_batch"] = [_P, _I64, _P, _P]
 
 
+class Segment(ctypes.Structure):
+    """hi2x_packed_segment (include/hi2x.h)."""
+
+    _fields_ = [("codes", _I64), ("params", _I64), ("frag0", ctypes.c_int32),
+                ("frags", ctypes.c_int32), ("nbits", ctypes.c_int32), ("block", ctypes.c_int32)]
+
+
 class Packed(ctypes.Structure):
     """hi2x_packed (include/hi2x.h): tensors laid out for products."""
 
     _fields_ = [("codes", _P), ("params", _P), ("rows", _P), ("segments", _P),
                 ("experts", _I64), ("n", _I64), ("k", _I64), ("kp", _I64), ("frags", _I64),
-                ("max_frags", _I64), ("max_tiles", _I64 * 3)]
+                ("max_frags", _I64), ("max_tiles", _I64 * 3), ("had", _P), ("col_scale", _P),
+                ("per_expert", _I64), ("first", Segment * 9)]
 
 
 class ActivationsDesc(ctypes.Structure):
@@ -118,10 +126,11 @@ class Epilogue(ctypes.Structure):
 
 
 SIGNATURES["hi2x_packed_layout"] = [_P, _P, _P, _P, _P, _P, _P]
-SIGNATURES["hi2x_packed_activations"] = [_P, _I, _I64, _I64, _I64, _P, _P, _P, _P, _I64, _P, _P]
-SIGNATURES["hi2x_packed_linear"] = [_P, _P, _P, _P, _I64, _P, _P]
-SIGNATURES["hi2x_packed_linear_few"] = [_P, _P, _I, _I64, _I64, _I, _P, _P, _I, _P, _P, _I64,
-                                        _P, _P]
+SIGNATURES["hi2x_packed_activations"] = [_P, _P, _I, _I64, _I64, _P, _P, _P, _P]
+SIGNATURES["hi2x_packed_linear"] = [_P, _P, _I, _I64, _I64, _I, _P, _P, _I64, _P, _P, _I64, _P]
+SIGNATURES["hi2x_packed_linear_activations"] = [_P, _P, _P, _P, _I64, _P, _P, _I64, _P]
+SIGNATURES["hi2x_moe_mlp"] = [_P, _P, _P, _P, _I, _I64, _I64, _I64, _I, _I, _I, _I, _P, _P, _P, _P,
+                              _P, _I, _P, _I, _P, _I64, _P]
 SIGNATURES["hi2x_route"] = [_P, _I, _I64, _I64, _I64, _I64, _I, _P, _I64, _I64, _I, _F, _P, _P,
                             _P, _P, _P, _P, _I64, _P]
 SIGNATURES["hi2x_route_backward"] = [_P, _I, _I64, _I64, _I64, _I64, _I, _I, _F, _P, _P, _P, _P]
@@ -136,7 +145,8 @@ SIZES = {
     "hi2x_chol_batched_workspace_bytes": [_I64, _I64],
     "hi2x_refine_workspace_bytes": [_I64, _I64, _I64],
     "hi2x_colstats_workspace_bytes": [_I64, _I64],
-    "hi2x_packed_few_rows": [_I64, _I],
+    "hi2x_packed_workspace_bytes": [_P, _I64, _I, _I, _I64, _I, _I],
+    "hi2x_moe_mlp_workspace_bytes": [_P, _P, _P, _I64, _I64, _I, _I, _I],
     "hi2x_route_workspace_bytes": [_I64, _I64],
 }
 

@@ -18,6 +18,40 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr int PK_CHUNK = 128;
 constexpr int PK_SEGS = HI2X_PACKED_SEGMENTS;
 
+// Lane exchanges within rows of 16 lanes.
+template <int CTRL>
+__device__ __forceinline__ int dpp(int x) {
+  return __builtin_amdgcn_update_dpp(x, x, CTRL, 0xf, 0xf, false);
+}
+// Reductions over each row of 16 lanes: neighbours, pairs, halves mirrored, row mirrored.
+#define HI2X_ROW16(x, OP)   \
+  x = OP(x, dpp<0xB1>(x));  \
+  x = OP(x, dpp<0x4E>(x));  \
+  x = OP(x, dpp<0x141>(x)); \
+  x = OP(x, dpp<0x140>(x));
+
+__device__ __forceinline__ int umax_(int a, int b) {
+  return (int)((uint32_t)a > (uint32_t)b ? (uint32_t)a : (uint32_t)b);
+}
+__device__ __forceinline__ int umin_(int a, int b) {
+  return (int)((uint32_t)a < (uint32_t)b ? (uint32_t)a : (uint32_t)b);
+}
+__device__ __forceinline__ int or_(int a, int b) { return a | b; }
+__device__ __forceinline__ uint32_t row_umax(uint32_t v) {
+  int x = (int)v;
+  HI2X_ROW16(x, umax_)
+  return (uint32_t)x;
+}
+__device__ __forceinline__ uint32_t row_umin(uint32_t v) {
+  int x = (int)v;
+  HI2X_ROW16(x, umin_)
+  return (uint32_t)x;
+}
+__device__ __forceinline__ uint32_t row_or(uint32_t v) {
+  int x = (int)v;
+  HI2X_ROW16(x, or_)
+  return (uint32_t)x;
+}
 // Loads of a row operand (bias, factor, residual) by its type.
 __device__ __forceinline__ float load_as_f32(const void* p, int64_t i, int dtype) {
   if (dtype == 0) return static_cast<const float*>(p)[i];
@@ -60,9 +94,17 @@ __device__ __forceinline__ float activate(float y, int act) {
 // codes as pairs (bits f and 16 + f), so masking one pair leaves two codes in the
 // mantissas of two halves; with the exponent of 1024 or-ed in, each half is exactly
 // 1024 + code 2^f, and one exact packed fma (or add) takes that to the code itself.
+// `magic` is DECODE_MAGIC in a vector register (decode_magic), which lets mask and or be one
+// instruction.
+constexpr uint32_t DECODE_MAGIC = 0x64006400u;
+__device__ __forceinline__ uint32_t decode_magic() {
+  uint32_t m = DECODE_MAGIC;
+  asm("" : "+v"(m));
+  return m;
+}
 template <int BITS>
 __device__ __forceinline__ h16x8 decode_step(const uint32_t (&cw)[BITS], int s, h16x2 lo,
-                                             h16x2 st) {
+                                             h16x2 st, uint32_t magic) {
   h16x8 out;
 #pragma unroll
   for (int p = 0; p < 4; ++p) {
@@ -79,7 +121,7 @@ __device__ __forceinline__ h16x8 decode_step(const uint32_t (&cw)[BITS], int s, 
       f = 0;
     }
     constexpr uint32_t M = (1u << BITS) - 1u;
-    const uint32_t x = (w & ((M << f) | (M << (16 + f)))) | 0x64006400u;
+    const uint32_t x = (w & ((M << f) | (M << (16 + f)))) | magic;
     const h16x2 v = __builtin_bit_cast(h16x2, x);
     h16x2 c;
     if (f == 0) {
@@ -163,27 +205,64 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc(const void* base, int64_t
                                            0x00020000);
 }
 
-// A tile of up to `per` fragments of one segment.
+// A tile of up to `per` fragments of one segment: number t of expert e's, segment by segment.
+// One expert's table comes with the arguments; of several, each lane reads one segment, so
+// that finding the tile costs one load's latency.
 struct Tile {
-  hi2x_packed_segment sg;
-  int first;  // fragment in the segment
+  int64_t codes, params;
+  int nbits, block;
+  int frag;   // first fragment, over all experts
+  int first;  // and in its segment
   int count;
 };
 
 __device__ __forceinline__ bool find_tile(const hi2x_packed& w, int e, int t, int per,
                                           Tile& out) {
-  for (int i = 0; i < PK_SEGS; ++i) {
-    const hi2x_packed_segment sg = w.segments[e * PK_SEGS + i];
-    const int n = (sg.frags + per - 1) / per;
-    if (t < n) {
-      out.sg = sg;
-      out.first = t * per;
-      out.count = sg.frags - out.first < per ? sg.frags - out.first : per;
-      return true;
+  if (w.experts == 1) {
+#pragma unroll
+    for (int i = 0; i < PK_SEGS; ++i) {
+      const hi2x_packed_segment& sg = w.first[i];
+      const int n = (sg.frags + per - 1) / per;
+      if (t >= 0 && t < n) {
+        out.codes = sg.codes;
+        out.params = sg.params;
+        out.nbits = sg.nbits;
+        out.block = sg.block;
+        out.first = t * per;
+        out.frag = sg.frag0 + out.first;
+        out.count = sg.frags - out.first < per ? sg.frags - out.first : per;
+        return true;
+      }
+      t -= n;
     }
-    t -= n;
+    return false;
   }
-  return false;
+  const int lane = threadIdx.x & 63;
+  hi2x_packed_segment sg{};
+  if (lane < PK_SEGS) sg = w.segments[e * PK_SEGS + lane];
+  const int n = (sg.frags + per - 1) / per;
+  int upto = n;
+#pragma unroll
+  for (int d = 1; d < 16; d <<= 1) {
+    const int o = __shfl_up(upto, d);
+    if (lane >= d) upto += o;
+  }
+  const unsigned long long hit = __ballot(lane < PK_SEGS && t < upto && t >= upto - n);
+  if (!hit) return false;
+  const int l = __builtin_ctzll(hit);
+  auto at = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+  auto at64 = [&](int64_t v) {
+    return (int64_t)(uint32_t)at((int)v) | (int64_t)at((int)(v >> 32)) << 32;
+  };
+  out.codes = at64(sg.codes);
+  out.params = at64(sg.params);
+  out.nbits = at(sg.nbits);
+  out.block = at(sg.block);
+  out.first = (t - at(upto - n)) * per;
+  out.frag = at(sg.frag0) + out.first;
+  const int left = at(sg.frags) - out.first;
+  out.count = left < per ? left : per;
+  return true;
 }
 
 template <int BITS>
@@ -202,15 +281,6 @@ __device__ __forceinline__ void load_codes(__amdgpu_buffer_rsrc_t rs, int lane, 
       for (int i = 0; i < 4; ++i) cw[4 * h + i] = v[i];
     }
   }
-}
-
-// What a product becomes: out[o][n] from its sum y (bias already looked up).
-__device__ __forceinline__ void finish(const hi2x_epilogue& E, float y, float bias, int64_t o,
-                                       int64_t n) {
-  y = activate(y + bias, E.act);
-  if (E.mul) y = y * load_as_f32(E.mul, o * E.ld_mul + n, E.dt_mul);
-  if (E.residual) y = y + load_as_f32(E.residual, o * E.ld_residual + n, E.dt_residual);
-  store_from_f32(E.out, o * E.ld_out + n, E.dt_out, y);
 }
 
 // 16 neighbouring activations, 16-byte aligned.
@@ -239,8 +309,53 @@ __device__ __forceinline__ void load16(const void* x, int64_t at, int dtype, flo
   }
 }
 
-// Few rows: the epilogue's arguments as for hi2x_packed_linear (packed_few.hip).
-int packed_few(const GemmArgs& g, hipStream_t s);
+// Whether a product goes to packed_few: its rows fit one operand (each expert's do on
+// average).  A wave of it walks an eighth of the columns alone: 4096 x 14336 at 16 rows took
+// 33 us so and 23 us in 64 x 64 tiles with the columns in eight shares, 4096 x 4096 13 and 14,
+// 14336 x 4096 16 and 20, 28672 x 8192 34 and 43.
+inline bool few_rows_product(const hi2x_packed& w, int64_t slots, bool ranges) {
+  if (ranges) return slots <= 16 * w.experts;
+  return slots <= 16 && (w.kp <= 8192 || w.max_frags >= 512);
+}
+
+constexpr int64_t FEW_RAW = 8;  // rows the few-rows kernel transforms for itself
+
+// Activations as they are: rows ldx elements apart; with x2 (same type and pitch, 32 bits)
+// act(x) * x2 elementwise.
+struct RawRows {
+  const void* x;
+  int dtype;
+  int64_t ldx, rows;
+  int npl;  // planes of their transform
+  const float* x2 = nullptr;
+  int act = 0;
+};
+
+// Products of `count` (1 or 2) tensors of one shape from the same activations; the epilogue's
+// arguments as for hi2x_packed_linear.
+struct GemmPair {
+  GemmArgs g[2];
+};
+int packed_few(const GemmPair& g, int count, hipStream_t s);
+int packed_few_raw(const GemmPair& g, int count, const RawRows& x, hipStream_t s);
+int packed_product(const GemmPair& g, int count, void* work, int64_t work_bytes, hipStream_t s);
+int64_t packed_part_bytes(const hi2x_packed& w, int64_t slots, bool ranges, int npl);
+int launch_activations(const RawRows& x, const hi2x_packed& w, const int64_t* src,
+                       const int64_t* offs, const hi2x_activations& out, hipStream_t s);
+int launch_combine(const void* y, int dt_y, int64_t y_rows, int64_t n, const int64_t* slots,
+                   const float* weights, int64_t t, int64_t top_k, const void* residual,
+                   int dt_residual, void* out, int dt_out, hipStream_t s);
+
+// Whether a product takes its activations as they are and transforms them inside (of
+// experts: two rows each on average).
+inline bool few_raw_product(const hi2x_packed& w, int64_t slots, bool ranges) {
+  return ranges ? slots <= 2 * w.experts : slots <= FEW_RAW;
+}
+
+inline int64_t plane_bytes(const hi2x_packed& w, int64_t rows, int npl) {
+  return rows * w.kp * 2 * npl;  // a multiple of 256
+}
+inline int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 
 inline int check_packed(const hi2x_packed* w, const char* what) {
   HI2X_REQUIRE(w, "%s: null tensor", what);

@@ -65,23 +65,42 @@ __global__ __launch_bounds__(256) void layout_params_kernel(
 }
 
 // ---- activations -------------------------------------------------------------------------
-// A workgroup transforms one row.  First pass: the largest finite |x / s|; the rotation can
+// The 16 values of group g of a row, divided by their smoothing: of x, or (GLU) of
+// act(x) * x2.
+template <int DT, bool GLU>
+__device__ __forceinline__ void group_values(const RawRows& x, int64_t base, int g,
+                                             const uint16_t* cs, float (&v)[16]) {
+  load16(x.x, base + 16 * (int64_t)g, DT, v);
+  if constexpr (GLU) {
+    float u[16];
+    load16(x.x2, base + 16 * (int64_t)g, 0, u);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = activate(v[i], x.act) * u[i];
+  }
+  if (cs) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = v[i] / f16_from_bits(cs[16 * g + i]);
+  }
+}
+
+// A workgroup transforms one row.  The largest finite |x / s| comes first; the rotation can
 // grow it fourfold at most, so 2^(13 - exponent) brings every value to at most 2^15, with
-// nothing of the row below fp16's normal range unless it is 2^-27 of the largest.  Second
-// pass: scaled (exact), rotated by butterflies in f32, rounded to fp16.  That rounding
-// (2^-12 of each value, independent) is below the output's own for bf16 and as large as
-// fp16's; nplanes 2 keeps the rest of it in a second plane.
-template <int DT>
+// nothing of the row below fp16's normal range unless it is 2^-27 of the largest.  Then the
+// values are scaled (exact), rotated by butterflies in f32 and rounded to fp16.  That
+// rounding (2^-12 of each value, independent) is below the output's own for bf16 and as
+// large as fp16's; nplanes 2 keeps the rest of it in a second plane.  A thread keeps its
+// group's values between the two where one group a thread is all there is (KEEP, 4096
+// columns); rows beyond are read twice, the second time from L2.
+template <int DT, bool GLU, bool KEEP>
 __global__ __launch_bounds__(256) void activations_kernel(
-    const void* __restrict__ x, int64_t ldx, int64_t x_rows, int64_t k,
-    const int64_t* __restrict__ src, const uint8_t* __restrict__ had,
+    RawRows x, int64_t k, const int64_t* __restrict__ src, const uint8_t* __restrict__ had,
     const uint16_t* __restrict__ cs, const int64_t* __restrict__ offs, int experts,
     hi2x_activations out) {
   const int64_t row = blockIdx.x;
   const int tid = threadIdx.x;
   const int64_t from = src ? src[row] : row;
-  const bool bad = from < 0 || from >= x_rows;
-  const int64_t base = bad ? 0 : from * ldx;
+  const bool bad = from < 0 || from >= x.rows;
+  const int64_t base = bad ? 0 : from * x.ldx;
   if (offs) {
     int lo = 0, hi = experts - 1;  // the expert whose range holds the row
     while (lo < hi) {
@@ -95,16 +114,15 @@ __global__ __launch_bounds__(256) void activations_kernel(
     if (cs) cs += (int64_t)lo * k;
   }
   const int groups = (int)(k / 16), all = (int)(out.kp / 16);
-  float m = 0.0f;
+  float v[16], m = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = 0.0f;
   if (!bad) {
     for (int g = tid; g < groups; g += 256) {
-      float v[16];
-      load16(x, base + 16 * (int64_t)g, DT, v);
+      group_values<DT, GLU>(x, base, g, cs, v);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        float a = v[i];
-        if (cs) a = a / f16_from_bits(cs[16 * g + i]);
-        a = fabsf(a);
+        const float a = fabsf(v[i]);
         m = fmaxf(m, a < __builtin_inff() ? a : 0.0f);
       }
     }
@@ -121,19 +139,13 @@ __global__ __launch_bounds__(256) void activations_kernel(
   const int e = 13 - ex > 126 ? 126 : (13 - ex < -126 ? -126 : 13 - ex);
   const float sc = ldexpf(1.0f, e);
   if (tid == 0) out.scale[row] = bad ? __builtin_nanf("") : ldexpf(1.0f, -e);
-  uint16_t* dst = out.planes + row * out.kp;
-  const int64_t plane = out.rows * out.kp;
+  uint16_t* dst = out.planes + row * out.kp * out.nplanes;
   for (int g = tid; g < all; g += 256) {
-    float v[16];
     if (bad || g >= groups) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) v[i] = 0.0f;
     } else {
-      load16(x, base + 16 * (int64_t)g, DT, v);
-      if (cs) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = v[i] / f16_from_bits(cs[16 * g + i]);
-      }
+      if constexpr (!KEEP) group_values<DT, GLU>(x, base, g, cs, v);
 #pragma unroll
       for (int i = 0; i < 16; ++i) v[i] *= sc;
       if (had[g]) {
@@ -150,26 +162,51 @@ __global__ __launch_bounds__(256) void activations_kernel(
         for (int i = 0; i < 16; ++i) v[i] *= 0.25f;
       }
     }
-    uint32_t h[8], l[8];
+    uint32_t h[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint16_t a = f16_bits(v[2 * i]), b = f16_bits(v[2 * i + 1]);
-      h[i] = (uint32_t)a | (uint32_t)b << 16;
-      l[i] = (uint32_t)f16_bits(v[2 * i] - f16_from_bits(a)) |
-             (uint32_t)f16_bits(v[2 * i + 1] - f16_from_bits(b)) << 16;
-    }
-    u32x4* d = reinterpret_cast<u32x4*>(dst + 16 * (int64_t)g);
+    for (int i = 0; i < 8; ++i)
+      h[i] = (uint32_t)f16_bits(v[2 * i]) | (uint32_t)f16_bits(v[2 * i + 1]) << 16;
+    uint16_t* at = dst + (int64_t)(g >> 3) * (PK_CHUNK * out.nplanes) + 16 * (g & 7);
+    u32x4* d = reinterpret_cast<u32x4*>(at);
     d[0] = u32x4{h[0], h[1], h[2], h[3]};
     d[1] = u32x4{h[4], h[5], h[6], h[7]};
     if (out.nplanes == 2) {
-      d = reinterpret_cast<u32x4*>(dst + plane + 16 * (int64_t)g);
-      d[0] = u32x4{l[0], l[1], l[2], l[3]};
-      d[1] = u32x4{l[4], l[5], l[6], l[7]};
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        h[i] = (uint32_t)f16_bits(v[2 * i] - f16_from_bits((uint16_t)h[i])) |
+               (uint32_t)f16_bits(v[2 * i + 1] - f16_from_bits((uint16_t)(h[i] >> 16))) << 16;
+      d = reinterpret_cast<u32x4*>(at + PK_CHUNK);
+      d[0] = u32x4{h[0], h[1], h[2], h[3]};
+      d[1] = u32x4{h[4], h[5], h[6], h[7]};
     }
   }
 }
 
 }  // namespace
+
+int launch_activations(const RawRows& x, const hi2x_packed& w, const int64_t* src,
+                       const int64_t* offs, const hi2x_activations& out, hipStream_t s) {
+  const dim3 grid((unsigned)out.rows);
+#define HI2X_ROWS(DT, GLU)                                                                   \
+  if (w.kp <= 4096)                                                                          \
+    activations_kernel<DT, GLU, true><<<grid, 256, 0, s>>>(x, w.k, src, w.had, w.col_scale,  \
+                                                           offs, (int)w.experts, out);       \
+  else                                                                                       \
+    activations_kernel<DT, GLU, false><<<grid, 256, 0, s>>>(x, w.k, src, w.had, w.col_scale, \
+                                                            offs, (int)w.experts, out);
+  if (x.x2) {
+    HI2X_ROWS(0, true)
+  } else if (x.dtype == 0) {
+    HI2X_ROWS(0, false)
+  } else if (x.dtype == 1) {
+    HI2X_ROWS(1, false)
+  } else {
+    HI2X_ROWS(2, false)
+  }
+#undef HI2X_ROWS
+  return launch_status("packed_activations");
+}
+
 }  // namespace hi2x
 
 using namespace hi2x;
@@ -195,38 +232,26 @@ extern "C" int hi2x_packed_layout(const hi2x_packed* w, const int32_t* codes,
   return launch_status("packed_layout");
 }
 
-extern "C" int hi2x_packed_activations(const void* x, int dtype, int64_t ldx, int64_t x_rows,
-                                       int64_t k, const int64_t* src, const uint8_t* had,
-                                       const uint16_t* col_scale, const int64_t* offs,
-                                       int64_t experts, const hi2x_activations* out,
+extern "C" int hi2x_packed_activations(const hi2x_packed* w, const void* x, int dtype,
+                                       int64_t ldx, int64_t x_rows, const int64_t* src,
+                                       const int64_t* offs, const hi2x_activations* out,
                                        void* stream) {
   clear_error();
   HI2X_REQUIRE(out, "packed_activations: null output");
-  if (int rc = check_x(x, dtype, ldx, x_rows, k, "packed_activations")) return rc;
-  HI2X_REQUIRE(k >= 16 && k % 16 == 0 && out->kp % PK_CHUNK == 0 && out->kp >= k &&
-                   out->kp < k + PK_CHUNK,
-               "packed_activations: %lld columns (a multiple of 16), %lld padded", (long long)k,
-               (long long)out->kp);
+  if (int rc = check_packed(w, "packed_activations")) return rc;
+  if (int rc = check_x(x, dtype, ldx, x_rows, w->k, "packed_activations")) return rc;
+  HI2X_REQUIRE(out->kp == w->kp, "packed_activations: %lld padded columns, %lld needed",
+               (long long)out->kp, (long long)w->kp);
   HI2X_REQUIRE(out->nplanes == 1 || out->nplanes == 2, "packed_activations: %d planes",
                out->nplanes);
   HI2X_REQUIRE(out->rows >= 0 && out->rows < (1ll << 31), "packed_activations: bad shape");
-  HI2X_REQUIRE(!offs || experts >= 1, "packed_activations: ranges without experts");
+  HI2X_REQUIRE(offs || !w->per_expert, "packed_activations: %lld transforms without ranges",
+               (long long)w->experts);
   if (out->rows == 0) return HI2X_OK;
-  HI2X_REQUIRE(had && out->planes && out->scale,
-               "packed_activations: null buffer");
+  HI2X_REQUIRE(out->planes && out->scale, "packed_activations: null buffer");
   HI2X_REQUIRE(src || out->rows <= x_rows, "packed_activations: %lld rows of %lld",
                (long long)out->rows, (long long)x_rows);
   HI2X_REQUIRE(((uintptr_t)out->planes & 255) == 0, "packed_activations: planes not aligned");
-  const hipStream_t s = as_stream(stream);
-  const dim3 grid((unsigned)out->rows);
-  if (dtype == 0)
-    activations_kernel<0><<<grid, 256, 0, s>>>(x, ldx, x_rows, k, src, had, col_scale, offs,
-                                               (int)experts, *out);
-  else if (dtype == 1)
-    activations_kernel<1><<<grid, 256, 0, s>>>(x, ldx, x_rows, k, src, had, col_scale, offs,
-                                               (int)experts, *out);
-  else
-    activations_kernel<2><<<grid, 256, 0, s>>>(x, ldx, x_rows, k, src, had, col_scale, offs,
-                                               (int)experts, *out);
-  return launch_status("packed_activations");
+  return launch_activations(RawRows{x, dtype, ldx, x_rows, out->nplanes}, *w, src,
+                            w->per_expert ? offs : nullptr, *out, as_stream(stream));
 }

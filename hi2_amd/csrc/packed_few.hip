@@ -1,101 +1,122 @@
 // Products of few rows by packed tensors: single tokens, small batches of them, and the
 // experts' products of a decode step.  Bound by reading the packed weights once.
 //
-// A workgroup of 8 waves takes FR fragments (16 FR rows of the tensor) and up to 16 MF
+// A workgroup of 8 waves takes FR fragments (16 FR rows of the tensor) and up to MT
 // activation rows; the columns are split over the waves by chunks of 128, and the partial
-// sums meet in LDS, so nothing is joined across workgroups.  A wave keeps D chunks of codes
-// in flight (one 16-byte load a lane holds a fragment's whole chunk at 4 bits).
+// sums meet in LDS, so nothing is joined across workgroups.  A wave keeps UN chunks of codes
+// in flight (one 16-byte load a lane holds a fragment's whole chunk at 4 bits).  The loops
+// stay rolled: unrolled, the code of a short call outgrows the instruction cache.
 #include "packed.h"
 
 namespace hi2x {
 namespace {
 
-constexpr int FW = 8;  // waves
-
 struct FewArgs {
-  GemmArgs g;
-  // fused: the activations as they are, transformed here
-  const void* x;
-  int dtype;
-  int64_t ldx, x_rows;
-  const uint8_t* had;
-  const uint16_t* cs;
-  int per_expert;  // had and cs hold one transform per expert
-  int npl;         // fp16 planes of the transformed activations
-  int mt;          // activation rows of a workgroup
+  GemmPair two;  // blockIdx.z picks
+  RawRows x;     // activations that are transformed here
 };
 
-// The transform of a wave's own columns (chunks w, w + 8, ...) into LDS, one 16-column group
-// of one row per lane and pass.  As in the separate pass (activations_kernel) each row is
-// scaled by a power of two, here by the largest value among the wave's columns.  Row r of
-// chunk i lies at (i R + r) 256 with its 16-byte pieces p at p ^ (r % 16); R = mt npl, the
-// second plane's rows behind the first's.
-__device__ __forceinline__ void few_transform(const FewArgs& a, int e, int64_t first, int live,
-                                              int w, int nc, char* xl, uint32_t* mx,
-                                              float* unscale) {
-  const int lane = threadIdx.x & 63;
-  const int k = (int)a.g.w.k;
-  const int R = a.mt * a.npl;
-  const uint8_t* had = a.had + (a.per_expert ? (int64_t)e * (k / 16) : 0);
-  const uint16_t* cs = a.cs ? a.cs + (a.per_expert ? (int64_t)e * k : 0) : nullptr;
-  const int total = nc * 8 * live;
-  const int passes = (total + 63) / 64;
-  if (lane < 16) mx[lane] = 0;
-  float v[16];
-  auto load = [&](int p, int& row, int& i, int& g) {
-    const int j = p * 64 + lane;
-    row = j / (nc * 8);
-    const int rest = j - row * (nc * 8);
-    i = rest >> 3;
-    g = 8 * (w + FW * i) + (rest & 7);  // group of 16 columns
-    const bool in = j < total;
-    const int64_t src = in ? (a.g.src ? a.g.src[first + row] : first + row) : -1;
-    if (src < 0 || src >= a.x_rows || 16 * g >= k) {
+// activations: transformed, or as they are (16 bits, 32 bits, act(x) * x2 of 32 bits)
+enum { GIVEN = 0, RAW16 = 1, RAW32 = 2, GLU32 = 3 };
+
+// One pass of the transform: the wave's next CP = 8 / MP chunks of up to MP rows (a power of
+// two), a 16-column group of one row per lane.  As in the separate pass (activations_kernel)
+// a row is scaled by a power of two, here by its largest value among the pass's columns; the
+// products of a pass are summed apart and unscaled.  Row r of chunk i lies in LDS at
+// (i R + r) 256 with its 16-byte pieces p at p ^ (r % 16); R = MP npl, the second plane's
+// rows behind the first's.
+template <int MODE, int MP, int FW>
+struct FewPass {
+  static constexpr bool F32 = MODE != RAW16, GLU = MODE == GLU32;
+  static constexpr int CP = 8 / MP, V = F32 ? 4 : 2;  // chunks; 16-byte pieces of a group
+  u32x4 raw[V], up[GLU ? V : 1];
+
+  __device__ __forceinline__ static int group(int w, int i0) {  // of 16 columns
+    const int r = threadIdx.x & (64 / MP - 1);
+    return 8 * (w + FW * (i0 + (r >> 3))) + (r & 7);
+  }
+
+  // `src`: the lane's row of the activations, negative for none
+  __device__ __forceinline__ void load(const FewArgs& a, int k, int64_t src, int w, int i0) {
+    const int g = group(w, i0);
 #pragma unroll
-      for (int t = 0; t < 16; ++t) v[t] = 0.0f;
-      return in;
+    for (int v = 0; v < V; ++v) raw[v] = up[GLU ? v : 0] = u32x4{0u, 0u, 0u, 0u};
+    if (src >= 0 && 16 * g < k) {
+      const u32x4* from = reinterpret_cast<const u32x4*>(
+          static_cast<const char*>(a.x.x) + (src * a.x.ldx + 16 * g) * (F32 ? 4 : 2));
+#pragma unroll
+      for (int v = 0; v < V; ++v) raw[v] = from[v];
+      if constexpr (GLU) {
+        from = reinterpret_cast<const u32x4*>(a.x.x2 + src * a.x.ldx + 16 * g);
+#pragma unroll
+        for (int v = 0; v < V; ++v) up[v] = from[v];
+      }
     }
-    load16(a.x, src * a.ldx + 16 * g, a.dtype, v);
-    if (cs) {
+  }
+
+  // Returns the factor that unscales the lane's row.
+  __device__ __forceinline__ float store(const FewArgs& a, int k, const uint8_t* had,
+                                         const uint16_t* cs, int w, int i0, char* xl) const {
+    const int lane = threadIdx.x & 63, g = group(w, i0);
+    const bool in = 16 * g < k;
+    float v[16];
+    if constexpr (F32) {
+#pragma unroll
+      for (int t = 0; t < 16; ++t) v[t] = __uint_as_float(raw[t >> 2][t & 3]);
+      if constexpr (GLU) {
+#pragma unroll
+        for (int t = 0; t < 16; ++t)
+          v[t] = activate(v[t], a.x.act) * __uint_as_float(up[t >> 2][t & 3]);
+      }
+    } else if (a.x.dtype == 1) {
+#pragma unroll
+      for (int t = 0; t < 16; ++t)
+        v[t] = f16_from_bits((uint16_t)(raw[t >> 3][(t >> 1) & 3] >> (16 * (t & 1))));
+    } else {
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        const uint32_t u = raw[t >> 2][t & 3];
+        v[2 * t] = __uint_as_float(u << 16);
+        v[2 * t + 1] = __uint_as_float(u & 0xffff0000u);
+      }
+    }
+    if (cs && in) {
 #pragma unroll
       for (int t = 0; t < 16; ++t) v[t] = v[t] / f16_from_bits(cs[16 * g + t]);
     }
-    return in;
-  };
-  int row, i, g;
-  bool in = false;
-  for (int p = 0; p < passes; ++p) {
-    in = load(p, row, i, g);
     float m = 0.0f;
 #pragma unroll
-    for (int t = 0; t < 16; ++t) {
-      const float b = fabsf(v[t]);
-      m = fmaxf(m, b < __builtin_inff() ? b : 0.0f);
+    for (int t = 0; t < 16; ++t) m = fmaxf(m, fabsf(v[t]));  // NaN is passed over
+    if (m == __builtin_inff()) {
+      m = 0.0f;
+#pragma unroll
+      for (int t = 0; t < 16; ++t) {
+        const float b = fabsf(v[t]);
+        m = fmaxf(m, b < __builtin_inff() ? b : 0.0f);
+      }
     }
-    if (in && m > 0.0f) atomicMax(&mx[row], __float_as_uint(m));
-  }
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup", "local");  // the wave's own values
-  if (lane < 16) {
-    const float m = __uint_as_float(mx[lane]);
+    uint32_t mb = __float_as_uint(m);  // the order of non-negative floats
+    if constexpr (MP <= 4) {
+      mb = row_umax(mb);
+#pragma unroll
+      for (int d = 16; d < 64 / MP; d <<= 1) {
+        const uint32_t o = __shfl_xor(mb, d);
+        mb = o > mb ? o : mb;
+      }
+    } else {
+#pragma unroll
+      for (int d = 1; d < 64 / MP; d <<= 1) {
+        const uint32_t o = __shfl_xor(mb, d);
+        mb = o > mb ? o : mb;
+      }
+    }
     int ex = 0;
-    if (m > 0.0f) (void)frexpf(m, &ex);
+    if (mb) (void)frexpf(__uint_as_float(mb), &ex);
     const int s = 13 - ex > 126 ? 126 : (13 - ex < -126 ? -126 : 13 - ex);
-    mx[lane] = (uint32_t)s;
-    bool bad = false;
-    if (lane < live && a.g.src) {
-      const int64_t src = a.g.src[first + lane];
-      bad = src < 0 || src >= a.x_rows;
-    }
-    unscale[lane] = bad ? __builtin_nanf("") : ldexpf(1.0f, -s);
-  }
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup", "local");
-  for (int p = 0; p < passes; ++p) {
-    if (passes > 1) in = load(p, row, i, g);
-    if (!in) continue;
-    const float sc = ldexpf(1.0f, (int)mx[row]);
+    const float sc = ldexpf(1.0f, s);
 #pragma unroll
     for (int t = 0; t < 16; ++t) v[t] *= sc;
-    if (16 * g < k && had[g]) {
+    if (in && had[g]) {
 #pragma unroll
       for (int d = 1; d < 16; d <<= 1)
 #pragma unroll
@@ -108,81 +129,72 @@ __device__ __forceinline__ void few_transform(const FewArgs& a, int e, int64_t f
 #pragma unroll
       for (int t = 0; t < 16; ++t) v[t] *= 0.25f;
     }
-    uint32_t h[8], l[8];
+    const int R = MP * a.x.npl, p0 = 2 * (g & 7);
+    const int r = lane / (64 / MP), chunk = (lane & (64 / MP - 1)) >> 3;
+    uint32_t h[8];
 #pragma unroll
-    for (int t = 0; t < 8; ++t) {
-      const uint16_t x = f16_bits(v[2 * t]), y = f16_bits(v[2 * t + 1]);
-      h[t] = (uint32_t)x | (uint32_t)y << 16;
-      l[t] = (uint32_t)f16_bits(v[2 * t] - f16_from_bits(x)) |
-             (uint32_t)f16_bits(v[2 * t + 1] - f16_from_bits(y)) << 16;
+    for (int t = 0; t < 8; ++t)
+      h[t] = (uint32_t)f16_bits(v[2 * t]) | (uint32_t)f16_bits(v[2 * t + 1]) << 16;
+    char* d = xl + (chunk * R + r) * 256;
+    *reinterpret_cast<u32x4*>(d + 16 * (p0 ^ r)) = u32x4{h[0], h[1], h[2], h[3]};
+    *reinterpret_cast<u32x4*>(d + 16 * ((p0 + 1) ^ r)) = u32x4{h[4], h[5], h[6], h[7]};
+    if (a.x.npl == 2) {
+      const int r2 = MP + r;
+#pragma unroll
+      for (int t = 0; t < 8; ++t)
+        h[t] = (uint32_t)f16_bits(v[2 * t] - f16_from_bits((uint16_t)h[t])) |
+               (uint32_t)f16_bits(v[2 * t + 1] - f16_from_bits((uint16_t)(h[t] >> 16))) << 16;
+      d = xl + (chunk * R + r2) * 256;
+      *reinterpret_cast<u32x4*>(d + 16 * (p0 ^ r2)) = u32x4{h[0], h[1], h[2], h[3]};
+      *reinterpret_cast<u32x4*>(d + 16 * ((p0 + 1) ^ r2)) = u32x4{h[4], h[5], h[6], h[7]};
     }
-    const int p0 = 2 * (g & 7);
-    {
-      char* d = xl + (i * R + row) * 256;
-      *reinterpret_cast<u32x4*>(d + 16 * (p0 ^ (row & 15))) = u32x4{h[0], h[1], h[2], h[3]};
-      *reinterpret_cast<u32x4*>(d + 16 * ((p0 + 1) ^ (row & 15))) = u32x4{h[4], h[5], h[6], h[7]};
-    }
-    if (a.npl == 2) {
-      const int r = a.mt + row;
-      char* d = xl + (i * R + r) * 256;
-      *reinterpret_cast<u32x4*>(d + 16 * (p0 ^ (r & 15))) = u32x4{l[0], l[1], l[2], l[3]};
-      *reinterpret_cast<u32x4*>(d + 16 * ((p0 + 1) ^ (r & 15))) = u32x4{l[4], l[5], l[6], l[7]};
-    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup", "local");  // read by this wave only
+    return ldexpf(1.0f, -s);
   }
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup", "local");
-}
+};
 
-template <int BITS, bool B16, int FR, int MF, bool FUSED>
-__device__ __forceinline__ void few_loop(const FewArgs& a, const Tile& tile, int e, int64_t first,
-                                         int live, char* xl, uint32_t* mx, float* unscale,
-                                         f32x4v (&acc)[FR][MF]) {
-  constexpr int D = FUSED ? (FR == 1 ? 4 : 2) : (FR * MF <= 2 ? 3 : 2);  // chunks in flight
-  const GemmArgs& g = a.g;
-  const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4;
+// MT: activation rows of the workgroup; as they are, a power of two up to 8, transformed, 16,
+// 32 or 64.  A step is one chunk and plane; the codes (and transformed activations) of UN
+// steps are fetched while the UN before them are multiplied.
+template <int BITS, int FR, int MT, int MODE, int FW>
+__device__ __forceinline__ void few_loop(const FewArgs& a, const GemmArgs& g, const Tile& tile, int e, int64_t first,
+                                         int live, char* xl,
+                                         f32x4v (&acc)[FR][MODE == GIVEN ? MT / 16 : 1]) {
+  constexpr bool RAW = MODE != GIVEN;
+  constexpr int MF = RAW ? 1 : MT / 16, MP = RAW ? MT : 1;
+  constexpr int CP = 8 / MP;
+  // (what 128 registers hold)
+  constexpr int RU = BITS == 8 || MODE == GLU32 || (MODE == RAW32 && BITS == 4) ? 2 : 4;
+  constexpr int UN = RAW ? (CP < RU ? CP : RU) : (FR * MF <= 2 ? 2 : 1);
+  const int k = (int)g.w.k;
+  const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4, col = lane & 15;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int nch = (int)(g.w.kp / PK_CHUNK);
   const int nc = w < nch ? (nch - w + FW - 1) / FW : 0;
-  const int64_t nblk = g.w.kp / tile.sg.block;
+  const int psh = RAW ? 0 : g.x.nplanes - 1;
+  const int steps = nc << psh;
+  const int64_t nblk = g.w.kp / tile.block;
   const uint32_t cfrag = (uint32_t)nch * (256 * BITS), pfrag = (uint32_t)nblk * 64;
   const __amdgpu_buffer_rsrc_t cr =
-      rsrc(static_cast<const char*>(g.w.codes) + tile.sg.codes + (int64_t)tile.first * cfrag,
+      rsrc(static_cast<const char*>(g.w.codes) + tile.codes + (int64_t)tile.first * cfrag,
            (int64_t)tile.count * cfrag);
   const __amdgpu_buffer_rsrc_t pr =
-      rsrc(static_cast<const char*>(g.w.params) + tile.sg.params + (int64_t)tile.first * pfrag,
+      rsrc(static_cast<const char*>(g.w.params) + tile.params + (int64_t)tile.first * pfrag,
            (int64_t)tile.count * pfrag);
-  const int bsh = tile.sg.block == 64 ? 6 : (tile.sg.block == 32 ? 5 : 4);
+  const int bsh = tile.block == 64 ? 6 : (tile.block == 32 ? 5 : 4);
   const uint32_t poff = 64 * ((32 * q) >> bsh) + 4 * (lane & 15);
-  uint32_t cw[D][FR][BITS], pw[D][FR][2];
-  auto fetch = [&](int d, int i) {
-    const int c = w + FW * i;
-#pragma unroll
-    for (int f = 0; f < FR; ++f) {
-      load_codes<BITS>(cr, lane, f * cfrag + (uint32_t)c * (256 * BITS), cw[d][f]);
-      const uint32_t so = f * pfrag + ((uint32_t)(c * PK_CHUNK) >> bsh) * 64;
-      pw[d][f][0] = __builtin_amdgcn_raw_buffer_load_b32(pr, (int)poff, (int)so, 0);
-      pw[d][f][1] = B16 ? __builtin_amdgcn_raw_buffer_load_b32(pr, (int)poff + 64, (int)so, 0) : 0u;
-    }
+  const uint32_t poff2 = poff + (tile.block == 16 ? 64 : 0);  // of columns 16..31
+  const uint32_t magic = decode_magic();
+  struct Group {
+    uint32_t cw[UN][FR][BITS], pw[UN][FR][2];
+    h16x8 b[RAW ? 1 : UN][4][MF];
   };
-#pragma unroll
-  for (int d = 0; d < D; ++d)
-    if (d < nc) fetch(d, d);
-  // where this lane's activation rows are
-  const int col = lane & 15;
-  const char* xrow = nullptr;
-  int xr = 0, R = 0;
+  Group cur, nxt;
   uint32_t xoff[MF];
   __amdgpu_buffer_rsrc_t xs;
-  int64_t plane = 0;
-  if constexpr (FUSED) {
-    few_transform(a, e, first, live, w, nc, xl, mx, unscale);
-    R = a.mt * a.npl;
-    xr = a.npl == 2 ? ((col & 7) < live ? (col >> 3) * a.mt + (col & 7) : 0)
-                    : (col < live ? col : 0);
-    xrow = xl + xr * 256;
-  } else {
-    const uint32_t pitch = (uint32_t)g.x.kp * 2;
+  if constexpr (!RAW) {
+    const uint32_t pitch = (uint32_t)g.x.kp * 2 * g.x.nplanes;
     const int64_t row0 = g.src ? 0 : first;
-    plane = g.x.rows * (int64_t)pitch;
     xs = rsrc(reinterpret_cast<const char*>(g.x.planes) + row0 * pitch,
               (g.x.rows - row0) * pitch);
 #pragma unroll
@@ -195,63 +207,117 @@ __device__ __forceinline__ void few_loop(const FewArgs& a, const Tile& tile, int
       xoff[m] = (uint32_t)r * pitch + 64 * q;
     }
   }
-  const int npl = FUSED ? 1 : g.x.nplanes;
-  for (int i0 = 0; i0 < nc; i0 += D) {
+  auto fetch = [&](int s0, Group& to) {
 #pragma unroll
-    for (int d = 0; d < D; ++d) {
-      const int i = i0 + d;
-      if (i < nc) {
-        for (int pl = 0; pl < npl; ++pl) {
-          h16x8 b[4][MF];
+    for (int u = 0; u < UN; ++u) {
+      if (s0 + u >= steps) continue;
+      const int c = w + FW * ((s0 + u) >> psh);
 #pragma unroll
-          for (int s = 0; s < 4; ++s)
+      for (int f = 0; f < FR; ++f) {
+        load_codes<BITS>(cr, lane, f * cfrag + (uint32_t)c * (256 * BITS), to.cw[u][f]);
+        const uint32_t so = f * pfrag + ((uint32_t)(c * PK_CHUNK) >> bsh) * 64;
+        to.pw[u][f][0] = __builtin_amdgcn_raw_buffer_load_b32(pr, (int)poff, (int)so, 0);
+        to.pw[u][f][1] = __builtin_amdgcn_raw_buffer_load_b32(pr, (int)poff2, (int)so, 0);
+      }
+      if constexpr (!RAW) {
+        const int at = ((c << psh) + ((s0 + u) & psh)) * 256;
 #pragma unroll
-            for (int m = 0; m < MF; ++m) {
-              if constexpr (FUSED)
-                b[s][m] = *reinterpret_cast<const h16x8*>(xrow + i * R * 256 +
-                                                          16 * ((4 * q + s) ^ (xr & 15)));
-              else
-                b[s][m] = __builtin_bit_cast(
-                    h16x8, __builtin_amdgcn_raw_buffer_load_b128(
-                               pl ? rsrc(reinterpret_cast<const char*>(g.x.planes) + plane +
-                                             (g.src ? 0 : first) * (int64_t)(g.x.kp * 2),
-                                         (g.x.rows - (g.src ? 0 : first)) * (int64_t)(g.x.kp * 2))
-                                  : xs,
-                               (int)xoff[m] + 16 * s, (w + FW * i) * 256, 0));
-            }
+        for (int s = 0; s < 4; ++s)
 #pragma unroll
-          for (int s = 0; s < 4; ++s)
+          for (int m = 0; m < MF; ++m)
+            to.b[u][s][m] = __builtin_bit_cast(
+                h16x8, __builtin_amdgcn_raw_buffer_load_b128(xs, (int)xoff[m] + 16 * s, at, 0));
+      }
+    }
+  };
+  // raw: the lane's row to transform, and the row its operand column reads
+  FewPass<RAW ? MODE : RAW16, MP, FW> pass;
+  int64_t src = -1;
+  int R = 0, xr = 0, from = 0;
+  float unscale = 1.0f;
+  const uint8_t* had = nullptr;
+  const uint16_t* cs = nullptr;
+  f32x4v part[FR];
+  if constexpr (RAW) {
+    const int row = lane / (64 / MP);
+    if (row < live) {
+      src = g.src ? g.src[first + row] : first + row;
+      if (src >= a.x.rows) src = -1;
+    }
+    pass.load(a, k, src, w, 0);
+    had = g.w.had + (g.w.per_expert ? (int64_t)e * (g.w.k / 16) : 0);
+    cs = g.w.col_scale;
+    if (cs && g.w.per_expert) cs += (int64_t)e * g.w.k;
+    R = MP * a.x.npl;
+    const int t = a.x.npl == 2 ? col & 7 : col, plane = a.x.npl == 2 ? col >> 3 : 0;
+    xr = t < MP ? plane * MP + t : 0;
+    from = t < MP ? t * (64 / MP) : 0;
+  }
+  fetch(0, nxt);
+  for (int s0 = 0; s0 < steps; s0 += UN) {
+    cur = nxt;
+    if constexpr (RAW) {
+      if (s0 % CP == 0) {
+        const FewPass<RAW ? MODE : RAW16, MP, FW> now = pass;
+        if (s0 + CP < steps) pass.load(a, k, src, w, s0 + CP);
+        fetch(s0 + UN, nxt);
+        unscale = now.store(a, k, had, cs, w, s0, xl);
+        unscale = __shfl(src < 0 ? __builtin_nanf("") : unscale, from);
 #pragma unroll
-            for (int f = 0; f < FR; ++f) {
-              const h16x2 ls =
-                  __builtin_bit_cast(h16x2, B16 && s >= 2 ? pw[d][f][1] : pw[d][f][0]);
-              const h16x8 av =
-                  decode_step<BITS>(cw[d][f], s, (h16x2){ls[0], ls[0]}, (h16x2){ls[1], ls[1]});
+        for (int f = 0; f < FR; ++f) part[f] = f32x4v{0.0f, 0.0f, 0.0f, 0.0f};
+      } else {
+        fetch(s0 + UN, nxt);
+      }
+    } else {
+      fetch(s0 + UN, nxt);
+    }
 #pragma unroll
-              for (int m = 0; m < MF; ++m)
-                acc[f][m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, b[s][m], acc[f][m], 0, 0, 0);
-            }
+    for (int u = 0; u < UN; ++u) {
+      if (s0 + u >= steps) break;
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        h16x8 x;
+        if constexpr (RAW)
+          x = *reinterpret_cast<const h16x8*>(xl + (((s0 + u) % CP) * R + xr) * 256 +
+                                              16 * ((4 * q + s) ^ xr));
+#pragma unroll
+        for (int f = 0; f < FR; ++f) {
+          const h16x2 ls = __builtin_bit_cast(h16x2, cur.pw[u][f][s >> 1]);
+          const h16x8 av = decode_step<BITS>(cur.cw[u][f], s, (h16x2){ls[0], ls[0]},
+                                             (h16x2){ls[1], ls[1]}, magic);
+          if constexpr (RAW) {
+            part[f] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, x, part[f], 0, 0, 0);
+          } else {
+#pragma unroll
+            for (int m = 0; m < MF; ++m)
+              acc[f][m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, cur.b[u][s][m], acc[f][m],
+                                                                 0, 0, 0);
+          }
         }
-        if (i + D < nc) fetch(d, i + D);
+      }
+    }
+    if constexpr (RAW) {
+      if (s0 % CP + UN >= CP || s0 + UN >= steps) {
+#pragma unroll
+        for (int f = 0; f < FR; ++f)
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+            acc[f][0][t] = __builtin_fmaf(part[f][t], unscale, acc[f][0][t]);
       }
     }
   }
-  if constexpr (FUSED) {
-    const float u = unscale[a.npl == 2 ? col & 7 : col];
-#pragma unroll
-    for (int f = 0; f < FR; ++f)
-#pragma unroll
-      for (int t = 0; t < 4; ++t) acc[f][0][t] *= nc ? u : 1.0f;
-  }
 }
 
-template <int FR, int MF, bool FUSED>
-__global__ __launch_bounds__(64 * FW) void packed_few_kernel(FewArgs a) {
-  extern __shared__ char lds[];
-  __shared__ uint32_t mx[FW][16];
-  __shared__ float unscale[FW][16];
-  const GemmArgs& g = a.g;
-  const PkWork wk = find_work(g.offs, (int)g.w.experts, g.slots, a.mt, blockIdx.y);
+template <int FR, int MT, int MODE, int FW>
+__global__ __launch_bounds__(
+    64 * FW, MODE == GIVEN ? 1 : (MODE == GLU32 ? 2 : (MT == 2 ? 3 : 4))) void packed_few_kernel(FewArgs a) {
+  constexpr bool RAW = MODE != GIVEN;
+  constexpr int MF = RAW ? 1 : MT / 16;
+  constexpr int XW = RAW ? 4096 : 0;         // bytes of transformed rows of a wave
+  constexpr int RED = FW * FR * MF * 1024;   // the partial sums
+  __shared__ __attribute__((aligned(16))) char lds[FW * XW > RED ? FW * XW : RED];
+  const GemmArgs& g = a.two.g[blockIdx.z];
+  const PkWork wk = find_work(g.offs, (int)g.w.experts, g.slots, MT, blockIdx.y);
   const int e = __builtin_amdgcn_readfirstlane(wk.e);
   if (e < 0) return;
   Tile tile;
@@ -259,30 +325,37 @@ __global__ __launch_bounds__(64 * FW) void packed_few_kernel(FewArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int64_t first = __builtin_amdgcn_readfirstlane((int)wk.first);  // slots < 2^31
   const int64_t left = __builtin_amdgcn_readfirstlane((int)wk.end) - first;
-  const int live = (int)(left < a.mt ? left : a.mt);
+  const int live = (int)(left < MT ? left : MT);
+  // what the epilogue needs of this thread's first output is on its way meanwhile
+  const hi2x_epilogue& E = g.epi;
+  int n = -1, t = 0;
+  float bias = 0.0f, mul = 1.0f, res = 0.0f;
+  auto operands = [&](int o) {
+    const int f = (o >> 8) / MF;
+    t = 16 * ((o >> 8) % MF) + ((o >> 4) & 15);
+    n = t < live && f < tile.count ? g.w.rows[(int64_t)(tile.frag + f) * 16 + (o & 15)] : -1;
+    if (n < 0) return;
+    if (E.bias) bias = load_as_f32(E.bias, n, E.dt_bias);
+    if (E.mul) mul = load_as_f32(E.mul, (first + t) * E.ld_mul + n, E.dt_mul);
+    if (E.residual) res = load_as_f32(E.residual, (first + t) * E.ld_residual + n, E.dt_residual);
+  };
+  if (tid < 256 * FR * MF) operands(tid);
   f32x4v acc[FR][MF];
 #pragma unroll
   for (int f = 0; f < FR; ++f)
 #pragma unroll
     for (int m = 0; m < MF; ++m) acc[f][m] = f32x4v{0.0f, 0.0f, 0.0f, 0.0f};
-  const int nch = (int)(g.w.kp / PK_CHUNK);
-  char* xl = lds + (size_t)w * ((nch + FW - 1) / FW) * a.mt * a.npl * 256;
-#define HI2X_FEW(BITS)                                                                     \
-  if (tile.sg.block == 16)                                                                 \
-    few_loop<BITS, true, FR, MF, FUSED>(a, tile, e, first, live, xl, mx[w], unscale[w], acc); \
-  else                                                                                     \
-    few_loop<BITS, false, FR, MF, FUSED>(a, tile, e, first, live, xl, mx[w], unscale[w], acc);
-  switch (tile.sg.nbits) {
+  char* xl = lds + w * XW;
+  switch (tile.nbits) {
     case 2:
-      HI2X_FEW(2)
+      few_loop<2, FR, MT, MODE, FW>(a, g, tile, e, first, live, xl, acc);
       break;
     case 4:
-      HI2X_FEW(4)
+      few_loop<4, FR, MT, MODE, FW>(a, g, tile, e, first, live, xl, acc);
       break;
     default:
-      HI2X_FEW(8)
+      few_loop<8, FR, MT, MODE, FW>(a, g, tile, e, first, live, xl, acc);
   }
-#undef HI2X_FEW
   // the waves' partial sums: [fragment][row of activations][slot]
   float* red = reinterpret_cast<float*>(lds);
   __syncthreads();
@@ -294,112 +367,88 @@ __global__ __launch_bounds__(64 * FW) void packed_few_kernel(FewArgs a) {
                                  4 * (lane >> 4)) = acc[f][m];
   __syncthreads();
   for (int o = tid; o < 256 * FR * MF; o += 64 * FW) {
-    const int slot = o & 15, row = (o >> 4) & 15, m = (o >> 8) % MF, f = (o >> 8) / MF;
-    const int t = 16 * m + row;
-    if (t >= live || f >= tile.count) continue;
-    const int n = g.w.rows[(int64_t)(tile.sg.frag0 + tile.first + f) * 16 + slot];
+    if (o != tid) operands(o);
     if (n < 0) continue;
     float y = 0.0f;
 #pragma unroll
     for (int v = 0; v < FW; ++v) {
-      const float* p = red + ((v * FR + f) * MF + m) * 256 + slot;
-      y += p[row * 16];
-      if (FUSED && a.npl == 2) y += p[(row + 8) * 16];
+      const float* p = red + v * (FR * MF * 256) + o;
+      y += p[0];
+      if (RAW && a.x.npl == 2) y += p[128];  // the second plane's, 8 rows on
     }
     const int64_t at = first + t;
-    if (!FUSED) {
+    if (!RAW) {
       const int64_t r = g.src ? g.src[at] : at;
       y *= r >= 0 && r < g.x.rows ? g.x.scale[r] : __builtin_nanf("");
     }
-    const float bias = g.epi.bias ? load_as_f32(g.epi.bias, n, g.epi.dt_bias) : 0.0f;
-    finish(g.epi, y, bias, at, n);
+    y = activate(y + bias, E.act);
+    if (E.mul) y = y * mul;
+    if (E.residual) y = y + res;
+    store_from_f32(E.out, at * E.ld_out + n, E.dt_out, y);
   }
 }
 
-template <int FR, int MF, bool FUSED>
-int launch(const FewArgs& a, hipStream_t s) {
-  const hi2x_packed& w = a.g.w;
-  const int64_t nch = w.kp / PK_CHUNK;
-  const size_t x = FUSED ? (size_t)FW * ((nch + FW - 1) / FW) * a.mt * a.npl * 256 : 0;
-  const size_t red = (size_t)FW * FR * MF * 1024;
-  const size_t dyn = x > red ? x : red;
+template <int FR, int MT, int MODE, int FW>
+int launch(const FewArgs& a, int count, hipStream_t s) {
+  const GemmArgs& g = a.two.g[0];
+  const hi2x_packed& w = g.w;
   // a segment's last tile may be partly filled
-  const int64_t nx = FR == 1 ? w.max_frags : w.max_frags / FR + PK_SEGS;
-  const int64_t part = a.g.offs ? (w.experts < a.g.slots ? w.experts : a.g.slots) : 1;
-  const int64_t ny = a.g.offs ? a.g.slots / a.mt + part : (a.g.slots + a.mt - 1) / a.mt;
+  int64_t nx = w.max_frags;
+  if (count > 1 && a.two.g[1].w.max_frags > nx) nx = a.two.g[1].w.max_frags;
+  if (FR > 1) nx = nx / FR + PK_SEGS;
+  const int64_t part = g.offs ? (w.experts < g.slots ? w.experts : g.slots) : 1;
+  const int64_t ny = g.offs ? g.slots / MT + part : (g.slots + MT - 1) / MT;
   HI2X_REQUIRE(nx < (1ll << 31) && ny <= 65535, "packed_linear: %lld rows are too many",
-               (long long)a.g.slots);
-  if (dyn > 32768)
-    HI2X_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(packed_few_kernel<FR, MF, FUSED>),
-                                 hipFuncAttributeMaxDynamicSharedMemorySize, (int)dyn));
-  packed_few_kernel<FR, MF, FUSED><<<dim3((unsigned)nx, (unsigned)ny), 64 * FW, dyn, s>>>(a);
+               (long long)g.slots);
+  packed_few_kernel<FR, MT, MODE, FW>
+      <<<dim3((unsigned)nx, (unsigned)ny, (unsigned)count), 64 * FW, 0, s>>>(a);
   return launch_status("packed_linear");
 }
 
 }  // namespace
 
-// Activation rows a workgroup can transform for itself: their planes in 64 KB of LDS (two
-// workgroups a CU), both planes' rows in one MFMA operand of 16.
-int64_t few_rows(int64_t k, int npl) {
-  const int64_t nch = (k + PK_CHUNK - 1) / PK_CHUNK;
-  const int64_t row = (nch + FW - 1) / FW * FW * 256 * npl;
-  const int64_t fit = 65536 / row;
-  return fit < 16 / npl ? fit : 16 / npl;
+int packed_few(const GemmPair& g, int count, hipStream_t s) {
+  FewArgs a{};
+  a.two = g;
+  const int64_t frags = g.g[0].w.max_frags;
+  return frags >= 1024 ? launch<4, 16, GIVEN, 8>(a, count, s)
+                       : (frags >= 512 ? launch<2, 16, GIVEN, 8>(a, count, s)
+                                       : launch<1, 16, GIVEN, 8>(a, count, s));
 }
 
-int packed_few(const GemmArgs& g, hipStream_t s) {
+int packed_few_raw(const GemmPair& g, int count, const RawRows& x, hipStream_t s) {
   FewArgs a{};
-  a.g = g;
-  a.npl = g.x.nplanes;
-  if (g.slots <= 16 || (g.offs && g.slots <= 16 * g.w.experts)) {
-    a.mt = 16;
-    return g.w.max_frags >= 1024 ? launch<4, 1, false>(a, s)
-                                 : (g.w.max_frags >= 512 ? launch<2, 1, false>(a, s)
-                                                         : launch<1, 1, false>(a, s));
+  a.two = g;
+  a.x = x;
+  const GemmArgs& g0 = g.g[0];
+  // Of experts most have one row in a decode step; a second tile reads the weights again.
+  const int rows = g0.offs ? (g0.slots <= 16 ? 1 : 2) : (int)g0.slots;
+  // Eight waves a workgroup shorten the walk along the columns; four of them transform the
+  // rows with half the instructions, which counts where workgroups share a CU: 4096 x 14336,
+  // one row, 16.8 against 18.2 us, 14336 x 4096 16.7 against 14.1.
+  const int64_t frags = g0.w.max_frags * count *
+                        (g0.offs ? (g0.slots < g0.w.experts ? g0.slots : g0.w.experts) : 1);
+  const bool wide = frags < 512;
+#define HI2X_RAW(MT)                                                                         \
+  if (x.dtype == 0)                                                                          \
+    return wide ? launch<1, MT, RAW32, 8>(a, count, s) : launch<1, MT, RAW32, 4>(a, count, s); \
+  return wide ? launch<1, MT, RAW16, 8>(a, count, s) : launch<1, MT, RAW16, 4>(a, count, s);
+  if (x.x2)  // (experts' only)
+    return rows <= 1 ? (wide ? launch<1, 1, GLU32, 8>(a, count, s)
+                             : launch<1, 1, GLU32, 4>(a, count, s))
+                     : (wide ? launch<1, 2, GLU32, 8>(a, count, s)
+                             : launch<1, 2, GLU32, 4>(a, count, s));
+  if (rows <= 1) {
+    HI2X_RAW(1)
   }
-  if (g.slots <= 32) {
-    a.mt = 32;
-    return g.w.max_frags >= 512 ? launch<2, 2, false>(a, s) : launch<1, 2, false>(a, s);
+  if (rows <= 2) {
+    HI2X_RAW(2)
   }
-  a.mt = 64;
-  return g.w.max_frags >= 512 ? launch<2, 4, false>(a, s) : launch<1, 4, false>(a, s);
+  if (rows <= 4) {
+    HI2X_RAW(4)
+  }
+  HI2X_RAW(8)
+#undef HI2X_RAW
 }
 
 }  // namespace hi2x
-
-using namespace hi2x;
-
-extern "C" int64_t hi2x_packed_few_rows(int64_t k, int nplanes) {
-  if (k < 16 || k % 16 || nplanes < 1 || nplanes > 2) return -1;
-  return few_rows(k, nplanes);
-}
-
-extern "C" int hi2x_packed_linear_few(const hi2x_packed* w, const void* x, int dtype, int64_t ldx,
-                                      int64_t x_rows, int nplanes, const uint8_t* had,
-                                      const uint16_t* col_scale, int per_expert,
-                                      const int64_t* src, const int64_t* offs, int64_t slots,
-                                      const hi2x_epilogue* epi, void* stream) {
-  clear_error();
-  HI2X_REQUIRE(w && epi, "packed_linear_few: null argument");
-  if (int rc = check_packed(w, "packed_linear_few")) return rc;
-  if (int rc = check_product(w, src, offs, slots, x_rows, epi, "packed_linear_few")) return rc;
-  if (int rc = check_x(x, dtype, ldx, x_rows, w->k, "packed_linear_few")) return rc;
-  HI2X_REQUIRE(nplanes == 1 || nplanes == 2, "packed_linear_few: %d planes", nplanes);
-  const int64_t mt = few_rows(w->k, nplanes);
-  HI2X_REQUIRE(mt >= 1, "packed_linear_few: %lld columns do not fit", (long long)w->k);
-  if (slots == 0) return HI2X_OK;
-  HI2X_REQUIRE(had, "packed_linear_few: null flags");
-  FewArgs a{};
-  a.g = GemmArgs{*w, hi2x_activations{}, src, offs, slots, *epi};
-  a.x = x;
-  a.dtype = dtype;
-  a.ldx = ldx;
-  a.x_rows = x_rows;
-  a.had = had;
-  a.cs = col_scale;
-  a.per_expert = per_expert;
-  a.npl = nplanes;
-  a.mt = (int)mt;
-  const hipStream_t s = as_stream(stream);
-  return w->max_frags >= 1024 ? launch<2, 1, true>(a, s) : launch<1, 1, true>(a, s);
-}

@@ -21,39 +21,6 @@ constexpr int RG = 64;      // most groups
 constexpr int SCAN_OVER = 512;  // workgroups from which the counts get a scan of their own
 
 template <int CTRL>
-__device__ __forceinline__ int dpp(int x) {
-  return __builtin_amdgcn_update_dpp(x, x, CTRL, 0xf, 0xf, false);
-}
-// Reductions over each row of 16 lanes: neighbours, pairs, halves mirrored, row mirrored.
-#define HI2X_ROW16(x, OP)   \
-  x = OP(x, dpp<0xB1>(x));  \
-  x = OP(x, dpp<0x4E>(x));  \
-  x = OP(x, dpp<0x141>(x)); \
-  x = OP(x, dpp<0x140>(x));
-
-__device__ __forceinline__ int umax_(int a, int b) {
-  return (int)((uint32_t)a > (uint32_t)b ? (uint32_t)a : (uint32_t)b);
-}
-__device__ __forceinline__ int umin_(int a, int b) {
-  return (int)((uint32_t)a < (uint32_t)b ? (uint32_t)a : (uint32_t)b);
-}
-__device__ __forceinline__ int or_(int a, int b) { return a | b; }
-__device__ __forceinline__ uint32_t row_umax(uint32_t v) {
-  int x = (int)v;
-  HI2X_ROW16(x, umax_)
-  return (uint32_t)x;
-}
-__device__ __forceinline__ uint32_t row_umin(uint32_t v) {
-  int x = (int)v;
-  HI2X_ROW16(x, umin_)
-  return (uint32_t)x;
-}
-__device__ __forceinline__ uint32_t row_or(uint32_t v) {
-  int x = (int)v;
-  HI2X_ROW16(x, or_)
-  return (uint32_t)x;
-}
-template <int CTRL>
 __device__ __forceinline__ double dpp_d(double v) {
   const long long b = __builtin_bit_cast(long long, v);
   const uint32_t lo = (uint32_t)dpp<CTRL>((int)b), hi = (uint32_t)dpp<CTRL>((int)(b >> 32));
@@ -489,6 +456,36 @@ __global__ void zero_i64_kernel(int64_t* p, int64_t n) {
 }
 
 }  // namespace
+
+int launch_combine(const void* y, int dt_y, int64_t y_rows, int64_t n, const int64_t* slots,
+                   const float* weights, int64_t t, int64_t top_k, const void* residual,
+                   int dt_residual, void* out, int dt_out, hipStream_t s) {
+  const bool vec = n % 4 == 0 && (uintptr_t)y % 16 == 0;
+  const int64_t cols = (n + (vec ? 1023 : 255)) / (vec ? 1024 : 256);
+  const dim3 grid((unsigned)t, (unsigned)(cols < 64 ? cols : 64));
+#define HI2X_COMBINE(DT, V)                                                                  \
+  combine_kernel<DT, V><<<grid, 256, 0, s>>>(y, y_rows, n, slots, weights, (int)top_k,       \
+                                             residual, dt_residual, out, dt_out)
+  if (dt_y == 0) {
+    if (vec)
+      HI2X_COMBINE(0, 4);
+    else
+      HI2X_COMBINE(0, 1);
+  } else if (dt_y == 1) {
+    if (vec)
+      HI2X_COMBINE(1, 4);
+    else
+      HI2X_COMBINE(1, 1);
+  } else {
+    if (vec)
+      HI2X_COMBINE(2, 4);
+    else
+      HI2X_COMBINE(2, 1);
+  }
+#undef HI2X_COMBINE
+  return launch_status("moe_combine");
+}
+
 }  // namespace hi2x
 
 using namespace hi2x;
@@ -598,29 +595,6 @@ extern "C" int hi2x_moe_combine(const void* y, int dt_y, int64_t y_rows, int64_t
                "moe_combine: bad shape");
   if (t == 0) return HI2X_OK;
   HI2X_REQUIRE((y || y_rows == 0) && slots && weights && out, "moe_combine: null buffer");
-  const hipStream_t s = as_stream(stream);
-  const bool vec = n % 4 == 0 && (uintptr_t)y % 16 == 0;
-  const int64_t cols = (n + (vec ? 1023 : 255)) / (vec ? 1024 : 256);
-  const dim3 grid((unsigned)t, (unsigned)(cols < 64 ? cols : 64));
-#define HI2X_COMBINE(DT, V)                                                                  \
-  combine_kernel<DT, V><<<grid, 256, 0, s>>>(y, y_rows, n, slots, weights, (int)top_k,       \
-                                             residual, dt_residual, out, dt_out)
-  if (dt_y == 0) {
-    if (vec)
-      HI2X_COMBINE(0, 4);
-    else
-      HI2X_COMBINE(0, 1);
-  } else if (dt_y == 1) {
-    if (vec)
-      HI2X_COMBINE(1, 4);
-    else
-      HI2X_COMBINE(1, 1);
-  } else {
-    if (vec)
-      HI2X_COMBINE(2, 4);
-    else
-      HI2X_COMBINE(2, 1);
-  }
-#undef HI2X_COMBINE
-  return launch_status("moe_combine");
+  return launch_combine(y, dt_y, y_rows, n, slots, weights, t, top_k, residual, dt_residual, out,
+                        dt_out, as_stream(stream));
 }

@@ -127,11 +127,6 @@ class _Packed:
         self._params = torch.empty(params_at, dtype=torch.uint8, device=dev)
         self._rows = _lib.h2d(torch.from_numpy(np.concatenate(slot_rows)), dev)
         self._segments = _lib.h2d(torch.from_numpy(segs.reshape(-1).view(np.uint8)), dev)
-        self._few = [int(_lib.lib().hi2x_packed_few_rows(k, p)) for p in (1, 2)]
-        self.desc = _lib.Packed(self._codes.data_ptr(), self._params.data_ptr(),
-                                self._rows.data_ptr(), self._segments.data_ptr(), e, n, k, kp,
-                                frag, most, (ctypes.c_int64 * 3)(*(int(v) for v in tiles)))
-
         def flat(parts, dtype):
             parts = [_lib.to_device(p.reshape(-1), dev, dtype) for p in parts]
             return (parts[0] if len(parts) == 1 else torch.cat(parts)).contiguous()
@@ -147,8 +142,6 @@ class _Packed:
             np.concatenate([t.param_off.cpu().numpy()[:-1].astype(np.int64) + a
                             for t, a in zip(tensors, po)])])
         offs = _lib.h2d(torch.from_numpy(offs), dev)
-        _lib.call("hi2x_packed_layout", dev, ctypes.byref(self.desc), _lib.ptr(words),
-                  _lib.ptr(offs[0]), _lib.ptr(bytes_), _lib.ptr(offs[1]), _lib.ptr(consts))
         # the transform: one for all where every expert has the same
         had = [t.had.reshape(-1).cpu().to(torch.uint8).numpy() for t in tensors]
         cs = [None if t.col_scale is None else
@@ -165,6 +158,16 @@ class _Packed:
         self._had = _lib.h2d(torch.from_numpy(np.stack(had[:own])), dev)
         self._scale = None if cs[0] is None else \
             _lib.h2d(torch.from_numpy(np.stack(cs[:own])), dev)
+        first = (_lib.Segment * len(CLASSES)).from_buffer_copy(segs[0].tobytes())
+        #: hi2x_packed: the layout, the tables and the transform
+        self.desc = _lib.Packed(
+            self._codes.data_ptr(), self._params.data_ptr(), self._rows.data_ptr(),
+            self._segments.data_ptr(), e, n, k, kp, frag, most,
+            (ctypes.c_int64 * 3)(*(int(v) for v in tiles)), self._had.data_ptr(),
+            None if self._scale is None else self._scale.data_ptr(), int(self.transform is None), first)
+        self._ref = ctypes.byref(self.desc)
+        _lib.call("hi2x_packed_layout", dev, self._ref, _lib.ptr(words),
+                  _lib.ptr(offs[0]), _lib.ptr(bytes_), _lib.ptr(offs[1]), _lib.ptr(consts))
 
     @property
     def nbytes(self) -> int:
@@ -190,7 +193,7 @@ class Activations:
     """Transformed activations (:func:`activations`): usable with every tensor whose
     transform is ``transform``."""
 
-    planes: torch.Tensor  # float16 [nplanes, rows, kp]
+    planes: torch.Tensor  # float16 [rows, kp / 128, nplanes, 128]
     scale: torch.Tensor  # float32 [rows]
     k: int
     dtype: torch.dtype  # of the activations they were made from
@@ -239,23 +242,6 @@ def _aligned(x: torch.Tensor) -> torch.Tensor:
     return x.clone() if x.data_ptr() % 16 else x
 
 
-def _transformed(x: torch.Tensor, w: _Packed, src=None, offs=None, rows=None, npl=None
-                 ) -> Activations:
-    dev = w.device
-    dt = _dtype(x, "x")
-    x = _rows_of(x, w.k, "x")
-    rows = x.shape[0] if rows is None else rows
-    x = _aligned(x)
-    npl = npl or _planes(x.dtype, w)
-    planes = torch.empty(npl, rows, w.kp, dtype=torch.float16, device=dev)
-    scale = torch.empty(rows, dtype=torch.float32, device=dev)
-    desc = _lib.ActivationsDesc(planes.data_ptr(), scale.data_ptr(), rows, w.kp, npl, 0)
-    _lib.call("hi2x_packed_activations", dev, _lib.ptr(x), dt, _pitch(x), x.shape[0], w.k,
-              _lib.ptr(src), _lib.ptr(w._had), _lib.ptr(w._scale), _lib.ptr(offs),
-              w.experts, ctypes.byref(desc))
-    return Activations(planes, scale, w.k, x.dtype, w.transform, desc)
-
-
 def activations(x: torch.Tensor, w: PackedLinear | PackedExperts) -> Activations:
     """``T(x)`` for ``w`` and every tensor with the same transform, to be handed to
     :func:`packed_linear` or :func:`experts_linear` in the place of ``x [..., K]``.  The
@@ -265,70 +251,63 @@ def activations(x: torch.Tensor, w: PackedLinear | PackedExperts) -> Activations
     _no_grad_inputs("activations", x)
     if w.transform is None:
         raise ValueError("the experts have transforms of their own: give experts_linear x itself")
-    return _transformed(x, w)
+    dt = _dtype(x, "x")
+    x = _aligned(_rows_of(x, w.k, "x"))
+    rows, npl = x.shape[0], _planes(x.dtype, w)
+    planes = torch.empty(rows, w.kp // CHUNK, npl, CHUNK, dtype=torch.float16, device=w.device)
+    scale = torch.empty(rows, dtype=torch.float32, device=w.device)
+    desc = _lib.ActivationsDesc(planes.data_ptr(), scale.data_ptr(), rows, w.kp, npl, 0)
+    _lib.call("hi2x_packed_activations", w.device, w._ref, _lib.ptr(x), dt, _pitch(x), rows, None,
+              None, ctypes.byref(desc))
+    return Activations(planes, scale, w.k, x.dtype, w.transform, desc)
 
 
-def _epilogue(w, slots, bias, activation, mul, residual, out, what):
-    if activation not in ACTIVATIONS:
-        raise ValueError(f"activation {activation!r} ({', '.join(ACTIVATIONS)})")
-    e = _lib.Epilogue()
-    e.act = ACTIVATIONS[activation]
-    keep = []
-    if bias is not None:
-        if bias.numel() != w.n:
-            raise ValueError(f"bias has {bias.numel()} entries, expected {w.n}")
-        bias = bias.reshape(-1).contiguous()
-        e.bias, e.dt_bias = bias.data_ptr(), _dtype(bias, "bias")
-        keep.append(bias)
-    for name, t in (("mul", mul), ("residual", residual)):
-        if t is None:
-            continue
-        if t.numel() != slots * w.n:
-            raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {slots} rows of {w.n}")
-        dt = _dtype(t, name)
-        t = _rows_of(t, w.n, name)
-        keep.append(t)
-        setattr(e, name, t.data_ptr())
-        setattr(e, "ld_" + name, _pitch(t))
-        setattr(e, "dt_" + name, dt)
-    e.out, e.ld_out, e.dt_out = out.data_ptr(), w.n, _dtype(out, "out_dtype")
-    return e, keep
+def _operand(t, slots, n, name):
+    """(tensor, address, pitch, dtype) of a factor or residual."""
+    if t is None:
+        return None, None, 0, 0
+    if t.numel() != slots * n:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {slots} rows of {n}")
+    dt = _dtype(t, name)
+    t = _rows_of(t, n, name)
+    return t, t.data_ptr(), _pitch(t), dt
 
 
-def _few(x, w, npl, slots, offs):
-    """Whether a product takes its activations as they are and transforms them inside: the
-    rows fit one workgroup tile (of each expert on average at most two)."""
-    fit = w._few[npl - 1]
-    return fit >= 1 and (slots <= fit if offs is None else slots <= min(2, fit) * w.experts)
-
-
-def _product(w, x, src, offs, slots, bias, activation, mul, residual, out_dtype, what, npl=None):
-    dev = w.device
-    if _lib.require_gpu(x if isinstance(x, torch.Tensor) else x.planes, bias, mul,
-                        residual, src, offs) != dev:
+def _product(w, x, src, offs, slots, bias, activation, mul, residual, out_dtype, what):
+    dev, n = w.device, w.n
+    given = not isinstance(x, torch.Tensor)
+    if _lib.require_gpu(x.planes if given else x, bias, mul, residual, src, offs) != dev:
         raise RuntimeError(f"{what}: inputs are not on the weights' device {dev}")
-    out = torch.empty(slots, w.n, dtype=out_dtype, device=dev)
-    epi, keep = _epilogue(w, slots, bias, activation, mul, residual, out, what)
+    act = ACTIVATIONS.get(activation)
+    if act is None:
+        raise ValueError(f"activation {activation!r} ({', '.join(ACTIVATIONS)})")
+    if bias is not None:
+        if bias.numel() != n:
+            raise ValueError(f"bias has {bias.numel()} entries, expected {n}")
+        bias = bias.reshape(-1).contiguous()
+    mul, mul_p, mul_ld, mul_dt = _operand(mul, slots, n, "mul")
+    residual, res_p, res_ld, res_dt = _operand(residual, slots, n, "residual")
+    out_dt = _dtype(out_dtype, "out_dtype")
+    dt = 0 if given else _dtype(x, "x")
+    out = torch.empty(slots, n, dtype=out_dtype, device=dev)
     if not slots:
         return out
-    if isinstance(x, torch.Tensor):
-        dt = _dtype(x, "x")
-        npl = npl or _planes(x.dtype, w)
-        if _few(x, w, npl, slots, offs):
-            x = _aligned(_rows_of(x, w.k, "x"))
-            _lib.call("hi2x_packed_linear_few", dev, ctypes.byref(w.desc), _lib.ptr(x), dt,
-                      _pitch(x), x.shape[0], npl, _lib.ptr(w._had), _lib.ptr(w._scale),
-                      int(w.transform is None), _lib.ptr(src), _lib.ptr(offs), slots,
-                      ctypes.byref(epi))
-            return out
-        if w.transform is not None:
-            act = _transformed(x, w, npl=npl)
-        else:  # every slot through its own expert's transform
-            act, src = _transformed(x, w, src=src, offs=offs, rows=slots, npl=npl), None
+    epi = _lib.Epilogue(None if bias is None else bias.data_ptr(), mul_p, res_p, out.data_ptr(),
+                        mul_ld, res_ld, n, 0 if bias is None else _dtype(bias, "bias"), mul_dt,
+                        res_dt, out_dt, act, 0)
+    if not given:
+        x = _aligned(x)
+    npl = x.desc.nplanes if given else _planes(x.dtype, w)
+    rows = x.scale.numel() if given else x.shape[0]
+    size = _lib.lib().hi2x_packed_workspace_bytes(
+        w._ref, rows, npl, given, slots, src is not None, offs is not None)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size > 0 else None
+    if given:
+        _lib.call("hi2x_packed_linear_activations", dev, w._ref, ctypes.byref(x.desc),
+                  _lib.ptr(src), _lib.ptr(offs), slots, ctypes.byref(epi), _lib.ptr(ws), size)
     else:
-        act = x
-    _lib.call("hi2x_packed_linear", dev, ctypes.byref(w.desc), ctypes.byref(act.desc),
-              _lib.ptr(src), _lib.ptr(offs), slots, ctypes.byref(epi))
+        _lib.call("hi2x_packed_linear", dev, w._ref, _lib.ptr(x), dt, _pitch(x), rows, npl,
+                  _lib.ptr(src), _lib.ptr(offs), slots, ctypes.byref(epi), _lib.ptr(ws), size)
     return out
 
 
@@ -374,7 +353,7 @@ def _routed(offs, rows, w, what):
 
 def experts_linear(x: torch.Tensor | Activations, w: PackedExperts, offs: torch.Tensor,
                    rows: torch.Tensor | None = None, activation: str = "none", mul=None,
-                   residual=None, out_dtype=None, *, _npl=None) -> torch.Tensor:
+                   residual=None, out_dtype=None) -> torch.Tensor:
     """``[S, N]``: row j is expert e's product for the routed slot j of its range
     ``offs[e]:offs[e + 1]``, which reads row ``rows[j]`` of ``x`` (row j itself without
     ``rows``), with the epilogue of :func:`packed_linear`.  ``offs`` (device int64, E + 1
@@ -394,7 +373,7 @@ def experts_linear(x: torch.Tensor | Activations, w: PackedExperts, offs: torch.
         x = _rows_of(x, w.k, "x")
     slots = rows.numel() if rows is not None else (x.scale.numel() if given else x.shape[0])
     return _product(w, x, rows, offs, slots, None, activation, mul, residual,
-                    out_dtype or x.dtype, "experts_linear", _npl)
+                    out_dtype or x.dtype, "experts_linear")
 
 
 def combine(y: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor, residual=None,
@@ -443,20 +422,37 @@ def moe_mlp(x: torch.Tensor, routing, gate: PackedExperts, up: PackedExperts,
     if _lib.require_gpu(x) != gate.device:
         raise RuntimeError(f"x is on {x.device}, the experts on {gate.device}")
     _no_grad_inputs("moe_mlp", x, routing.weights, residual)
-    flat = _rows_of(x, gate.k, "x")
-    if routing.index.shape[0] != flat.shape[0]:
-        raise ValueError(f"routing of {routing.index.shape[0]} tokens for {flat.shape[0]}")
+    act = ACTIVATIONS.get(activation)
+    if act is None:
+        raise ValueError(f"activation {activation!r} ({', '.join(ACTIVATIONS)})")
+    flat = _aligned(_rows_of(x, gate.k, "x"))
+    t = flat.shape[0]
+    index, weights, slots = routing.index, routing.weights, routing.slots
+    if index.shape[0] != t:
+        raise ValueError(f"routing of {index.shape[0]} tokens for {t}")
+    if routing.offs.numel() != gate.experts + 1:
+        raise ValueError(f"routing over {routing.offs.numel() - 1} experts for {gate.experts}")
+    if residual is not None:
+        if residual.numel() != t * gate.k:
+            raise ValueError(f"residual has shape {tuple(residual.shape)}, expected {(t, gate.k)}")
+        residual = residual.contiguous()
+    if _lib.require_gpu(flat, weights, residual) != gate.device:
+        raise RuntimeError(f"moe_mlp: inputs are not on the experts' device {gate.device}")
+    dt = _dtype(x, "x")
+    out = torch.empty(x.shape, dtype=x.dtype, device=gate.device)
+    if not t:
+        return out
+    # one fp16 plane of the hidden values is well below a bf16 result's own rounding, and half
+    # the products; next to an fp16 result it would show
+    npl, mid = _planes(x.dtype, gate), 1 if x.dtype == torch.bfloat16 else 2
+    top_k = index.shape[1]
     shared = gate.transform is not None and gate.transform == up.transform
-    offs, rows = routing.offs, routing.rows
-    few = _few(flat, gate, _planes(x.dtype, gate), rows.numel(), offs)
-    inp = activations(flat, gate) if shared and not few else flat
-    g = experts_linear(inp, gate, offs, rows, activation=activation, out_dtype=torch.float32)
-    h = experts_linear(inp, up, offs, rows, mul=g, out_dtype=torch.float32)
-    del g
-    # one fp16 plane of the hidden values is well below a bf16 result's own rounding, and
-    # half the products; next to an fp16 result it would show
-    y = experts_linear(h, down, offs, out_dtype=torch.float32,
-                       _npl=1 if x.dtype == torch.bfloat16 else 2)
-    res = None if residual is None else residual.reshape(flat.shape)
-    out = combine(y, routing.slots, routing.weights, residual=res, out_dtype=x.dtype)
-    return out.reshape(x.shape)
+    size = _lib.lib().hi2x_moe_mlp_workspace_bytes(gate._ref, up._ref, down._ref, t, top_k, npl,
+                                                   mid, shared)
+    ws = torch.empty(max(size, 1), dtype=torch.uint8, device=gate.device)
+    _lib.call("hi2x_moe_mlp", gate.device, gate._ref, up._ref, down._ref, _lib.ptr(flat), dt,
+              _pitch(flat), t, top_k, npl, mid, shared, act, _lib.ptr(routing.rows),
+              _lib.ptr(routing.offs), _lib.ptr(slots), _lib.ptr(weights), _lib.ptr(residual),
+              0 if residual is None else _dtype(residual, "residual"), _lib.ptr(out), dt,
+              _lib.ptr(ws), size)
+    return out

@@ -546,6 +546,10 @@ typedef struct {
   int64_t frags;                       /* fragments of all experts */
   int64_t max_frags;                   /* most fragments of one expert */
   int64_t max_tiles[3];                /* most tiles of one expert, of 4, 8 and 16 fragments */
+  const uint8_t* had;                  /* [k / 16] rotation flags of the 16-column groups */
+  const uint16_t* col_scale;           /* [k] fp16 smoothing, or NULL */
+  int64_t per_expert;                  /* had and col_scale hold one row per expert */
+  hi2x_packed_segment first[HI2X_PACKED_SEGMENTS]; /* expert 0's segments (host copy) */
 } hi2x_packed;
 
 /* Fills w->codes and w->params.  codes i32 words, blk_params u8 pairs, row_consts fp16
@@ -559,7 +563,7 @@ int hi2x_packed_layout(const hi2x_packed* w, const int32_t* codes, const int64_t
  * two that puts its values in fp16's range, and that factor's inverse in scale.  With
  * nplanes 2 a second plane holds what the first one's rounding left (together 22 bits). */
 typedef struct {
-  uint16_t* planes; /* [nplanes][rows][kp] fp16, 256-byte aligned, columns from k on zero */
+  uint16_t* planes; /* fp16 [rows][kp / 128][nplanes][128], 256-byte aligned; zero from k on */
   float* scale;     /* [rows] */
   int64_t rows;
   int64_t kp;
@@ -567,17 +571,14 @@ typedef struct {
   int32_t pad_;
 } hi2x_activations;
 
-/* T(x) = H16(x / col_scale) on the flagged 16-column groups, x / col_scale elsewhere.
- * x [.., k] f32 (dtype 0), fp16 (1) or bf16 (2), rows ldx elements apart, each at a
- * multiple of 16 bytes; row i of the
- * result is row src[i] of x (src NULL: row i; an index outside [0, x_rows): a row of NaN).
- * had [k / 16] u8 and col_scale [k] fp16 or NULL.  With offs (experts + 1 row ranges on
- * the device) row i belongs to the expert whose range holds it and uses that expert's
- * had [experts][k / 16] and col_scale [experts][k]. */
-int hi2x_packed_activations(const void* x, int dtype, int64_t ldx, int64_t x_rows, int64_t k,
-                            const int64_t* src, const uint8_t* had, const uint16_t* col_scale,
-                            const int64_t* offs, int64_t experts, const hi2x_activations* out,
-                            void* stream);
+/* T(x) = H16(x / col_scale) on w's flagged 16-column groups, x / col_scale elsewhere.
+ * x [.., k] f32 (dtype 0), fp16 (1) or bf16 (2), rows ldx elements apart, each at a multiple
+ * of 16 bytes; row i of the result is row src[i] of x (src NULL: row i; an index outside
+ * [0, x_rows): a row of NaN).  Where w holds one transform per expert, offs (experts + 1 row
+ * ranges on the device) says whose row i is. */
+int hi2x_packed_activations(const hi2x_packed* w, const void* x, int dtype, int64_t ldx,
+                            int64_t x_rows, const int64_t* src, const int64_t* offs,
+                            const hi2x_activations* out, void* stream);
 
 #define HI2X_ACT_NONE 0
 #define HI2X_ACT_RELU 1
@@ -599,24 +600,27 @@ typedef struct {
   int32_t pad_;
 } hi2x_epilogue;
 
-/* out[slot] = epilogue(T(x)[src[slot]] Wq^T) for every slot (src NULL: the slot itself).
- * With several experts offs [experts + 1] gives each one's slot range and must cover all
- * slots; offs NULL: one expert. */
-int hi2x_packed_linear(const hi2x_packed* w, const hi2x_activations* x, const int64_t* src,
-                       const int64_t* offs, int64_t slots, const hi2x_epilogue* epi,
+/* out[slot] = epilogue(T(x)[src[slot]] Wq^T) for every slot (src NULL: the slot itself; an
+ * index outside [0, x_rows): a row of NaN).  With several experts offs [experts + 1] gives
+ * each one's slot range and must cover all slots; offs NULL: one expert.  x as for
+ * hi2x_packed_activations; nplanes 1 or 2: the planes its transform is held in.  Few rows
+ * are transformed inside the product, in one launch; others in a pass of their own.
+ * Workspace: hi2x_packed_workspace_bytes. */
+int hi2x_packed_linear(const hi2x_packed* w, const void* x, int dtype, int64_t ldx,
+                       int64_t x_rows, int nplanes, const int64_t* src, const int64_t* offs,
+                       int64_t slots, const hi2x_epilogue* epi, void* ws, int64_t ws_bytes,
                        void* stream);
 
-/* hi2x_packed_linear for few rows, with the transform of hi2x_packed_activations inside:
- * x, had, col_scale and src as there (per_expert: one transform per expert), nplanes 1 or
- * 2 the planes the transformed rows are held in.  One launch; meant for up to
- * hi2x_packed_few_rows(k, nplanes) rows (per expert: more are taken in several tiles, each
- * reading the weights again), which is 0 where k columns do not fit. */
-int hi2x_packed_linear_few(const hi2x_packed* w, const void* x, int dtype, int64_t ldx,
-                           int64_t x_rows, int nplanes, const uint8_t* had,
-                           const uint16_t* col_scale, int per_expert, const int64_t* src,
-                           const int64_t* offs, int64_t slots, const hi2x_epilogue* epi,
-                           void* stream);
-int64_t hi2x_packed_few_rows(int64_t k, int nplanes);
+/* The same from transformed activations (tensors that share their input). */
+int hi2x_packed_linear_activations(const hi2x_packed* w, const hi2x_activations* x,
+                                   const int64_t* src, const int64_t* offs, int64_t slots,
+                                   const hi2x_epilogue* epi, void* ws, int64_t ws_bytes,
+                                   void* stream);
+
+/* Workspace of a product of `slots` rows from x_rows rows in nplanes planes (given: of
+ * hi2x_packed_linear_activations; indexed: src is given; ranges: offs is given). */
+int64_t hi2x_packed_workspace_bytes(const hi2x_packed* w, int64_t x_rows, int nplanes, int given,
+                                    int64_t slots, int indexed, int ranges);
 
 /* ---- routing ------------------------------------------------------------------------------ */
 
@@ -649,6 +653,24 @@ int hi2x_route_backward(const void* logits, int dtype, int64_t ld, int64_t t, in
 int hi2x_moe_combine(const void* y, int dt_y, int64_t y_rows, int64_t n, const int64_t* slots,
                      const float* weights, int64_t t, int64_t top_k, const void* residual,
                      int dt_residual, void* out, int dt_out, void* stream);
+
+/* The gated MLP of experts over routed tokens, from one call:
+ *   out[t] = residual[t] + sum_j weights[t][j] y[slots[t][j]],
+ *   y = down(act(gate(x)) * up(x)) for every routed slot.
+ * x [t][h] as for hi2x_packed_activations; rows, offs, slots and weights as hi2x_route gives
+ * them for t tokens and top_k choices; residual (or NULL) and out [t][h] contiguous.  The
+ * experts' values in between are f32; nplanes and nplanes_mid are the planes of the tokens'
+ * and the hidden values' transforms, shared says that gate's and up's transforms are the
+ * same.  Workspace: hi2x_moe_mlp_workspace_bytes. */
+int hi2x_moe_mlp(const hi2x_packed* gate, const hi2x_packed* up, const hi2x_packed* down,
+                 const void* x, int dtype, int64_t ldx, int64_t t, int64_t top_k, int nplanes,
+                 int nplanes_mid, int shared, int act, const int64_t* rows, const int64_t* offs,
+                 const int64_t* slots, const float* weights, const void* residual,
+                 int dt_residual, void* out, int dt_out, void* ws, int64_t ws_bytes,
+                 void* stream);
+int64_t hi2x_moe_mlp_workspace_bytes(const hi2x_packed* gate, const hi2x_packed* up,
+                                     const hi2x_packed* down, int64_t t, int64_t top_k,
+                                     int nplanes, int nplanes_mid, int shared);
 
 /* ---- streams ---------------------------------------------------------------------------- */
 
