@@ -309,16 +309,17 @@ __device__ __forceinline__ void load16(const void* x, int64_t at, int dtype, flo
   }
 }
 
-// Whether a product goes to packed_few: its rows fit one operand (each expert's do on
-// average).  A wave of it walks an eighth of the columns alone: 4096 x 14336 at 16 rows took
-// 33 us so and 23 us in 64 x 64 tiles with the columns in eight shares, 4096 x 4096 13 and 14,
-// 14336 x 4096 16 and 20, 28672 x 8192 34 and 43.
+// Whether a product goes to packed_few: its rows fit one operand.  A wave of it walks an
+// eighth of the columns alone: 4096 x 14336 at 16 rows took 33 us so and 23 us in 64 x 64
+// tiles with the columns in eight shares, 4096 x 4096 13 and 14, 14336 x 4096 16 and 20,
+// 28672 x 8192 34 and 43.  Experts' rows take tiles: a layer of 64 experts at 64 tokens,
+// eight each, took 315 us so and 128 us in tiles.
 inline bool few_rows_product(const hi2x_packed& w, int64_t slots, bool ranges) {
-  if (ranges) return slots <= 16 * w.experts;
-  return slots <= 16 && (w.kp <= 8192 || w.max_frags >= 512);
+  return !ranges && slots <= 16 && (w.kp <= 8192 || w.max_frags >= 512);
 }
 
-constexpr int64_t FEW_RAW = 8;  // rows the few-rows kernel transforms for itself
+constexpr int64_t FEW_RAW = 8;      // rows the few-rows kernel transforms for itself,
+constexpr int64_t FEW_RANGES = 16;  // and of all experts together
 
 // Activations as they are: rows ldx elements apart; with x2 (same type and pitch, 32 bits)
 // act(x) * x2 elementwise.
@@ -346,10 +347,11 @@ int launch_combine(const void* y, int dt_y, int64_t y_rows, int64_t n, const int
                    const float* weights, int64_t t, int64_t top_k, const void* residual,
                    int dt_residual, void* out, int dt_out, hipStream_t s);
 
-// Whether a product takes its activations as they are and transforms them inside (of
-// experts: two rows each on average).
-inline bool few_raw_product(const hi2x_packed& w, int64_t slots, bool ranges) {
-  return ranges ? slots <= 2 * w.experts : slots <= FEW_RAW;
+// Whether a product takes its activations as they are and transforms them inside.  Of
+// experts most have one row then: at 64 experts and 8 choices, two tokens 62 us so and 74 in
+// tiles, four 84 and 75.
+inline bool few_raw_product(const hi2x_packed&, int64_t slots, bool ranges) {
+  return slots <= (ranges ? FEW_RANGES : FEW_RAW);
 }
 
 inline int64_t plane_bytes(const hi2x_packed& w, int64_t rows, int npl) {

@@ -83,7 +83,7 @@ __device__ __forceinline__ void group_values(const RawRows& x, int64_t base, int
   }
 }
 
-// A workgroup transforms one row.  The largest finite |x / s| comes first; the rotation can
+// TPR threads transform a row, 256 / TPR rows to a workgroup.  The largest finite |x / s| comes first; the rotation can
 // grow it fourfold at most, so 2^(13 - exponent) brings every value to at most 2^15, with
 // nothing of the row below fp16's normal range unless it is 2^-27 of the largest.  Then the
 // values are scaled (exact), rotated by butterflies in f32 and rounded to fp16.  That
@@ -91,17 +91,18 @@ __device__ __forceinline__ void group_values(const RawRows& x, int64_t base, int
 // large as fp16's; nplanes 2 keeps the rest of it in a second plane.  A thread keeps its
 // group's values between the two where one group a thread is all there is (KEEP, 4096
 // columns); rows beyond are read twice, the second time from L2.
-template <int DT, bool GLU, bool KEEP>
+template <int DT, bool GLU, bool KEEP, int TPR>
 __global__ __launch_bounds__(256) void activations_kernel(
     RawRows x, int64_t k, const int64_t* __restrict__ src, const uint8_t* __restrict__ had,
     const uint16_t* __restrict__ cs, const int64_t* __restrict__ offs, int experts,
     hi2x_activations out) {
-  const int64_t row = blockIdx.x;
-  const int tid = threadIdx.x;
-  const int64_t from = src ? src[row] : row;
+  const int64_t row = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+  const int tid = threadIdx.x % TPR;
+  const bool none = row >= out.rows;
+  const int64_t from = none ? -1 : (src ? src[row] : row);
   const bool bad = from < 0 || from >= x.rows;
   const int64_t base = bad ? 0 : from * x.ldx;
-  if (offs) {
+  if (offs && !none) {
     int lo = 0, hi = experts - 1;  // the expert whose range holds the row
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
@@ -118,7 +119,7 @@ __global__ __launch_bounds__(256) void activations_kernel(
 #pragma unroll
   for (int i = 0; i < 16; ++i) v[i] = 0.0f;
   if (!bad) {
-    for (int g = tid; g < groups; g += 256) {
+    for (int g = tid; g < groups; g += TPR) {
       group_values<DT, GLU>(x, base, g, cs, v);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
@@ -129,10 +130,14 @@ __global__ __launch_bounds__(256) void activations_kernel(
   }
 #pragma unroll
   for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
-  __shared__ float red[4];
-  if ((tid & 63) == 0) red[tid >> 6] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  if constexpr (TPR > 64) {
+    __shared__ float red[4];
+    const int w = threadIdx.x >> 6;
+    if ((tid & 63) == 0) red[w] = m;
+    __syncthreads();
+    m = TPR == 128 ? fmaxf(red[w & 2], red[w | 1]) : fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  }
+  if (none) return;
   int ex = 0;
   if (m > 0.0f) (void)frexpf(m, &ex);
   // the exponent stays where both 2^e and 2^-e are normal
@@ -140,7 +145,7 @@ __global__ __launch_bounds__(256) void activations_kernel(
   const float sc = ldexpf(1.0f, e);
   if (tid == 0) out.scale[row] = bad ? __builtin_nanf("") : ldexpf(1.0f, -e);
   uint16_t* dst = out.planes + row * out.kp * out.nplanes;
-  for (int g = tid; g < all; g += 256) {
+  for (int g = tid; g < all; g += TPR) {
     if (bad || g >= groups) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) v[i] = 0.0f;
@@ -186,14 +191,19 @@ __global__ __launch_bounds__(256) void activations_kernel(
 
 int launch_activations(const RawRows& x, const hi2x_packed& w, const int64_t* src,
                        const int64_t* offs, const hi2x_activations& out, hipStream_t s) {
-  const dim3 grid((unsigned)out.rows);
-#define HI2X_ROWS(DT, GLU)                                                                   \
-  if (w.kp <= 4096)                                                                          \
-    activations_kernel<DT, GLU, true><<<grid, 256, 0, s>>>(x, w.k, src, w.had, w.col_scale,  \
-                                                           offs, (int)w.experts, out);       \
-  else                                                                                       \
-    activations_kernel<DT, GLU, false><<<grid, 256, 0, s>>>(x, w.k, src, w.had, w.col_scale, \
-                                                            offs, (int)w.experts, out);
+#define HI2X_ROWS_(DT, GLU, KEEP, TPR)                                                    \
+  activations_kernel<DT, GLU, KEEP, TPR>                                                  \
+      <<<dim3((unsigned)((out.rows * TPR + 255) / 256)), 256, 0, s>>>(                    \
+          x, w.k, src, w.had, w.col_scale, offs, (int)w.experts, out)
+#define HI2X_ROWS(DT, GLU)                 \
+  if (w.kp <= 1024)                        \
+    HI2X_ROWS_(DT, GLU, true, 64);         \
+  else if (w.kp <= 2048)                   \
+    HI2X_ROWS_(DT, GLU, true, 128);        \
+  else if (w.kp <= 4096)                   \
+    HI2X_ROWS_(DT, GLU, true, 256);        \
+  else                                     \
+    HI2X_ROWS_(DT, GLU, false, 256);
   if (x.x2) {
     HI2X_ROWS(0, true)
   } else if (x.dtype == 0) {
@@ -204,6 +214,7 @@ int launch_activations(const RawRows& x, const hi2x_packed& w, const int64_t* sr
     HI2X_ROWS(2, false)
   }
 #undef HI2X_ROWS
+#undef HI2X_ROWS_
   return launch_status("packed_activations");
 }
 

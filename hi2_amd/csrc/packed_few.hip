@@ -65,8 +65,10 @@ struct FewPass {
       for (int t = 0; t < 16; ++t) v[t] = __uint_as_float(raw[t >> 2][t & 3]);
       if constexpr (GLU) {
 #pragma unroll
-        for (int t = 0; t < 16; ++t)
+        for (int t = 0; t < 16; ++t) {
           v[t] = activate(v[t], a.x.act) * __uint_as_float(up[t >> 2][t & 3]);
+          __builtin_amdgcn_sched_barrier(0);  // one after the other: few registers
+        }
       }
     } else if (a.x.dtype == 1) {
 #pragma unroll
@@ -82,7 +84,10 @@ struct FewPass {
     }
     if (cs && in) {
 #pragma unroll
-      for (int t = 0; t < 16; ++t) v[t] = v[t] / f16_from_bits(cs[16 * g + t]);
+      for (int t = 0; t < 16; ++t) {
+        v[t] = v[t] / f16_from_bits(cs[16 * g + t]);
+        if (t & 1) __builtin_amdgcn_sched_barrier(0);  // two at a time: few registers
+      }
     }
     float m = 0.0f;
 #pragma unroll
@@ -158,13 +163,15 @@ struct FewPass {
 // steps are fetched while the UN before them are multiplied.
 template <int BITS, int FR, int MT, int MODE, int FW>
 __device__ __forceinline__ void few_loop(const FewArgs& a, const GemmArgs& g, const Tile& tile, int e, int64_t first,
-                                         int live, char* xl,
+                                         int live, FewPass<MODE == GIVEN ? RAW16 : MODE,
+                                                           MODE == GIVEN ? 1 : MT, FW> pass,
+                                         int64_t src, char* xl,
                                          f32x4v (&acc)[FR][MODE == GIVEN ? MT / 16 : 1]) {
   constexpr bool RAW = MODE != GIVEN;
   constexpr int MF = RAW ? 1 : MT / 16, MP = RAW ? MT : 1;
   constexpr int CP = 8 / MP;
-  // (what 128 registers hold)
-  constexpr int RU = BITS == 8 || MODE == GLU32 || (MODE == RAW32 && BITS == 4) ? 2 : 4;
+  // what the registers hold: 128 with eight waves, of which a CU takes two workgroups
+  constexpr int RU = BITS == 8 ? 1 : (MODE != RAW16 || FW == 8 ? 2 : 4);
   constexpr int UN = RAW ? (CP < RU ? CP : RU) : (FR * MF <= 2 ? 2 : 1);
   const int k = (int)g.w.k;
   const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4, col = lane & 15;
@@ -230,21 +237,13 @@ __device__ __forceinline__ void few_loop(const FewArgs& a, const GemmArgs& g, co
       }
     }
   };
-  // raw: the lane's row to transform, and the row its operand column reads
-  FewPass<RAW ? MODE : RAW16, MP, FW> pass;
-  int64_t src = -1;
+  // raw: the row this lane's operand column reads, and which lane transforms it
   int R = 0, xr = 0, from = 0;
   float unscale = 1.0f;
   const uint8_t* had = nullptr;
   const uint16_t* cs = nullptr;
   f32x4v part[FR];
   if constexpr (RAW) {
-    const int row = lane / (64 / MP);
-    if (row < live) {
-      src = g.src ? g.src[first + row] : first + row;
-      if (src >= a.x.rows) src = -1;
-    }
-    pass.load(a, k, src, w, 0);
     had = g.w.had + (g.w.per_expert ? (int64_t)e * (g.w.k / 16) : 0);
     cs = g.w.col_scale;
     if (cs && g.w.per_expert) cs += (int64_t)e * g.w.k;
@@ -258,10 +257,9 @@ __device__ __forceinline__ void few_loop(const FewArgs& a, const GemmArgs& g, co
     cur = nxt;
     if constexpr (RAW) {
       if (s0 % CP == 0) {
-        const FewPass<RAW ? MODE : RAW16, MP, FW> now = pass;
-        if (s0 + CP < steps) pass.load(a, k, src, w, s0 + CP);
         fetch(s0 + UN, nxt);
-        unscale = now.store(a, k, had, cs, w, s0, xl);
+        unscale = pass.store(a, k, had, cs, w, s0, xl);
+        if (s0 + CP < steps) pass.load(a, k, src, w, s0 + CP);
         unscale = __shfl(src < 0 ? __builtin_nanf("") : unscale, from);
 #pragma unroll
         for (int f = 0; f < FR; ++f) part[f] = f32x4v{0.0f, 0.0f, 0.0f, 0.0f};
@@ -310,22 +308,40 @@ __device__ __forceinline__ void few_loop(const FewArgs& a, const GemmArgs& g, co
 
 template <int FR, int MT, int MODE, int FW>
 __global__ __launch_bounds__(
-    64 * FW, MODE == GIVEN ? 1 : (MODE == GLU32 ? 2 : (MT == 2 ? 3 : 4))) void packed_few_kernel(FewArgs a) {
+    64 * FW, MODE == GIVEN ? 1 : (MODE != RAW16 ? 2 : (FW == 8 ? 4 : 3))) void packed_few_kernel(FewArgs a) {
   constexpr bool RAW = MODE != GIVEN;
   constexpr int MF = RAW ? 1 : MT / 16;
   constexpr int XW = RAW ? 4096 : 0;         // bytes of transformed rows of a wave
   constexpr int RED = FW * FR * MF * 1024;   // the partial sums
   __shared__ __attribute__((aligned(16))) char lds[FW * XW > RED ? FW * XW : RED];
   const GemmArgs& g = a.two.g[blockIdx.z];
-  const PkWork wk = find_work(g.offs, (int)g.w.experts, g.slots, MT, blockIdx.y);
-  const int e = __builtin_amdgcn_readfirstlane(wk.e);
-  if (e < 0) return;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int e = 0, live = 1;
+  int64_t first = blockIdx.y;  // tiles of one row: the tile is its slot
+  if constexpr (MT > 1) {      // (one tensor)
+    first *= MT;
+    live = (int)(g.slots - first < MT ? g.slots - first : MT);
+  }
+  // the rows to transform come first, behind nothing but their index
+  FewPass<RAW ? MODE : RAW16, RAW ? MT : 1, FW> pass;
+  int64_t src = -1;
+  if constexpr (RAW) {
+    const int row = lane / (64 / MT);
+    if (row < live) {
+      src = g.src ? g.src[first + row] : first + row;
+      if (src >= a.x.rows) src = -1;
+    }
+    pass.load(a, (int)g.w.k, src, w, 0);
+  }
+  if (MT == 1 && g.offs) {  // the expert: as many as end at or before the slot come before it
+    for (int e0 = 0; e0 < (int)g.w.experts; e0 += 64) {
+      const bool before = e0 + lane < (int)g.w.experts && g.offs[e0 + lane + 1] <= first;
+      e += __builtin_popcountll(__ballot(before));
+    }
+    if (e >= (int)g.w.experts) return;  // (ranges that end before the last slot)
+  }
   Tile tile;
   if (!find_tile(g.w, e, blockIdx.x, FR, tile)) return;
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  const int64_t first = __builtin_amdgcn_readfirstlane((int)wk.first);  // slots < 2^31
-  const int64_t left = __builtin_amdgcn_readfirstlane((int)wk.end) - first;
-  const int live = (int)(left < MT ? left : MT);
   // what the epilogue needs of this thread's first output is on its way meanwhile
   const hi2x_epilogue& E = g.epi;
   int n = -1, t = 0;
@@ -348,13 +364,13 @@ __global__ __launch_bounds__(
   char* xl = lds + w * XW;
   switch (tile.nbits) {
     case 2:
-      few_loop<2, FR, MT, MODE, FW>(a, g, tile, e, first, live, xl, acc);
+      few_loop<2, FR, MT, MODE, FW>(a, g, tile, e, first, live, pass, src, xl, acc);
       break;
     case 4:
-      few_loop<4, FR, MT, MODE, FW>(a, g, tile, e, first, live, xl, acc);
+      few_loop<4, FR, MT, MODE, FW>(a, g, tile, e, first, live, pass, src, xl, acc);
       break;
     default:
-      few_loop<8, FR, MT, MODE, FW>(a, g, tile, e, first, live, xl, acc);
+      few_loop<8, FR, MT, MODE, FW>(a, g, tile, e, first, live, pass, src, xl, acc);
   }
   // the waves' partial sums: [fragment][row of activations][slot]
   float* red = reinterpret_cast<float*>(lds);
@@ -396,13 +412,35 @@ int launch(const FewArgs& a, int count, hipStream_t s) {
   int64_t nx = w.max_frags;
   if (count > 1 && a.two.g[1].w.max_frags > nx) nx = a.two.g[1].w.max_frags;
   if (FR > 1) nx = nx / FR + PK_SEGS;
-  const int64_t part = g.offs ? (w.experts < g.slots ? w.experts : g.slots) : 1;
-  const int64_t ny = g.offs ? g.slots / MT + part : (g.slots + MT - 1) / MT;
+  const int64_t ny = (g.slots + MT - 1) / MT;
   HI2X_REQUIRE(nx < (1ll << 31) && ny <= 65535, "packed_linear: %lld rows are too many",
                (long long)g.slots);
   packed_few_kernel<FR, MT, MODE, FW>
       <<<dim3((unsigned)nx, (unsigned)ny, (unsigned)count), 64 * FW, 0, s>>>(a);
   return launch_status("packed_linear");
+}
+
+// One row (a tile of one of an expert's): the eight chunks of a pass keep all lanes of the
+// transform busy, so a wave takes eight chunks where there are workgroups enough (2 a CU),
+// and fewer where there are not: 4096 x 14336 16.8 us with eight waves and 18.2 with four,
+// 14336 x 4096 16.7 and 13.3, the down projection of eight experts (2048 x 1024) 16.2 with
+// four and 13.1 with one.
+template <int MODE>
+int launch_one(const FewArgs& a, int count, int64_t frags, hipStream_t s) {
+  const int64_t nch = a.two.g[0].w.kp / PK_CHUNK;
+  int waves = nch <= 8 ? 1 : (nch <= 16 ? 2 : (nch <= 32 ? 4 : 8));
+  if (frags < 512 && waves < 8) waves *= 2;
+  if (MODE != RAW16 && waves > 4) waves = 4;  // (more registers a wave)
+  switch (waves) {
+    case 1:
+      return launch<1, 1, MODE, 1>(a, count, s);
+    case 2:
+      return launch<1, 1, MODE, 2>(a, count, s);
+    case 4:
+      return launch<1, 1, MODE, 4>(a, count, s);
+    default:
+      return launch<1, 1, MODE, MODE == RAW16 ? 8 : 4>(a, count, s);
+  }
 }
 
 }  // namespace
@@ -421,30 +459,22 @@ int packed_few_raw(const GemmPair& g, int count, const RawRows& x, hipStream_t s
   a.two = g;
   a.x = x;
   const GemmArgs& g0 = g.g[0];
-  // Of experts most have one row in a decode step; a second tile reads the weights again.
-  const int rows = g0.offs ? (g0.slots <= 16 ? 1 : 2) : (int)g0.slots;
-  // Eight waves a workgroup shorten the walk along the columns; four of them transform the
-  // rows with half the instructions, which counts where workgroups share a CU: 4096 x 14336,
-  // one row, 16.8 against 18.2 us, 14336 x 4096 16.7 against 14.1.
-  const int64_t frags = g0.w.max_frags * count *
-                        (g0.offs ? (g0.slots < g0.w.experts ? g0.slots : g0.w.experts) : 1);
+  const int64_t live = !g0.offs ? 1 : (g0.slots < g0.w.experts ? g0.slots : g0.w.experts);
+  const int64_t frags = g0.w.max_frags * count * live;
+  if (g0.offs || g0.slots == 1)
+    return x.x2 ? launch_one<GLU32>(a, count, frags, s)
+                : (x.dtype == 0 ? launch_one<RAW32>(a, count, frags, s)
+                                : launch_one<RAW16>(a, count, frags, s));
+  // Eight waves shorten the walk along the columns, four transform the rows with half the
+  // instructions, which counts where workgroups share a CU.
   const bool wide = frags < 512;
 #define HI2X_RAW(MT)                                                                         \
-  if (x.dtype == 0)                                                                          \
-    return wide ? launch<1, MT, RAW32, 8>(a, count, s) : launch<1, MT, RAW32, 4>(a, count, s); \
+  if (x.dtype == 0) return launch<1, MT, RAW32, 4>(a, count, s);                             \
   return wide ? launch<1, MT, RAW16, 8>(a, count, s) : launch<1, MT, RAW16, 4>(a, count, s);
-  if (x.x2)  // (experts' only)
-    return rows <= 1 ? (wide ? launch<1, 1, GLU32, 8>(a, count, s)
-                             : launch<1, 1, GLU32, 4>(a, count, s))
-                     : (wide ? launch<1, 2, GLU32, 8>(a, count, s)
-                             : launch<1, 2, GLU32, 4>(a, count, s));
-  if (rows <= 1) {
-    HI2X_RAW(1)
-  }
-  if (rows <= 2) {
+  if (g0.slots <= 2) {
     HI2X_RAW(2)
   }
-  if (rows <= 4) {
+  if (g0.slots <= 4) {
     HI2X_RAW(4)
   }
   HI2X_RAW(8)

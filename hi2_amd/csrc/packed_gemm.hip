@@ -206,13 +206,24 @@ __device__ __forceinline__ float row_scale(const GemmArgs& g, int64_t first, int
   return r >= 0 && r < g.x.rows ? g.x.scale[r] : __builtin_nanf("");
 }
 
-// The work of a workgroup: its expert, tile of fragments and tile of activation rows.
+// The work of a workgroup: its expert, tile of fragments and tile of activation rows.  Of
+// several experts the grid is (tiles x tiles of rows) long: workgroups go to the eight XCDs
+// in turn, so an XCD takes all tiles of four neighbouring row tiles one after the other, and
+// the rows (and mostly the expert's weights) come to its L2 once.
 template <int NF, int MF>
-__device__ __forceinline__ bool find(const GemmArgs& g, Tile& tile, int64_t& first, int& live) {
-  const PkWork wk = find_work(g.offs, (int)g.w.experts, g.slots, 16 * MF, blockIdx.y);
+__device__ __forceinline__ bool find(const GemmArgs& g, int nx, Tile& tile, int64_t& first,
+                                     int& live) {
+  int x = blockIdx.x;
+  int64_t y = blockIdx.y;
+  if (g.offs) {
+    const int xcd = x & 7, j = x >> 3, r = j / nx;
+    x = j - r * nx;
+    y = ((int64_t)(r >> 2) * 8 + xcd) * 4 + (r & 3);
+  }
+  const PkWork wk = find_work(g.offs, (int)g.w.experts, g.slots, 16 * MF, y);
   const int e = __builtin_amdgcn_readfirstlane(wk.e);
   if (e < 0) return false;
-  if (!find_tile(g.w, e, blockIdx.x, 4 * NF, tile)) return false;
+  if (!find_tile(g.w, e, x, 4 * NF, tile)) return false;
   first = __builtin_amdgcn_readfirstlane((int)wk.first);  // slots < 2^31
   const int64_t left = __builtin_amdgcn_readfirstlane((int)wk.end) - first;
   live = (int)(left < 16 * MF ? left : 16 * MF);
@@ -230,7 +241,7 @@ __device__ __forceinline__ int slot_row(const GemmArgs& g, const Tile& tile, int
 // the accumulators hold them.
 template <int NF, int MF, bool SPLIT>
 __global__ __launch_bounds__(256, NF == 4 ? 2 : 4) void packed_gemm_kernel(GemmPair two, float* part,
-                                                                           int per) {
+                                                                           int per, int nx) {
   const GemmArgs& g = two.g[SPLIT ? 0 : blockIdx.z];
   constexpr int MT = 16 * MF, NS = 64 * NF;
   constexpr int XB = 2 * MT * 256;  // two stages of activations
@@ -244,7 +255,7 @@ __global__ __launch_bounds__(256, NF == 4 ? 2 : 4) void packed_gemm_kernel(GemmP
   Tile tile;
   int64_t first;
   int live;
-  if (!find<NF, MF>(g, tile, first, live)) return;
+  if (!find<NF, MF>(g, nx, tile, first, live)) return;
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
   // Where the rows this lane stages begin.  Rows past the end read zeros or another
   // tile's, and are not stored; indices outside the activations read row 0 (and come out as
@@ -327,7 +338,7 @@ __global__ __launch_bounds__(256) void packed_join_kernel(GemmArgs g, const floa
   Tile tile;
   int64_t first;
   int live;
-  if (!find<NF, MF>(g, tile, first, live)) return;
+  if (!find<NF, MF>(g, 1, tile, first, live)) return;
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, m = blockIdx.z;
   const int rows = live - 16 * m < 16 ? live - 16 * m : 16;
   if (rows <= 0) return;
@@ -355,13 +366,13 @@ __global__ __launch_bounds__(256) void packed_join_kernel(GemmArgs g, const floa
 
 template <int NF, int MF>
 int launch_gemm(const GemmPair& g, int count, float* part, int splits, int per, dim3 grid,
-                hipStream_t s) {
+                int nx, hipStream_t s) {
   if (splits == 1) {
     grid.z = count;
-    packed_gemm_kernel<NF, MF, false><<<grid, 256, 0, s>>>(g, nullptr, 0);
+    packed_gemm_kernel<NF, MF, false><<<grid, 256, 0, s>>>(g, nullptr, 0, nx);
   } else {
     grid.z = splits;
-    packed_gemm_kernel<NF, MF, true><<<grid, 256, 0, s>>>(g, part, per);
+    packed_gemm_kernel<NF, MF, true><<<grid, 256, 0, s>>>(g, part, per, nx);
     grid.z = MF;
     packed_join_kernel<NF, MF><<<grid, 256, 0, s>>>(g.g[0], part, splits);
   }
@@ -446,19 +457,21 @@ int packed_product(const GemmPair& two, int count, void* work, int64_t work_byte
     const int64_t other = m[p.nf == 1 ? 0 : (p.nf == 2 ? 1 : 2)];
     nx = nx > other ? nx : other;
   }
-  HI2X_REQUIRE(nx < (1ll << 31) && p.ny <= 65535, "packed_linear: %lld rows are too many",
-               (long long)g.slots);
+  const int64_t padded = (p.ny + 31) / 32 * 32;  // whole rounds of four tiles to each XCD
+  HI2X_REQUIRE(nx < (1ll << 31) && (g.offs ? nx * padded < (1ll << 31) : p.ny <= 65535),
+               "packed_linear: %lld rows are too many", (long long)g.slots);
   Workspace ws;
   if (int rc = take_workspace(ws, work, work_bytes, (size_t)p.part_bytes(), s, "packed_linear"))
     return rc;
   float* part = reinterpret_cast<float*>(ws.p);
-  const dim3 grid((unsigned)nx, (unsigned)p.ny, (unsigned)count);
+  const dim3 grid((unsigned)(g.offs ? nx * padded : nx), (unsigned)(g.offs ? 1 : p.ny),
+                  (unsigned)count);
   if (p.nf == 4) {
-    packed_gemm_kernel<4, 8, false><<<grid, 256, 0, s>>>(two, nullptr, 0);
+    packed_gemm_kernel<4, 8, false><<<grid, 256, 0, s>>>(two, nullptr, 0, (int)nx);
     return launch_status("packed_linear");
   }
-  return p.nf == 2 ? launch_gemm<2, 4>(two, count, part, p.splits, p.per, grid, s)
-                   : launch_gemm<1, 4>(two, count, part, p.splits, p.per, grid, s);
+  return p.nf == 2 ? launch_gemm<2, 4>(two, count, part, p.splits, p.per, grid, (int)nx, s)
+                   : launch_gemm<1, 4>(two, count, part, p.splits, p.per, grid, (int)nx, s);
 }
 
 }  // namespace hi2x
