@@ -4,8 +4,8 @@
 // 16 lanes hold one token's E scores (expert 16 i + lane in register i), so four tokens
 // share a wave and every reduction over the experts is four DPP steps without LDS.  The
 // passes read a few MB at most: what bounds them is launches and the latency of the top-k
-// loop, so a workgroup does 64 tokens from logits to indices, and up to 64 tokens in all
-// the slot order too.  That order needs no sort: a token chooses an expert at most once,
+// loop, so a workgroup does up to 64 tokens from logits to indices, and where they are all there
+// are the slot order too.  That order needs no sort: a token chooses an expert at most once,
 // so 64 tokens' choices of an expert are one 64-bit mask, a choice's rank is the number of
 // lower bits, and the stable order follows from the masks' popcounts.
 #include "packed.h"
@@ -13,12 +13,10 @@
 namespace hi2x {
 namespace {
 
-constexpr int RT = 64;      // tokens per workgroup (half as many above 256 experts, where a
-                            // token's registers leave room for half the waves)
 constexpr int RK = 32;      // most choices
 constexpr int RE = 512;     // most experts
 constexpr int RG = 64;      // most groups
-constexpr int SCAN_OVER = 512;  // workgroups from which the counts get a scan of their own
+constexpr int SCAN_OVER = 1024;  // workgroups above which the counts get a scan of their own
 
 template <int CTRL>
 __device__ __forceinline__ double dpp_d(double v) {
@@ -48,12 +46,22 @@ __device__ __forceinline__ void token_scores(const void* logits, int dtype, int6
                                              int scoring, int l16, float (&v)[EPL],
                                              float (&p)[EPL]) {
   const float ninf = -__builtin_inff();
+  // all loads in flight before the first conversion (past the end: the last expert's)
+  if (dtype == 0) {
+    const float* p = static_cast<const float*>(logits) + at;
 #pragma unroll
-  for (int i = 0; i < EPL; ++i) {
-    const int x = 16 * i + l16;
-    float a = x < e ? load_as_f32(logits, at + x, dtype) : ninf;
-    v[i] = a == a ? a : ninf;
+    for (int i = 0; i < EPL; ++i) v[i] = p[16 * i + l16 < e ? 16 * i + l16 : e - 1];
+  } else {
+    const uint16_t* p = static_cast<const uint16_t*>(logits) + at;
+    uint16_t r[EPL];
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) r[i] = p[16 * i + l16 < e ? 16 * i + l16 : e - 1];
+#pragma unroll
+    for (int i = 0; i < EPL; ++i)
+      v[i] = dtype == 1 ? f16_from_bits(r[i]) : __uint_as_float((uint32_t)r[i] << 16);
   }
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) v[i] = 16 * i + l16 < e && v[i] == v[i] ? v[i] : ninf;
   if (scoring == 1) {
 #pragma unroll
     for (int i = 0; i < EPL; ++i) p[i] = 1.0f / (1.0f + expf(-v[i]));
@@ -78,6 +86,26 @@ __device__ __forceinline__ void token_scores(const void* logits, int dtype, int6
   for (int i = 0; i < EPL; ++i) p[i] = s > 0.0f ? p[i] / s : (s == s ? 0.0f : s);
 }
 
+// The best two values of a row of lanes, from each lane's two.
+template <int CTRL>
+__device__ __forceinline__ void best2_step(float& b1, float& b2) {
+  const float o1 = __int_as_float(dpp<CTRL>(__float_as_int(b1)));
+  const float o2 = __int_as_float(dpp<CTRL>(__float_as_int(b2)));
+  b2 = fmaxf(fminf(b1, o1), fmaxf(b2, o2));
+  b1 = fmaxf(b1, o1);
+}
+__device__ __forceinline__ void row_best2(float& b1, float& b2) {
+  best2_step<0xB1>(b1, b2);
+  best2_step<0x4E>(b1, b2);
+  best2_step<0x141>(b1, b2);
+  best2_step<0x140>(b1, b2);
+}
+
+// Whether groups of gs experts are whole registers of a token, at most one to a lane.
+__host__ __device__ inline bool whole_rows(int64_t gs, int64_t groups) {
+  return gs % 16 == 0 && groups <= 16;
+}
+
 struct RouteArgs {
   const void* logits;
   int dtype;
@@ -91,22 +119,32 @@ struct RouteArgs {
   int64_t* rows;
   int64_t* offs;
   int64_t* slots;
-  uint8_t* hist;    // [workgroups][e] tokens per expert
-  int32_t* prefix;  // [workgroups][e] tokens of earlier workgroups, or null
+  uint8_t* hist;    // [e][nbp] tokens of each workgroup
+  int32_t* prefix;  // [e][nbp] tokens of earlier workgroups, or null
+  int nbp;          // workgroups, up to a multiple of 16 (the rest counts nothing)
 };
 
-// cnt[0..e) -> exclusive prefix in place, by a workgroup of at least e threads.
+// cnt[0..e) -> running sums in place, by the first wave.
 __device__ __forceinline__ void scan_experts(int* cnt, int e) {
-  const int tid = threadIdx.x;
-  for (int d = 1; d < e; d <<= 1) {
-    int a = 0;
-    if (tid < e && tid >= d) a = cnt[tid - d];
-    __syncthreads();
-    if (tid < e) cnt[tid] += a;
-    __syncthreads();
+  if (threadIdx.x < 64) {
+    const int lane = threadIdx.x;
+    int before = 0;
+    for (int e0 = 0; e0 < e; e0 += 64) {
+      int v = e0 + lane < e ? cnt[e0 + lane] : 0;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(v, d);
+        if (lane >= d) v += o;
+      }
+      v += before;
+      if (e0 + lane < e) cnt[e0 + lane] = v;
+      before = __shfl(v, 63);
+    }
   }
+  __syncthreads();
 }
 
+// NT / 16 tokens to a workgroup.
 template <int EPL, int NT>
 __global__ __launch_bounds__(NT) void route_kernel(RouteArgs a) {
   constexpr int RT = NT / 16;
@@ -125,30 +163,53 @@ __global__ __launch_bounds__(NT) void route_kernel(RouteArgs a) {
   // the keys the experts are ranked by; 0: taken, or not taking part
   const float ninf = -__builtin_inff();
   uint32_t key[EPL];
+  if (a.bias) {
+    float b[EPL];
 #pragma unroll
-  for (int i = 0; i < EPL; ++i) {
-    const int x = 16 * i + l16;
-    if (a.bias && v[i] > ninf) {
-      const float c = p[i] + (x < e ? a.bias[x] : 0.0f);
-      v[i] = c == c ? c : ninf;
+    for (int i = 0; i < EPL; ++i) b[i] = a.bias[16 * i + l16 < e ? 16 * i + l16 : e - 1];
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) {
+      const float c = p[i] + b[i];
+      v[i] = v[i] > ninf && c == c ? c : ninf;
     }
-    key[i] = x < e ? order_key(v[i]) : 0u;
   }
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) key[i] = 16 * i + l16 < e ? order_key(v[i]) : 0u;
   if (a.top_groups < a.groups) {
     const int gs = e / a.groups, pitch = e + a.groups;
     const float inv = 1.0f / (float)gs;
-#pragma unroll
-    for (int i = 0; i < EPL; ++i) {
-      const int x = 16 * i + l16;
-      if (x < e) keys[tok * pitch + x + (int)(((float)x + 0.5f) * inv)] = v[i];
-    }
-    __syncthreads();
     uint32_t gk[RG / 16];
 #pragma unroll
-    for (int i = 0; i < RG / 16; ++i) {
-      const int g = 16 * i + l16;
-      gk[i] = 0;
-      if (g < a.groups) {
+    for (int i = 0; i < RG / 16; ++i) gk[i] = 0;
+    if (whole_rows(gs, a.groups)) {
+      // whole registers to a group: its best two by exchanges over the 16 lanes
+      float b1 = ninf, b2 = ninf;
+      int left = gs / 16, g = 0;
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) {
+        b2 = v[i] > b1 ? b1 : (v[i] > b2 ? v[i] : b2);
+        b1 = v[i] > b1 ? v[i] : b1;
+        if (--left == 0) {
+          row_best2(b1, b2);
+          const float s = a.bias ? b1 + b2 : b1;
+          if (l16 == g) gk[0] = order_key(s == s ? s : ninf);
+          b1 = b2 = ninf;
+          left = gs / 16;
+          ++g;
+        }
+      }
+      if (l16 >= a.groups) gk[0] = 0;
+    } else {
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) {
+        const int x = 16 * i + l16;
+        if (x < e) keys[tok * pitch + x + (int)(((float)x + 0.5f) * inv)] = v[i];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < RG / 16; ++i) {
+        const int g = 16 * i + l16;
+        if (g >= a.groups) continue;
         float b1 = ninf, b2 = ninf;
         for (int x = 0; x < gs; ++x) {
           const float c = keys[tok * pitch + g * (gs + 1) + x];
@@ -186,23 +247,23 @@ __global__ __launch_bounds__(NT) void route_kernel(RouteArgs a) {
   }
   for (int j = 0; j < k; ++j) {
     uint32_t bk = 0;
-    int be = RE;
-    float bp = 0.0f;
 #pragma unroll
-    for (int i = 0; i < EPL; ++i)
-      if (key[i] > bk) {
-        bk = key[i];
-        be = 16 * i + l16;
-        bp = p[i];
-      }
+    for (int i = 0; i < EPL; ++i) bk = key[i] > bk ? key[i] : bk;
     const uint32_t m = row_umax(bk);
-    const int w = (int)row_umin(bk == m ? (uint32_t)be : 0xffffu);
-    if (be == w) {
-      sel_e[tok][j] = w;
-      sel_p[tok][j] = bp;
+    uint32_t be = RE;
 #pragma unroll
-      for (int i = 0; i < EPL; ++i)
-        if (16 * i + l16 == w) key[i] = 0;
+    for (int i = EPL - 1; i >= 0; --i) be = key[i] == m ? (uint32_t)(16 * i + l16) : be;
+    const uint32_t w = row_umin(be);
+    if (be == w) {
+      float bp = 0.0f;
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) {
+        const bool it = (uint32_t)(16 * i + l16) == w;
+        bp = it ? p[i] : bp;
+        key[i] = it ? 0u : key[i];
+      }
+      sel_e[tok][j] = (int)w;
+      sel_p[tok][j] = bp;
     }
   }
   __syncthreads();
@@ -219,16 +280,21 @@ __global__ __launch_bounds__(NT) void route_kernel(RouteArgs a) {
   }
   __syncthreads();
   if (a.hist) {
-    for (int i = tid; i < e; i += NT)
-      a.hist[(int64_t)blockIdx.x * e + i] =
+    for (int i = tid; i < e; i += NT) {
+      uint8_t* h = a.hist + (int64_t)i * a.nbp;
+      h[blockIdx.x] =
           (uint8_t)(__builtin_popcount(mask[i][0]) + __builtin_popcount(mask[i][1]));
+      if (blockIdx.x == gridDim.x - 1)
+        for (int b = gridDim.x; b < a.nbp; ++b) h[b] = 0;
+    }
     return;
   }
   // one workgroup in all: the slot order at once
-  if (tid < e) cnt[tid] = __builtin_popcount(mask[tid][0]) + __builtin_popcount(mask[tid][1]);
+  for (int i = tid; i < e; i += NT)
+    cnt[i] = __builtin_popcount(mask[i][0]) + __builtin_popcount(mask[i][1]);
   __syncthreads();
   scan_experts(cnt, e);
-  if (tid < e) a.offs[tid + 1] = cnt[tid];
+  for (int i = tid; i < e; i += NT) a.offs[i + 1] = cnt[i];
   if (tid == 0) a.offs[0] = 0;
   for (int j = l16; j < k; j += 16) {
     if (!live) break;
@@ -244,26 +310,34 @@ __global__ __launch_bounds__(NT) void route_kernel(RouteArgs a) {
   }
 }
 
-// prefix[b][x] = sum of hist[b'][x] over b' < b; a workgroup takes 64 experts, 16 runs of
-// workgroups side by side.
+// prefix[x][b] = sum of hist[x][b'] over b' < b, a workgroup for each expert.
 __global__ __launch_bounds__(1024) void route_scan_kernel(const uint8_t* __restrict__ hist,
-                                                          int nb, int e,
-                                                          int32_t* __restrict__ prefix) {
-  __shared__ int part[16][64];
-  const int x = blockIdx.x * 64 + (threadIdx.x & 63), r = threadIdx.x >> 6;
-  const int run = (nb + 15) / 16, b0 = r * run, b1 = b0 + run < nb ? b0 + run : nb;
-  int s = 0;
-  if (x < e)
-    for (int b = b0; b < b1; ++b) s += hist[(int64_t)b * e + x];
-  part[r][threadIdx.x & 63] = s;
-  __syncthreads();
-  s = 0;
-  for (int i = 0; i < r; ++i) s += part[i][threadIdx.x & 63];
-  if (x < e)
-    for (int b = b0; b < b1; ++b) {
-      prefix[(int64_t)b * e + x] = s;
-      s += hist[(int64_t)b * e + x];
+                                                          int nbp, int32_t* __restrict__ prefix) {
+  __shared__ int part[16];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const uint8_t* h = hist + (int64_t)blockIdx.x * nbp;
+  int32_t* p = prefix + (int64_t)blockIdx.x * nbp;
+  int before = 0;
+  for (int b0 = 0; b0 < nbp; b0 += 1024) {
+    const int b = b0 + threadIdx.x;
+    const int own = b < nbp ? h[b] : 0;
+    int v = own;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int o = __shfl_up(v, d);
+      if (lane >= d) v += o;
     }
+    if (lane == 63) part[w] = v;
+    __syncthreads();
+    int front = before, all = before;
+    for (int i = 0; i < 16; ++i) {
+      front += i < w ? part[i] : 0;
+      all += part[i];
+    }
+    if (b < nbp) p[b] = front + v - own;
+    before = all;
+    __syncthreads();
+  }
 }
 
 // The slot order of workgroup b's tokens, given every workgroup's counts.
@@ -285,21 +359,29 @@ __global__ __launch_bounds__(1024) void route_order_kernel(RouteArgs a, int nb, 
       atomicOr(&mask[(int)a.index[t * k + j]][tok >> 5], 1u << (tok & 31));
   if (a.prefix) {
     for (int x = tid; x < e; x += 1024) {
-      base[x] = a.prefix[(int64_t)b * e + x];
-      cnt[x] = a.prefix[(int64_t)(nb - 1) * e + x] + a.hist[(int64_t)(nb - 1) * e + x];
+      const int64_t at = (int64_t)x * a.nbp;
+      base[x] = a.prefix[at + b];
+      cnt[x] = a.prefix[at + nb - 1] + a.hist[at + nb - 1];
     }
   } else {
     const int ep = e <= 64 ? 64 : (e <= 128 ? 128 : (e <= 256 ? 256 : 512));
     const int x = tid & (ep - 1), parts = 1024 / ep;
     if (x < e) {
-      int all = 0, pre = 0;
-      for (int i = tid / ep; i < nb; i += parts) {
-        const int h = a.hist[(int64_t)i * e + x];
-        all += h;
-        pre += i < b ? h : 0;
+      // 16 workgroups' counts a load, four a sum of bytes
+      uint32_t all = 0, pre = 0;
+      const u32x4* h = reinterpret_cast<const u32x4*>(a.hist + (int64_t)x * a.nbp);
+      for (int i = tid / ep; i < a.nbp / 16; i += parts) {
+        const u32x4 v = h[i];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int n = b - 16 * i - 4 * q;  // of these four, how many come before
+          const uint32_t m = n <= 0 ? 0u : (n >= 4 ? ~0u : (1u << (8 * n)) - 1u);
+          all = __builtin_amdgcn_sad_u8(v[q], 0u, all);
+          pre = __builtin_amdgcn_sad_u8(v[q] & m, 0u, pre);
+        }
       }
-      atomicAdd(&cnt[x], all);
-      atomicAdd(&base[x], pre);
+      atomicAdd(&cnt[x], (int)all);
+      atomicAdd(&base[x], (int)pre);
     }
   }
   __syncthreads();
@@ -447,7 +529,14 @@ int check_route(const char* what, const void* logits, int dtype, int64_t ld, int
   return HI2X_OK;
 }
 
-int route_tokens(int64_t e) { return e <= 256 ? RT : RT / 2; }
+// Tokens to a workgroup.  Four where that is all there are (barriers of one wave: one token
+// of 64 experts 7.2 -> 5.6 us); up to the 64 that one launch orders (32 above 256 experts,
+// whose registers leave room for half the waves) one workgroup; up to 4096 16, which spreads
+// them over the CUs (4096 tokens of 256 experts in groups 20 -> 9 us); then 64 again.
+int route_tokens(int64_t t, int64_t e) {
+  const int most = e <= 256 ? 64 : 32;
+  return t <= 4 ? 4 : (t <= most ? most : (t <= 4096 ? 16 : most));
+}
 
 // Clears offs where there are no tokens.
 __global__ void zero_i64_kernel(int64_t* p, int64_t n) {
@@ -492,10 +581,10 @@ using namespace hi2x;
 
 extern "C" int64_t hi2x_route_workspace_bytes(int64_t t, int64_t e) {
   if (t < 0 || e < 1 || e > RE) return -1;
-  const int64_t nb = (t + route_tokens(e) - 1) / route_tokens(e);
+  const int64_t nb = (t + route_tokens(t, e) - 1) / route_tokens(t, e);
   if (nb <= 1) return 0;
-  const int64_t hist = (nb * e + 255) / 256 * 256;
-  return hist + (nb > SCAN_OVER ? nb * e * 4 : 0);
+  const int64_t nbp = (nb + 15) / 16 * 16;
+  return align256(nbp * e) + (nb > SCAN_OVER ? nbp * e * 4 : 0);
 }
 
 extern "C" int hi2x_route(const void* logits, int dtype, int64_t ld, int64_t t, int64_t e,
@@ -517,27 +606,37 @@ extern "C" int hi2x_route(const void* logits, int dtype, int64_t ld, int64_t t, 
     zero_i64_kernel<<<dim3((unsigned)(e / 256 + 1)), 256, 0, s>>>(offs, e + 1);
     return launch_status("route");
   }
-  const int rt = route_tokens(e);
+  const int rt = route_tokens(t, e);
   const int64_t nb = (t + rt - 1) / rt;
   Workspace w;
   const int64_t need = hi2x_route_workspace_bytes(t, e);
   if (int rc = take_workspace(w, ws, ws_bytes, (size_t)need, s, "route")) return rc;
   RouteArgs a{logits, dtype,  ld,      t,     (int)e, (int)top_k, scoring, bias,
               (int)groups, (int)top_groups, renormalise, scale, index, weights, rows, offs,
-              slots, nullptr, nullptr};
+              slots, nullptr, nullptr, 0};
   if (nb > 1) {
+    a.nbp = (int)((nb + 15) / 16 * 16);
     a.hist = reinterpret_cast<uint8_t*>(w.p);
     if (nb > SCAN_OVER)
-      a.prefix = reinterpret_cast<int32_t*>(w.p + (nb * e + 255) / 256 * 256);
+      a.prefix = reinterpret_cast<int32_t*>(w.p + align256((int64_t)a.nbp * e));
   }
-  const size_t dyn = top_groups < groups ? (size_t)rt * (e + groups) * 4 : 0;
+  const size_t dyn = top_groups < groups && !whole_rows(e / groups, groups) ? (size_t)rt * (e + groups) * 4 : 0;
   const dim3 grid((unsigned)nb);
-#define HI2X_ROUTE(EPL, NT)                                                                    \
+#define HI2X_ROUTE_(EPL, NT)                                                                   \
   {                                                                                            \
     if (dyn > 32768)                                                                           \
       HI2X_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(route_kernel<EPL, NT>),       \
                                    hipFuncAttributeMaxDynamicSharedMemorySize, (int)dyn));     \
     route_kernel<EPL, NT><<<grid, NT, dyn, s>>>(a);                                            \
+  }
+#define HI2X_ROUTE(EPL, MOST)                       \
+  {                                                 \
+    if (rt == 4)                                    \
+      HI2X_ROUTE_(EPL, 64)                          \
+    else if (rt == 16)                              \
+      HI2X_ROUTE_(EPL, 256)                         \
+    else                                            \
+      HI2X_ROUTE_(EPL, MOST)                        \
   }
   if (e <= 64)
     HI2X_ROUTE(4, 1024)
@@ -547,11 +646,11 @@ extern "C" int hi2x_route(const void* logits, int dtype, int64_t ld, int64_t t, 
     HI2X_ROUTE(16, 1024)
   else
     HI2X_ROUTE(32, 512)
+#undef HI2X_ROUTE_
 #undef HI2X_ROUTE
   if (nb > 1) {
     if (a.prefix)
-      route_scan_kernel<<<dim3((unsigned)((e + 63) / 64)), 1024, 0, s>>>(a.hist, (int)nb, (int)e,
-                                                                        a.prefix);
+      route_scan_kernel<<<dim3((unsigned)e), 1024, 0, s>>>(a.hist, a.nbp, a.prefix);
     route_order_kernel<<<grid, 1024, 0, s>>>(a, (int)nb, rt);
   }
   return launch_status("route");
