@@ -419,15 +419,23 @@ __global__ __launch_bounds__(256) void route_backward_kernel(
   const int64_t t = live ? tt : n_tok - 1;
   float v[EPL], p[EPL], d[EPL];
   bool chosen[EPL];
+  __shared__ int64_t at[16][RK];
+  __shared__ float up[16][RK];
+  const int tok = threadIdx.x >> 4;
+  for (int j = l16; j < k; j += 16) {
+    at[tok][j] = index[t * k + j];
+    up[tok][j] = grad[t * k + j];
+  }
   token_scores<EPL>(logits, dtype, t * ld, e, scoring, l16, v, p);
+  __syncthreads();
 #pragma unroll
   for (int i = 0; i < EPL; ++i) {
     d[i] = 0.0f;
     chosen[i] = false;
   }
   for (int j = 0; j < k; ++j) {
-    const int64_t x = index[t * k + j];
-    const float g = grad[t * k + j];
+    const int64_t x = at[tok][j];
+    const float g = up[tok][j];
 #pragma unroll
     for (int i = 0; i < EPL; ++i)
       if (x == 16 * i + l16) {

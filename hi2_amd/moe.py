@@ -57,24 +57,27 @@ class _Weights(torch.autograd.Function):
     """The weights' gradient to the logits (``hi2x_route_backward``)."""
 
     @staticmethod
-    def forward(ctx, logits, out, scoring, renormalise, scale):
-        ctx.save_for_backward(logits, out[0])
-        ctx.args = (scoring, renormalise, scale)
-        return out[1]
+    def forward(ctx, logits, weights, index, args):
+        ctx.save_for_backward(logits, index)
+        ctx.args = args
+        ctx.mark_dirty(weights)
+        return weights
 
     @staticmethod
+    @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         logits, index = ctx.saved_tensors
         scoring, renormalise, scale = ctx.args
         t, e = logits.shape
         d = torch.empty(t, e, dtype=logits.dtype, device=logits.device)
-        grad = grad.to(torch.float32).contiguous()
+        if grad.dtype != torch.float32 or not grad.is_contiguous():
+            grad = grad.to(torch.float32).contiguous()
         if t:
-            _lib.call("hi2x_route_backward", logits.device, _lib.ptr(logits),
+            _lib.call("hi2x_route_backward", logits.device, logits.data_ptr(),
                       _FLOATS[logits.dtype], logits.stride(0) if t > 1 else e, t, e,
-                      index.shape[1], scoring, renormalise, scale, _lib.ptr(index),
-                      _lib.ptr(grad), _lib.ptr(d))
-        return d, None, None, None, None
+                      index.shape[1], scoring, renormalise, scale, index.data_ptr(),
+                      grad.data_ptr(), d.data_ptr())
+        return d, None, None, None
 
 
 def route(logits: torch.Tensor, top_k: int, scoring: str = "softmax", bias=None,
@@ -110,23 +113,21 @@ def route(logits: torch.Tensor, top_k: int, scoring: str = "softmax", bias=None,
     x = logits.detach()
     if (e > 1 and x.stride(1) != 1) or (t > 1 and x.stride(0) < e):
         x = x.contiguous()
-    # one allocation: int64 index, rows, slots and offs, then the weights
     k = max(top_k, 0)
-    n = t * k
-    i64 = torch.empty(3 * n + e + 1, dtype=torch.int64, device=dev)
+    index, slots, rows = torch.empty(3, t, k, dtype=torch.int64, device=dev).unbind()
+    rows = rows.view(-1)
+    offs = torch.empty(e + 1, dtype=torch.int64, device=dev)
     weights = torch.empty(t, k, dtype=torch.float32, device=dev)
-    index, slots = i64[:n].view(t, k), i64[n:2 * n].view(t, k)
-    rows, offs = i64[2 * n:3 * n], i64[3 * n:]
     size = _lib.lib().hi2x_route_workspace_bytes(t, e)
     ws = torch.empty(size, dtype=torch.uint8, device=dev) if size > 0 else None
-    _lib.call("hi2x_route", dev, _lib.ptr(x), _FLOATS[x.dtype], x.stride(0) if t > 1 else e, t,
+    _lib.call("hi2x_route", dev, x.data_ptr(), _FLOATS[x.dtype], x.stride(0) if t > 1 else e, t,
               e, top_k, SCORING[scoring], _lib.ptr(b), groups, top_groups, int(renormalise),
-              float(scale), _lib.ptr(index), _lib.ptr(weights), _lib.ptr(rows), _lib.ptr(offs),
-              _lib.ptr(slots), _lib.ptr(ws), max(size, 0))
+              float(scale), index.data_ptr(), weights.data_ptr(), rows.data_ptr(),
+              offs.data_ptr(), slots.data_ptr(), _lib.ptr(ws), max(size, 0))
     if logits.requires_grad and torch.is_grad_enabled():
         weights = _Weights.apply(logits if x.data_ptr() == logits.data_ptr() else
-                                 logits.contiguous(), (index, weights), SCORING[scoring],
-                                 int(renormalise), float(scale))
+                                 logits.contiguous(), weights, index,
+                                 (SCORING[scoring], int(renormalise), float(scale)))
     return Routing(index, weights, rows, offs, slots)
 
 

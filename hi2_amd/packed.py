@@ -246,8 +246,7 @@ def activations(x: torch.Tensor, w: PackedLinear | PackedExperts) -> Activations
     """``T(x)`` for ``w`` and every tensor with the same transform, to be handed to
     :func:`packed_linear` or :func:`experts_linear` in the place of ``x [..., K]``.  The
     product then has one row per row of ``x``."""
-    if _lib.require_gpu(x) != w.device:
-        raise RuntimeError(f"x is on {x.device}, the weights on {w.device}")
+    _same_device(w, "activations", x)
     _no_grad_inputs("activations", x)
     if w.transform is None:
         raise ValueError("the experts have transforms of their own: give experts_linear x itself")
@@ -274,17 +273,19 @@ def _operand(t, slots, n, name):
 
 
 def _product(w, x, src, offs, slots, bias, activation, mul, residual, out_dtype, what):
+    """The product of :func:`packed_linear` and :func:`experts_linear`; ``x`` is rows
+    ``[rows, K]`` or :class:`Activations`, both on the weights' device already."""
     dev, n = w.device, w.n
     given = not isinstance(x, torch.Tensor)
-    if _lib.require_gpu(x.planes if given else x, bias, mul, residual, src, offs) != dev:
-        raise RuntimeError(f"{what}: inputs are not on the weights' device {dev}")
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"activation {activation!r} ({', '.join(ACTIVATIONS)})")
+    bias_p = bias_dt = 0
     if bias is not None:
         if bias.numel() != n:
             raise ValueError(f"bias has {bias.numel()} entries, expected {n}")
         bias = bias.reshape(-1).contiguous()
+        bias_p, bias_dt = bias.data_ptr(), _dtype(bias, "bias")
     mul, mul_p, mul_ld, mul_dt = _operand(mul, slots, n, "mul")
     residual, res_p, res_ld, res_dt = _operand(residual, slots, n, "residual")
     out_dt = _dtype(out_dtype, "out_dtype")
@@ -292,23 +293,32 @@ def _product(w, x, src, offs, slots, bias, activation, mul, residual, out_dtype,
     out = torch.empty(slots, n, dtype=out_dtype, device=dev)
     if not slots:
         return out
-    epi = _lib.Epilogue(None if bias is None else bias.data_ptr(), mul_p, res_p, out.data_ptr(),
-                        mul_ld, res_ld, n, 0 if bias is None else _dtype(bias, "bias"), mul_dt,
-                        res_dt, out_dt, act, 0)
-    if not given:
-        x = _aligned(x)
-    npl = x.desc.nplanes if given else _planes(x.dtype, w)
-    rows = x.scale.numel() if given else x.shape[0]
-    size = _lib.lib().hi2x_packed_workspace_bytes(
-        w._ref, rows, npl, given, slots, src is not None, offs is not None)
-    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size > 0 else None
+    epi = _lib.Epilogue(bias_p or None, mul_p, res_p, out.data_ptr(), mul_ld, res_ld, n, bias_dt,
+                        mul_dt, res_dt, out_dt, act, 0)
     if given:
-        _lib.call("hi2x_packed_linear_activations", dev, w._ref, ctypes.byref(x.desc),
-                  _lib.ptr(src), _lib.ptr(offs), slots, ctypes.byref(epi), _lib.ptr(ws), size)
+        rows, npl = x.scale.numel(), x.desc.nplanes
     else:
-        _lib.call("hi2x_packed_linear", dev, w._ref, _lib.ptr(x), dt, _pitch(x), rows, npl,
-                  _lib.ptr(src), _lib.ptr(offs), slots, ctypes.byref(epi), _lib.ptr(ws), size)
+        x = _aligned(x)
+        rows, npl = x.shape[0], _planes(x.dtype, w)
+    size = _lib.lib().hi2x_packed_workspace_bytes(w._ref, rows, npl, given, slots,
+                                                  src is not None, offs is not None)
+    ws = torch.empty(size, dtype=torch.uint8, device=dev) if size > 0 else None
+    src_p = None if src is None else src.data_ptr()
+    offs_p = None if offs is None else offs.data_ptr()
+    ws_p = None if ws is None else ws.data_ptr()
+    if given:
+        _lib.call("hi2x_packed_linear_activations", dev, w._ref, ctypes.byref(x.desc), src_p,
+                  offs_p, slots, ctypes.byref(epi), ws_p, size)
+    else:
+        _lib.call("hi2x_packed_linear", dev, w._ref, x.data_ptr(), dt, _pitch(x), rows, npl,
+                  src_p, offs_p, slots, ctypes.byref(epi), ws_p, size)
     return out
+
+
+def _same_device(w, what, *tensors):
+    dev = _lib.require_gpu(*tensors)
+    if dev != w.device:
+        raise RuntimeError(f"{what}: inputs are on {dev}, the weights on {w.device}")
 
 
 def _check_activations(x: Activations, w):
@@ -328,18 +338,16 @@ def packed_linear(x: torch.Tensor | Activations, w: PackedLinear, bias=None,
         raise TypeError(f"packed_linear takes a PackedLinear, got {type(w).__name__}")
     if isinstance(x, Activations):
         _check_activations(x, w)
-        lead, slots, dtype = (x.scale.numel(),), x.scale.numel(), x.dtype
+        _same_device(w, "packed_linear", x.planes, bias, mul, residual)
         _no_grad_inputs("packed_linear", bias, mul, residual)
-    else:
-        if _lib.require_gpu(x) != w.device:
-            raise RuntimeError(f"x is on {x.device}, the weights on {w.device}")
-        _no_grad_inputs("packed_linear", x, bias, mul, residual)
-        lead, dtype = tuple(x.shape[:-1]), x.dtype
-        x = _rows_of(x, w.k, "x")
-        slots = x.shape[0]
-    y = _product(w, x, None, None, slots, bias, activation, mul, residual,
-                 out_dtype or dtype, "packed_linear")
-    return y.reshape(*lead, w.n)
+        return _product(w, x, None, None, x.scale.numel(), bias, activation, mul, residual,
+                        out_dtype or x.dtype, "packed_linear")
+    _same_device(w, "packed_linear", x, bias, mul, residual)
+    _no_grad_inputs("packed_linear", x, bias, mul, residual)
+    rows = _rows_of(x, w.k, "x")
+    y = _product(w, rows, None, None, rows.shape[0], bias, activation, mul, residual,
+                 out_dtype or x.dtype, "packed_linear")
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], w.n)
 
 
 def _routed(offs, rows, w, what):
@@ -363,8 +371,7 @@ def experts_linear(x: torch.Tensor | Activations, w: PackedExperts, offs: torch.
     if not isinstance(w, PackedExperts):
         raise TypeError(f"experts_linear takes PackedExperts, got {type(w).__name__}")
     given = isinstance(x, Activations)
-    if _lib.require_gpu(offs, rows, x.planes if given else x) != w.device:
-        raise RuntimeError(f"experts_linear: inputs are not on the weights' device {w.device}")
+    _same_device(w, "experts_linear", offs, rows, x.planes if given else x, mul, residual)
     offs, rows = _routed(offs, rows, w, "experts_linear")
     _no_grad_inputs("experts_linear", None if given else x, mul, residual)
     if given:
@@ -419,8 +426,11 @@ def moe_mlp(x: torch.Tensor, routing, gate: PackedExperts, up: PackedExperts,
     if (gate.n, gate.k, gate.experts) != (up.n, up.k, up.experts) or \
             (down.k, down.n, down.experts) != (gate.n, gate.k, gate.experts):
         raise ValueError("gate and up [I, K] and down [K, I] of the same experts expected")
-    if _lib.require_gpu(x) != gate.device:
-        raise RuntimeError(f"x is on {x.device}, the experts on {gate.device}")
+    _same_device(gate, "moe_mlp", x, residual)
+    if up.device != gate.device or down.device != gate.device:
+        raise RuntimeError("gate, up and down are on different devices")
+    if routing is None:
+        raise TypeError("moe_mlp takes a Routing")
     _no_grad_inputs("moe_mlp", x, routing.weights, residual)
     act = ACTIVATIONS.get(activation)
     if act is None:
@@ -436,8 +446,7 @@ def moe_mlp(x: torch.Tensor, routing, gate: PackedExperts, up: PackedExperts,
         if residual.numel() != t * gate.k:
             raise ValueError(f"residual has shape {tuple(residual.shape)}, expected {(t, gate.k)}")
         residual = residual.contiguous()
-    if _lib.require_gpu(flat, weights, residual) != gate.device:
-        raise RuntimeError(f"moe_mlp: inputs are not on the experts' device {gate.device}")
+    _same_device(gate, "moe_mlp", weights, slots)
     dt = _dtype(x, "x")
     out = torch.empty(x.shape, dtype=x.dtype, device=gate.device)
     if not t:
