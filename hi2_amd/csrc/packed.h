@@ -309,13 +309,12 @@ __device__ __forceinline__ void load16(const void* x, int64_t at, int dtype, flo
   }
 }
 
-// Whether a product goes to packed_few: its rows fit one operand.  A wave of it walks an
-// eighth of the columns alone: 4096 x 14336 at 16 rows took 33 us so and 23 us in 64 x 64
-// tiles with the columns in eight shares, 4096 x 4096 13 and 14, 14336 x 4096 16 and 20,
-// 28672 x 8192 34 and 43.  Experts' rows take tiles: a layer of 64 experts at 64 tokens,
-// eight each, took 315 us so and 128 us in tiles.
-inline bool few_rows_product(const hi2x_packed& w, int64_t slots, bool ranges) {
-  return !ranges && slots <= 16 && (w.kp <= 8192 || w.max_frags >= 512);
+// Whether a product goes to packed_few: its rows fit one operand (4096 x 14336 at 16 rows
+// takes 20 us so, 23 in 64 x 64 tiles with the columns in eight shares; 28672 x 8192 30 and
+// 43).  Experts' rows take tiles: a layer of 64 experts at 64 tokens, eight each, took 315 us
+// so and 128 us in tiles.
+inline bool few_rows_product(const hi2x_packed&, int64_t slots, bool ranges) {
+  return !ranges && slots <= 16;
 }
 
 constexpr int64_t FEW_RAW = 8;      // rows the few-rows kernel transforms for itself,

@@ -83,20 +83,21 @@ __device__ __forceinline__ void group_values(const RawRows& x, int64_t base, int
   }
 }
 
-// TPR threads transform a row, 256 / TPR rows to a workgroup.  The largest finite |x / s| comes first; the rotation can
+// TPR threads transform a row, several rows to a workgroup of 256 where that leaves room.  The largest finite |x / s| comes first; the rotation can
 // grow it fourfold at most, so 2^(13 - exponent) brings every value to at most 2^15, with
 // nothing of the row below fp16's normal range unless it is 2^-27 of the largest.  Then the
 // values are scaled (exact), rotated by butterflies in f32 and rounded to fp16.  That
 // rounding (2^-12 of each value, independent) is below the output's own for bf16 and as
 // large as fp16's; nplanes 2 keeps the rest of it in a second plane.  A thread keeps its
-// group's values between the two where one group a thread is all there is (KEEP, 4096
+// group's values between the two where one group a thread is all there is (KEEP, up to 16384
 // columns); rows beyond are read twice, the second time from L2.
 template <int DT, bool GLU, bool KEEP, int TPR>
-__global__ __launch_bounds__(256) void activations_kernel(
+__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void activations_kernel(
     RawRows x, int64_t k, const int64_t* __restrict__ src, const uint8_t* __restrict__ had,
     const uint16_t* __restrict__ cs, const int64_t* __restrict__ offs, int experts,
     hi2x_activations out) {
-  const int64_t row = (int64_t)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+  constexpr int NT = TPR > 256 ? TPR : 256;
+  const int64_t row = (int64_t)blockIdx.x * (NT / TPR) + threadIdx.x / TPR;
   const int tid = threadIdx.x % TPR;
   const bool none = row >= out.rows;
   const int64_t from = none ? -1 : (src ? src[row] : row);
@@ -131,11 +132,12 @@ __global__ __launch_bounds__(256) void activations_kernel(
 #pragma unroll
   for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
   if constexpr (TPR > 64) {
-    __shared__ float red[4];
-    const int w = threadIdx.x >> 6;
+    __shared__ float red[NT / 64];
+    const int w = threadIdx.x >> 6, w0 = w - (tid >> 6);  // the row's waves
     if ((tid & 63) == 0) red[w] = m;
     __syncthreads();
-    m = TPR == 128 ? fmaxf(red[w & 2], red[w | 1]) : fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+#pragma unroll
+    for (int i = 0; i < TPR / 64; ++i) m = fmaxf(m, red[w0 + i]);
   }
   if (none) return;
   int ex = 0;
@@ -193,8 +195,9 @@ int launch_activations(const RawRows& x, const hi2x_packed& w, const int64_t* sr
                        const int64_t* offs, const hi2x_activations& out, hipStream_t s) {
 #define HI2X_ROWS_(DT, GLU, KEEP, TPR)                                                    \
   activations_kernel<DT, GLU, KEEP, TPR>                                                  \
-      <<<dim3((unsigned)((out.rows * TPR + 255) / 256)), 256, 0, s>>>(                    \
-          x, w.k, src, w.had, w.col_scale, offs, (int)w.experts, out)
+      <<<dim3((unsigned)(TPR < 256 ? (out.rows * TPR + 255) / 256 : out.rows)),           \
+         TPR < 256 ? 256 : TPR, 0, s>>>(x, w.k, src, w.had, w.col_scale, offs,            \
+                                        (int)w.experts, out)
 #define HI2X_ROWS(DT, GLU)                 \
   if (w.kp <= 1024)                        \
     HI2X_ROWS_(DT, GLU, true, 64);         \
@@ -202,8 +205,12 @@ int launch_activations(const RawRows& x, const hi2x_packed& w, const int64_t* sr
     HI2X_ROWS_(DT, GLU, true, 128);        \
   else if (w.kp <= 4096)                   \
     HI2X_ROWS_(DT, GLU, true, 256);        \
+  else if (w.kp <= 8192)                   \
+    HI2X_ROWS_(DT, GLU, true, 512);        \
+  else if (w.kp <= 16384)                  \
+    HI2X_ROWS_(DT, GLU, true, 1024);       \
   else                                     \
-    HI2X_ROWS_(DT, GLU, false, 256);
+    HI2X_ROWS_(DT, GLU, false, 1024);
   if (x.x2) {
     HI2X_ROWS(0, true)
   } else if (x.dtype == 0) {

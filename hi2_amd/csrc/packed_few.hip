@@ -172,7 +172,8 @@ __device__ __forceinline__ void few_loop(const FewArgs& a, const GemmArgs& g, co
   constexpr int CP = 8 / MP;
   // what the registers hold: 128 with eight waves, of which a CU takes two workgroups
   constexpr int RU = BITS == 8 ? 1 : (MODE != RAW16 || FW == 8 ? 2 : 4);
-  constexpr int UN = RAW ? (CP < RU ? CP : RU) : (FR * MF <= 2 ? 2 : 1);
+  constexpr int UN = RAW ? (CP < RU ? CP : RU) : (FR == 1 && BITS < 8 ? 2 : 1);
+  constexpr bool AHEAD = RAW || BITS < 8 || FR == 1;
   const int k = (int)g.w.k;
   const int tid = threadIdx.x, lane = tid & 63, q = lane >> 4, col = lane & 15;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -252,9 +253,12 @@ __device__ __forceinline__ void few_loop(const FewArgs& a, const GemmArgs& g, co
     xr = t < MP ? plane * MP + t : 0;
     from = t < MP ? t * (64 / MP) : 0;
   }
-  fetch(0, nxt);
+  if constexpr (AHEAD) fetch(0, nxt);
   for (int s0 = 0; s0 < steps; s0 += UN) {
-    cur = nxt;
+    if constexpr (AHEAD)
+      cur = nxt;
+    else
+      fetch(s0, cur);
     if constexpr (RAW) {
       if (s0 % CP == 0) {
         fetch(s0 + UN, nxt);
@@ -266,7 +270,7 @@ __device__ __forceinline__ void few_loop(const FewArgs& a, const GemmArgs& g, co
       } else {
         fetch(s0 + UN, nxt);
       }
-    } else {
+    } else if constexpr (AHEAD) {
       fetch(s0 + UN, nxt);
     }
 #pragma unroll
@@ -308,7 +312,7 @@ __device__ __forceinline__ void few_loop(const FewArgs& a, const GemmArgs& g, co
 
 template <int FR, int MT, int MODE, int FW>
 __global__ __launch_bounds__(
-    64 * FW, MODE == GIVEN ? 1 : (MODE != RAW16 ? 2 : (FW == 8 ? 4 : 3))) void packed_few_kernel(FewArgs a) {
+    64 * FW, MODE == GIVEN ? 4 : (MODE != RAW16 ? 2 : (FW == 8 ? 4 : 3))) void packed_few_kernel(FewArgs a) {
   constexpr bool RAW = MODE != GIVEN;
   constexpr int MF = RAW ? 1 : MT / 16;
   constexpr int XW = RAW ? 4096 : 0;         // bytes of transformed rows of a wave
@@ -448,10 +452,14 @@ int launch_one(const FewArgs& a, int count, int64_t frags, hipStream_t s) {
 int packed_few(const GemmPair& g, int count, hipStream_t s) {
   FewArgs a{};
   a.two = g;
+  // More fragments a wave share their activation reads, while there are workgroups enough:
+  // at 16 rows 28672 x 8192 takes 29.9 us with four, 37.6 with two and 61 with one, 8192 x
+  // 8192 18.0 and 21.2, 4096 x 4096 11.6, 9.2 and 11.3, 1024 x 4096 8.4 with one and 10.4
+  // with two.
   const int64_t frags = g.g[0].w.max_frags;
-  return frags >= 1024 ? launch<4, 16, GIVEN, 8>(a, count, s)
-                       : (frags >= 512 ? launch<2, 16, GIVEN, 8>(a, count, s)
-                                       : launch<1, 16, GIVEN, 8>(a, count, s));
+  return frags >= 512 ? launch<4, 16, GIVEN, 8>(a, count, s)
+                      : (frags >= 192 ? launch<2, 16, GIVEN, 8>(a, count, s)
+                                      : launch<1, 16, GIVEN, 8>(a, count, s));
 }
 
 int packed_few_raw(const GemmPair& g, int count, const RawRows& x, hipStream_t s) {

@@ -57,15 +57,17 @@ class _Weights(torch.autograd.Function):
     """The weights' gradient to the logits (``hi2x_route_backward``)."""
 
     @staticmethod
-    def forward(ctx, logits, weights, index, args):
-        ctx.save_for_backward(logits, index)
+    def forward(ctx, logits, routed, args):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(logits, routed[1])
         ctx.args = args
-        ctx.mark_dirty(weights)
-        return weights
+        return routed[0]
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
+        if grad is None:
+            return None, None, None
         logits, index = ctx.saved_tensors
         scoring, renormalise, scale = ctx.args
         t, e = logits.shape
@@ -77,7 +79,7 @@ class _Weights(torch.autograd.Function):
                       _FLOATS[logits.dtype], logits.stride(0) if t > 1 else e, t, e,
                       index.shape[1], scoring, renormalise, scale, index.data_ptr(),
                       grad.data_ptr(), d.data_ptr())
-        return d, None, None, None
+        return d, None, None
 
 
 def route(logits: torch.Tensor, top_k: int, scoring: str = "softmax", bias=None,
@@ -126,7 +128,7 @@ def route(logits: torch.Tensor, top_k: int, scoring: str = "softmax", bias=None,
               offs.data_ptr(), slots.data_ptr(), _lib.ptr(ws), max(size, 0))
     if logits.requires_grad and torch.is_grad_enabled():
         weights = _Weights.apply(logits if x.data_ptr() == logits.data_ptr() else
-                                 logits.contiguous(), weights, index,
+                                 logits.contiguous(), (weights, index),
                                  (SCORING[scoring], int(renormalise), float(scale)))
     return Routing(index, weights, rows, offs, slots)
 
