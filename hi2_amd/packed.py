@@ -42,6 +42,10 @@ CLASSES = [(nb, b) for nb in (2, 4, 8) for b in (16, 32, 64)]
 DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 
+_CLASS_AT = np.full((256, 256), -1, np.int64)  # class of [nbits, block]
+for _i, (_nb, _b) in enumerate(CLASSES):
+    _CLASS_AT[_nb, _b] = _i
+
 _SEGMENT = np.dtype([("codes", np.int64), ("params", np.int64), ("frag0", np.int32),
                      ("frags", np.int32), ("nbits", np.int32), ("block", np.int32)])
 
@@ -51,14 +55,13 @@ def _classes_of(t: HI2Tensor, what: str) -> np.ndarray:
     r, k = t.shape
     if k % GROUP or k < GROUP or r < 1:
         raise ValueError(f"{what}: shape {tuple(t.shape)} (columns a multiple of {GROUP})")
-    nb = t.row_nbits.cpu().numpy().astype(np.int64)
-    blk = t.row_block.cpu().numpy().astype(np.int64)
-    if nb.shape != (r,) or blk.shape != (r,):
-        raise ValueError(f"{what}: {nb.size} row widths and {blk.size} blocks for {r} rows")
-    cls = np.full(r, -1, np.int64)
-    for i, (b, w) in enumerate(CLASSES):
-        cls[(nb == b) & (blk == w)] = i
-    if (cls < 0).any():
+    nb8, blk8 = t.row_nbits.cpu().numpy(), t.row_block.cpu().numpy()
+    if nb8.shape != (r,) or blk8.shape != (r,):
+        raise ValueError(f"{what}: {nb8.size} row widths and {blk8.size} blocks for {r} rows")
+    nb, blk = nb8.astype(np.int64), blk8.astype(np.int64)
+    cls = _CLASS_AT[nb, blk] if 0 <= min(nb.min(), blk.min()) and \
+        max(nb.max(), blk.max()) < 256 else np.full(r, -1)
+    if cls.min() < 0:
         at = int(np.argmax(cls < 0))
         raise ValueError(f"{what}: row {at} is INT{nb[at]} in blocks of {blk[at]}")
     if (k % blk).any():
@@ -111,9 +114,13 @@ class _Packed:
             cls = _classes_of(t, "tensor" if e == 1 else f"expert {i}")
             first = frag
             cut = np.zeros(3, np.int64)
-            for c in np.unique(cls):
+            order = np.argsort(cls, kind="stable").astype(np.int32)
+            ends = np.cumsum(np.bincount(cls, minlength=len(CLASSES)))
+            for c in range(len(CLASSES)):
+                rows = order[ends[c - 1] if c else 0:ends[c]]
+                if not rows.size:
+                    continue
                 nb, blk = CLASSES[c]
-                rows = np.flatnonzero(cls == c).astype(np.int32)
                 f = -(-rows.size // FRAG)
                 slot_rows += [rows, np.full(f * FRAG - rows.size, -1, np.int32)]
                 segs[i, c] = (codes_at, params_at, frag, f, nb, blk)
@@ -143,9 +150,15 @@ class _Packed:
                             for t, a in zip(tensors, po)])])
         offs = _lib.h2d(torch.from_numpy(offs), dev)
         # the transform: one for all where every expert has the same
-        had = [t.had.reshape(-1).cpu().to(torch.uint8).numpy() for t in tensors]
-        cs = [None if t.col_scale is None else
-              t.col_scale.reshape(-1).cpu().to(torch.float16).numpy() for t in tensors]
+        seen: dict = {}  # experts often share the tensors themselves (all alive here)
+
+        def host(v, dtype):
+            if v is not None and id(v) not in seen:
+                seen[id(v)] = v.reshape(-1).cpu().to(dtype).numpy()
+            return None if v is None else seen[id(v)]
+
+        had = [host(t.had, torch.uint8) for t in tensors]
+        cs = [host(t.col_scale, torch.float16) for t in tensors]
         if any(c is None for c in cs) and not all(c is None for c in cs):
             cs = [np.ones(k, np.float16) if c is None else c for c in cs]
         keys = [(h.astype(bool).tobytes(), b"" if c is None else c.tobytes())
