@@ -283,6 +283,13 @@ __device__ __forceinline__ void load_codes(__amdgpu_buffer_rsrc_t rs, int lane, 
   }
 }
 
+// What fp16 `h` leaves of v, as fp16: the second plane's value.  Infinities are whole in the
+// first (their difference, a NaN, would take the product's sign).
+__device__ __forceinline__ uint32_t rest_bits(float v, uint32_t h) {
+  const float r = v - f16_from_bits((uint16_t)h);
+  return f16_bits(r == r ? r : 0.0f);
+}
+
 // 16 neighbouring activations, 16-byte aligned.
 __device__ __forceinline__ void load16(const void* x, int64_t at, int dtype, float (&v)[16]) {
   if (dtype == 0) {

@@ -180,8 +180,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void activations_kernel(
     if (out.nplanes == 2) {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        h[i] = (uint32_t)f16_bits(v[2 * i] - f16_from_bits((uint16_t)h[i])) |
-               (uint32_t)f16_bits(v[2 * i + 1] - f16_from_bits((uint16_t)(h[i] >> 16))) << 16;
+        h[i] = rest_bits(v[2 * i], h[i]) | rest_bits(v[2 * i + 1], h[i] >> 16) << 16;
       d = reinterpret_cast<u32x4*>(at + PK_CHUNK);
       d[0] = u32x4{h[0], h[1], h[2], h[3]};
       d[1] = u32x4{h[4], h[5], h[6], h[7]};

@@ -147,8 +147,7 @@ struct FewPass {
       const int r2 = MP + r;
 #pragma unroll
       for (int t = 0; t < 8; ++t)
-        h[t] = (uint32_t)f16_bits(v[2 * t] - f16_from_bits((uint16_t)h[t])) |
-               (uint32_t)f16_bits(v[2 * t + 1] - f16_from_bits((uint16_t)(h[t] >> 16))) << 16;
+        h[t] = rest_bits(v[2 * t], h[t]) | rest_bits(v[2 * t + 1], h[t] >> 16) << 16;
       d = xl + (chunk * R + r2) * 256;
       *reinterpret_cast<u32x4*>(d + 16 * (p0 ^ r2)) = u32x4{h[0], h[1], h[2], h[3]};
       *reinterpret_cast<u32x4*>(d + 16 * ((p0 + 1) ^ r2)) = u32x4{h[4], h[5], h[6], h[7]};
