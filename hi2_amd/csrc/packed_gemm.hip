@@ -24,14 +24,14 @@ constexpr int waitcnt(int vm, int lgkm) {
 }
 
 // The main loop of one tile: 4 waves of NF fragments x 16 MF slots each, all reading the
-// same activations from LDS.  A stage of 16 MF slots x 128 columns is 256 bytes a slot in
+// same activations from LDS, in a workgroup's accumulators of AF x AM.  A stage of 16 MF slots x 128 columns is 256 bytes a slot in
 // 16 pieces; piece p of slot t lies at p ^ (t % 16), so that the 16 slots a fragment read
 // touches at one piece fall on different banks.
-template <int BITS, bool B16, int NF, int MF>
+template <int BITS, bool B16, int NF, int MF, int AF, int AM>
 __device__ __forceinline__ void gemm_loop(const GemmArgs& g, const Tile& tile, char* lds,
                                           const char* xb, int64_t xbytes,
-                                          const uint32_t (&xoff)[MF], int c0, int c1,
-                                          f32x4v (&acc)[NF][MF]) {
+                                          const uint32_t (&xoff)[AM], int c0, int c1,
+                                          f32x4v (&acc)[AF][AM]) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int q = lane >> 4;
@@ -236,6 +236,33 @@ __device__ __forceinline__ int slot_row(const GemmArgs& g, const Tile& tile, int
              : -1;
 }
 
+// The least of MOST, its half and its quarter that holds n.
+template <int MOST>
+__device__ __forceinline__ int share_of(int n) {
+  if (MOST >= 4 && n <= MOST / 4) return MOST / 4;
+  return MOST >= 2 && n <= MOST / 2 ? MOST / 2 : MOST;
+}
+
+// The loop for the tile's own nf fragments a wave and 16 mf rows: an expert's last rows and a
+// class's last fragments fill a tile in part only, and most tiles of a small batch are such
+// (64 experts, 8 choices: 64 tokens 127 us in whole tiles and 107 so, 2048 tokens 433 and
+// 417).  (128 x 64 tiles share by rows alone: both would not fit their registers.)
+template <int BITS, bool B16, int N, int M, int NF, int MF>
+__device__ __forceinline__ void sized_loop(const GemmArgs& g, const Tile& tile, char* lds,
+                                           const char* xb, int64_t xbytes,
+                                           const uint32_t (&xoff)[MF], int nf, int mf, int c0,
+                                           int c1, f32x4v (&acc)[NF][MF]) {
+  if constexpr (NF != 2 && N > 1 && 4 * N > NF) {
+    if (nf < N)
+      return sized_loop<BITS, B16, N / 2, M>(g, tile, lds, xb, xbytes, xoff, nf, mf, c0, c1, acc);
+  }
+  if constexpr (M > 1 && 4 * M > MF) {
+    if (mf < M)
+      return sized_loop<BITS, B16, N, M / 2>(g, tile, lds, xb, xbytes, xoff, nf, mf, c0, c1, acc);
+  }
+  gemm_loop<BITS, B16, N, M>(g, tile, lds, xb, xbytes, xoff, c0, c1, acc);
+}
+
 // One workgroup: 64 NF slots of w's layout (one segment) x 16 MF activation rows, over all
 // columns or (SPLIT) the blockIdx.z-th share of their chunks.  A split's sums go to `part` as
 // the accumulators hold them.
@@ -257,6 +284,8 @@ __global__ __launch_bounds__(256, NF == 4 ? 2 : 4) void packed_gemm_kernel(GemmP
   int live;
   if (!find<NF, MF>(g, nx, tile, first, live)) return;
   const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  const int nf = SPLIT || NF == 2 ? NF : share_of<NF>((tile.count + 3) / 4);
+  const int mf = SPLIT ? MF : share_of<MF>((live + 15) / 16);
   // Where the rows this lane stages begin.  Rows past the end read zeros or another
   // tile's, and are not stored; indices outside the activations read row 0 (and come out as
   // NaN below).  Without src the resource begins at the tile's own rows.
@@ -267,7 +296,7 @@ __global__ __launch_bounds__(256, NF == 4 ? 2 : 4) void packed_gemm_kernel(GemmP
   const int64_t xbytes = (g.x.rows - row0) * pitch;
 #pragma unroll
   for (int i = 0; i < MF; ++i) {
-    const int t = 4 * (wv * MF + i) + (lane >> 4);
+    const int t = 4 * (wv * mf + i) + (lane >> 4);
     int64_t r = t;
     if (g.src) {
       r = t < live ? g.src[first + t] : 0;
@@ -284,20 +313,25 @@ __global__ __launch_bounds__(256, NF == 4 ? 2 : 4) void packed_gemm_kernel(GemmP
   for (int f = 0; f < NF; ++f)
 #pragma unroll
     for (int m = 0; m < MF; ++m) acc[f][m] = f32x4v{0.0f, 0.0f, 0.0f, 0.0f};
-#define HI2X_LOOP(BITS)                                                                \
-  if (tile.block == 16)                                                             \
-    gemm_loop<BITS, true, NF, MF>(g, tile, lds, xb, xbytes, xoff, c0, c1, acc);        \
-  else                                                                                 \
-    gemm_loop<BITS, false, NF, MF>(g, tile, lds, xb, xbytes, xoff, c0, c1, acc);
-  switch (tile.nbits) {
-    case 2:
-      HI2X_LOOP(2)
-      break;
+#define HI2X_LOOP(BITS, B16)                                                                \
+  if constexpr (SPLIT)                                                                    \
+    gemm_loop<BITS, B16, NF, MF>(g, tile, lds, xb, xbytes, xoff, c0, c1, acc);            \
+  else                                                                                    \
+    sized_loop<BITS, B16, NF, MF>(g, tile, lds, xb, xbytes, xoff, nf, mf, c0, c1, acc);   \
+  break;
+  switch (2 * tile.nbits + (tile.block == 16)) {
     case 4:
-      HI2X_LOOP(4)
-      break;
+      HI2X_LOOP(2, false)
+    case 5:
+      HI2X_LOOP(2, true)
+    case 8:
+      HI2X_LOOP(4, false)
+    case 9:
+      HI2X_LOOP(4, true)
+    case 16:
+      HI2X_LOOP(8, false)
     default:
-      HI2X_LOOP(8)
+      HI2X_LOOP(8, true)
   }
 #undef HI2X_LOOP
   if constexpr (SPLIT) {
@@ -315,13 +349,15 @@ __global__ __launch_bounds__(256, NF == 4 ? 2 : 4) void packed_gemm_kernel(GemmP
   const float bias = g.epi.bias && n >= 0 ? load_as_f32(g.epi.bias, n, g.epi.dt_bias) : 0.0f;
 #pragma unroll
   for (int p = 0; p < MT / EH; ++p) {
+    if (p * EH >= live) break;
     __syncthreads();
 #pragma unroll
     for (int m = 0; m < EH / 16; ++m)
 #pragma unroll
       for (int f = 0; f < NF; ++f)
-        *reinterpret_cast<f32x4v*>(ep + (16 * m + (lane & 15)) * PITCH + (wv * NF + f) * 16 +
-                                   4 * (lane >> 4)) = acc[f][p * (EH / 16) + m];
+        if (f < nf)
+          *reinterpret_cast<f32x4v*>(ep + (16 * m + (lane & 15)) * PITCH + (wv * nf + f) * 16 +
+                                     4 * (lane >> 4)) = acc[f][p * (EH / 16) + m];
     __syncthreads();
     store_pass<NS, PITCH, EH, 8>(g.epi, ep, xscale + p * EH, n, bias, first + p * EH,
                                  live - p * EH < EH ? live - p * EH : EH);
