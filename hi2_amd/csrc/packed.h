@@ -89,6 +89,30 @@ __device__ __forceinline__ float activate(float y, int act) {
   }
 }
 
+// The same of several values, the choice made once.
+template <int N>
+__device__ __forceinline__ void activate_all(float (&y)[N], int act) {
+#define HI2X_EACH(A)                                   \
+  _Pragma("unroll") for (int i = 0; i < N; ++i) y[i] = activate(y[i], A);
+  switch (act) {
+    case HI2X_ACT_RELU:
+      HI2X_EACH(HI2X_ACT_RELU)
+      break;
+    case HI2X_ACT_SILU:
+      HI2X_EACH(HI2X_ACT_SILU)
+      break;
+    case HI2X_ACT_GELU:
+      HI2X_EACH(HI2X_ACT_GELU)
+      break;
+    case HI2X_ACT_GELU_TANH:
+      HI2X_EACH(HI2X_ACT_GELU_TANH)
+      break;
+    default:
+      break;
+  }
+#undef HI2X_EACH
+}
+
 // The steps s of a chunk's weights from a lane's codes, as the MFMA's A operand: fp16
 // (lo + code step) with one rounding, which is the format's own decode.  A dword holds its
 // codes as pairs (bits f and 16 + f), so masking one pair leaves two codes in the
@@ -187,6 +211,8 @@ __device__ __forceinline__ PkWork find_work(const int64_t* offs, int experts, in
   return w;
 }
 
+// `scaled16`: the result is handed on in fp16 without its row's factor and times 2^-c of
+// sum_exponent, for a kernel that reads it with a RowFactor.
 struct GemmArgs {
   hi2x_packed w;
   hi2x_activations x;
@@ -194,7 +220,30 @@ struct GemmArgs {
   const int64_t* offs;
   int64_t slots;
   hi2x_epilogue epi;
+  bool scaled16 = false;
 };
+
+// c with |sum| < 2^15 2^c for any row's product with k weights: its activations are at most
+// 2^15, the weights *largest.
+__device__ __forceinline__ int sum_exponent(const float* largest, int64_t k) {
+  const float most = *largest * (float)k;
+  int c = 0;
+  if (most > 0.0f) (void)frexpf(most, &c);
+  return c;
+}
+
+// What takes rows of a scaled16 product back: 2^c and the factor of the row's activations.
+struct RowFactor {
+  const float* scale = nullptr;  // null: the rows are as they are
+  const int64_t* index = nullptr;
+  int64_t rows = 0;  // of scale
+  const float* largest = nullptr;
+  int64_t k = 0;
+};
+__device__ __forceinline__ float row_factor(const RowFactor& f, int64_t row) {
+  const int64_t r = f.index ? f.index[row] : row;
+  return r >= 0 && r < f.rows ? f.scale[r] : __builtin_nanf("");
+}
 
 // Loads go through buffer resources: a lane's offset is one 32-bit register, the walk along
 // the columns is a scalar offset, and what lies past the resource reads as zero.
@@ -327,15 +376,16 @@ inline bool few_rows_product(const hi2x_packed&, int64_t slots, bool ranges) {
 constexpr int64_t FEW_RAW = 8;      // rows the few-rows kernel transforms for itself,
 constexpr int64_t FEW_RANGES = 16;  // and of all experts together
 
-// Activations as they are: rows ldx elements apart; with x2 (same type and pitch, 32 bits)
-// act(x) * x2 elementwise.
+// Activations as they are: rows ldx elements apart; with x2 (same type and pitch, 32 bits or
+// scaled16) act(x) * x2 elementwise.
 struct RawRows {
   const void* x;
   int dtype;
   int64_t ldx, rows;
   int npl;  // planes of their transform
-  const float* x2 = nullptr;
+  const void* x2 = nullptr;
   int act = 0;
+  RowFactor f1, f2;  // dtype 1 with x2: of both
 };
 
 // Products of `count` (1 or 2) tensors of one shape from the same activations; the epilogue's
@@ -349,9 +399,9 @@ int packed_product(const GemmPair& g, int count, void* work, int64_t work_bytes,
 int64_t packed_part_bytes(const hi2x_packed& w, int64_t slots, bool ranges, int npl);
 int launch_activations(const RawRows& x, const hi2x_packed& w, const int64_t* src,
                        const int64_t* offs, const hi2x_activations& out, hipStream_t s);
-int launch_combine(const void* y, int dt_y, int64_t y_rows, int64_t n, const int64_t* slots,
-                   const float* weights, int64_t t, int64_t top_k, const void* residual,
-                   int dt_residual, void* out, int dt_out, hipStream_t s);
+int launch_combine(const void* y, int dt_y, const RowFactor& f, int64_t y_rows, int64_t n,
+                   const int64_t* slots, const float* weights, int64_t t, int64_t top_k,
+                   const void* residual, int dt_residual, void* out, int dt_out, hipStream_t s);
 
 // Whether a product takes its activations as they are and transforms them inside.  Of
 // experts most have one row then: at 64 experts and 8 choices, two tokens 62 us so and 74 in

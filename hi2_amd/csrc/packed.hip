@@ -17,6 +17,7 @@ __global__ __launch_bounds__(256) void layout_codes_kernel(hi2x_packed w,
   const int64_t e = blockIdx.y / PK_SEGS;
   const int64_t nch = w.kp / PK_CHUNK;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i == 0 && blockIdx.y == 0) *w.largest = 0.0f;  // (layout_params_kernel comes next)
   if (i >= sg.frags * nch * 64) return;
   const int lane = (int)(i & 63);
   const int64_t c = (i >> 6) % nch, f = (i >> 6) / nch;
@@ -49,10 +50,11 @@ __global__ __launch_bounds__(256) void layout_params_kernel(
   const int64_t e = blockIdx.y / PK_SEGS;
   const int64_t nblk = w.kp / sg.block;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= sg.frags * nblk * 16) return;
+  const bool in = i < sg.frags * nblk * 16;
   const int64_t b = (i >> 4) % nblk, f = (i >> 4) / nblk;
-  const int row = w.rows[(sg.frag0 + f) * 16 + (i & 15)];
+  const int row = in ? w.rows[(sg.frag0 + f) * 16 + (i & 15)] : -1;
   uint32_t v = 0;
+  float most = 0.0f;  // of |weight|: at the first or the last step of a ladder
   if (row >= 0 && b < w.k / sg.block) {
     const int64_t r = e * w.n + row;
     const uint8_t* p = params + 2 * (param_off[r] + b);
@@ -60,22 +62,40 @@ __global__ __launch_bounds__(256) void layout_params_kernel(
                                     f16_from_bits(consts[3 * r]));
     const float st = (float)p[1] * f16_from_bits(consts[3 * r + 2]);
     v = (uint32_t)f16_bits(lo) | (uint32_t)f16_bits(st) << 16;
+    const float l = f16_from_bits((uint16_t)v), steps = (float)((1 << sg.nbits) - 1);
+    const float h = f16_from_bits(f16_bits(__builtin_fmaf(steps, f16_from_bits(v >> 16), l)));
+    most = fmaxf(fabsf(l), fabsf(h));
+    most = most < __builtin_inff() ? most : 0.0f;
   }
-  reinterpret_cast<uint32_t*>(static_cast<char*>(w.params) + sg.params)[i] = v;
+  if (in) reinterpret_cast<uint32_t*>(static_cast<char*>(w.params) + sg.params)[i] = v;
+#pragma unroll
+  for (int d = 32; d; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
+  unsigned* to = reinterpret_cast<unsigned*>(w.largest);  // non-negative floats, by their bits
+  if ((threadIdx.x & 63) == 0 &&
+      __float_as_uint(most) > __hip_atomic_load(to, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT))
+    atomicMax(to, __float_as_uint(most));
 }
 
 // ---- activations -------------------------------------------------------------------------
 // The 16 values of group g of a row, divided by their smoothing: of x, or (GLU) of
 // act(x) * x2.
 template <int DT, bool GLU>
-__device__ __forceinline__ void group_values(const RawRows& x, int64_t base, int g,
-                                             const uint16_t* cs, float (&v)[16]) {
+__device__ __forceinline__ void group_values(const RawRows& x, const float (&rf)[4], int64_t base,
+                                             int g, const uint16_t* cs, float (&v)[16]) {
   load16(x.x, base + 16 * (int64_t)g, DT, v);
   if constexpr (GLU) {
     float u[16];
-    load16(x.x2, base + 16 * (int64_t)g, 0, u);
+    load16(x.x2, base + 16 * (int64_t)g, DT, u);
+    if constexpr (DT == 1) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = activate(v[i], x.act) * u[i];
+      for (int i = 0; i < 16; ++i) {
+        v[i] = v[i] * rf[0] * rf[1];
+        u[i] = u[i] * rf[2] * rf[3];
+      }
+    }
+    activate_all(v, x.act);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] *= u[i];
   }
   if (cs) {
 #pragma unroll
@@ -116,12 +136,21 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void activations_kernel(
     if (cs) cs += (int64_t)lo * k;
   }
   const int groups = (int)(k / 16), all = (int)(out.kp / 16);
+  float rf[4] = {};  // 2^c and factor of the rows of x and x2
+  if constexpr (GLU && DT == 1) {
+    if (!bad) {
+      rf[0] = ldexpf(1.0f, sum_exponent(x.f1.largest, x.f1.k));
+      rf[1] = row_factor(x.f1, from);
+      rf[2] = ldexpf(1.0f, sum_exponent(x.f2.largest, x.f2.k));
+      rf[3] = row_factor(x.f2, from);
+    }
+  }
   float v[16], m = 0.0f;
 #pragma unroll
   for (int i = 0; i < 16; ++i) v[i] = 0.0f;
   if (!bad) {
     for (int g = tid; g < groups; g += TPR) {
-      group_values<DT, GLU>(x, base, g, cs, v);
+      group_values<DT, GLU>(x, rf, base, g, cs, v);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const float a = fabsf(v[i]);
@@ -152,7 +181,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void activations_kernel(
 #pragma unroll
       for (int i = 0; i < 16; ++i) v[i] = 0.0f;
     } else {
-      if constexpr (!KEEP) group_values<DT, GLU>(x, base, g, cs, v);
+      if constexpr (!KEEP) group_values<DT, GLU>(x, rf, base, g, cs, v);
 #pragma unroll
       for (int i = 0; i < 16; ++i) v[i] *= sc;
       if (had[g]) {
@@ -210,7 +239,9 @@ int launch_activations(const RawRows& x, const hi2x_packed& w, const int64_t* sr
     HI2X_ROWS_(DT, GLU, true, 1024);       \
   else                                     \
     HI2X_ROWS_(DT, GLU, false, 1024);
-  if (x.x2) {
+  if (x.x2 && x.dtype == 1) {
+    HI2X_ROWS(1, true)
+  } else if (x.x2) {
     HI2X_ROWS(0, true)
   } else if (x.dtype == 0) {
     HI2X_ROWS(0, false)
@@ -234,6 +265,7 @@ extern "C" int hi2x_packed_layout(const hi2x_packed* w, const int32_t* codes,
                                   void* stream) {
   clear_error();
   if (int rc = check_packed(w, "packed_layout")) return rc;
+  HI2X_REQUIRE(w->largest, "packed_layout: null buffer");
   HI2X_REQUIRE(codes && code_off && blk_params && param_off && row_consts,
                "packed_layout: null buffer");
   const hipStream_t s = as_stream(stream);

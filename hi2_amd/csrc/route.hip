@@ -474,50 +474,69 @@ __global__ __launch_bounds__(256) void route_backward_kernel(
   }
 }
 
-// out[t] = residual[t] + sum_j w[t][j] y[slots[t][j]]: a workgroup per token, four columns
-// per thread and step.  Bound by reading y once.
-template <int DT>
-__device__ __forceinline__ f32x4v load4(const void* p, int64_t at) {
-  if constexpr (DT == 0) {
-    return *reinterpret_cast<const f32x4v*>(static_cast<const float*>(p) + at);
-  } else {
-    const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + at);
-    const uint16_t h[4] = {(uint16_t)u.x, (uint16_t)(u.x >> 16), (uint16_t)u.y,
-                           (uint16_t)(u.y >> 16)};
-    f32x4v r;
+// out[t] = residual[t] + sum_j w[t][j] y[slots[t][j]]: 64, 128 or 256 threads (TPT) on a
+// token, 16 bytes of a row of y at a time, four rows in flight.  Bound by reading y once.
+template <int DT, int V>
+struct Piece {  // V neighbouring values of y
+  static constexpr int W = V == 1 ? 1 : V * (DT == 0 ? 4 : 2) / 4;
+  uint32_t u[W];
+  __device__ __forceinline__ void load(const void* p, int64_t at) {
+    if constexpr (V == 1) {
+      if constexpr (DT == 0)
+        u[0] = static_cast<const uint32_t*>(p)[at];
+      else
+        u[0] = static_cast<const uint16_t*>(p)[at];
+    } else {
+      const u32x4 v = *reinterpret_cast<const u32x4*>(static_cast<const char*>(p) +
+                                                      at * (DT == 0 ? 4 : 2));
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      r[i] = DT == 1 ? f16_from_bits(h[i]) : __uint_as_float((uint32_t)h[i] << 16);
-    return r;
+      for (int i = 0; i < 4; ++i) u[i] = v[i];
+    }
   }
-}
+  __device__ __forceinline__ float operator[](int i) const {
+    if constexpr (DT == 0) return __uint_as_float(u[i]);
+    const uint32_t h = V == 1 ? u[0] : u[i >> 1] >> (16 * (i & 1));
+    if constexpr (DT == 1) return f16_from_bits((uint16_t)h);
+    return __uint_as_float(h << 16);
+  }
+};
 
 template <int DT, int V>
 __global__ __launch_bounds__(256) void combine_kernel(
-    const void* __restrict__ y, int64_t y_rows, int64_t n, const int64_t* __restrict__ slots,
-    const float* __restrict__ weights, int k, const void* __restrict__ residual, int dt_res,
-    void* __restrict__ out, int dt_out) {
-  const int64_t t = blockIdx.x;
-  for (int64_t c = ((int64_t)blockIdx.y * 256 + threadIdx.x) * V; c < n;
-       c += (int64_t)gridDim.y * 256 * V) {
+    const void* __restrict__ y, RowFactor f, int64_t y_rows, int64_t n,
+    const int64_t* __restrict__ slots, const float* __restrict__ weights, int64_t tokens, int k,
+    int tpt, const void* __restrict__ residual, int dt_res, void* __restrict__ out, int dt_out) {
+  const int at = __builtin_amdgcn_readfirstlane(threadIdx.x / tpt);
+  const int64_t t = (int64_t)blockIdx.x * (256 / tpt) + at;
+  if (t >= tokens) return;
+  const float up = f.scale ? ldexpf(1.0f, sum_exponent(f.largest, f.k)) : 1.0f;
+  for (int64_t c = ((int64_t)blockIdx.y * tpt + (threadIdx.x - at * tpt)) * V; c < n;
+       c += (int64_t)gridDim.y * tpt * V) {
     float acc[V];
 #pragma unroll
     for (int i = 0; i < V; ++i)
       acc[i] = residual ? load_as_f32(residual, t * n + c + i, dt_res) : 0.0f;
-    for (int j = 0; j < k; ++j) {
-      const int64_t s = slots[t * k + j];
-      const float w = weights[t * k + j];
-      if (s < 0 || s >= y_rows) {
+    for (int j0 = 0; j0 < k; j0 += 4) {
+      Piece<DT, V> p[4];
+      float w[4], rf[4];
 #pragma unroll
-        for (int i = 0; i < V; ++i) acc[i] = __builtin_nanf("");
-        continue;
+      for (int u = 0; u < 4; ++u) {
+        const int j = j0 + u < k ? j0 + u : k - 1;
+        int64_t s = slots[t * k + j];
+        w[u] = weights[t * k + j];
+        if (s < 0 || s >= y_rows) {
+          w[u] = __builtin_nanf("");
+          s = 0;
+        }
+        rf[u] = f.scale && y_rows ? f.scale[s] : 1.0f;
+        if (y_rows) p[u].load(y, s * n + c);
       }
-      if constexpr (V == 4) {
-        const f32x4v r = load4<DT>(y, s * n + c);
 #pragma unroll
-        for (int i = 0; i < V; ++i) acc[i] = __builtin_fmaf(w, r[i], acc[i]);
-      } else {
-        acc[0] = __builtin_fmaf(w, load_as_f32(y, s * n + c, DT), acc[0]);
+      for (int u = 0; u < 4; ++u) {
+        if (j0 + u >= k) break;
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          acc[i] = __builtin_fmaf(w[u], y_rows ? p[u][i] * up * rf[u] : 0.0f, acc[i]);
       }
     }
 #pragma unroll
@@ -554,28 +573,31 @@ __global__ void zero_i64_kernel(int64_t* p, int64_t n) {
 
 }  // namespace
 
-int launch_combine(const void* y, int dt_y, int64_t y_rows, int64_t n, const int64_t* slots,
-                   const float* weights, int64_t t, int64_t top_k, const void* residual,
-                   int dt_residual, void* out, int dt_out, hipStream_t s) {
-  const bool vec = n % 4 == 0 && (uintptr_t)y % 16 == 0;
-  const int64_t cols = (n + (vec ? 1023 : 255)) / (vec ? 1024 : 256);
-  const dim3 grid((unsigned)t, (unsigned)(cols < 64 ? cols : 64));
-#define HI2X_COMBINE(DT, V)                                                                  \
-  combine_kernel<DT, V><<<grid, 256, 0, s>>>(y, y_rows, n, slots, weights, (int)top_k,       \
-                                             residual, dt_residual, out, dt_out)
+int launch_combine(const void* y, int dt_y, const RowFactor& f, int64_t y_rows, int64_t n,
+                   const int64_t* slots, const float* weights, int64_t t, int64_t top_k,
+                   const void* residual, int dt_residual, void* out, int dt_out, hipStream_t s) {
+  const int wide = dt_y == 0 ? 4 : 8;
+  const int v = n % wide == 0 && (uintptr_t)y % 16 == 0 ? wide : 1;
+  const int64_t pieces = n / v;
+  const int tpt = pieces <= 64 ? 64 : (pieces <= 128 ? 128 : 256);
+  const int64_t cols = (pieces + tpt - 1) / tpt;
+  const dim3 grid((unsigned)((t + 256 / tpt - 1) / (256 / tpt)), (unsigned)(cols < 64 ? cols : 64));
+#define HI2X_COMBINE(DT, V)                                                                    \
+  combine_kernel<DT, V><<<grid, 256, 0, s>>>(y, f, y_rows, n, slots, weights, t, (int)top_k,   \
+                                             tpt, residual, dt_residual, out, dt_out)
   if (dt_y == 0) {
-    if (vec)
+    if (v == 4)
       HI2X_COMBINE(0, 4);
     else
       HI2X_COMBINE(0, 1);
   } else if (dt_y == 1) {
-    if (vec)
-      HI2X_COMBINE(1, 4);
+    if (v == 8)
+      HI2X_COMBINE(1, 8);
     else
       HI2X_COMBINE(1, 1);
   } else {
-    if (vec)
-      HI2X_COMBINE(2, 4);
+    if (v == 8)
+      HI2X_COMBINE(2, 8);
     else
       HI2X_COMBINE(2, 1);
   }
@@ -702,6 +724,6 @@ extern "C" int hi2x_moe_combine(const void* y, int dt_y, int64_t y_rows, int64_t
                "moe_combine: bad shape");
   if (t == 0) return HI2X_OK;
   HI2X_REQUIRE((y || y_rows == 0) && slots && weights && out, "moe_combine: null buffer");
-  return launch_combine(y, dt_y, y_rows, n, slots, weights, t, top_k, residual, dt_residual, out,
+  return launch_combine(y, dt_y, RowFactor{}, y_rows, n, slots, weights, t, top_k, residual, dt_residual, out,
                         dt_out, as_stream(stream));
 }

@@ -171,13 +171,15 @@ class _Packed:
         self._had = _lib.h2d(torch.from_numpy(np.stack(had[:own])), dev)
         self._scale = None if cs[0] is None else \
             _lib.h2d(torch.from_numpy(np.stack(cs[:own])), dev)
+        self._largest = torch.empty(1, device=dev)
         first = (_lib.Segment * len(CLASSES)).from_buffer_copy(segs[0].tobytes())
         #: hi2x_packed: the layout, the tables and the transform
         self.desc = _lib.Packed(
             self._codes.data_ptr(), self._params.data_ptr(), self._rows.data_ptr(),
             self._segments.data_ptr(), e, n, k, kp, frag, most,
             (ctypes.c_int64 * 3)(*(int(v) for v in tiles)), self._had.data_ptr(),
-            None if self._scale is None else self._scale.data_ptr(), int(self.transform is None), first)
+            None if self._scale is None else self._scale.data_ptr(), int(self.transform is None),
+            self._largest.data_ptr(), first)
         self._ref = ctypes.byref(self.desc)
         _lib.call("hi2x_packed_layout", dev, self._ref, _lib.ptr(words),
                   _lib.ptr(offs[0]), _lib.ptr(bytes_), _lib.ptr(offs[1]), _lib.ptr(consts))
@@ -431,8 +433,10 @@ def moe_mlp(x: torch.Tensor, routing, gate: PackedExperts, up: PackedExperts,
             down: PackedExperts, activation: str = "silu", residual=None) -> torch.Tensor:
     """The gated MLP of packed experts over routed tokens:
     ``residual + sum_j w_j down(activation(gate(x)) * up(x))`` for ``x [..., K]`` and the
-    :class:`hi2_amd.moe.Routing` of its tokens, as x's shape and type.  What the experts
-    hand on stays in float32; the rounding to x's type is one, at the end."""
+    :class:`hi2_amd.moe.Routing` of its tokens, as x's shape and type.  Sums are float32 and the
+    rounding to x's type is one, at the end; what the experts hand on is float32, for bfloat16
+    inputs of more than a few tokens fp16 of 11 bits under a scale (2^-12 of each value, a
+    sixteenth of the result's own rounding)."""
     for name, p in (("gate", gate), ("up", up), ("down", down)):
         if not isinstance(p, PackedExperts):
             raise TypeError(f"{name} is {type(p).__name__}, expected PackedExperts")
@@ -464,8 +468,8 @@ def moe_mlp(x: torch.Tensor, routing, gate: PackedExperts, up: PackedExperts,
     out = torch.empty(x.shape, dtype=x.dtype, device=gate.device)
     if not t:
         return out
-    # one fp16 plane of the hidden values is well below a bf16 result's own rounding, and half
-    # the products; next to an fp16 result it would show
+    # one fp16 plane of the hidden values (and fp16 between the products) is well below a bf16
+    # result's own rounding, and half the products; next to an fp16 result it would show
     npl, mid = _planes(x.dtype, gate), 1 if x.dtype == torch.bfloat16 else 2
     top_k = index.shape[1]
     shared = gate.transform is not None and gate.transform == up.transform

@@ -549,6 +549,7 @@ typedef struct {
   const uint8_t* had;                  /* [k / 16] rotation flags of the 16-column groups */
   const uint16_t* col_scale;           /* [k] fp16 smoothing, or NULL */
   int64_t per_expert;                  /* had and col_scale hold one row per expert */
+  float* largest;                      /* the largest |weight| (hi2x_packed_layout writes it) */
   hi2x_packed_segment first[HI2X_PACKED_SEGMENTS]; /* expert 0's segments (host copy) */
 } hi2x_packed;
 
@@ -659,9 +660,10 @@ int hi2x_moe_combine(const void* y, int dt_y, int64_t y_rows, int64_t n, const i
  *   y = down(act(gate(x)) * up(x)) for every routed slot.
  * x [t][h] as for hi2x_packed_activations; rows, offs, slots and weights as hi2x_route gives
  * them for t tokens and top_k choices; residual (or NULL) and out [t][h] contiguous.  The
- * experts' values in between are f32; nplanes and nplanes_mid are the planes of the tokens'
- * and the hidden values' transforms, shared says that gate's and up's transforms are the
- * same.  Workspace: hi2x_moe_mlp_workspace_bytes. */
+ * nplanes and nplanes_mid are the planes of the tokens' and the hidden values' transforms,
+ * shared says that gate's and up's transforms are the same.  The experts' values in between
+ * are f32; with one plane of the hidden values, and more than 16 slots, fp16 times a power of
+ * two that their sums cannot exceed (from `largest`).  Workspace: hi2x_moe_mlp_workspace_bytes. */
 int hi2x_moe_mlp(const hi2x_packed* gate, const hi2x_packed* up, const hi2x_packed* down,
                  const void* x, int dtype, int64_t ldx, int64_t t, int64_t top_k, int nplanes,
                  int nplanes_mid, int shared, int act, const int64_t* rows, const int64_t* offs,

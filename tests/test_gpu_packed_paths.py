@@ -172,3 +172,34 @@ def test_gated_mlp_of_unlike_tensors(t, e, k, h, i, dt, dev):
         np.add.at(want, tok, w[tok, c][:, None] * (stored(a, ds[0][j]) @ ds[1][j].T))
     rel = np.linalg.norm(N(got) - want) / np.linalg.norm(want)
     assert rel < {"bf16": 2.0 ** -8, "f32": 2.0 ** -19}[dt], rel
+
+
+@pytest.mark.parametrize("size", [1e-30, 1.0, 1e18])
+def test_gated_mlp_at_any_scale(size, dev):
+    """What the experts hand on is scaled, so that neither tiny nor huge tokens overflow or
+    vanish on the way; a token with an infinity and one with a NaN keep to themselves."""
+    from hi2_amd.moe import route
+    from hi2_amd.packed import PackedExperts, moe_mlp
+
+    t, e, k, h, i = 60, 4, 2, 128, 192
+    gs, us, ds = _experts(e, i, h, 100), _experts(e, i, h, 200), _experts(e, h, i, 300)
+    plans = [PackedExperts(s[0], dev) for s in (gs, us, ds)]
+    x = (tokens(t, h, torch.float32, 4, dev) * size).bfloat16()
+    x[3, 5], x[7, 9] = float("inf"), float("nan")
+    r = route(torch.randn(t, e, generator=torch.Generator().manual_seed(3)).to(dev), k)
+    got = moe_mlp(x, r, *plans, activation="relu")
+    ok = np.setdiff1d(np.arange(t), [3, 7])
+    assert not torch.isfinite(got[3]).any() and torch.isnan(got[7]).all()
+    index, w = N(r.index).astype(int), N(r.weights)
+    want = np.zeros((t, h))
+    for j in range(e):
+        tok, c = np.nonzero(index == j)
+        c, tok = c[np.isin(tok, ok)], tok[np.isin(tok, ok)]
+        a = act64(stored(N(x)[tok], gs[0][j]) @ gs[1][j].T, "relu")
+        a = a * (stored(N(x)[tok], us[0][j]) @ us[1][j].T)
+        np.add.at(want, tok, w[tok, c][:, None] * (stored(a, ds[0][j]) @ ds[1][j].T))
+    if size < 1e-20:  # (products below the smallest float32)
+        assert np.abs(N(got)[ok]).max() <= 1e-37
+    else:
+        rel = np.linalg.norm(N(got)[ok] - want[ok]) / np.linalg.norm(want[ok])
+        assert rel < 2.0 ** -8, rel
