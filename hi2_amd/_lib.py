@@ -134,6 +134,8 @@ SIGNATURES["hi2x_moe_mlp"] = [_P, _P, _P, _P, _I, _I64, _I64, _I64, _I, _I, _I, 
 SIGNATURES["hi2x_route"] = [_P, _I, _I64, _I64, _I64, _I64, _I, _P, _I64, _I64, _I, _F, _P, _P,
                             _P, _P, _P, _P, _I64, _P]
 SIGNATURES["hi2x_route_backward"] = [_P, _I, _I64, _I64, _I64, _I64, _I, _I, _F, _P, _P, _P, _P]
+SIGNATURES["hi2x_moe_combine_backward"] = [_P, _I, _P, _I, _I64, _I64, _P, _P, _I64, _I64, _P, _P,
+                                           _P]
 SIGNATURES["hi2x_moe_combine"] = [_P, _I, _I64, _I64, _P, _P, _I64, _I64, _P, _I, _P, _I, _P]
 
 # workspace sizes (int64 bytes, -1 for bad arguments): name -> argtypes

@@ -544,6 +544,59 @@ __global__ __launch_bounds__(256) void combine_kernel(
   }
 }
 
+// The weighted sum's gradients, a wave on a slot (t, j): dw = sum_c g[t][c] y[slot][c], dy[slot]
+// = w g[t].  Bound by reading y and writing dy once (g's rows are read by their k slots from
+// cache).
+template <int DT, int V>
+__device__ __forceinline__ void load_values(const void* p, int64_t at, float (&v)[V]) {
+  if constexpr (V == 1) {
+    v[0] = load_as_f32(p, at, DT);
+  } else if constexpr (DT == 0) {
+    const f32x4v u = *reinterpret_cast<const f32x4v*>(static_cast<const float*>(p) + at);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = u[i];
+  } else {
+    const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + at);
+    const uint32_t h[4] = {u.x & 0xffffu, u.x >> 16, u.y & 0xffffu, u.y >> 16};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      v[i] = DT == 1 ? f16_from_bits((uint16_t)h[i]) : __uint_as_float(h[i] << 16);
+  }
+}
+
+template <int DG, int DT, int V>
+__global__ __launch_bounds__(256) void combine_backward_kernel(
+    const void* __restrict__ grad, const void* __restrict__ y, int64_t y_rows, int64_t n,
+    const int64_t* __restrict__ slots, const float* __restrict__ weights, int64_t count, int k,
+    float* __restrict__ dw, void* __restrict__ dy) {
+  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  if (i >= count) return;
+  const int64_t t = i / k, s = slots[i];
+  if (s < 0 || s >= y_rows) {
+    if (dw && lane == 0) dw[i] = __builtin_nanf("");
+    return;
+  }
+  const float w = weights[i];
+  float sum = 0.0f;
+  for (int64_t c = lane * V; c < n; c += 64 * V) {
+    float g[V], v[V];
+    load_values<DG, V>(grad, t * n + c, g);
+    if (dw) {
+      load_values<DT, V>(y, s * n + c, v);
+#pragma unroll
+      for (int u = 0; u < V; ++u) sum = __builtin_fmaf(g[u], v[u], sum);
+    }
+    if (dy) {
+#pragma unroll
+      for (int u = 0; u < V; ++u) store_from_f32(dy, s * n + c + u, DT, w * g[u]);
+    }
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+  if (dw && lane == 0) dw[i] = sum;
+}
+
 int check_route(const char* what, const void* logits, int dtype, int64_t ld, int64_t t,
                 int64_t e, int64_t k, int scoring) {
   HI2X_REQUIRE(dtype >= 0 && dtype <= 2, "%s: dtype %d", what, dtype);
@@ -726,4 +779,51 @@ extern "C" int hi2x_moe_combine(const void* y, int dt_y, int64_t y_rows, int64_t
   HI2X_REQUIRE((y || y_rows == 0) && slots && weights && out, "moe_combine: null buffer");
   return launch_combine(y, dt_y, RowFactor{}, y_rows, n, slots, weights, t, top_k, residual, dt_residual, out,
                         dt_out, as_stream(stream));
+}
+
+extern "C" int hi2x_moe_combine_backward(const void* grad, int dt_grad, const void* y, int dt_y,
+                                         int64_t y_rows, int64_t n, const int64_t* slots,
+                                         const float* weights, int64_t t, int64_t top_k,
+                                         float* grad_weights, void* grad_y, void* stream) {
+  clear_error();
+  for (int d : {dt_grad, dt_y})
+    HI2X_REQUIRE(d >= 0 && d <= 2, "moe_combine_backward: dtype %d", d);
+  HI2X_REQUIRE(y_rows >= 0 && n >= 0 && t >= 0 && t < (1ll << 31) && top_k >= 1 &&
+                   top_k < (1 << 20) && t * top_k < (1ll << 32),
+               "moe_combine_backward: bad shape");
+  if (t == 0 || (!grad_weights && !grad_y)) return HI2X_OK;
+  HI2X_REQUIRE((grad || n == 0) && (y || y_rows == 0 || n == 0) && slots && weights,
+               "moe_combine_backward: null buffer");
+  const int64_t count = t * top_k;
+  const hipStream_t s = as_stream(stream);
+  const dim3 grid((unsigned)((count + 3) / 4));
+  const bool vec = n % 4 == 0 &&
+                   (((uintptr_t)grad | (uintptr_t)y | (uintptr_t)grad_y) & 15) == 0;
+#define HI2X_BACK_(DG, DT, V)                                                              \
+  combine_backward_kernel<DG, DT, V><<<grid, 256, 0, s>>>(grad, y, y_rows, n, slots, weights, \
+                                                          count, (int)top_k, grad_weights, \
+                                                          grad_y);
+#define HI2X_BACK(DG)         \
+  if (vec && dt_y == 0)       \
+    HI2X_BACK_(DG, 0, 4)      \
+  else if (vec && dt_y == 1)  \
+    HI2X_BACK_(DG, 1, 4)      \
+  else if (vec)               \
+    HI2X_BACK_(DG, 2, 4)      \
+  else if (dt_y == 0)         \
+    HI2X_BACK_(DG, 0, 1)      \
+  else if (dt_y == 1)         \
+    HI2X_BACK_(DG, 1, 1)      \
+  else                        \
+    HI2X_BACK_(DG, 2, 1)
+  if (dt_grad == 0) {
+    HI2X_BACK(0)
+  } else if (dt_grad == 1) {
+    HI2X_BACK(1)
+  } else {
+    HI2X_BACK(2)
+  }
+#undef HI2X_BACK
+#undef HI2X_BACK_
+  return launch_status("moe_combine_backward");
 }

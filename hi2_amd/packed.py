@@ -17,8 +17,9 @@ registers on the way.
   (q, k, v; gate, up) to be multiplied one after the other.
 
 Inputs are float32, float16 or bfloat16; products are summed in float32 and rounded once,
-to ``out_dtype``.  Nothing here has a gradient (the codes are integers; inputs that
-require one are refused while gradients are recorded).
+to ``out_dtype``.  The products have no gradient (the codes are integers; inputs that
+require one are refused while gradients are recorded); :func:`combine` has, and
+:func:`moe_mlp` to the routing's weights, so that a router can be trained on frozen experts.
 """
 
 from __future__ import annotations
@@ -398,14 +399,42 @@ def experts_linear(x: torch.Tensor | Activations, w: PackedExperts, offs: torch.
                     out_dtype or x.dtype, "experts_linear")
 
 
+class _Combine(torch.autograd.Function):
+    """:func:`combine` with gradients to y, the weights and the residual."""
+
+    @staticmethod
+    def forward(ctx, y, weights, residual, slots, out_dtype):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(y, weights, slots)
+        ctx.res = None if residual is None else (residual.shape, residual.dtype)
+        return _combine(y, slots, weights, residual, out_dtype)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        if grad is None:
+            return (None,) * 5
+        y, weights, slots = ctx.saved_tensors
+        need_y, need_w, need_r = ctx.needs_input_grad[:3]
+        grad = grad.contiguous()
+        dw = torch.empty_like(weights) if need_w else None
+        dy = torch.zeros_like(y) if need_y else None
+        if need_w or need_y:
+            _lib.call("hi2x_moe_combine_backward", y.device, _lib.ptr(grad), _dtype(grad, "grad"),
+                      _lib.ptr(y), _dtype(y, "y"), y.shape[0], y.shape[1], _lib.ptr(slots),
+                      _lib.ptr(weights), slots.shape[0], slots.shape[1], _lib.ptr(dw),
+                      _lib.ptr(dy))
+        return dy, dw, grad.to(ctx.res[1]).view(ctx.res[0]) if need_r else None, None, None
+
+
 def combine(y: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor, residual=None,
             out_dtype=None) -> torch.Tensor:
     """``out[t] = residual[t] + sum_j weights[t, j] * y[slots[t, j]]`` over ``y [S, N]``, with
     ``slots`` (int64) and ``weights`` (float32) ``[T, k]`` of :func:`hi2_amd.moe.route`: summed
     in float32 in the order of j, rounded once to ``out_dtype`` (default: residual's, else
-    y's)."""
-    dev = _lib.require_gpu(y, slots, weights, residual)
-    _no_grad_inputs("combine", y, weights, residual)
+    y's).  y, the weights and the residual have gradients where they require them (y's row by
+    row: no row of y may then be named twice, and :func:`hi2_amd.moe.route` names none twice)."""
+    _lib.require_gpu(y, slots, weights, residual)
     if y.dim() != 2:
         raise ValueError(f"y has shape {tuple(y.shape)}, expected [S, N]")
     if slots.dim() != 2 or weights.shape != slots.shape or slots.shape[1] < 1:
@@ -418,11 +447,19 @@ def combine(y: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor, residua
     if residual is not None and residual.numel() != t * n:
         raise ValueError(f"residual has shape {tuple(residual.shape)}, expected {(t, n)}")
     y, slots, weights = y.contiguous(), slots.contiguous(), weights.contiguous()
+    if torch.is_grad_enabled() and (y.requires_grad or weights.requires_grad or
+                                    residual is not None and residual.requires_grad):
+        return _Combine.apply(y, weights, residual, slots, out_dtype)
+    return _combine(y, slots, weights, residual, out_dtype)
+
+
+def _combine(y, slots, weights, residual, out_dtype):
+    t, n = slots.shape[0], y.shape[1]
     res = None if residual is None else residual.contiguous()
     out_dtype = out_dtype or (y.dtype if res is None else res.dtype)
-    out = torch.empty(t, n, dtype=out_dtype, device=dev)
+    out = torch.empty(t, n, dtype=out_dtype, device=y.device)
     if t and n:
-        _lib.call("hi2x_moe_combine", dev, _lib.ptr(y), _dtype(y, "y"), y.shape[0], n,
+        _lib.call("hi2x_moe_combine", y.device, _lib.ptr(y), _dtype(y, "y"), y.shape[0], n,
                   _lib.ptr(slots), _lib.ptr(weights), t, slots.shape[1], _lib.ptr(res),
                   0 if res is None else _dtype(res, "residual"), _lib.ptr(out),
                   _dtype(out_dtype, "out_dtype"))
@@ -436,7 +473,8 @@ def moe_mlp(x: torch.Tensor, routing, gate: PackedExperts, up: PackedExperts,
     :class:`hi2_amd.moe.Routing` of its tokens, as x's shape and type.  Sums are float32 and the
     rounding to x's type is one, at the end; what the experts hand on is float32, for bfloat16
     inputs of more than a few tokens fp16 of 11 bits under a scale (2^-12 of each value, a
-    sixteenth of the result's own rounding)."""
+    sixteenth of the result's own rounding).  Where the routing's weights (or the residual)
+    require a gradient they have one, from the parts' own calls, in float32 between them."""
     for name, p in (("gate", gate), ("up", up), ("down", down)):
         if not isinstance(p, PackedExperts):
             raise TypeError(f"{name} is {type(p).__name__}, expected PackedExperts")
@@ -448,7 +486,7 @@ def moe_mlp(x: torch.Tensor, routing, gate: PackedExperts, up: PackedExperts,
         raise RuntimeError("gate, up and down are on different devices")
     if routing is None:
         raise TypeError("moe_mlp takes a Routing")
-    _no_grad_inputs("moe_mlp", x, routing.weights, residual)
+    _no_grad_inputs("moe_mlp", x)
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"activation {activation!r} ({', '.join(ACTIVATIONS)})")
@@ -462,8 +500,18 @@ def moe_mlp(x: torch.Tensor, routing, gate: PackedExperts, up: PackedExperts,
     if residual is not None:
         if residual.numel() != t * gate.k:
             raise ValueError(f"residual has shape {tuple(residual.shape)}, expected {(t, gate.k)}")
-        residual = residual.contiguous()
+        residual = residual.reshape(t, gate.k).contiguous()
     _same_device(gate, "moe_mlp", weights, slots)
+    if torch.is_grad_enabled() and (weights.requires_grad or
+                                    residual is not None and residual.requires_grad):
+        with torch.no_grad():
+            def part(p, v, **more):
+                return experts_linear(v, p, routing.offs, out_dtype=torch.float32, **more)
+
+            h = part(up, flat, rows=routing.rows)
+            h = part(gate, flat, rows=routing.rows, activation=activation, mul=h)
+            y = part(down, h)
+        return combine(y, slots, weights, residual, x.dtype).view(x.shape)
     dt = _dtype(x, "x")
     out = torch.empty(x.shape, dtype=x.dtype, device=gate.device)
     if not t:

@@ -655,6 +655,16 @@ int hi2x_moe_combine(const void* y, int dt_y, int64_t y_rows, int64_t n, const i
                      const float* weights, int64_t t, int64_t top_k, const void* residual,
                      int dt_residual, void* out, int dt_out, void* stream);
 
+/* Its gradients, from grad [t][n] contiguous: grad_weights f32 [t][top_k] (or NULL), each
+ * sum over n in f32, and grad_y [y_rows][n] in y's type (or NULL), whose rows that a slot
+ * names are written: weights[t][j] * grad[t] (a row that several slots name takes one of
+ * theirs; hi2x_route names none twice).  A slot outside [0, y_rows) has the weight gradient
+ * NaN.  The residual's gradient is grad. */
+int hi2x_moe_combine_backward(const void* grad, int dt_grad, const void* y, int dt_y,
+                              int64_t y_rows, int64_t n, const int64_t* slots,
+                              const float* weights, int64_t t, int64_t top_k,
+                              float* grad_weights, void* grad_y, void* stream);
+
 /* The gated MLP of experts over routed tokens, from one call:
  *   out[t] = residual[t] + sum_j weights[t][j] y[slots[t][j]],
  *   y = down(act(gate(x)) * up(x)) for every routed slot.
