@@ -527,6 +527,7 @@ extern "C" int hi2x_packed_linear_activations(const hi2x_packed* w, const hi2x_a
                "packed_linear: 4 GiB of activations or more cannot be taken by index");
   if (slots == 0) return HI2X_OK;
   HI2X_REQUIRE(x->rows > 0 && x->planes && x->scale, "packed_linear: null activations");
+  HI2X_REQUIRE(((uintptr_t)x->planes & 255) == 0, "packed_linear: planes not aligned");
   const GemmArgs g{*w, *x, src, offs, slots, *epi};
   return packed_product(GemmPair{{g, g}}, 1, work, work_bytes, as_stream(stream));
 }
