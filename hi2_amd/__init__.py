@@ -8,6 +8,9 @@ Drop-in for the reference's per-Linear encode numerics: the modules
 modules of the same names (``hi2.hessian`` ... ``hi2.checkpoint``) for the encode path
 and run every arithmetic step in the HIP kernels of ``libhi2x.so`` (C ABI:
 ``include/hi2x.h``).
+
+``hi2_amd.packed`` and ``hi2_amd.moe.route`` run what was encoded: products by packed tensors
+and experts, and the router in front of them.
 """
 
 __version__ = "0.1.0"

@@ -103,14 +103,17 @@ __device__ __forceinline__ void group_values(const RawRows& x, const float (&rf)
   }
 }
 
-// TPR threads transform a row, several rows to a workgroup of 256 where that leaves room.  The largest finite |x / s| comes first; the rotation can
-// grow it fourfold at most, so 2^(13 - exponent) brings every value to at most 2^15, with
-// nothing of the row below fp16's normal range unless it is 2^-27 of the largest.  Then the
-// values are scaled (exact), rotated by butterflies in f32 and rounded to fp16.  That
-// rounding (2^-12 of each value, independent) is below the output's own for bf16 and as
-// large as fp16's; nplanes 2 keeps the rest of it in a second plane.  A thread keeps its
-// group's values between the two where one group a thread is all there is (KEEP, up to 16384
-// columns); rows beyond are read twice, the second time from L2.
+// TPR threads transform a row, several rows to a workgroup of 256 where that leaves room.  The
+// largest finite |x / s| comes first; the rotation can grow it fourfold at most, so
+// 2^(13 - exponent) brings every value to at most 2^15, with nothing of the row below fp16's
+// normal range unless it is 2^-27 of the largest.  Then the values are scaled (exact), rotated
+// by butterflies in f32 and rounded to fp16.  That rounding (at most 2^-11 of a value) is an
+// eighth of a bf16 output's own and as large as an fp16 output's; nplanes 2 keeps the rest of it
+// in a second plane.  A thread keeps its group's values between the two where one group a thread
+// is all there is (KEEP, up to 16384 columns); rows beyond are read twice, the second time from
+// L2.  Bound by reading x and writing the planes: the hidden rows of 16384 tokens and 8 of 64
+// experts (131072 x 1024, two operands of 16 bits) take 196 us, 4.1 TB/s; with one group a lane
+// the gated form's arithmetic is hidden behind that.
 template <int DT, bool GLU, bool KEEP, int TPR>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void activations_kernel(
     RawRows x, int64_t k, const int64_t* __restrict__ src, const uint8_t* __restrict__ had,

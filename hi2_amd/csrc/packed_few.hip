@@ -158,13 +158,14 @@ struct FewPass {
   }
 };
 
-// MT: activation rows of the workgroup; as they are, a power of two up to 8, transformed, 16,
-// 32 or 64.  A step is one chunk and plane; the codes (and transformed activations) of UN
+// MT: activation rows of the workgroup; as they are, a power of two up to 8, transformed, 16.
+// A step is one chunk and plane; the codes (and transformed activations) of UN
 // steps are fetched while the UN before them are multiplied.
 template <int BITS, int FR, int MT, int MODE, int FW>
-__device__ __forceinline__ void few_loop(const FewArgs& a, const GemmArgs& g, const Tile& tile, int e, int64_t first,
-                                         int live, FewPass<MODE == GIVEN ? RAW16 : MODE,
-                                                           MODE == GIVEN ? 1 : MT, FW> pass,
+__device__ __forceinline__ void few_loop(const FewArgs& a, const GemmArgs& g, const Tile& tile,
+                                         int e, int64_t first, int live,
+                                         FewPass<MODE == GIVEN ? RAW16 : MODE,
+                                                 MODE == GIVEN ? 1 : MT, FW> pass,
                                          int64_t src, char* xl,
                                          f32x4v (&acc)[FR][MODE == GIVEN ? MT / 16 : 1]) {
   constexpr bool RAW = MODE != GIVEN;
@@ -311,8 +312,9 @@ __device__ __forceinline__ void few_loop(const FewArgs& a, const GemmArgs& g, co
 }
 
 template <int FR, int MT, int MODE, int FW>
-__global__ __launch_bounds__(
-    64 * FW, MODE == GIVEN ? 4 : (MODE != RAW16 ? 2 : (FW == 8 ? 4 : 3))) void packed_few_kernel(FewArgs a) {
+__global__ __launch_bounds__(64 * FW,
+                             MODE == GIVEN ? 4 : (MODE != RAW16 ? 2 : (FW == 8 ? 4 : 3)))
+void packed_few_kernel(FewArgs a) {
   constexpr bool RAW = MODE != GIVEN;
   constexpr int MF = RAW ? 1 : MT / 16;
   constexpr int XW = RAW ? 4096 : 0;         // bytes of transformed rows of a wave

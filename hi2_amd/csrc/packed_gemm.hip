@@ -23,10 +23,14 @@ constexpr int waitcnt(int vm, int lgkm) {
   return (vm & 15) | ((vm >> 4) << 14) | (7 << 4) | (lgkm << 8);
 }
 
-// The main loop of one tile: 4 waves of NF fragments x 16 MF slots each, all reading the
-// same activations from LDS, in a workgroup's accumulators of AF x AM.  A stage of 16 MF slots x 128 columns is 256 bytes a slot in
-// 16 pieces; piece p of slot t lies at p ^ (t % 16), so that the 16 slots a fragment read
-// touches at one piece fall on different banks.
+// The main loop of one tile: 4 waves of NF fragments x 16 MF slots each (of the AF and AM that
+// the accumulators hold), all reading the same activations from LDS.  A stage of 16 MF slots x
+// 128 columns is 256 bytes a slot in 16 pieces; piece p of slot t lies at p ^ (t % 16), so that
+// the 16 slots a fragment read touches at one piece fall on different banks.  The activations of
+// the next stage are on their way while one is multiplied, and the matrix units are busy 52 % of
+// the cycles (14336 x 4096, 4096 rows, 470 us, 1020 TFLOP/s); the rest is decoding (28 % of the
+// issue slots) and waits.  A barrier in mid-stage with the decode a fragment further ahead took 3
+// to 8 % longer.
 template <int BITS, bool B16, int NF, int MF, int AF, int AM>
 __device__ __forceinline__ void gemm_loop(const GemmArgs& g, const Tile& tile, char* lds,
                                           const char* xb, int64_t xbytes,
@@ -265,8 +269,8 @@ __device__ __forceinline__ void sized_loop(const GemmArgs& g, const Tile& tile, 
 // columns or (SPLIT) the blockIdx.z-th share of their chunks.  A split's sums go to `part` as
 // the accumulators hold them.
 template <int NF, int MF, bool SPLIT>
-__global__ __launch_bounds__(256, NF == 4 ? 2 : 4) void packed_gemm_kernel(GemmPair two, float* part,
-                                                                           int per, int nx) {
+__global__ __launch_bounds__(256, NF == 4 ? 2 : 4)
+void packed_gemm_kernel(GemmPair two, float* part, int per, int nx) {
   const GemmArgs& g = two.g[SPLIT ? 0 : blockIdx.z];
   constexpr int MT = 16 * MF, NS = 64 * NF;
   constexpr int XB = 2 * MT * 256;  // two stages of activations
@@ -424,7 +428,7 @@ struct GemmPlan {
 };
 
 // Large tiles feed the matrix units best, but only where there are enough of them: 256 x 128
-// (two workgroups a CU) reaches 1080 TFLOP/s at 14336 x 4096 and 4096 rows, but takes 2 us a
+// (two workgroups a CU) reaches 1020 TFLOP/s at 14336 x 4096 and 4096 rows, but takes 2 us a
 // chunk where a workgroup has its CU to itself.  The choice is the least of the estimates
 //   5.5 us + chunks x (a + b x workgroups on a CU), for each round of them,
 // and for splits the joining pass, 3.5 us + 0.45 us a share + the partial sums at 4.5 TB/s.
@@ -605,7 +609,7 @@ MlpSpace mlp_space(const hi2x_packed& gate, const hi2x_packed& up, const hi2x_pa
     at += align256(n);
     return a;
   };
-  // Results of 16 bits hide the rounding of scaled16 (2^-12) as they hide that of one plane;
+  // A bf16 result hides the rounding of scaled16 (2^-11) as it hides that of one plane;
   // writing and reading the three is what the large calls are short of: 64 experts of
   // 2048 x 1024, 8 choices, 16384 tokens 2680 us in f32, 2370 so.  Short calls keep f32.
   m.half = npl_mid == 1 && !few_raw_product(gate, slots, true);

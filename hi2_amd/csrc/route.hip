@@ -474,8 +474,10 @@ __global__ __launch_bounds__(256) void route_backward_kernel(
   }
 }
 
-// out[t] = residual[t] + sum_j w[t][j] y[slots[t][j]]: 64, 128 or 256 threads (TPT) on a
-// token, 16 bytes of a row of y at a time, four rows in flight.  Bound by reading y once.
+// out[t] = residual[t] + sum_j w[t][j] y[slots[t][j]]: 64, 128 or 256 threads (tpt) on a
+// token, 16 bytes of a row of y at a time, four rows in flight.  Bound by reading y once: 16384
+// tokens of 8 rows of 2048 in fp16 157 us, 3.4 TB/s (one row in flight, twice the bytes in f32:
+// 267 us, 4.0 TB/s).
 template <int DT, int V>
 struct Piece {  // V neighbouring values of y
   static constexpr int W = V == 1 ? 1 : V * (DT == 0 ? 4 : 2) / 4;
@@ -612,7 +614,7 @@ int check_route(const char* what, const void* logits, int dtype, int64_t ld, int
 // Tokens to a workgroup.  Four where that is all there are (barriers of one wave: one token
 // of 64 experts 7.2 -> 5.6 us); up to the 64 that one launch orders (32 above 256 experts,
 // whose registers leave room for half the waves) one workgroup; up to 4096 16, which spreads
-// them over the CUs (4096 tokens of 256 experts in groups 20 -> 9 us); then 64 again.
+// them over the CUs (4096 tokens of 256 experts in groups 20 -> 11.5 us); then 64 again.
 int route_tokens(int64_t t, int64_t e) {
   const int most = e <= 256 ? 64 : 32;
   return t <= 4 ? 4 : (t <= most ? most : (t <= 4096 ? 16 : most));
@@ -703,7 +705,9 @@ extern "C" int hi2x_route(const void* logits, int dtype, int64_t ld, int64_t t, 
     if (nb > SCAN_OVER)
       a.prefix = reinterpret_cast<int32_t*>(w.p + align256((int64_t)a.nbp * e));
   }
-  const size_t dyn = top_groups < groups && !whole_rows(e / groups, groups) ? (size_t)rt * (e + groups) * 4 : 0;
+  const size_t dyn = top_groups < groups && !whole_rows(e / groups, groups)
+                         ? (size_t)rt * (e + groups) * 4
+                         : 0;
   const dim3 grid((unsigned)nb);
 #define HI2X_ROUTE_(EPL, NT)                                                                   \
   {                                                                                            \
@@ -777,8 +781,8 @@ extern "C" int hi2x_moe_combine(const void* y, int dt_y, int64_t y_rows, int64_t
                "moe_combine: bad shape");
   if (t == 0) return HI2X_OK;
   HI2X_REQUIRE((y || y_rows == 0) && slots && weights && out, "moe_combine: null buffer");
-  return launch_combine(y, dt_y, RowFactor{}, y_rows, n, slots, weights, t, top_k, residual, dt_residual, out,
-                        dt_out, as_stream(stream));
+  return launch_combine(y, dt_y, RowFactor{}, y_rows, n, slots, weights, t, top_k, residual,
+                        dt_residual, out, dt_out, as_stream(stream));
 }
 
 extern "C" int hi2x_moe_combine_backward(const void* grad, int dt_grad, const void* y, int dt_y,
