@@ -106,7 +106,8 @@ class Packed(ctypes.Structure):
     _fields_ = [("codes", _P), ("params", _P), ("rows", _P), ("segments", _P),
                 ("experts", _I64), ("n", _I64), ("k", _I64), ("kp", _I64), ("frags", _I64),
                 ("max_frags", _I64), ("max_tiles", _I64 * 3), ("had", _P), ("col_scale", _P),
-                ("per_expert", _I64), ("largest", _P), ("first", Segment * 9)]
+                ("per_expert", _I64), ("largest", _P), ("places", _P),
+                ("first", Segment * 9)]
 
 
 class ActivationsDesc(ctypes.Structure):

@@ -77,22 +77,68 @@ __global__ __launch_bounds__(256) void layout_params_kernel(
 }
 
 // ---- activations -------------------------------------------------------------------------
+// Rows of SlotRows on their way through LDS: `a` and `b` hold them slot by slot, then column by
+// column.  Lanes take neighbouring columns, whose places are almost neighbours too, so that the
+// reads by place meet on few banks; all of a row's loads are in flight before the first is
+// waited for (131072 x 1024 hidden rows of 64 experts 386 us without that).
+struct SlotRow {
+  uint16_t *a, *b;
+  float up[2], factor[2];
+};
+template <int TPR>
+struct SlotColumns {
+  u32x4 raw[3];       // the row's slots, 8 at a time
+  uint32_t place[8];  // of the columns' pairs
+  __device__ __forceinline__ void load(const SlotRows& s, int64_t row, int tid) {
+    const u32x4* from = reinterpret_cast<const u32x4*>(s.v + row * s.pitch);
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+      raw[i] = tid + TPR * i < s.pitch / 8 ? from[tid + TPR * i] : u32x4{0u, 0u, 0u, 0u};
+  }
+  __device__ __forceinline__ void load_places(const SlotRows& s, int expert, int tid) {
+    const uint32_t* from = reinterpret_cast<const uint32_t*>(s.places + expert * s.n);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      place[i] = 2 * (tid + TPR * i) < s.n ? from[tid + TPR * i] : 0u;
+  }
+  __device__ __forceinline__ void put_slots(const SlotRows& s, uint16_t* row, int tid) const {
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+      if (tid + TPR * i < s.pitch / 8) reinterpret_cast<u32x4*>(row)[tid + TPR * i] = raw[i];
+  }
+  __device__ __forceinline__ void take_columns(const uint16_t* row) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      place[i] = (uint32_t)row[place[i] & 0xffffu] | (uint32_t)row[place[i] >> 16] << 16;
+  }
+  __device__ __forceinline__ void put_columns(const SlotRows& s, uint16_t* row, int tid) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (2 * (tid + TPR * i) < s.n) reinterpret_cast<uint32_t*>(row)[tid + TPR * i] = place[i];
+  }
+};
+
 // The 16 values of group g of a row, divided by their smoothing: of x, or (GLU) of
-// act(x) * x2.
+// act(x) * x2, or (SLOTS) of act(s1) * s2 from LDS.
+constexpr int SLOTS = 3;  // a type of its own
 template <int DT, bool GLU>
-__device__ __forceinline__ void group_values(const RawRows& x, const float (&rf)[4], int64_t base,
+__device__ __forceinline__ void group_values(const RawRows& x, const SlotRow& sr, int64_t base,
                                              int g, const uint16_t* cs, float (&v)[16]) {
-  load16(x.x, base + 16 * (int64_t)g, DT, v);
+  auto scaled = [&](const uint16_t* row, int o, float (&u)[16]) {
+    load16(row, 16 * (int64_t)g, 1, u);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) u[i] = u[i] * sr.up[o] * sr.factor[o];
+  };
+  if constexpr (DT == SLOTS)
+    scaled(sr.a, 0, v);
+  else
+    load16(x.x, base + 16 * (int64_t)g, DT, v);
   if constexpr (GLU) {
     float u[16];
-    load16(x.x2, base + 16 * (int64_t)g, DT, u);
-    if constexpr (DT == 1) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        v[i] = v[i] * rf[0] * rf[1];
-        u[i] = u[i] * rf[2] * rf[3];
-      }
-    }
+    if constexpr (DT == SLOTS)
+      scaled(sr.b, 1, u);
+    else
+      load16(x.x2, base + 16 * (int64_t)g, 0, u);
     activate_all(v, x.act);
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] *= u[i];
@@ -126,34 +172,53 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void activations_kernel(
   const int64_t from = none ? -1 : (src ? src[row] : row);
   const bool bad = from < 0 || from >= x.rows;
   const int64_t base = bad ? 0 : from * x.ldx;
-  if (offs && !none) {
-    int lo = 0, hi = experts - 1;  // the expert whose range holds the row
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (offs[mid + 1] > row)
-        hi = mid;
+  SlotColumns<TPR> ca, cb;
+  if constexpr (DT == SLOTS) {  // (the rows' loads before what their places wait for)
+    ca.load(x.s1, none ? 0 : row, tid);
+    cb.load(x.s2, none ? 0 : row, tid);
+  }
+  const int64_t* ranges = DT == SLOTS ? x.offs : offs;
+  const int expert =
+      ranges ? expert_of(range_ends(ranges, experts), ranges, experts, none ? 0 : row) : 0;
+  if (offs) {
+    had += (int64_t)expert * (k / 16);
+    if (cs) cs += (int64_t)expert * k;
+  }
+  SlotRow sr;
+  if constexpr (DT == SLOTS) {
+    extern __shared__ __attribute__((aligned(16))) uint16_t rows16[];
+    uint16_t* a = rows16 + (threadIdx.x / TPR) * (x.s1.pitch + x.s2.pitch);
+    uint16_t* b = a + x.s1.pitch;
+    sr = SlotRow{a, b, {}, {}};
+    ca.load_places(x.s1, expert, tid);
+    cb.load_places(x.s2, expert, tid);
+    sr.up[0] = ldexpf(1.0f, sum_exponent(x.s1.largest, x.s1.k));
+    sr.factor[0] = row_factor(x.s1, none ? 0 : row);
+    sr.up[1] = ldexpf(1.0f, sum_exponent(x.s2.largest, x.s2.k));
+    sr.factor[1] = row_factor(x.s2, none ? 0 : row);
+    auto meet = [] {  // of the row's threads
+      if constexpr (TPR > 64)
+        __syncthreads();
       else
-        lo = mid + 1;
-    }
-    had += (int64_t)lo * (k / 16);
-    if (cs) cs += (int64_t)lo * k;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup", "local");
+    };
+    ca.put_slots(x.s1, a, tid);
+    cb.put_slots(x.s2, b, tid);
+    meet();
+    ca.take_columns(a);
+    cb.take_columns(b);
+    meet();
+    ca.put_columns(x.s1, a, tid);
+    cb.put_columns(x.s2, b, tid);
+    meet();
   }
   const int groups = (int)(k / 16), all = (int)(out.kp / 16);
-  float rf[4] = {};  // 2^c and factor of the rows of x and x2
-  if constexpr (GLU && DT == 1) {
-    if (!bad) {
-      rf[0] = ldexpf(1.0f, sum_exponent(x.f1.largest, x.f1.k));
-      rf[1] = row_factor(x.f1, from);
-      rf[2] = ldexpf(1.0f, sum_exponent(x.f2.largest, x.f2.k));
-      rf[3] = row_factor(x.f2, from);
-    }
-  }
   float v[16], m = 0.0f;
 #pragma unroll
   for (int i = 0; i < 16; ++i) v[i] = 0.0f;
   if (!bad) {
     for (int g = tid; g < groups; g += TPR) {
-      group_values<DT, GLU>(x, rf, base, g, cs, v);
+      group_values<DT, GLU>(x, sr, base, g, cs, v);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const float a = fabsf(v[i]);
@@ -184,7 +249,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void activations_kernel(
 #pragma unroll
       for (int i = 0; i < 16; ++i) v[i] = 0.0f;
     } else {
-      if constexpr (!KEEP) group_values<DT, GLU>(x, rf, base, g, cs, v);
+      if constexpr (!KEEP) group_values<DT, GLU>(x, sr, base, g, cs, v);
 #pragma unroll
       for (int i = 0; i < 16; ++i) v[i] *= sc;
       if (had[g]) {
@@ -227,8 +292,9 @@ int launch_activations(const RawRows& x, const hi2x_packed& w, const int64_t* sr
 #define HI2X_ROWS_(DT, GLU, KEEP, TPR)                                                    \
   activations_kernel<DT, GLU, KEEP, TPR>                                                  \
       <<<dim3((unsigned)(TPR < 256 ? (out.rows * TPR + 255) / 256 : out.rows)),           \
-         TPR < 256 ? 256 : TPR, 0, s>>>(x, w.k, src, w.had, w.col_scale, offs,            \
-                                        (int)w.experts, out)
+         TPR < 256 ? 256 : TPR,                                                           \
+         DT == SLOTS ? (TPR < 256 ? 256 / TPR : 1) * (x.s1.pitch + x.s2.pitch) * 2 : 0,   \
+         s>>>(x, w.k, src, w.had, w.col_scale, offs, (int)w.experts, out)
 #define HI2X_ROWS(DT, GLU)                 \
   if (w.kp <= 1024)                        \
     HI2X_ROWS_(DT, GLU, true, 64);         \
@@ -238,12 +304,14 @@ int launch_activations(const RawRows& x, const hi2x_packed& w, const int64_t* sr
     HI2X_ROWS_(DT, GLU, true, 256);        \
   else if (w.kp <= 8192)                   \
     HI2X_ROWS_(DT, GLU, true, 512);        \
-  else if (w.kp <= 16384)                  \
-    HI2X_ROWS_(DT, GLU, true, 1024);       \
-  else                                     \
-    HI2X_ROWS_(DT, GLU, false, 1024);
-  if (x.x2 && x.dtype == 1) {
-    HI2X_ROWS(1, true)
+  else if constexpr (DT != SLOTS) {        \
+    if (w.kp <= 16384)                     \
+      HI2X_ROWS_(DT, GLU, true, 1024);     \
+    else                                   \
+      HI2X_ROWS_(DT, GLU, false, 1024);    \
+  }
+  if (!x.x) {
+    HI2X_ROWS(SLOTS, true)
   } else if (x.x2) {
     HI2X_ROWS(0, true)
   } else if (x.dtype == 0) {

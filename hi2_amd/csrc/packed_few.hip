@@ -47,8 +47,7 @@ struct FewPass {
 #pragma unroll
       for (int v = 0; v < V; ++v) raw[v] = from[v];
       if constexpr (GLU) {
-        from = reinterpret_cast<const u32x4*>(static_cast<const float*>(a.x.x2) + src * a.x.ldx +
-                                              16 * g);
+        from = reinterpret_cast<const u32x4*>(a.x.x2 + src * a.x.ldx + 16 * g);
 #pragma unroll
         for (int v = 0; v < V; ++v) up[v] = from[v];
       }

@@ -200,10 +200,31 @@ __device__ __forceinline__ void store_pass(const hi2x_epilogue& E, const float* 
   }
 }
 
+// The store of a pass of a scaled16 product: the slots as they lie, 8 to a thread, from slot
+// `at` of the output's rows on.
+template <int NS, int PITCH>
+__device__ __forceinline__ void store_slots(const hi2x_epilogue& E, const float* ep, float scale,
+                                            int at, int slots, int64_t o0, int rows) {
+  constexpr int TPR = NS / 8;
+  const int slot = threadIdx.x % TPR * 8;
+  if (slot >= slots) return;
+  uint16_t* out = static_cast<uint16_t*>(E.out) + o0 * E.ld_out + at + slot;
+  for (int t = threadIdx.x / TPR; t < rows; t += 256 / TPR) {
+    const f32x4v* from = reinterpret_cast<const f32x4v*>(ep + t * PITCH + slot);
+    const f32x4v a = from[0], b = from[1];
+    u32x4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float x = i < 2 ? a[2 * i] : b[2 * i - 4], y = i < 2 ? a[2 * i + 1] : b[2 * i - 3];
+      v[i] = (uint32_t)f16_bits(x * scale) | (uint32_t)f16_bits(y * scale) << 16;
+    }
+    *reinterpret_cast<u32x4*>(out + t * E.ld_out) = v;
+  }
+}
+
 // Row `t` of a tile's factor of scale: 0 past the end, NaN for an index outside.
 __device__ __forceinline__ float row_scale(const GemmArgs& g, int64_t first, int t, int live) {
   if (t >= live) return 0.0f;
-  if (g.scaled16) return ldexpf(1.0f, -sum_exponent(g.w.largest, g.w.k));
   const int64_t r = g.src ? g.src[first + t] : first + t;
   return r >= 0 && r < g.x.rows ? g.x.scale[r] : __builtin_nanf("");
 }
@@ -307,6 +328,7 @@ void packed_gemm_kernel(GemmPair two, float* part, int per, int nx) {
     xoff[i] = (uint32_t)r * pitch + 16 * ((lane & 15) ^ (t & 15));
   }
   if (tid < MT) xscale[tid] = row_scale(g, first, tid, live);
+  const float scale = g.scaled16 ? ldexpf(1.0f, -sum_exponent(g.w.largest, g.w.k)) : 0.0f;
   const int nch = (int)(g.w.kp / PK_CHUNK);
   const int c0 = SPLIT ? (int)blockIdx.z * per : 0;
   const int c1 = SPLIT && c0 + per < nch ? c0 + per : nch;
@@ -361,8 +383,12 @@ void packed_gemm_kernel(GemmPair two, float* part, int per, int nx) {
           *reinterpret_cast<f32x4v*>(ep + (16 * m + (lane & 15)) * PITCH + (wv * nf + f) * 16 +
                                      4 * (lane >> 4)) = acc[f][p * (EH / 16) + m];
     __syncthreads();
-    store_pass<NS, PITCH, EH, 8>(g.epi, ep, xscale + p * EH, n, bias, first + p * EH,
-                                 live - p * EH < EH ? live - p * EH : EH);
+    const int rows = live - p * EH < EH ? live - p * EH : EH;
+    if (g.scaled16)
+      store_slots<NS, PITCH>(g.epi, ep, scale, 16 * (tile.frag - tile.base), 16 * tile.count,
+                             first + p * EH, rows);
+    else
+      store_pass<NS, PITCH, EH, 8>(g.epi, ep, xscale + p * EH, n, bias, first + p * EH, rows);
   }
 }
 
@@ -611,12 +637,15 @@ MlpSpace mlp_space(const hi2x_packed& gate, const hi2x_packed& up, const hi2x_pa
   };
   // A bf16 result hides the rounding of scaled16 (2^-11) as it hides that of one plane;
   // writing and reading the three is what the large calls are short of: 64 experts of
-  // 2048 x 1024, 8 choices, 16384 tokens 2680 us in f32, 2370 so.  Short calls keep f32.
+  // 2048 x 1024, 8 choices, 16384 tokens 2680 us in f32, 2080 so.  Short calls keep f32.
   m.half = npl_mid == 1 && !few_raw_product(gate, slots, true);
+  for (const hi2x_packed* p : {&gate, &up, &down})
+    m.half = m.half && p->places && p->largest && 16 * p->max_frags <= SLOTS16 &&
+             16 * p->max_frags <= p->n + 16 * PK_SEGS;  // (as many as the readers' loads take)
   const int64_t size = m.half ? 2 : 4;
-  m.gate = take(slots * gate.n * size);
-  m.up = take(slots * gate.n * size);
-  m.y = take(slots * down.n * size);
+  m.gate = take(slots * (m.half ? 16 * gate.max_frags : gate.n) * size);
+  m.up = take(slots * (m.half ? 16 * up.max_frags : gate.n) * size);
+  m.y = take(slots * (m.half ? 16 * down.max_frags : down.n) * size);
   if (!few_raw_product(gate, slots, true)) {
     for (int i = 0; i < (shared ? 1 : 2); ++i) {
       m.in_rows[i] = (i ? up : gate).per_expert ? slots : t;
@@ -673,28 +702,26 @@ extern "C" int hi2x_moe_mlp(const hi2x_packed* gate, const hi2x_packed* up,
   for (int d : {dt_residual, dt_out})
     HI2X_REQUIRE(d >= 0 && d <= 2, "moe_mlp: dtype %d", d);
   if (t == 0) return HI2X_OK;
-  HI2X_REQUIRE(rows && offs && slots && weights && out && gate->largest && up->largest &&
-                   down->largest,
-               "moe_mlp: null buffer");
+  HI2X_REQUIRE(rows && offs && slots && weights && out, "moe_mlp: null buffer");
   HI2X_REQUIRE(t * gate->kp * 2 * nplanes < (1ll << 32) - 1 || few_raw_product(*gate, n, true),
                "moe_mlp: 4 GiB of activations or more cannot be taken by index");
   const hipStream_t s = as_stream(stream);
   const MlpSpace m = mlp_space(*gate, *up, *down, t, n, nplanes, nplanes_mid, shared);
   Workspace w;
   if (int rc = take_workspace(w, ws, ws_bytes, (size_t)m.bytes, s, "moe_mlp")) return rc;
-  auto to = [&](int64_t at, int64_t cols) {
+  auto to = [&](int64_t at, const hi2x_packed& p) {
     hi2x_epilogue e{};
     e.out = w.p + at;
-    e.ld_out = cols;
-    e.dt_out = m.half ? 1 : 0;
+    e.ld_out = m.half ? 16 * p.max_frags : p.n;
     return e;
   };
-  GemmPair in{{GemmArgs{*gate, hi2x_activations{}, rows, offs, n, to(m.gate, gate->n), m.half},
-               GemmArgs{*up, hi2x_activations{}, rows, offs, n, to(m.up, gate->n), m.half}}};
-  GemmArgs last{*down, hi2x_activations{}, nullptr, offs, n, to(m.y, down->n), m.half};
+  GemmPair in{{GemmArgs{*gate, hi2x_activations{}, rows, offs, n, to(m.gate, *gate), m.half},
+               GemmArgs{*up, hi2x_activations{}, rows, offs, n, to(m.up, *up), m.half}}};
+  GemmArgs last{*down, hi2x_activations{}, nullptr, offs, n, to(m.y, *down), m.half};
   const RawRows tokens{x, dtype, ldx, t, nplanes};
-  RawRows hidden{w.p + m.gate, m.half ? 1 : 0, gate->n, n, nplanes_mid, w.p + m.up, act};
-  RowFactor results;
+  RawRows hidden{w.p + m.gate, 0, gate->n, n, nplanes_mid,
+                 reinterpret_cast<const float*>(w.p + m.up), act};
+  SlotRows results;
   if (few_raw_product(*gate, n, true)) {
     if (int rc = packed_few_raw(in, 2, tokens, s)) return rc;
     if (int rc = packed_few_raw(GemmPair{{last, last}}, 1, hidden, s)) return rc;
@@ -712,13 +739,17 @@ extern "C" int hi2x_moe_mlp(const hi2x_packed* gate, const hi2x_packed* up,
       if (p.per_expert) in.g[i].src = nullptr;
     }
     if (m.half) {
-      auto factor = [](const GemmArgs& g) {
-        return RowFactor{g.x.scale, g.src, g.x.rows, g.w.largest, g.w.k};
+      auto rows_of = [](const GemmArgs& g) {
+        return SlotRows{static_cast<const uint16_t*>(g.epi.out), (int)g.epi.ld_out, g.w.places,
+                        g.x.scale, g.src, g.x.rows, g.w.largest, g.w.n, g.w.k};
       };
-      hidden.f1 = factor(in.g[0]);
-      hidden.f2 = factor(in.g[1]);
-      results = RowFactor{reinterpret_cast<const float*>(w.p + m.mid_scale), nullptr, n,
-                          down->largest, down->k};
+      hidden.x = nullptr;
+      hidden.s1 = rows_of(in.g[0]);
+      hidden.s2 = rows_of(in.g[1]);
+      hidden.offs = offs;
+      last.x.scale = reinterpret_cast<float*>(w.p + m.mid_scale);
+      last.x.rows = n;
+      results = rows_of(last);
     }
     const int64_t part = m.bytes - m.part;
     if (int rc = packed_product(in, 2, w.p + m.part, part, s)) return rc;
@@ -730,6 +761,9 @@ extern "C" int hi2x_moe_mlp(const hi2x_packed* gate, const hi2x_packed* up,
       return rc;
     if (int rc = packed_product(GemmPair{{last, last}}, 1, w.p + m.part, part, s)) return rc;
   }
-  return launch_combine(w.p + m.y, m.half ? 1 : 0, results, n, down->n, slots, weights, t, top_k,
-                        residual, dt_residual, out, dt_out, s);
+  if (m.half)
+    return launch_combine(results, offs, (int)down->experts, n, slots, weights, t, top_k, residual,
+                          dt_residual, out, dt_out, s);
+  return launch_combine(w.p + m.y, 0, n, down->n, slots, weights, t, top_k, residual, dt_residual,
+                        out, dt_out, s);
 }

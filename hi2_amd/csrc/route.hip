@@ -505,13 +505,12 @@ struct Piece {  // V neighbouring values of y
 
 template <int DT, int V>
 __global__ __launch_bounds__(256) void combine_kernel(
-    const void* __restrict__ y, RowFactor f, int64_t y_rows, int64_t n,
+    const void* __restrict__ y, int64_t y_rows, int64_t n,
     const int64_t* __restrict__ slots, const float* __restrict__ weights, int64_t tokens, int k,
     int tpt, const void* __restrict__ residual, int dt_res, void* __restrict__ out, int dt_out) {
   const int at = __builtin_amdgcn_readfirstlane(threadIdx.x / tpt);
   const int64_t t = (int64_t)blockIdx.x * (256 / tpt) + at;
   if (t >= tokens) return;
-  const float up = f.scale ? ldexpf(1.0f, sum_exponent(f.largest, f.k)) : 1.0f;
   for (int64_t c = ((int64_t)blockIdx.y * tpt + (threadIdx.x - at * tpt)) * V; c < n;
        c += (int64_t)gridDim.y * tpt * V) {
     float acc[V];
@@ -520,7 +519,7 @@ __global__ __launch_bounds__(256) void combine_kernel(
       acc[i] = residual ? load_as_f32(residual, t * n + c + i, dt_res) : 0.0f;
     for (int j0 = 0; j0 < k; j0 += 4) {
       Piece<DT, V> p[4];
-      float w[4], rf[4];
+      float w[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int j = j0 + u < k ? j0 + u : k - 1;
@@ -530,7 +529,6 @@ __global__ __launch_bounds__(256) void combine_kernel(
           w[u] = __builtin_nanf("");
           s = 0;
         }
-        rf[u] = f.scale && y_rows ? f.scale[s] : 1.0f;
         if (y_rows) p[u].load(y, s * n + c);
       }
 #pragma unroll
@@ -538,11 +536,102 @@ __global__ __launch_bounds__(256) void combine_kernel(
         if (j0 + u >= k) break;
 #pragma unroll
         for (int i = 0; i < V; ++i)
-          acc[i] = __builtin_fmaf(w[u], y_rows ? p[u][i] * up * rf[u] : 0.0f, acc[i]);
+          acc[i] = __builtin_fmaf(w[u], y_rows ? p[u][i] : 0.0f, acc[i]);
       }
     }
 #pragma unroll
     for (int i = 0; i < V; ++i) store_from_f32(out, t * n + c + i, dt_out, acc[i]);
+  }
+}
+
+// The same of SlotRows: four rows at a time go through LDS, from where columns are taken by
+// their places, a pair of neighbours to a thread (and CH pairs tpt apart), so that a wave's reads
+// meet on few banks: 157 us where rows lie in their own order, TODO so.
+template <int CH>
+__global__ __launch_bounds__(256) void combine_slots_kernel(
+    SlotRows y, const int64_t* __restrict__ offs, int experts, int64_t y_rows,
+    const int64_t* __restrict__ slots, const float* __restrict__ weights, int64_t tokens, int k,
+    int tpt, const void* __restrict__ residual, int dt_res, void* __restrict__ out, int dt_out) {
+  extern __shared__ __attribute__((aligned(16))) uint16_t rows16[];
+  const int at = __builtin_amdgcn_readfirstlane(threadIdx.x / tpt), tid = threadIdx.x - at * tpt;
+  const int64_t tt = (int64_t)blockIdx.x * (256 / tpt) + at;
+  const bool live = tt < tokens;  // (all threads meet at the barriers)
+  const int64_t t = live ? tt : tokens - 1;
+  const int n = (int)y.n;
+  uint16_t* rows = rows16 + at * 4 * y.pitch;
+  const float up = ldexpf(1.0f, sum_exponent(y.largest, y.k));
+  float acc[CH][2];
+#pragma unroll
+  for (int h = 0; h < CH; ++h)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int c = 2 * (tid + h * tpt) + i;
+      acc[h][i] = residual && c < n ? load_as_f32(residual, t * n + c, dt_res) : 0.0f;
+    }
+  constexpr int IT = CH == 4 ? 2 : 4;  // pieces of a row's slots a thread
+  const int64_t ends = range_ends(offs, experts);
+  for (int j0 = 0; j0 < k; j0 += 4) {
+    const uint32_t* places[4];
+    float w[4], factor[4];
+    u32x4 raw[4][IT];
+    uint32_t p[CH][4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int j = j0 + u < k ? j0 + u : k - 1;
+      int64_t s = slots[t * k + j];
+      w[u] = weights[t * k + j];
+      if (s < 0 || s >= y_rows) {
+        w[u] = __builtin_nanf("");
+        s = 0;
+      }
+      factor[u] = y.scale[s];
+      places[u] = reinterpret_cast<const uint32_t*>(
+          y.places + (int64_t)expert_of(ends, offs, experts, s) * n);
+      const u32x4* from = reinterpret_cast<const u32x4*>(y.v + s * y.pitch);
+#pragma unroll
+      for (int i = 0; i < IT; ++i)
+        if (tid + i * tpt < y.pitch / 8) raw[u][i] = from[tid + i * tpt];
+    }
+#pragma unroll
+    for (int h = 0; h < CH; ++h)
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (2 * (tid + h * tpt) < n) p[h][u] = places[u][tid + h * tpt];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int i = 0; i < IT; ++i)
+        if (tid + i * tpt < y.pitch / 8)
+          reinterpret_cast<u32x4*>(rows + u * y.pitch)[tid + i * tpt] = raw[u][i];
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < CH; ++h) {
+      const int c = tid + h * tpt;
+      if (2 * c >= n) break;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (j0 + u >= k) break;
+        const uint16_t* row = rows + u * y.pitch;
+        const float a = f16_from_bits(row[p[h][u] & 0xffffu]) * up * factor[u];
+        const float b = f16_from_bits(row[p[h][u] >> 16]) * up * factor[u];
+        acc[h][0] = __builtin_fmaf(w[u], a, acc[h][0]);
+        acc[h][1] = __builtin_fmaf(w[u], b, acc[h][1]);
+      }
+    }
+    __syncthreads();
+  }
+  if (!live) return;
+#pragma unroll
+  for (int h = 0; h < CH; ++h) {
+    const int c = tid + h * tpt;
+    if (2 * c >= n) break;
+    const int64_t o = t * n + 2 * c;  // (even)
+    if (dt_out == 0)
+      *reinterpret_cast<float2*>(static_cast<float*>(out) + o) = make_float2(acc[h][0], acc[h][1]);
+    else
+      *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(out) + o) =
+          dt_out == 1 ? (uint32_t)f16_bits(acc[h][0]) | (uint32_t)f16_bits(acc[h][1]) << 16
+                      : (uint32_t)bf16_bits(acc[h][0]) | (uint32_t)bf16_bits(acc[h][1]) << 16;
   }
 }
 
@@ -628,9 +717,27 @@ __global__ void zero_i64_kernel(int64_t* p, int64_t n) {
 
 }  // namespace
 
-int launch_combine(const void* y, int dt_y, const RowFactor& f, int64_t y_rows, int64_t n,
+int launch_combine(const SlotRows& y, const int64_t* offs, int experts, int64_t y_rows,
                    const int64_t* slots, const float* weights, int64_t t, int64_t top_k,
                    const void* residual, int dt_residual, void* out, int dt_out, hipStream_t s) {
+  const int64_t pieces = y.n / 8;  // (n is a multiple of 16)
+  const int tpt = pieces <= 64 ? 64 : (pieces <= 128 ? 128 : 256), each = 256 / tpt;
+  const dim3 grid((unsigned)((t + each - 1) / each));
+  const size_t lds = (size_t)each * 4 * y.pitch * 2;
+  if (pieces <= 256)
+    combine_slots_kernel<4><<<grid, 256, lds, s>>>(y, offs, experts, y_rows, slots, weights, t,
+                                                   (int)top_k, tpt, residual, dt_residual, out,
+                                                   dt_out);
+  else
+    combine_slots_kernel<16><<<grid, 256, lds, s>>>(y, offs, experts, y_rows, slots, weights, t,
+                                                   (int)top_k, tpt, residual, dt_residual, out,
+                                                   dt_out);
+  return launch_status("moe_combine");
+}
+
+int launch_combine(const void* y, int dt_y, int64_t y_rows, int64_t n, const int64_t* slots,
+                   const float* weights, int64_t t, int64_t top_k, const void* residual,
+                   int dt_residual, void* out, int dt_out, hipStream_t s) {
   const int wide = dt_y == 0 ? 4 : 8;
   const int v = n % wide == 0 && (uintptr_t)y % 16 == 0 ? wide : 1;
   const int64_t pieces = n / v;
@@ -638,7 +745,7 @@ int launch_combine(const void* y, int dt_y, const RowFactor& f, int64_t y_rows, 
   const int64_t cols = (pieces + tpt - 1) / tpt;
   const dim3 grid((unsigned)((t + 256 / tpt - 1) / (256 / tpt)), (unsigned)(cols < 64 ? cols : 64));
 #define HI2X_COMBINE(DT, V)                                                                    \
-  combine_kernel<DT, V><<<grid, 256, 0, s>>>(y, f, y_rows, n, slots, weights, t, (int)top_k,   \
+  combine_kernel<DT, V><<<grid, 256, 0, s>>>(y, y_rows, n, slots, weights, t, (int)top_k,      \
                                              tpt, residual, dt_residual, out, dt_out)
   if (dt_y == 0) {
     if (v == 4)
@@ -781,7 +888,7 @@ extern "C" int hi2x_moe_combine(const void* y, int dt_y, int64_t y_rows, int64_t
                "moe_combine: bad shape");
   if (t == 0) return HI2X_OK;
   HI2X_REQUIRE((y || y_rows == 0) && slots && weights && out, "moe_combine: null buffer");
-  return launch_combine(y, dt_y, RowFactor{}, y_rows, n, slots, weights, t, top_k, residual,
+  return launch_combine(y, dt_y, y_rows, n, slots, weights, t, top_k, residual,
                         dt_residual, out, dt_out, as_stream(stream));
 }
 

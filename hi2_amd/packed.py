@@ -110,10 +110,11 @@ class _Packed:
         segs = np.zeros((e, len(CLASSES)), _SEGMENT)
         slot_rows = []
         codes_at = params_at = frag = 0
-        most, tiles = 0, np.zeros(3, np.int64)
+        most, tiles, starts = 0, np.zeros(3, np.int64), np.zeros(e, np.int64)
         for i, t in enumerate(tensors):
             cls = _classes_of(t, "tensor" if e == 1 else f"expert {i}")
             first = frag
+            starts[i] = FRAG * frag
             cut = np.zeros(3, np.int64)
             order = np.argsort(cls, kind="stable").astype(np.int32)
             ends = np.cumsum(np.bincount(cls, minlength=len(CLASSES)))
@@ -133,7 +134,15 @@ class _Packed:
             tiles = np.maximum(tiles, cut)
         self._codes = torch.empty(codes_at, dtype=torch.uint8, device=dev)
         self._params = torch.empty(params_at, dtype=torch.uint8, device=dev)
-        self._rows = _lib.h2d(torch.from_numpy(np.concatenate(slot_rows)), dev)
+        rows = np.concatenate(slot_rows)
+        self._rows = _lib.h2d(torch.from_numpy(rows), dev)
+        self._places = None
+        if 16 * most <= 8192:  # (beyond, nothing reads them)
+            places = np.empty((e, n), np.uint16)
+            at = np.flatnonzero(rows >= 0)
+            of = np.searchsorted(starts, at, side="right") - 1  # the expert of each slot
+            places[of, rows[at]] = at - starts[of]
+            self._places = _lib.h2d(torch.from_numpy(places.view(np.int16)), dev)
         self._segments = _lib.h2d(torch.from_numpy(segs.reshape(-1).view(np.uint8)), dev)
         def flat(parts, dtype):
             parts = [_lib.to_device(p.reshape(-1), dev, dtype) for p in parts]
@@ -180,7 +189,8 @@ class _Packed:
             self._segments.data_ptr(), e, n, k, kp, frag, most,
             (ctypes.c_int64 * 3)(*(int(v) for v in tiles)), self._had.data_ptr(),
             None if self._scale is None else self._scale.data_ptr(), int(self.transform is None),
-            self._largest.data_ptr(), first)
+            self._largest.data_ptr(), None if self._places is None else self._places.data_ptr(),
+            first)
         self._ref = ctypes.byref(self.desc)
         _lib.call("hi2x_packed_layout", dev, self._ref, _lib.ptr(words),
                   _lib.ptr(offs[0]), _lib.ptr(bytes_), _lib.ptr(offs[1]), _lib.ptr(consts))

@@ -550,6 +550,9 @@ typedef struct {
   const uint16_t* col_scale;           /* [k] fp16 smoothing, or NULL */
   int64_t per_expert;                  /* had and col_scale hold one row per expert */
   float* largest;                      /* the largest |weight| (hi2x_packed_layout writes it) */
+  const uint16_t* places;              /* [experts][n] the slot of each row in its expert, or
+                                          NULL (then, and past 8192 slots, hi2x_moe_mlp keeps
+                                          f32 between its products) */
   hi2x_packed_segment first[HI2X_PACKED_SEGMENTS]; /* expert 0's segments (host copy) */
 } hi2x_packed;
 

@@ -144,7 +144,9 @@ def test_tiles_of_experts(n, k, t, e, own, dev):
 
 
 @pytest.mark.parametrize("t,e,k,h,i", [(2, 8, 4, 1088, 256), (1, 2, 1, 128, 2304),
-                                       (2, 3, 2, 192, 1152), (40, 4, 2, 256, 512)])
+                                       (2, 3, 2, 192, 1152), (40, 4, 2, 256, 512),
+                                       (20, 2, 1, 2304, 1152), (20, 2, 1, 8256, 64),
+                                       (30, 70, 2, 128, 64), (9, 3, 3, 64, 5120)])
 @pytest.mark.parametrize("dt", ["bf16", "f32"])
 def test_gated_mlp_of_unlike_tensors(t, e, k, h, i, dt, dev):
     """gate, up and down cut into rows of different classes, gate and up of different
