@@ -491,35 +491,41 @@ def moe_mlp(x: torch.Tensor, routing, gate: PackedExperts, up: PackedExperts,
     if (gate.n, gate.k, gate.experts) != (up.n, up.k, up.experts) or \
             (down.k, down.n, down.experts) != (gate.n, gate.k, gate.experts):
         raise ValueError("gate and up [I, K] and down [K, I] of the same experts expected")
-    _same_device(gate, "moe_mlp", x, residual)
     if up.device != gate.device or down.device != gate.device:
         raise RuntimeError("gate, up and down are on different devices")
     if routing is None:
         raise TypeError("moe_mlp takes a Routing")
+    rows, offs = routing.rows.contiguous(), routing.offs.contiguous()
+    slots, weights = routing.slots.contiguous(), routing.weights.contiguous()
+    _same_device(gate, "moe_mlp", x, residual, rows, offs, slots, weights)
     _no_grad_inputs("moe_mlp", x)
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"activation {activation!r} ({', '.join(ACTIVATIONS)})")
     flat = _aligned(_rows_of(x, gate.k, "x"))
     t = flat.shape[0]
-    index, weights, slots = routing.index, routing.weights, routing.slots
-    if index.shape[0] != t:
-        raise ValueError(f"routing of {index.shape[0]} tokens for {t}")
-    if routing.offs.numel() != gate.experts + 1:
-        raise ValueError(f"routing over {routing.offs.numel() - 1} experts for {gate.experts}")
+    if slots.dim() != 2 or slots.shape[0] != t:
+        raise ValueError(f"routing of {slots.shape[0]} tokens for {t}")
+    if offs.numel() != gate.experts + 1:
+        raise ValueError(f"routing over {offs.numel() - 1} experts for {gate.experts}")
+    if weights.shape != slots.shape or rows.numel() != slots.numel() or slots.shape[1] < 1:
+        raise ValueError(f"routing: weights {tuple(weights.shape)}, slots {tuple(slots.shape)} "
+                         f"and {rows.numel()} rows do not belong together")
+    if rows.dtype != torch.int64 or offs.dtype != torch.int64 or slots.dtype != torch.int64 or \
+            weights.dtype != torch.float32:
+        raise ValueError("routing: rows, offs and slots int64 and weights float32 expected")
     if residual is not None:
         if residual.numel() != t * gate.k:
             raise ValueError(f"residual has shape {tuple(residual.shape)}, expected {(t, gate.k)}")
         residual = residual.reshape(t, gate.k).contiguous()
-    _same_device(gate, "moe_mlp", weights, slots)
     if torch.is_grad_enabled() and (weights.requires_grad or
                                     residual is not None and residual.requires_grad):
         with torch.no_grad():
             def part(p, v, **more):
-                return experts_linear(v, p, routing.offs, out_dtype=torch.float32, **more)
+                return experts_linear(v, p, offs, out_dtype=torch.float32, **more)
 
-            h = part(up, flat, rows=routing.rows)
-            h = part(gate, flat, rows=routing.rows, activation=activation, mul=h)
+            h = part(up, flat, rows=rows)
+            h = part(gate, flat, rows=rows, activation=activation, mul=h)
             y = part(down, h)
         return combine(y, slots, weights, residual, x.dtype).view(x.shape)
     dt = _dtype(x, "x")
@@ -528,15 +534,16 @@ def moe_mlp(x: torch.Tensor, routing, gate: PackedExperts, up: PackedExperts,
         return out
     # one fp16 plane of the hidden values (and fp16 between the products) is well below a bf16
     # result's own rounding, and half the products; next to an fp16 result it would show
-    npl, mid = _planes(x.dtype, gate), 1 if x.dtype == torch.bfloat16 else 2
-    top_k = index.shape[1]
+    npl, mid = max(_planes(x.dtype, gate), _planes(x.dtype, up)), 1 if dt == 2 else 2
+    top_k = slots.shape[1]
     shared = gate.transform is not None and gate.transform == up.transform
     size = _lib.lib().hi2x_moe_mlp_workspace_bytes(gate._ref, up._ref, down._ref, t, top_k, npl,
                                                    mid, shared)
     ws = torch.empty(max(size, 1), dtype=torch.uint8, device=gate.device)
-    _lib.call("hi2x_moe_mlp", gate.device, gate._ref, up._ref, down._ref, _lib.ptr(flat), dt,
-              _pitch(flat), t, top_k, npl, mid, shared, act, _lib.ptr(routing.rows),
-              _lib.ptr(routing.offs), _lib.ptr(slots), _lib.ptr(weights), _lib.ptr(residual),
-              0 if residual is None else _dtype(residual, "residual"), _lib.ptr(out), dt,
-              _lib.ptr(ws), size)
+    _lib.call("hi2x_moe_mlp", gate.device, gate._ref, up._ref, down._ref, flat.data_ptr(), dt,
+              _pitch(flat), t, top_k, npl, mid, shared, act, rows.data_ptr(), offs.data_ptr(),
+              slots.data_ptr(), weights.data_ptr(),
+              None if residual is None else residual.data_ptr(),
+              0 if residual is None else _dtype(residual, "residual"), out.data_ptr(), dt,
+              ws.data_ptr(), size)
     return out

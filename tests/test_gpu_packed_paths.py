@@ -205,3 +205,56 @@ def test_gated_mlp_at_any_scale(size, dev):
     else:
         rel = np.linalg.norm(N(got)[ok] - want[ok]) / np.linalg.norm(want[ok])
         assert rel < 2.0 ** -8, rel
+
+
+def test_gated_mlp_refuses_what_is_no_routing_of_its_tokens(dev):
+    from dataclasses import replace
+
+    from hi2_amd.moe import route
+    from hi2_amd.packed import PackedExperts, moe_mlp
+
+    gate, down = (PackedExperts(_experts(3, n, k, 5)[0], dev) for n, k in ((64, 128), (128, 64)))
+    x = tokens(6, 128, torch.bfloat16, 1, dev)
+    r = route(torch.randn(6, 3, generator=torch.Generator().manual_seed(2)).to(dev), 2)
+    good = moe_mlp(x, r, gate, gate, down)
+    for wrong, match in ((dict(rows=r.rows[:3]), "belong together"),
+                         (dict(weights=r.weights[:, :1]), "belong together"),
+                         (dict(slots=r.slots[:4]), "of 4 tokens for 6"),
+                         (dict(offs=r.offs[:3]), "over 2 experts for 3"),
+                         (dict(rows=r.rows.int()), "int64"),
+                         (dict(slots=r.slots.int()), "int64"),
+                         (dict(weights=r.weights.double()), "float32")):
+        with pytest.raises(ValueError, match=match):
+            moe_mlp(x, replace(r, **wrong), gate, gate, down)
+    with pytest.raises(RuntimeError):
+        moe_mlp(x, replace(r, offs=r.offs.cpu()), gate, gate, down)
+    same = replace(r, slots=r.slots.t().contiguous().t(), weights=r.weights.t().contiguous().t())
+    assert not same.slots.is_contiguous()
+    assert torch.equal(moe_mlp(x, same, gate, gate, down), good)
+
+
+def test_half_precision_mlp_with_one_plain_projection(dev):
+    """fp16 tokens that gate takes as they are and up rotates: the rotated ones need both
+    planes."""
+    from hi2_amd.moe import route
+    from hi2_amd.packed import PackedExperts, moe_mlp
+
+    t, e, k, h, i = 40, 3, 2, 128, 64
+    gs, us, ds = _experts(e, i, h, 100), _experts(e, i, h, 200), _experts(e, h, i, 300)
+    for g in gs[0]:
+        g.had[:] = 0
+    plans = [PackedExperts(s[0], dev) for s in (gs, us, ds)]
+    assert plans[0].plain and not plans[1].plain
+    x = tokens(t, h, torch.float16, 4, dev)
+    r = route(torch.randn(t, e, generator=torch.Generator().manual_seed(3)).to(dev), k)
+    got = moe_mlp(x, r, *plans)
+    index, w = N(r.index).astype(int), N(r.weights)
+    want = np.zeros((t, h))
+    for j in range(e):
+        tok, c = np.nonzero(index == j)
+        a = act64(stored(N(x)[tok], gs[0][j]) @ gs[1][j].T, "silu")
+        a = a * (stored(N(x)[tok], us[0][j]) @ us[1][j].T)
+        np.add.at(want, tok, w[tok, c][:, None] * (stored(a, ds[0][j]) @ ds[1][j].T))
+    # only the result's rounding: half an ulp of each, at most 2^-11 (one plane would add as much)
+    off = np.abs(N(got) - want) - 2.0 ** -11 * np.abs(want)
+    assert off.max() < 2.0 ** -13 * np.abs(want).max()
