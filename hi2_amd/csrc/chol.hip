@@ -660,8 +660,9 @@ __device__ __forceinline__ void g3_dma16(__amdgpu_buffer_rsrc_t rs, uint32_t vof
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
   // as inline assembly: the compiler would otherwise take the asynchronous LDS write for
-  // an alias of every later LDS read and wait for all loads in flight before each one
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+  // an alias of every later LDS read and wait for all loads in flight before each one (and would
+  // not add the wait state that the write of m0 needs in front of the load)
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                :
                : "s"(la), "v"(voff), "s"(rs)
                : "m0");

@@ -401,13 +401,14 @@ constexpr uint32_t SYRK_PB = 0u | 2u << 2 | 1u << 4 | 0u << 6 | 1u << 8 | 0u << 
 // wave-uniform).  Issued as inline assembly so that the compiler does not treat the
 // asynchronous LDS write as aliasing every later LDS read (it would wait for all loads
 // in flight before the first one); the kernel orders the writes itself with vmcnt waits
-// and barriers.  m0 holds the LDS address only for this instruction.
+// and barriers.  m0 holds the LDS address only for this instruction; the hardware wants one
+// wait state between its write and the load, which the compiler does not add in here.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void lds_dma16(__amdgpu_buffer_rsrc_t rs, uint32_t voff, void* lds) {
   const uint32_t la = __builtin_amdgcn_readfirstlane(
       (uint32_t)(size_t)(__attribute__((address_space(3))) void*)lds);
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                :
                : "s"(la), "v"(voff), "s"(rs)
                : "m0");

@@ -7,12 +7,13 @@ namespace {
 
 // 64 lanes x 16 bytes from global memory straight into LDS at byte `la` (+ 16 lane).  As
 // inline assembly: the compiler would otherwise take the asynchronous write for an alias of
-// every later LDS read and wait for all loads in flight before each one.
+// every later LDS read and wait for all loads in flight before each one.  The hardware wants one
+// wait state between the write of M0 and the load, which the compiler does not add in here.
 __device__ __forceinline__ void dma16(__amdgpu_buffer_rsrc_t rs, uint32_t voff, uint32_t soff,
                                       uint32_t la) {
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                :
                : "s"(la), "v"(voff), "s"(rs), "s"(soff)
                : "m0");
