@@ -405,7 +405,8 @@ constexpr int64_t FEW_RAW = 8;      // rows the few-rows kernel transforms for i
 constexpr int64_t FEW_RANGES = 16;  // and of all experts together
 
 // Activations as they are: rows ldx elements apart; with x2 (same type and pitch, 32 bits)
-// act(x) * x2 elementwise; without x act(s1) * s2, of the experts of `offs`.
+// act(x) * x2 elementwise; where s1 holds rows (s1.v) act(s1) * s2 instead, of the experts of
+// `offs`.  x may be null where there are no rows.
 struct RawRows {
   const void* x;
   int dtype;
@@ -444,6 +445,14 @@ inline bool few_raw_product(const hi2x_packed&, int64_t slots, bool ranges) {
 
 inline int64_t plane_bytes(const hi2x_packed& w, int64_t rows, int npl) {
   return rows * w.kp * 2 * npl;  // a multiple of 256
+}
+// Rows of the transform in front of a product: those of x, or every slot's by its own expert's
+// transform.  Of no rows at all (each index lies outside) it makes every slot a row of NaN.
+inline bool transform_slots(const hi2x_packed& w, int64_t x_rows) {
+  return w.per_expert || x_rows == 0;
+}
+inline int64_t transform_rows(const hi2x_packed& w, int64_t x_rows, bool indexed, int64_t slots) {
+  return !indexed || transform_slots(w, x_rows) ? slots : x_rows;
 }
 inline int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 

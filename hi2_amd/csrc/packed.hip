@@ -289,6 +289,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void activations_kernel(
 
 int launch_activations(const RawRows& x, const hi2x_packed& w, const int64_t* src,
                        const int64_t* offs, const hi2x_activations& out, hipStream_t s) {
+  if (out.rows == 0) return HI2X_OK;
 #define HI2X_ROWS_(DT, GLU, KEEP, TPR)                                                    \
   activations_kernel<DT, GLU, KEEP, TPR>                                                  \
       <<<dim3((unsigned)(TPR < 256 ? (out.rows * TPR + 255) / 256 : out.rows)),           \
@@ -310,7 +311,7 @@ int launch_activations(const RawRows& x, const hi2x_packed& w, const int64_t* sr
     else                                   \
       HI2X_ROWS_(DT, GLU, false, 1024);    \
   }
-  if (!x.x) {
+  if (x.s1.v) {
     HI2X_ROWS(SLOTS, true)
   } else if (x.x2) {
     HI2X_ROWS(0, true)

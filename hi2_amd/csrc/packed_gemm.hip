@@ -578,10 +578,10 @@ extern "C" int hi2x_packed_linear(const hi2x_packed* w, const void* x, int dtype
   const RawRows raw{x, dtype, ldx, x_rows, nplanes};
   GemmArgs g{*w, hi2x_activations{}, src, offs, slots, *epi};
   if (few_raw_product(*w, slots, offs)) return packed_few_raw(GemmPair{{g, g}}, 1, raw, s);
-  // the transform of the rows of x, or of every slot by its own expert's
-  const int64_t rows = w->per_expert ? slots : (src ? x_rows : slots);
+  const bool each = transform_slots(*w, x_rows);
+  const int64_t rows = transform_rows(*w, x_rows, src, slots);
   HI2X_REQUIRE(rows < (1ll << 31), "packed_linear: too many rows");
-  HI2X_REQUIRE(!src || w->per_expert || rows * w->kp * 2 * nplanes < (1ll << 32) - 1,
+  HI2X_REQUIRE(!src || each || rows * w->kp * 2 * nplanes < (1ll << 32) - 1,
                "packed_linear: 4 GiB of activations or more cannot be taken by index");
   Workspace ws;
   const int64_t need = hi2x_packed_workspace_bytes(w, x_rows, nplanes, 0, slots, src != nullptr,
@@ -590,10 +590,10 @@ extern "C" int hi2x_packed_linear(const hi2x_packed* w, const void* x, int dtype
   const int64_t pb = plane_bytes(*w, rows, nplanes);
   g.x = hi2x_activations{reinterpret_cast<uint16_t*>(ws.p), reinterpret_cast<float*>(ws.p + pb),
                          rows, w->kp, nplanes, 0};
-  if (int rc = launch_activations(raw, *w, w->per_expert ? src : nullptr,
-                                  w->per_expert ? offs : nullptr, g.x, s))
+  if (int rc = launch_activations(raw, *w, each ? src : nullptr, w->per_expert ? offs : nullptr,
+                                  g.x, s))
     return rc;
-  if (w->per_expert) g.src = nullptr;
+  if (each) g.src = nullptr;
   const int64_t used = pb + align256(rows * 4);
   return packed_product(GemmPair{{g, g}}, 1, ws.p + used, need - used, s);
 }
@@ -608,7 +608,7 @@ extern "C" int64_t hi2x_packed_workspace_bytes(const hi2x_packed* w, int64_t x_r
   int64_t front = 0;
   if (!given) {
     if (few_raw_product(*w, slots, ranges)) return 0;
-    const int64_t rows = w->per_expert ? slots : (indexed ? x_rows : slots);
+    const int64_t rows = transform_rows(*w, x_rows, indexed, slots);
     front = plane_bytes(*w, rows, nplanes) + align256(rows * 4);
   }
   return front + packed_part_bytes(*w, slots, ranges, nplanes);

@@ -605,17 +605,17 @@ typedef struct {
 } hi2x_epilogue;
 
 /* out[slot] = epilogue(T(x)[src[slot]] Wq^T) for every slot (src NULL: the slot itself; an
- * index outside [0, x_rows): a row of NaN).  With several experts offs [experts + 1] gives
- * each one's slot range and must cover all slots; offs NULL: one expert.  x as for
- * hi2x_packed_activations; nplanes 1 or 2: the planes its transform is held in.  Few rows
- * are transformed inside the product, in one launch; others in a pass of their own.
- * Workspace: hi2x_packed_workspace_bytes. */
+ * index outside [0, x_rows), every one where x has no rows and may be NULL: a row of NaN).
+ * With several experts offs [experts + 1] gives each one's slot range and must cover all slots;
+ * offs NULL: one expert.  x as for hi2x_packed_activations; nplanes 1 or 2: the planes its
+ * transform is held in.  Few rows are transformed inside the product, in one launch; others in
+ * a pass of their own.  Workspace: hi2x_packed_workspace_bytes. */
 int hi2x_packed_linear(const hi2x_packed* w, const void* x, int dtype, int64_t ldx,
                        int64_t x_rows, int nplanes, const int64_t* src, const int64_t* offs,
                        int64_t slots, const hi2x_epilogue* epi, void* ws, int64_t ws_bytes,
                        void* stream);
 
-/* The same from transformed activations (tensors that share their input). */
+/* The same from transformed activations (tensors that share their input), one row at least. */
 int hi2x_packed_linear_activations(const hi2x_packed* w, const hi2x_activations* x,
                                    const int64_t* src, const int64_t* offs, int64_t slots,
                                    const hi2x_epilogue* epi, void* ws, int64_t ws_bytes,

@@ -1,0 +1,17 @@
+"""The host side of the packed products: sizes and checks that need no GPU."""
+
+import ctypes
+
+from hi2_amd import _lib
+from test_packed_abi import packed
+
+
+def test_workspace_of_slots_that_index_no_rows():
+    """Every index lies outside an empty batch: each slot becomes a row of NaN of its own, so
+    the workspace holds the slots' rows, not the batch's."""
+    size = _lib.lib().hi2x_packed_workspace_bytes
+    for w in (packed(), packed(experts=4), packed(experts=4, per_expert=1)):
+        ranges = int(w.experts > 1)
+        some = size(ctypes.byref(w), 0, 2, 0, 40, 1, ranges)
+        assert some >= 40 * 128 * 2 * 2 + 40 * 4
+        assert size(ctypes.byref(w), 0, 2, 0, 0, 1, ranges) == 0
