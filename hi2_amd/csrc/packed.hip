@@ -65,7 +65,7 @@ __global__ __launch_bounds__(256) void layout_params_kernel(
     const float l = f16_from_bits((uint16_t)v), steps = (float)((1 << sg.nbits) - 1);
     const float h = f16_from_bits(f16_bits(__builtin_fmaf(steps, f16_from_bits(v >> 16), l)));
     most = fmaxf(fabsf(l), fabsf(h));
-    most = most < __builtin_inff() ? most : 0.0f;
+    most = most < 65504.0f ? most : 65504.0f;  // (steps below an infinite one are finite)
   }
   if (in) reinterpret_cast<uint32_t*>(static_cast<char*>(w.params) + sg.params)[i] = v;
 #pragma unroll

@@ -2,10 +2,12 @@
 
 import ctypes
 
+import numpy as np
 import pytest
 import torch
 
-from test_gpu_packed import F, _experts
+from packed_data import act64, stored
+from test_gpu_packed import F, N, _experts, tokens
 
 pytestmark = pytest.mark.gpu
 
@@ -43,3 +45,52 @@ def test_activations_of_an_empty_batch_are_nan(own, dev):
     _lib.call("hi2x_packed_activations", dev, ctypes.byref(plan.desc), None, 2, 192, 0,
               _lib.ptr(src), _lib.ptr(offs), ctypes.byref(desc))
     assert torch.isnan(scale).all() and not planes.any()
+
+
+def mlp64(x, r, gate, up, down, act="relu"):
+    """The gated MLP in float64: gate, up and down each (tensors, decoded weights)."""
+    index, w = N(r.index).astype(int), N(r.weights)
+    out = np.zeros((len(x), down[1][0].shape[0]))
+    for e in range(len(gate[0])):
+        tok, c = np.nonzero(index == e)
+        if not len(tok):
+            continue
+        a = act64(stored(N(x)[tok], gate[0][e]) @ gate[1][e].T, act)
+        a = a * (stored(N(x)[tok], up[0][e]) @ up[1][e].T)
+        np.add.at(out, tok, w[tok, c][:, None] * (stored(a, down[0][e]) @ down[1][e].T))
+    return out
+
+
+def huge_row(t, w, row):
+    """Row `row` of INT4 in steps of about 5000, codes up to 11: its weights are finite, the
+    ladder's last step is not."""
+    k = t.shape[1]
+    assert t.row_nbits[row] == 4
+    t.row_consts[row] = torch.tensor([0.0, 0.0, 19.6]).half()
+    blocks = slice(2 * int(t.param_off[row]), 2 * int(t.param_off[row + 1]))
+    t.blk_params[blocks] = 255
+    words = t.codes[int(t.code_off[row]):int(t.code_off[row + 1])]
+    words &= int(np.uint32(0xBBBBBBBB).view(np.int32))
+    codes = (words.numpy().view(np.uint32)[:, None] >> (4 * np.arange(8, dtype=np.uint32))) & 15
+    step = np.float64(np.float16(np.float32(255 * np.float64(np.float16(19.6)))))
+    w[row] = (codes.reshape(k) * step).astype(np.float16).astype(np.float64)
+    assert np.isfinite(w[row]).all() and np.isinf(np.float16(15 * step))
+
+
+def test_mlp_of_weights_below_an_infinite_step(dev):
+    """A ladder whose last steps overflow fp16 and are not used: every weight and result is
+    finite, in one call as in its parts."""
+    from hi2_amd.moe import route
+    from hi2_amd.packed import PackedExperts, moe_mlp
+
+    t, e, k, h, i = 60, 3, 2, 128, 64
+    gs, us, ds = _experts(e, i, h, 100), _experts(e, i, h, 200), _experts(e, h, i, 300)
+    for ts, ws in (gs, us, ds):
+        huge_row(ts[1], ws[1], int(torch.nonzero(ts[1].row_nbits == 4)[0]))
+    plans = [PackedExperts(s[0], dev) for s in (gs, us, ds)]
+    x = tokens(t, h, torch.bfloat16, 4, dev)
+    r = route(torch.randn(t, e, generator=torch.Generator().manual_seed(3)).to(dev), k)
+    got, want = N(moe_mlp(x, r, *plans, activation="relu")), mlp64(x, r, gs, us, ds)
+    assert np.isfinite(got).all()
+    # the roundings of the tokens, the hidden values and the result, as in the other MLP tests
+    assert np.linalg.norm(got - want) < 2.0 ** -8 * np.linalg.norm(want)
