@@ -37,6 +37,7 @@ __device__ __forceinline__ int umin_(int a, int b) {
   return (int)((uint32_t)a < (uint32_t)b ? (uint32_t)a : (uint32_t)b);
 }
 __device__ __forceinline__ int or_(int a, int b) { return a | b; }
+__device__ __forceinline__ int imax_(int a, int b) { return a > b ? a : b; }
 __device__ __forceinline__ uint32_t row_umax(uint32_t v) {
   int x = (int)v;
   HI2X_ROW16(x, umax_)
@@ -211,11 +212,11 @@ __device__ __forceinline__ PkWork find_work(const int64_t* offs, int experts, in
   return w;
 }
 
-// `scaled16`: the result is handed on in fp16 without its row's factor and times 2^-c of
-// sum_exponent, each row in the order of its expert's slots, for a kernel that reads it with a
-// SlotRows.  (Scattered to the rows' own order, a lane would store single values: the stores
-// alone took a quarter of the products of 64 experts of 2048 x 1024 at 16384 tokens, gate and up
-// 1316 us and 1152 so, down 847 and 623.)
+// `exps`: the result is handed on in fp16 without its row's factor, each row in the order of its
+// expert's slots and each fragment of 16 slots under a power of two of its own, 2^c with c in
+// exps[slot][fragment], for a kernel that reads it with a SlotRows.  (Scattered to the rows' own
+// order, a lane would store single values: the stores alone took a quarter of the products of 64
+// experts of 2048 x 1024 at 16384 tokens, gate and up 1316 us and 1152 so, down 847 and 623.)
 struct GemmArgs {
   hi2x_packed w;
   hi2x_activations x;
@@ -223,35 +224,34 @@ struct GemmArgs {
   const int64_t* offs;
   int64_t slots;
   hi2x_epilogue epi;
-  bool scaled16 = false;
+  int8_t* exps = nullptr;
+  int ep = 0;  // bytes of a row of exps: the most fragments of an expert, a multiple of 4
 };
 
-// c with |sum| < 2^15 2^c for any row's product with k weights: its activations are at most
-// 2^15, the weights *largest.
-__device__ __forceinline__ int sum_exponent(const float* largest, int64_t k) {
-  const float most = *largest * (float)k;
-  int c = 0;
-  if (most > 0.0f) (void)frexpf(most, &c);
-  return c;
-}
+// The largest finite value of a fragment comes to [2^14, 2^15): its others keep fp16's 11 bits
+// down to 2^-28 of it, and what is lost below is 2^-39 of it, whatever the sizes of the experts,
+// the rows and their channels.  (Under one bound for all experts' sums a row far below it lost
+// its bits.)  EXP_LEAST keeps 2^c and 2^-c normal floats.
+constexpr int EXP_LEAST = -120;
+inline int exps_pitch(const hi2x_packed& w) { return (int)((w.max_frags + 3) / 4 * 4); }
 
-// Rows of a scaled16 product of w [n][k]: `pitch` values each; 2^c and the factor of the row's
-// activations take them back, `places` says where a column lies.
+// Rows of such a product of w [n][.]: `pitch` values each, of which `places` says where a column
+// lies; its fragment's exponent and the factor of the row's activations take it back.
 struct SlotRows {
   const uint16_t* v = nullptr;
   int pitch = 0;
   const uint16_t* places = nullptr;
+  const int8_t* exps = nullptr;
+  int ep = 0;
   const float* scale = nullptr;
   const int64_t* index = nullptr;  // row of scale, or null: the row itself
   int64_t rows = 0;                // of scale
-  const float* largest = nullptr;
-  int64_t n = 0, k = 0;
+  int64_t n = 0;
 };
 __device__ __forceinline__ float row_factor(const SlotRows& f, int64_t row) {
   const int64_t r = f.index ? f.index[row] : row;
   return r >= 0 && r < f.rows ? f.scale[r] : __builtin_nanf("");
 }
-
 // The expert whose range holds a slot (the same for the wave): as many as end at or before it
 // come before it; the last one where the ranges end too early.  `ends` are the lanes' own of
 // the first 64 experts (range_ends).
@@ -268,7 +268,7 @@ __device__ __forceinline__ int expert_of(int64_t ends, const int64_t* offs, int 
   }
   return e < experts ? e : experts - 1;
 }
-constexpr int SLOTS16 = 8192;  // most slots of a row of SlotRows (two of them, or four, in LDS)
+constexpr int SLOTS16 = 8192;  // most slots of a row of SlotRows (two of them lie in LDS)
 
 // Loads go through buffer resources: a lane's offset is one 32-bit register, the walk along
 // the columns is a scalar offset, and what lies past the resource reads as zero.

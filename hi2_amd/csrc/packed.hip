@@ -77,23 +77,22 @@ __global__ __launch_bounds__(256) void layout_params_kernel(
 }
 
 // ---- activations -------------------------------------------------------------------------
-// Rows of SlotRows on their way through LDS: `a` and `b` hold them slot by slot, then column by
-// column.  Lanes take neighbouring columns, whose places are almost neighbours too, so that the
-// reads by place meet on few banks; all of a row's loads are in flight before the first is
-// waited for (131072 x 1024 hidden rows of 64 experts 386 us without that).
-struct SlotRow {
-  uint16_t *a, *b;
-  float up[2], factor[2];
-};
+// Rows of SlotRows on their way through LDS: `a` and `b` hold them and their exponents slot by
+// slot, then act(a) * b column by column takes their room.  Lanes take neighbouring columns, whose
+// places are almost neighbours too, so that the reads by place meet on few banks; all of a row's
+// loads are in flight before the first is waited for (131072 x 1024 hidden rows of 64 experts 386
+// us without that).
 template <int TPR>
 struct SlotColumns {
   u32x4 raw[3];       // the row's slots, 8 at a time
+  uint32_t exps;      // four fragments' exponents
   uint32_t place[8];  // of the columns' pairs
   __device__ __forceinline__ void load(const SlotRows& s, int64_t row, int tid) {
     const u32x4* from = reinterpret_cast<const u32x4*>(s.v + row * s.pitch);
 #pragma unroll
     for (int i = 0; i < 3; ++i)
       raw[i] = tid + TPR * i < s.pitch / 8 ? from[tid + TPR * i] : u32x4{0u, 0u, 0u, 0u};
+    exps = 4 * tid < s.ep ? reinterpret_cast<const uint32_t*>(s.exps + row * s.ep)[tid] : 0u;
   }
   __device__ __forceinline__ void load_places(const SlotRows& s, int expert, int tid) {
     const uint32_t* from = reinterpret_cast<const uint32_t*>(s.places + expert * s.n);
@@ -101,44 +100,48 @@ struct SlotColumns {
     for (int i = 0; i < 8; ++i)
       place[i] = 2 * (tid + TPR * i) < s.n ? from[tid + TPR * i] : 0u;
   }
-  __device__ __forceinline__ void put_slots(const SlotRows& s, uint16_t* row, int tid) const {
+  __device__ __forceinline__ void put(const SlotRows& s, uint16_t* row, int8_t* ex,
+                                      int tid) const {
 #pragma unroll
     for (int i = 0; i < 3; ++i)
       if (tid + TPR * i < s.pitch / 8) reinterpret_cast<u32x4*>(row)[tid + TPR * i] = raw[i];
+    if (4 * tid < s.ep) reinterpret_cast<uint32_t*>(ex)[tid] = exps;
   }
-  __device__ __forceinline__ void take_columns(const uint16_t* row) {
+  __device__ __forceinline__ void take(const uint16_t* row, const int8_t* ex, float factor,
+                                       float (&v)[16]) const {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      place[i] = (uint32_t)row[place[i] & 0xffffu] | (uint32_t)row[place[i] >> 16] << 16;
-  }
-  __device__ __forceinline__ void put_columns(const SlotRows& s, uint16_t* row, int tid) const {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (2 * (tid + TPR * i) < s.n) reinterpret_cast<uint32_t*>(row)[tid + TPR * i] = place[i];
+    for (int i = 0; i < 16; ++i) {
+      const uint32_t p = i & 1 ? place[i >> 1] >> 16 : place[i >> 1] & 0xffffu;
+      v[i] = ldexpf(f16_from_bits(row[p]), ex[p >> 4]) * factor;
+    }
   }
 };
+// Bytes of a row's slots and exponents in LDS; the columns in the slots' room: 16-byte piece q
+// of group g at q ^ (g / 4 % 4), so that the lanes' reads of whole groups fall on different banks.
+__host__ __device__ inline int slot_bytes(const SlotRows& a, const SlotRows& b) {
+  return (2 * (a.pitch + b.pitch) + a.ep + b.ep + 15) / 16 * 16;
+}
+__device__ __forceinline__ int group_piece(int g, int q) { return 4 * g + (q ^ (g >> 2 & 3)); }
 
 // The 16 values of group g of a row, divided by their smoothing: of x, or (GLU) of
-// act(x) * x2, or (SLOTS) of act(s1) * s2 from LDS.
+// act(x) * x2, or (SLOTS) of `sr` in LDS.
 constexpr int SLOTS = 3;  // a type of its own
 template <int DT, bool GLU>
-__device__ __forceinline__ void group_values(const RawRows& x, const SlotRow& sr, int64_t base,
+__device__ __forceinline__ void group_values(const RawRows& x, const f32x4v* sr, int64_t base,
                                              int g, const uint16_t* cs, float (&v)[16]) {
-  auto scaled = [&](const uint16_t* row, int o, float (&u)[16]) {
-    load16(row, 16 * (int64_t)g, 1, u);
+  if constexpr (DT == SLOTS) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) u[i] = u[i] * sr.up[o] * sr.factor[o];
-  };
-  if constexpr (DT == SLOTS)
-    scaled(sr.a, 0, v);
-  else
+    for (int q = 0; q < 4; ++q) {
+      const f32x4v u = sr[group_piece(g, q)];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[4 * q + i] = u[i];
+    }
+  } else {
     load16(x.x, base + 16 * (int64_t)g, DT, v);
+  }
   if constexpr (GLU) {
     float u[16];
-    if constexpr (DT == SLOTS)
-      scaled(sr.b, 1, u);
-    else
-      load16(x.x2, base + 16 * (int64_t)g, 0, u);
+    load16(x.x2, base + 16 * (int64_t)g, 0, u);
     activate_all(v, x.act);
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] *= u[i];
@@ -184,32 +187,37 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void activations_kernel(
     had += (int64_t)expert * (k / 16);
     if (cs) cs += (int64_t)expert * k;
   }
-  SlotRow sr;
+  f32x4v* sr = nullptr;
   if constexpr (DT == SLOTS) {
-    extern __shared__ __attribute__((aligned(16))) uint16_t rows16[];
-    uint16_t* a = rows16 + (threadIdx.x / TPR) * (x.s1.pitch + x.s2.pitch);
-    uint16_t* b = a + x.s1.pitch;
-    sr = SlotRow{a, b, {}, {}};
+    extern __shared__ __attribute__((aligned(16))) char rows16[];
+    char* lds = rows16 + threadIdx.x / TPR * slot_bytes(x.s1, x.s2);
+    uint16_t *a = reinterpret_cast<uint16_t*>(lds), *b = a + x.s1.pitch;
+    int8_t *ea = reinterpret_cast<int8_t*>(b + x.s2.pitch), *eb = ea + x.s1.ep;
+    const float fa = row_factor(x.s1, none ? 0 : row), fb = row_factor(x.s2, none ? 0 : row);
+    sr = reinterpret_cast<f32x4v*>(lds);
     ca.load_places(x.s1, expert, tid);
     cb.load_places(x.s2, expert, tid);
-    sr.up[0] = ldexpf(1.0f, sum_exponent(x.s1.largest, x.s1.k));
-    sr.factor[0] = row_factor(x.s1, none ? 0 : row);
-    sr.up[1] = ldexpf(1.0f, sum_exponent(x.s2.largest, x.s2.k));
-    sr.factor[1] = row_factor(x.s2, none ? 0 : row);
     auto meet = [] {  // of the row's threads
       if constexpr (TPR > 64)
         __syncthreads();
       else
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup", "local");
     };
-    ca.put_slots(x.s1, a, tid);
-    cb.put_slots(x.s2, b, tid);
+    ca.put(x.s1, a, ea, tid);
+    cb.put(x.s2, b, eb, tid);
     meet();
-    ca.take_columns(a);
-    cb.take_columns(b);
+    float v[16], u[16];
+    ca.take(a, ea, fa, v);
+    cb.take(b, eb, fb, u);
     meet();
-    ca.put_columns(x.s1, a, tid);
-    cb.put_columns(x.s2, b, tid);
+    activate_all(v, x.act);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int p = tid + TPR * i;  // a pair of columns
+      if (2 * p < x.s1.n)
+        reinterpret_cast<float2*>(sr + group_piece(p >> 3, p >> 1 & 3))[p & 1] =
+            make_float2(v[2 * i] * u[2 * i], v[2 * i + 1] * u[2 * i + 1]);
+    }
     meet();
   }
   const int groups = (int)(k / 16), all = (int)(out.kp / 16);
@@ -294,7 +302,7 @@ int launch_activations(const RawRows& x, const hi2x_packed& w, const int64_t* sr
   activations_kernel<DT, GLU, KEEP, TPR>                                                  \
       <<<dim3((unsigned)(TPR < 256 ? (out.rows * TPR + 255) / 256 : out.rows)),           \
          TPR < 256 ? 256 : TPR,                                                           \
-         DT == SLOTS ? (TPR < 256 ? 256 / TPR : 1) * (x.s1.pitch + x.s2.pitch) * 2 : 0,   \
+         DT == SLOTS ? (TPR < 256 ? 256 / TPR : 1) * slot_bytes(x.s1, x.s2) : 0,          \
          s>>>(x, w.k, src, w.had, w.col_scale, offs, (int)w.experts, out)
 #define HI2X_ROWS(DT, GLU)                 \
   if (w.kp <= 1024)                        \
@@ -312,7 +320,7 @@ int launch_activations(const RawRows& x, const hi2x_packed& w, const int64_t* sr
       HI2X_ROWS_(DT, GLU, false, 1024);    \
   }
   if (x.s1.v) {
-    HI2X_ROWS(SLOTS, true)
+    HI2X_ROWS(SLOTS, false)
   } else if (x.x2) {
     HI2X_ROWS(0, true)
   } else if (x.dtype == 0) {

@@ -201,18 +201,36 @@ __device__ __forceinline__ void store_pass(const hi2x_epilogue& E, const float* 
   }
 }
 
-// The store of a pass of a scaled16 product: the slots as they lie, 8 to a thread, from slot
-// `at` of the output's rows on.
+// The store of a pass of a product with exponents: the slots as they lie, 8 to a thread and two
+// threads to a fragment, from slot `at` of the output's rows on.  (The exponents cost the products
+// of 64 experts at 16384 tokens 2 to 3 %; several rows of a thread at a time no less.)
 template <int NS, int PITCH>
-__device__ __forceinline__ void store_slots(const hi2x_epilogue& E, const float* ep, float scale,
-                                            int at, int slots, int64_t o0, int rows) {
+__device__ __forceinline__ void store_slots(const GemmArgs& g, const float* ep, int at, int slots,
+                                            int64_t o0, int rows) {
   constexpr int TPR = NS / 8;
   const int slot = threadIdx.x % TPR * 8;
   if (slot >= slots) return;
+  const hi2x_epilogue& E = g.epi;
   uint16_t* out = static_cast<uint16_t*>(E.out) + o0 * E.ld_out + at + slot;
+  int8_t* exps = g.exps + o0 * g.ep + (at + slot) / 16;
   for (int t = threadIdx.x / TPR; t < rows; t += 256 / TPR) {
     const f32x4v* from = reinterpret_cast<const f32x4v*>(ep + t * PITCH + slot);
     const f32x4v a = from[0], b = from[1];
+    float m = 0.0f;  // the largest finite one (NaN is passed over)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = fmaxf(m, fmaxf(fabsf(a[i]), fabsf(b[i])));
+    if (m == __builtin_inff()) {
+      m = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float x = fabsf(i < 4 ? a[i] : b[i - 4]);
+        m = fmaxf(m, x < __builtin_inff() ? x : 0.0f);
+      }
+    }
+    m = fmaxf(m, __int_as_float(dpp<0xB1>(__float_as_int(m))));
+    // by the bits of m: 2^(e - 127) <= m < 2^(e - 126), and 2^c is a normal float
+    const int c = m > 0.0f ? imax_((__float_as_int(m) >> 23) - 141, EXP_LEAST) : 0;
+    const float scale = __int_as_float((127 - c) << 23);  // 2^-c
     u32x4 v;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -220,6 +238,7 @@ __device__ __forceinline__ void store_slots(const hi2x_epilogue& E, const float*
       v[i] = (uint32_t)f16_bits(x * scale) | (uint32_t)f16_bits(y * scale) << 16;
     }
     *reinterpret_cast<u32x4*>(out + t * E.ld_out) = v;
+    if (!(slot & 8)) exps[t * g.ep] = (int8_t)c;
   }
 }
 
@@ -329,7 +348,6 @@ void packed_gemm_kernel(GemmPair two, float* part, int per, int nx) {
     xoff[i] = (uint32_t)r * pitch + 16 * ((lane & 15) ^ (t & 15));
   }
   if (tid < MT) xscale[tid] = row_scale(g, first, tid, live);
-  const float scale = g.scaled16 ? ldexpf(1.0f, -sum_exponent(g.w.largest, g.w.k)) : 0.0f;
   const int nch = (int)(g.w.kp / PK_CHUNK);
   const int c0 = SPLIT ? (int)blockIdx.z * per : 0;
   const int c1 = SPLIT && c0 + per < nch ? c0 + per : nch;
@@ -385,9 +403,9 @@ void packed_gemm_kernel(GemmPair two, float* part, int per, int nx) {
                                      4 * (lane >> 4)) = acc[f][p * (EH / 16) + m];
     __syncthreads();
     const int rows = live - p * EH < EH ? live - p * EH : EH;
-    if (g.scaled16)
-      store_slots<NS, PITCH>(g.epi, ep, scale, 16 * (tile.frag - tile.base), 16 * tile.count,
-                             first + p * EH, rows);
+    if (g.exps)
+      store_slots<NS, PITCH>(g, ep, 16 * (tile.frag - tile.base), 16 * tile.count, first + p * EH,
+                             rows);
     else
       store_pass<NS, PITCH, EH, 8>(g.epi, ep, xscale + p * EH, n, bias, first + p * EH, rows);
   }
@@ -619,8 +637,9 @@ namespace {
 
 // Where the parts of hi2x_moe_mlp's workspace begin.
 struct MlpSpace {
-  bool half;                    // gate, up and y as scaled16, else f32
+  bool half;                    // gate, up and y with exponents, else f32
   int64_t gate, up, y;          // [slots][i], [slots][i], [slots][h]
+  int64_t exps[3];              // their fragments' exponents
   int64_t in[2], in_scale[2];   // the transformed tokens: shared, or per tensor
   int64_t mid, mid_scale;       // the transformed hidden values
   int64_t in_rows[2];
@@ -636,17 +655,19 @@ MlpSpace mlp_space(const hi2x_packed& gate, const hi2x_packed& up, const hi2x_pa
     at += align256(n);
     return a;
   };
-  // A bf16 result hides the rounding of scaled16 (2^-11) as it hides that of one plane;
+  // A bf16 result hides the rounding to fp16 (2^-11) as it hides that of one plane;
   // writing and reading the three is what the large calls are short of: 64 experts of
   // 2048 x 1024, 8 choices, 16384 tokens 2680 us in f32, 2060 so.  Short calls keep f32.
   m.half = npl_mid == 1 && !few_raw_product(gate, slots, true);
   for (const hi2x_packed* p : {&gate, &up, &down})
-    m.half = m.half && p->places && p->largest && 16 * p->max_frags <= SLOTS16 &&
+    m.half = m.half && p->places && 16 * p->max_frags <= SLOTS16 &&
              16 * p->max_frags <= p->n + 16 * PK_SEGS;  // (as many as the readers' loads take)
   const int64_t size = m.half ? 2 : 4;
   m.gate = take(slots * (m.half ? 16 * gate.max_frags : gate.n) * size);
   m.up = take(slots * (m.half ? 16 * up.max_frags : gate.n) * size);
   m.y = take(slots * (m.half ? 16 * down.max_frags : down.n) * size);
+  const hi2x_packed* of[3] = {&gate, &up, &down};
+  for (int i = 0; i < 3 && m.half; ++i) m.exps[i] = take(slots * exps_pitch(*of[i]));
   if (!few_raw_product(gate, slots, true)) {
     for (int i = 0; i < (shared ? 1 : 2); ++i) {
       m.in_rows[i] = (i ? up : gate).per_expert ? slots : t;
@@ -710,15 +731,18 @@ extern "C" int hi2x_moe_mlp(const hi2x_packed* gate, const hi2x_packed* up,
   const MlpSpace m = mlp_space(*gate, *up, *down, t, n, nplanes, nplanes_mid, shared);
   Workspace w;
   if (int rc = take_workspace(w, ws, ws_bytes, (size_t)m.bytes, s, "moe_mlp")) return rc;
-  auto to = [&](int64_t at, const hi2x_packed& p) {
-    hi2x_epilogue e{};
-    e.out = w.p + at;
-    e.ld_out = m.half ? 16 * p.max_frags : p.n;
-    return e;
+  auto product = [&](const hi2x_packed& p, const int64_t* src, int64_t at, int64_t exps) {
+    GemmArgs g{p, hi2x_activations{}, src, offs, n, hi2x_epilogue{}};
+    g.epi.out = w.p + at;
+    g.epi.ld_out = m.half ? 16 * p.max_frags : p.n;
+    if (m.half) {
+      g.exps = reinterpret_cast<int8_t*>(w.p + exps);
+      g.ep = exps_pitch(p);
+    }
+    return g;
   };
-  GemmPair in{{GemmArgs{*gate, hi2x_activations{}, rows, offs, n, to(m.gate, *gate), m.half},
-               GemmArgs{*up, hi2x_activations{}, rows, offs, n, to(m.up, *up), m.half}}};
-  GemmArgs last{*down, hi2x_activations{}, nullptr, offs, n, to(m.y, *down), m.half};
+  GemmPair in{{product(*gate, rows, m.gate, m.exps[0]), product(*up, rows, m.up, m.exps[1])}};
+  GemmArgs last = product(*down, nullptr, m.y, m.exps[2]);
   const RawRows tokens{x, dtype, ldx, t, nplanes};
   RawRows hidden{w.p + m.gate, 0, gate->n, n, nplanes_mid,
                  reinterpret_cast<const float*>(w.p + m.up), act};
@@ -742,7 +766,7 @@ extern "C" int hi2x_moe_mlp(const hi2x_packed* gate, const hi2x_packed* up,
     if (m.half) {
       auto rows_of = [](const GemmArgs& g) {
         return SlotRows{static_cast<const uint16_t*>(g.epi.out), (int)g.epi.ld_out, g.w.places,
-                        g.x.scale, g.src, g.x.rows, g.w.largest, g.w.n, g.w.k};
+                        g.exps, g.ep, g.x.scale, g.src, g.x.rows, g.w.n};
       };
       hidden.x = nullptr;
       hidden.s1 = rows_of(in.g[0]);

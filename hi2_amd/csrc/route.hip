@@ -543,10 +543,11 @@ __global__ __launch_bounds__(256) void combine_kernel(
   }
 }
 
-// The same of SlotRows: four rows at a time go through LDS, from where columns are taken by
+// The same of SlotRows: two rows at a time go through LDS, from where columns are taken by
 // their places, a pair of neighbours to a thread (and CH pairs tpt apart), so that a wave's reads
-// meet on few banks: 16384 tokens of 8 rows of 2048 192 us (combine_kernel, rows in their own
-// order, 157; what the products' stores save is 390).
+// meet on few banks: 16384 tokens of 8 rows of 2048 197 us (four rows at a time, which leave room
+// for fewer waves, 232; combine_kernel, rows in their own order, 157; what the products' stores
+// save is 390).
 template <int CH>
 __global__ __launch_bounds__(256) void combine_slots_kernel(
     SlotRows y, const int64_t* __restrict__ offs, int experts, int64_t y_rows,
@@ -558,8 +559,10 @@ __global__ __launch_bounds__(256) void combine_slots_kernel(
   const bool live = tt < tokens;  // (all threads meet at the barriers)
   const int64_t t = live ? tt : tokens - 1;
   const int n = (int)y.n;
-  uint16_t* rows = rows16 + at * 4 * y.pitch;
-  const float up = ldexpf(1.0f, sum_exponent(y.largest, y.k));
+  constexpr int R = 2;
+  uint16_t* rows = rows16 + at * R * (y.pitch + y.ep / 2);
+  int8_t* ex = reinterpret_cast<int8_t*>(rows + R * y.pitch);  // their exponents
+  const int share = tpt / R, ei = tid & (share - 1);  // of the threads, to a row's exponents
   float acc[CH][2];
 #pragma unroll
   for (int h = 0; h < CH; ++h)
@@ -570,13 +573,14 @@ __global__ __launch_bounds__(256) void combine_slots_kernel(
     }
   constexpr int IT = CH == 4 ? 2 : 4;  // pieces of a row's slots a thread
   const int64_t ends = range_ends(offs, experts);
-  for (int j0 = 0; j0 < k; j0 += 4) {
-    const uint32_t* places[4];
-    float w[4], factor[4];
-    u32x4 raw[4][IT];
-    uint32_t p[CH][4];
+  for (int j0 = 0; j0 < k; j0 += R) {
+    const uint32_t* places[R];
+    float w[R], factor[R];
+    u32x4 raw[R][IT];
+    uint32_t exps = 0;  // four fragments'
+    uint32_t p[CH][R];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < R; ++u) {
       const int j = j0 + u < k ? j0 + u : k - 1;
       int64_t s = slots[t * k + j];
       w[u] = weights[t * k + j];
@@ -592,30 +596,39 @@ __global__ __launch_bounds__(256) void combine_slots_kernel(
       for (int i = 0; i < IT; ++i)
         if (tid + i * tpt < y.pitch / 8) raw[u][i] = from[tid + i * tpt];
     }
+    if (4 * ei < y.ep) {
+      const int j = j0 + tid / share;
+      const int64_t s = slots[t * k + (j < k ? j : k - 1)];
+      exps = reinterpret_cast<const uint32_t*>(y.exps +
+                                               (s < 0 || s >= y_rows ? 0 : s) * y.ep)[ei];
+    }
 #pragma unroll
     for (int h = 0; h < CH; ++h)
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
+      for (int u = 0; u < R; ++u)
         if (2 * (tid + h * tpt) < n) p[h][u] = places[u][tid + h * tpt];
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
+    for (int u = 0; u < R; ++u)
 #pragma unroll
       for (int i = 0; i < IT; ++i)
         if (tid + i * tpt < y.pitch / 8)
           reinterpret_cast<u32x4*>(rows + u * y.pitch)[tid + i * tpt] = raw[u][i];
+    if (4 * ei < y.ep) reinterpret_cast<uint32_t*>(ex + tid / share * y.ep)[ei] = exps;
     __syncthreads();
 #pragma unroll
     for (int h = 0; h < CH; ++h) {
       const int c = tid + h * tpt;
       if (2 * c >= n) break;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < R; ++u) {
         if (j0 + u >= k) break;
         const uint16_t* row = rows + u * y.pitch;
-        const float a = f16_from_bits(row[p[h][u] & 0xffffu]) * up * factor[u];
-        const float b = f16_from_bits(row[p[h][u] >> 16]) * up * factor[u];
-        acc[h][0] = __builtin_fmaf(w[u], a, acc[h][0]);
-        acc[h][1] = __builtin_fmaf(w[u], b, acc[h][1]);
+        const int8_t* by = ex + u * y.ep;
+        const uint32_t a = p[h][u] & 0xffffu, b = p[h][u] >> 16;
+        acc[h][0] = __builtin_fmaf(
+            w[u], ldexpf(f16_from_bits(row[a]), by[a >> 4]) * factor[u], acc[h][0]);
+        acc[h][1] = __builtin_fmaf(
+            w[u], ldexpf(f16_from_bits(row[b]), by[b >> 4]) * factor[u], acc[h][1]);
       }
     }
     __syncthreads();
@@ -723,15 +736,15 @@ int launch_combine(const SlotRows& y, const int64_t* offs, int experts, int64_t 
   const int64_t pieces = y.n / 8;  // (n is a multiple of 16)
   const int tpt = pieces <= 64 ? 64 : (pieces <= 128 ? 128 : 256), each = 256 / tpt;
   const dim3 grid((unsigned)((t + each - 1) / each));
-  const size_t lds = (size_t)each * 4 * y.pitch * 2;
+  const size_t lds = (size_t)each * 2 * (y.pitch * 2 + y.ep);  // (at most 33 KiB)
   if (pieces <= 256)
     combine_slots_kernel<4><<<grid, 256, lds, s>>>(y, offs, experts, y_rows, slots, weights, t,
                                                    (int)top_k, tpt, residual, dt_residual, out,
                                                    dt_out);
   else
     combine_slots_kernel<16><<<grid, 256, lds, s>>>(y, offs, experts, y_rows, slots, weights, t,
-                                                   (int)top_k, tpt, residual, dt_residual, out,
-                                                   dt_out);
+                                                    (int)top_k, tpt, residual, dt_residual, out,
+                                                    dt_out);
   return launch_status("moe_combine");
 }
 

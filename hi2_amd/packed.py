@@ -482,9 +482,10 @@ def moe_mlp(x: torch.Tensor, routing, gate: PackedExperts, up: PackedExperts,
     ``residual + sum_j w_j down(activation(gate(x)) * up(x))`` for ``x [..., K]`` and the
     :class:`hi2_amd.moe.Routing` of its tokens, as x's shape and type.  Sums are float32 and the
     rounding to x's type is one, at the end; what the experts hand on is float32, for bfloat16
-    inputs of more than a few tokens fp16 under a scale (at most 2^-11 of each value, an
-    eighth of the result's own rounding).  Where the routing's weights (or the residual)
-    require a gradient they have one, from the parts' own calls, in float32 between them."""
+    inputs of more than a few tokens fp16 with an exponent to every 16 values (2^-11 of each,
+    an eighth of the result's own rounding, and no less than 2^-39 of the largest of the 16).
+    Where the routing's weights (or the residual) require a gradient they have one, from the
+    parts' own calls, in float32 between them."""
     for name, p in (("gate", gate), ("up", up), ("down", down)):
         if not isinstance(p, PackedExperts):
             raise TypeError(f"{name} is {type(p).__name__}, expected PackedExperts")

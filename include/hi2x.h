@@ -549,7 +549,8 @@ typedef struct {
   const uint8_t* had;                  /* [k / 16] rotation flags of the 16-column groups */
   const uint16_t* col_scale;           /* [k] fp16 smoothing, or NULL */
   int64_t per_expert;                  /* had and col_scale hold one row per expert */
-  float* largest;                      /* the largest |weight| (hi2x_packed_layout writes it) */
+  float* largest;                      /* the largest |weight|, at most 65504, for the caller
+                                          (hi2x_packed_layout writes it) */
   const uint16_t* places;              /* [experts][n] the slot of each row in its expert, or
                                           NULL (then, and past 8192 slots, hi2x_moe_mlp keeps
                                           f32 between its products) */
@@ -675,8 +676,9 @@ int hi2x_moe_combine_backward(const void* grad, int dt_grad, const void* y, int 
  * them for t tokens and top_k choices; residual (or NULL) and out [t][h] contiguous.  The
  * nplanes and nplanes_mid are the planes of the tokens' and the hidden values' transforms,
  * shared says that gate's and up's transforms are the same.  The experts' values in between
- * are f32; with one plane of the hidden values, and more than 16 slots, fp16 times a power of
- * two that their sums cannot exceed (from `largest`).  Workspace: hi2x_moe_mlp_workspace_bytes. */
+ * are f32; with one plane of the hidden values, and more than 16 slots, fp16 with an exponent to
+ * every 16 of them: 2^-11 of each value, no less than 2^-39 of the largest of the 16.  Workspace:
+ * hi2x_moe_mlp_workspace_bytes. */
 int hi2x_moe_mlp(const hi2x_packed* gate, const hi2x_packed* up, const hi2x_packed* down,
                  const void* x, int dtype, int64_t ldx, int64_t t, int64_t top_k, int nplanes,
                  int nplanes_mid, int shared, int act, const int64_t* rows, const int64_t* offs,

@@ -94,3 +94,81 @@ def test_mlp_of_weights_below_an_infinite_step(dev):
     assert np.isfinite(got).all()
     # the roundings of the tokens, the hidden values and the result, as in the other MLP tests
     assert np.linalg.norm(got - want) < 2.0 ** -8 * np.linalg.norm(want)
+
+
+def decoded(t):
+    """The weights of a tensor by the format's definition, float64."""
+    n, k = t.shape
+    w = np.zeros((n, k))
+    params, words = t.blk_params.numpy().reshape(-1, 2), t.codes.numpy().view(np.uint32)
+    for r in range(n):
+        nb, b = int(t.row_nbits[r]), int(t.row_block[r])
+        c = t.row_consts[r].numpy().astype(np.float64)
+        v = words[int(t.code_off[r]):int(t.code_off[r + 1])]
+        codes = (v[:, None] >> (nb * np.arange(32 // nb, dtype=np.uint32))) & (2 ** nb - 1)
+        u = params[int(t.param_off[r]):int(t.param_off[r + 1])]
+        lo = (u[:, 0] * c[1] + c[0]).astype(np.float32).astype(np.float16).astype(np.float64)
+        st = (u[:, 1] * c[2]).astype(np.float32).astype(np.float16).astype(np.float64)
+        w[r] = (lo[:, None] + codes.reshape(-1, b) * st[:, None]).astype(np.float16).reshape(-1)
+    return w
+
+
+@pytest.mark.parametrize("channel", [0.0, 1e5, 1e7])
+def test_mlp_of_experts_of_unlike_magnitude(channel, dev):
+    """Experts with weights of 1e-3 and of 5e4 side by side, and tokens with a channel that
+    dwarfs the others and meets zero weights: every token's result is as exact as another's."""
+    from hi2_amd.moe import route
+    from hi2_amd.packed import PackedExperts, moe_mlp
+
+    t, e, h, i = 90, 3, 256, 128
+    sides = []
+    for n, k, seed in ((i, h, 100), (i, h, 200), (h, i, 300)):
+        ts, _ = _experts(e, n, k, seed)
+        for j, size in enumerate((1.0, 2.0 ** 18, 2.0 ** -6)):
+            consts = ts[j].row_consts.double() * size
+            ts[j].row_consts = consts.half()
+            ts[j].had[:] = 0
+            if k == h:  # columns 0 to 63 are zero: lo = u lo_scale + 0 and step 0 at u = 0
+                consts[:, 1], consts[:, 0] = consts[:, 0] / 255, 0.0
+                ts[j].row_consts = consts.half()
+                for r in range(n):
+                    b = 64 // int(ts[j].row_block[r])
+                    a = 2 * int(ts[j].param_off[r])
+                    ts[j].blk_params[a:a + 2 * b] = 0
+        ws = [decoded(q) for q in ts]
+        assert all(np.isfinite(v).all() for v in ws)
+        sides.append((ts, ws))
+    assert np.abs(sides[0][1][1]).max() > 2e4 and np.abs(sides[0][1][2]).max() < 4e-3
+    x = tokens(t, h, torch.float32, 4, dev)
+    x[:, 5] = channel
+    x = x.bfloat16()
+    index = torch.arange(t, device=dev) % e
+    logits = torch.zeros(t, e, device=dev)
+    logits[torch.arange(t, device=dev), index] = 4.0
+    r = route(logits, 1)
+    got = N(moe_mlp(x, r, *(PackedExperts(s[0], dev) for s in sides), activation="relu"))
+    want = mlp64(x, r, *sides)
+    off = np.linalg.norm(got - want, axis=1) / np.linalg.norm(want, axis=1)
+    # a token's own roundings: its values, the hidden ones, the result, 2^-9 or less each as rms
+    assert off.max() < 2.0 ** -7, off.reshape(-1, e).max(0)
+
+
+@pytest.mark.parametrize("h,i", [(8064, 64), (64, 8064), (4096, 2064), (528, 1040)])
+def test_mlp_of_wide_rows(h, i, dev):
+    """The widest rows that the experts hand on in slot order, and widths beside the steps of
+    the kernels that read them."""
+    from hi2_amd.moe import route
+    from hi2_amd.packed import PackedExperts, moe_mlp
+
+    t, e, k = 24, 2, 1
+    classes = [(2, 16), (4, 16)]
+    sides = [_experts(e, n, m, s, classes=classes) for n, m, s in ((i, h, 1), (i, h, 2), (h, i, 3))]
+    plans = [PackedExperts(s[0], dev) for s in sides]
+    x = tokens(t, h, torch.bfloat16, 4, dev)
+    r = route(torch.randn(t, e, generator=torch.Generator().manual_seed(3)).to(dev), k)
+    got, want = N(moe_mlp(x, r, *plans, residual=x)), mlp64(x, r, *sides, act="silu") + N(x)
+    assert np.isfinite(got).all()
+    # each element: the result's rounding, and that of the tokens, the hidden values and what
+    # is handed on, 2^-11 each, of sums whose terms cancel: as the row's norm, with margin
+    off = np.abs(got - want) - 2.0 ** -8 * np.abs(want)
+    assert off.max() < 2.0 ** -8 * np.abs(want).max()
