@@ -17,7 +17,8 @@ registers on the way.
   (q, k, v; gate, up) to be multiplied one after the other.
 
 Inputs are float32, float16 or bfloat16; products are summed in float32 and rounded once,
-to ``out_dtype``.  The products have no gradient (the codes are integers; inputs that
+to ``out_dtype``.  Their transformed activations have 22 bits, for bfloat16 results of
+bfloat16 inputs 11 (an eighth of the result's rounding).  The products have no gradient (the codes are integers; inputs that
 require one are refused while gradients are recorded); :func:`combine` has, and
 :func:`moe_mlp` to the routing's weights, so that a router can be trained on frozen experts.
 """
@@ -254,11 +255,13 @@ def _pitch(x: torch.Tensor) -> int:
     return x.stride(0) if x.shape[0] > 1 else x.shape[1]
 
 
-def _planes(dtype: torch.dtype, w: _Packed) -> int:
+def _planes(dtype: torch.dtype, w: _Packed, out_dtype: torch.dtype) -> int:
     """fp16 planes of the transformed activations.  One plane rounds each value by up to
-    2^-11, which a bf16 result's own rounding hides, but not an fp16 or fp32 one's: those
-    take two (22 bits), except fp16 values that the transform leaves as they are."""
-    return 1 if dtype == torch.bfloat16 or dtype == torch.float16 and w.plain else 2
+    2^-11, which a bf16 result of bf16 values hides, but not an fp16 or fp32 one: those
+    take two (22 bits), except 16-bit values that the transform leaves as they are."""
+    if w.plain and dtype != torch.float32:
+        return 1
+    return 1 if dtype == out_dtype == torch.bfloat16 else 2
 
 
 def _aligned(x: torch.Tensor) -> torch.Tensor:
@@ -268,17 +271,20 @@ def _aligned(x: torch.Tensor) -> torch.Tensor:
     return x.clone() if x.data_ptr() % 16 else x
 
 
-def activations(x: torch.Tensor, w: PackedLinear | PackedExperts) -> Activations:
+def activations(x: torch.Tensor, w: PackedLinear | PackedExperts, out_dtype=None
+                ) -> Activations:
     """``T(x)`` for ``w`` and every tensor with the same transform, to be handed to
     :func:`packed_linear` or :func:`experts_linear` in the place of ``x [..., K]``.  The
-    product then has one row per row of ``x``."""
+    product then has one row per row of ``x``.  ``out_dtype`` is the type of the results
+    (default: x's); where bfloat16 values are held to a bfloat16 result's bits, the products
+    refuse a wider one."""
     _same_device(w, "activations", x)
     _no_grad_inputs("activations", x)
     if w.transform is None:
         raise ValueError("the experts have transforms of their own: give experts_linear x itself")
     dt = _dtype(x, "x")
     x = _aligned(_rows_of(x, w.k, "x"))
-    rows, npl = x.shape[0], _planes(x.dtype, w)
+    rows, npl = x.shape[0], _planes(x.dtype, w, out_dtype or x.dtype)
     planes = torch.empty(rows, w.kp // CHUNK, npl, CHUNK, dtype=torch.float16, device=w.device)
     scale = torch.empty(rows, dtype=torch.float32, device=w.device)
     desc = _lib.ActivationsDesc(planes.data_ptr(), scale.data_ptr(), rows, w.kp, npl, 0)
@@ -315,6 +321,9 @@ def _product(w, x, src, offs, slots, bias, activation, mul, residual, out_dtype,
     mul, mul_p, mul_ld, mul_dt = _operand(mul, slots, n, "mul")
     residual, res_p, res_ld, res_dt = _operand(residual, slots, n, "residual")
     out_dt = _dtype(out_dtype, "out_dtype")
+    if given and x.desc.nplanes < _planes(x.dtype, w, out_dtype):
+        raise ValueError(f"activations of {x.dtype} made for results of that type: give "
+                         f"activations out_dtype={out_dtype}")
     dt = 0 if given else _dtype(x, "x")
     out = torch.empty(slots, n, dtype=out_dtype, device=dev)
     if not slots:
@@ -325,7 +334,7 @@ def _product(w, x, src, offs, slots, bias, activation, mul, residual, out_dtype,
         rows, npl = x.scale.numel(), x.desc.nplanes
     else:
         x = _aligned(x)
-        rows, npl = x.shape[0], _planes(x.dtype, w)
+        rows, npl = x.shape[0], _planes(x.dtype, w, out_dtype)
     size = _lib.lib().hi2x_packed_workspace_bytes(w._ref, rows, npl, given, slots,
                                                   src is not None, offs is not None)
     ws = torch.empty(size, dtype=torch.uint8, device=dev) if size > 0 else None
@@ -535,7 +544,8 @@ def moe_mlp(x: torch.Tensor, routing, gate: PackedExperts, up: PackedExperts,
         return out
     # one fp16 plane of the hidden values (and fp16 between the products) is well below a bf16
     # result's own rounding, and half the products; next to an fp16 result it would show
-    npl, mid = max(_planes(x.dtype, gate), _planes(x.dtype, up)), 1 if dt == 2 else 2
+    npl = max(_planes(x.dtype, gate, x.dtype), _planes(x.dtype, up, x.dtype))
+    mid = 1 if dt == 2 else 2
     top_k = slots.shape[1]
     shared = gate.transform is not None and gate.transform == up.transform
     size = _lib.lib().hi2x_moe_mlp_workspace_bytes(gate._ref, up._ref, down._ref, t, top_k, npl,

@@ -6,8 +6,8 @@ import numpy as np
 import pytest
 import torch
 
-from packed_data import act64, stored
-from test_gpu_packed import F, N, _experts, tokens
+from packed_data import act64, packed_tensor, stored
+from test_gpu_packed import F, MIX, N, _experts, tokens
 
 pytestmark = pytest.mark.gpu
 
@@ -172,3 +172,72 @@ def test_mlp_of_wide_rows(h, i, dev):
     # is handed on, 2^-11 each, of sums whose terms cancel: as the row's norm, with margin
     off = np.abs(got - want) - 2.0 ** -8 * np.abs(want)
     assert off.max() < 2.0 ** -8 * np.abs(want).max()
+
+
+def relative(got, want):
+    return np.linalg.norm(N(got) - want) / np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("t", [1, 8, 14, 90, 300])
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("out", ["f32", "f16"])
+def test_results_wider_than_bf16_keep_the_activations_bits(t, dt, out, dev):
+    """Rotated and smoothed activations of 16 bits take two planes where the result shows it."""
+    from hi2_amd.packed import PackedLinear, activations, packed_linear
+
+    n, k = 96, 256
+    p, w = packed_tensor(n, k, MIX, 9, smooth=True)
+    plan = PackedLinear(p, dev)
+    x = tokens(t, k, F[dt], 3, dev)
+    want = stored(N(x), p) @ w.T
+    got = packed_linear(x, plan, out_dtype=F[out])
+    # two planes leave 2^-22 of a value, sums in float32 about sqrt(k / 2) 2^-25 of the result;
+    # an fp16 result is at most half an ulp from its value.  (One plane: about 2^-13.)
+    lim = 2.0 ** -19 if out == "f32" else 2.0 ** -11.5
+    assert relative(got, want) < lim
+    if out == "f16":  # nothing beyond the result's own rounding
+        own = np.linalg.norm(want.astype(np.float16) - want) / np.linalg.norm(want)
+        assert relative(got, want) < own * (1 + 2.0 ** -7)
+    a = activations(x, plan, out_dtype=F[out])
+    assert relative(packed_linear(a, plan, out_dtype=F[out]), want) < lim
+
+
+def test_activations_made_for_bf16_results_refuse_wider_ones(dev):
+    from hi2_amd.packed import PackedLinear, activations, packed_linear
+
+    p, _ = packed_tensor(32, 128, MIX, 9)
+    plan = PackedLinear(p, dev)
+    x = tokens(4, 128, torch.bfloat16, 3, dev)
+    a = activations(x, plan)
+    assert packed_linear(a, plan).dtype == torch.bfloat16
+    with pytest.raises(ValueError, match="out_dtype"):
+        packed_linear(a, plan, out_dtype=torch.float32)
+    p.had[:] = 0  # bfloat16 values that nothing transforms are whole in one plane
+    plain = PackedLinear(p, dev)
+    got = packed_linear(activations(x, plain), plain, out_dtype=torch.float32)
+    assert torch.equal(got, packed_linear(x, plain, out_dtype=torch.float32))
+
+
+def test_gradient_of_the_mlps_weights_keeps_the_activations_bits(dev):
+    """The routing's weights have a float32 gradient, from float32 parts: nothing in it is left
+    to the 11 bits of one plane."""
+    from dataclasses import replace
+
+    from hi2_amd.moe import route
+    from hi2_amd.packed import PackedExperts, moe_mlp
+
+    t, e, k, h, i = 50, 4, 2, 128, 64
+    sides = _experts(e, i, h, 100), _experts(e, i, h, 200), _experts(e, h, i, 300)
+    plans = [PackedExperts(s[0], dev) for s in sides]
+    x = tokens(t, h, torch.bfloat16, 4, dev)
+    r = route(torch.randn(t, e, generator=torch.Generator().manual_seed(3)).to(dev), k)
+    weights = r.weights.clone().requires_grad_(True)
+    out = moe_mlp(x, replace(r, weights=weights), *plans, activation="relu")
+    c = torch.randn(t, h, generator=torch.Generator().manual_seed(6)).bfloat16().to(dev)
+    out.backward(c)
+    want = np.zeros((t, k))
+    for j in range(k):
+        only = torch.zeros_like(r.weights)
+        only[:, j] = 1.0
+        want[:, j] = (N(c) * mlp64(x, replace(r, weights=only), *sides)).sum(1)
+    assert relative(weights.grad, want) < 2.0 ** -17
