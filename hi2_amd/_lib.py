@@ -276,6 +276,17 @@ def require_gpu(*tensors: torch.Tensor) -> torch.device:
     return dev
 
 
+def refuse_tangents(what: str, *tensors) -> None:
+    """Raise where a tensor carries a forward-mode tangent: nothing here has such a derivative,
+    and the kernels would drop it without a word."""
+    fwd = torch.autograd.forward_ad
+    if fwd._current_level < 0:  # outside every dual level: no tangents
+        return
+    if any(t is not None and fwd.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{what} has no forward-mode derivative: its inputs must carry no "
+                           "tangent")
+
+
 def ptr(t: torch.Tensor | None):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
 

@@ -101,6 +101,7 @@ def route(logits: torch.Tensor, top_k: int, scoring: str = "softmax", bias=None,
     Limits: 512 experts, 32 choices, 64 groups.  One launch for up to 64 tokens (32 above
     256 experts), two above; the host never waits."""
     dev = _lib.require_gpu(logits, bias)
+    _lib.refuse_tangents("route", logits, bias)
     if logits.dim() != 2:
         raise ValueError(f"logits has shape {tuple(logits.shape)}, expected [T, E]")
     if logits.dtype not in _FLOATS:

@@ -229,6 +229,7 @@ class Activations:
 
 
 def _no_grad_inputs(what, *tensors):
+    _lib.refuse_tangents(what, *tensors)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad() or detach "
                            "its inputs")
@@ -454,6 +455,7 @@ def combine(y: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor, residua
     y's).  y, the weights and the residual have gradients where they require them (y's row by
     row: no row of y may then be named twice, and :func:`hi2_amd.moe.route` names none twice)."""
     _lib.require_gpu(y, slots, weights, residual)
+    _lib.refuse_tangents("combine", y, weights, residual)
     if y.dim() != 2:
         raise ValueError(f"y has shape {tuple(y.shape)}, expected [S, N]")
     if slots.dim() != 2 or weights.shape != slots.shape or slots.shape[1] < 1:
@@ -509,6 +511,7 @@ def moe_mlp(x: torch.Tensor, routing, gate: PackedExperts, up: PackedExperts,
     slots, weights = routing.slots.contiguous(), routing.weights.contiguous()
     _same_device(gate, "moe_mlp", x, residual, rows, offs, slots, weights)
     _no_grad_inputs("moe_mlp", x)
+    _lib.refuse_tangents("moe_mlp", weights, residual)
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"activation {activation!r} ({', '.join(ACTIVATIONS)})")

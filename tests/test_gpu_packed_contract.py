@@ -241,3 +241,38 @@ def test_gradient_of_the_mlps_weights_keeps_the_activations_bits(dev):
         only[:, j] = 1.0
         want[:, j] = (N(c) * mlp64(x, replace(r, weights=only), *sides)).sum(1)
     assert relative(weights.grad, want) < 2.0 ** -17
+
+
+def dual(t):
+    from torch.autograd import forward_ad
+
+    return forward_ad.make_dual(t, torch.ones_like(t))
+
+
+def test_forward_mode_tangents_are_refused(dev):
+    """None of these has a forward-mode derivative: a tangent is refused, not dropped."""
+    from torch.autograd import forward_ad
+
+    from hi2_amd.moe import route
+    from hi2_amd.packed import (PackedExperts, PackedLinear, activations, combine,
+                                experts_linear, moe_mlp, packed_linear)
+
+    p, _ = packed_tensor(128, 128, MIX, 9)
+    one, ex = PackedLinear(p, dev), PackedExperts([p, p], dev)
+    x = torch.randn(6, 128, device=dev)
+    logits = torch.randn(6, 2, device=dev)
+    r = route(logits, 1)
+    y = torch.randn(6, 8, device=dev)
+    calls = [lambda d: route(d(logits), 1), lambda d: route(logits, 1, bias=d(logits[0])),
+             lambda d: packed_linear(d(x), one), lambda d: packed_linear(x, one, mul=d(x)),
+             lambda d: packed_linear(x, one, bias=d(x[0])), lambda d: activations(d(x), one),
+             lambda d: experts_linear(x, ex, r.offs, r.rows, residual=d(x)),
+             lambda d: combine(d(y), r.slots, r.weights),
+             lambda d: combine(y, r.slots, d(r.weights)),
+             lambda d: combine(y, r.slots, r.weights, residual=d(y)),
+             lambda d: moe_mlp(d(x), r, ex, ex, ex), lambda d: moe_mlp(x, r, ex, ex, ex, residual=d(x))]
+    for call in calls:
+        with forward_ad.dual_level():
+            call(lambda v: v)
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call(dual)

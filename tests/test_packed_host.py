@@ -2,6 +2,9 @@
 
 import ctypes
 
+import pytest
+import torch
+
 from hi2_amd import _lib
 from test_packed_abi import packed
 
@@ -15,3 +18,17 @@ def test_workspace_of_slots_that_index_no_rows():
         some = size(ctypes.byref(w), 0, 2, 0, 40, 1, ranges)
         assert some >= 40 * 128 * 2 * 2 + 40 * 4
         assert size(ctypes.byref(w), 0, 2, 0, 0, 1, ranges) == 0
+
+
+def test_tangents_are_seen_with_and_without_gradients():
+    from torch.autograd import forward_ad
+
+    x = torch.ones(3)
+    _lib.refuse_tangents("this", x, None)
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, torch.ones(3))
+        _lib.refuse_tangents("this", x, None)
+        for ctx in (torch.no_grad(), torch.enable_grad()):
+            with ctx, pytest.raises(RuntimeError, match="this has no forward-mode"):
+                _lib.refuse_tangents("this", None, x, d)
+    _lib.refuse_tangents("this", d)  # the level's end takes its tangents along
