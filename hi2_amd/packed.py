@@ -419,6 +419,12 @@ def experts_linear(x: torch.Tensor | Activations, w: PackedExperts, offs: torch.
                     out_dtype or x.dtype, "experts_linear")
 
 
+def _check_residual(residual, t, n):
+    """``residual`` has t rows of n, in any leading dimensions."""
+    if residual is not None and (residual.numel() != t * n or residual.shape[-1:] != (n,)):
+        raise ValueError(f"residual has shape {tuple(residual.shape)}, expected {(t, n)}")
+
+
 class _Combine(torch.autograd.Function):
     """:func:`combine` with gradients to y, the weights and the residual."""
 
@@ -465,8 +471,7 @@ def combine(y: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor, residua
         raise ValueError(f"slots {slots.dtype} and weights {weights.dtype}: int64 and float32 "
                          "expected")
     t, n = slots.shape[0], y.shape[1]
-    if residual is not None and residual.numel() != t * n:
-        raise ValueError(f"residual has shape {tuple(residual.shape)}, expected {(t, n)}")
+    _check_residual(residual, t, n)
     y, slots, weights = y.contiguous(), slots.contiguous(), weights.contiguous()
     if torch.is_grad_enabled() and (y.requires_grad or weights.requires_grad or
                                     residual is not None and residual.requires_grad):
@@ -528,8 +533,7 @@ def moe_mlp(x: torch.Tensor, routing, gate: PackedExperts, up: PackedExperts,
             weights.dtype != torch.float32:
         raise ValueError("routing: rows, offs and slots int64 and weights float32 expected")
     if residual is not None:
-        if residual.numel() != t * gate.k:
-            raise ValueError(f"residual has shape {tuple(residual.shape)}, expected {(t, gate.k)}")
+        _check_residual(residual, t, gate.k)
         residual = residual.reshape(t, gate.k).contiguous()
     if torch.is_grad_enabled() and (weights.requires_grad or
                                     residual is not None and residual.requires_grad):

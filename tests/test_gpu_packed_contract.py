@@ -276,3 +276,25 @@ def test_forward_mode_tangents_are_refused(dev):
             call(lambda v: v)
             with pytest.raises(RuntimeError, match="forward-mode"):
                 call(dual)
+
+
+def test_residuals_of_another_shape_are_refused(dev):
+    from hi2_amd.moe import route
+    from hi2_amd.packed import PackedExperts, combine, moe_mlp
+
+    p, _ = packed_tensor(128, 128, MIX, 9)
+    ex = PackedExperts([p, p], dev)
+    x = torch.randn(2, 3, 128, device=dev)
+    r = route(torch.randn(6, 2, device=dev), 1)
+    y, res = torch.randn(6, 8, device=dev), torch.randn(6, 8, device=dev)
+    want = combine(y, r.slots, r.weights, residual=res)
+    for ok in (res.view(2, 3, 8), res.t().contiguous().t()):
+        assert torch.equal(combine(y, r.slots, r.weights, residual=ok), want)
+    for bad in (res.t(), res.reshape(-1), res[:5], res.view(6, 4, 2)):
+        with pytest.raises(ValueError, match="residual"):
+            combine(y, r.slots, r.weights, residual=bad)
+    want = moe_mlp(x, r, ex, ex, ex, residual=x)
+    assert torch.equal(moe_mlp(x, r, ex, ex, ex, residual=x.view(6, 128)), want)
+    for bad in (x.view(6, 128).t(), x.reshape(-1), x[:1]):
+        with pytest.raises(ValueError, match="residual"):
+            moe_mlp(x, r, ex, ex, ex, residual=bad)
