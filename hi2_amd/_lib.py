@@ -137,6 +137,8 @@ SIGNATURES["hi2x_route"] = [_P, _I, _I64, _I64, _I64, _I64, _I, _P, _I64, _I64, 
 SIGNATURES["hi2x_route_backward"] = [_P, _I, _I64, _I64, _I64, _I64, _I, _I, _F, _P, _P, _P, _P]
 SIGNATURES["hi2x_moe_combine_backward"] = [_P, _I, _P, _I, _I64, _I64, _P, _P, _I64, _I64, _P, _P,
                                            _P]
+SIGNATURES["hi2x_moe_combine_grad"] = [_P, _I, _P, _I, _I64, _I64, _P, _P, _I64, _I64, _P, _P, _P,
+                                       _I64, _P]
 SIGNATURES["hi2x_moe_combine"] = [_P, _I, _I64, _I64, _P, _P, _I64, _I64, _P, _I, _P, _I, _P]
 
 # workspace sizes (int64 bytes, -1 for bad arguments): name -> argtypes
@@ -151,6 +153,7 @@ SIZES = {
     "hi2x_packed_workspace_bytes": [_P, _I64, _I, _I, _I64, _I, _I],
     "hi2x_moe_mlp_workspace_bytes": [_P, _P, _P, _I64, _I64, _I, _I, _I],
     "hi2x_route_workspace_bytes": [_I64, _I64],
+    "hi2x_moe_combine_grad_workspace_bytes": [_I64],
 }
 
 

@@ -650,7 +650,8 @@ __global__ __launch_bounds__(256) void combine_slots_kernel(
 
 // The weighted sum's gradients, a wave on a slot (t, j): dw = sum_c g[t][c] y[slot][c], dy[slot]
 // = w g[t].  Bound by reading y and writing dy once (g's rows are read by their k slots from
-// cache).
+// cache).  A row of y that several slots name takes the sum of theirs: the wave of the first one
+// looks for the others between it and the last (`named`), and adds them in their order.
 template <int DT, int V>
 __device__ __forceinline__ void load_values(const void* p, int64_t at, float (&v)[V]) {
   if constexpr (V == 1) {
@@ -668,11 +669,22 @@ __device__ __forceinline__ void load_values(const void* p, int64_t at, float (&v
   }
 }
 
+// named[row] = {last + 1, count - first} of the slots that name a row of y, from zeros.
+__global__ void combine_named_kernel(const int64_t* __restrict__ slots, int64_t count,
+                                     int64_t y_rows, uint2* named) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= count) return;
+  const int64_t s = slots[i];
+  if (s < 0 || s >= y_rows) return;
+  atomicMax(&named[s].x, (uint32_t)(i + 1));
+  atomicMax(&named[s].y, (uint32_t)(count - i));
+}
+
 template <int DG, int DT, int V>
 __global__ __launch_bounds__(256) void combine_backward_kernel(
     const void* __restrict__ grad, const void* __restrict__ y, int64_t y_rows, int64_t n,
     const int64_t* __restrict__ slots, const float* __restrict__ weights, int64_t count, int k,
-    float* __restrict__ dw, void* __restrict__ dy) {
+    float* __restrict__ dw, void* __restrict__ dy, const uint2* __restrict__ named) {
   const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
   if (i >= count) return;
@@ -683,6 +695,11 @@ __global__ __launch_bounds__(256) void combine_backward_kernel(
   }
   const float w = weights[i];
   float sum = 0.0f;
+  int64_t first = i, last = i;
+  if (dy) {
+    last = (int64_t)named[s].x - 1;
+    first = count - (int64_t)named[s].y;
+  }
   for (int64_t c = lane * V; c < n; c += 64 * V) {
     float g[V], v[V];
     load_values<DG, V>(grad, t * n + c, g);
@@ -691,11 +708,32 @@ __global__ __launch_bounds__(256) void combine_backward_kernel(
 #pragma unroll
       for (int u = 0; u < V; ++u) sum = __builtin_fmaf(g[u], v[u], sum);
     }
-    if (dy) {
+    if (dy && first == last) {
 #pragma unroll
       for (int u = 0; u < V; ++u) store_from_f32(dy, s * n + c + u, DT, w * g[u]);
     }
   }
+  if (dy && i == first && first < last)
+    for (int64_t c0 = 0; c0 < n; c0 += 64 * V) {  // (the whole wave)
+      const int64_t c = c0 + lane * V;
+      float g[V], acc[V];
+#pragma unroll
+      for (int u = 0; u < V; ++u) acc[u] = 0.0f;
+      for (int64_t j0 = first; j0 <= last; j0 += 64) {
+        unsigned long long more = __ballot(j0 + lane <= last && slots[j0 + lane] == s);
+        for (; more; more &= more - 1) {
+          const int64_t j = j0 + __builtin_ctzll(more);
+          const float wj = weights[j];
+          if (c < n) load_values<DG, V>(grad, j / k * n + c, g);
+#pragma unroll
+          for (int u = 0; u < V; ++u)
+            if (c < n) acc[u] = __builtin_fmaf(wj, g[u], acc[u]);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < V; ++u)
+        if (c < n) store_from_f32(dy, s * n + c + u, DT, acc[u]);
+    }
 #pragma unroll
   for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
   if (dw && lane == 0) dw[i] = sum;
@@ -722,7 +760,7 @@ int route_tokens(int64_t t, int64_t e) {
   return t <= 4 ? 4 : (t <= most ? most : (t <= 4096 ? 16 : most));
 }
 
-// Clears offs where there are no tokens.
+// Clears offs where there are no tokens, and tables in front of their kernels.
 __global__ void zero_i64_kernel(int64_t* p, int64_t n) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i < n) p[i] = 0;
@@ -905,14 +943,27 @@ extern "C" int hi2x_moe_combine(const void* y, int dt_y, int64_t y_rows, int64_t
                         dt_residual, out, dt_out, as_stream(stream));
 }
 
+extern "C" int64_t hi2x_moe_combine_grad_workspace_bytes(int64_t y_rows) {
+  return y_rows < 0 ? -1 : align256(y_rows * (int64_t)sizeof(uint2));
+}
+
 extern "C" int hi2x_moe_combine_backward(const void* grad, int dt_grad, const void* y, int dt_y,
                                          int64_t y_rows, int64_t n, const int64_t* slots,
                                          const float* weights, int64_t t, int64_t top_k,
                                          float* grad_weights, void* grad_y, void* stream) {
+  return hi2x_moe_combine_grad(grad, dt_grad, y, dt_y, y_rows, n, slots, weights, t, top_k,
+                               grad_weights, grad_y, nullptr, 0, stream);
+}
+
+extern "C" int hi2x_moe_combine_grad(const void* grad, int dt_grad, const void* y, int dt_y,
+                                     int64_t y_rows, int64_t n, const int64_t* slots,
+                                     const float* weights, int64_t t, int64_t top_k,
+                                     float* grad_weights, void* grad_y, void* ws,
+                                     int64_t ws_bytes, void* stream) {
   clear_error();
   for (int d : {dt_grad, dt_y})
     HI2X_REQUIRE(d >= 0 && d <= 2, "moe_combine_backward: dtype %d", d);
-  HI2X_REQUIRE(y_rows >= 0 && n >= 0 && t >= 0 && t < (1ll << 31) && top_k >= 1 &&
+  HI2X_REQUIRE(y_rows >= 0 && y_rows < (1ll << 38) && n >= 0 && t >= 0 && t < (1ll << 31) && top_k >= 1 &&
                    top_k < (1 << 20) && t * top_k < (1ll << 32),
                "moe_combine_backward: bad shape");
   if (t == 0 || (!grad_weights && !grad_y)) return HI2X_OK;
@@ -920,13 +971,25 @@ extern "C" int hi2x_moe_combine_backward(const void* grad, int dt_grad, const vo
                "moe_combine_backward: null buffer");
   const int64_t count = t * top_k;
   const hipStream_t s = as_stream(stream);
+  Workspace w;
+  if (grad_y) {
+    const size_t need = (size_t)hi2x_moe_combine_grad_workspace_bytes(y_rows);
+    if (int rc = take_workspace(w, ws, ws_bytes, need, s, "moe_combine_backward")) return rc;
+    if (y_rows > 0) {
+      zero_i64_kernel<<<dim3((unsigned)(y_rows / 256 + 1)), 256, 0, s>>>(
+          reinterpret_cast<int64_t*>(w.p), y_rows);
+      combine_named_kernel<<<dim3((unsigned)((count + 255) / 256)), 256, 0, s>>>(
+          slots, count, y_rows, reinterpret_cast<uint2*>(w.p));
+    }
+  }
+  const uint2* named = reinterpret_cast<const uint2*>(w.p);
   const dim3 grid((unsigned)((count + 3) / 4));
   const bool vec = n % 4 == 0 &&
                    (((uintptr_t)grad | (uintptr_t)y | (uintptr_t)grad_y) & 15) == 0;
 #define HI2X_BACK_(DG, DT, V)                                                              \
   combine_backward_kernel<DG, DT, V><<<grid, 256, 0, s>>>(grad, y, y_rows, n, slots, weights, \
                                                           count, (int)top_k, grad_weights, \
-                                                          grad_y);
+                                                          grad_y, named);
 #define HI2X_BACK(DG)         \
   if (vec && dt_y == 0)       \
     HI2X_BACK_(DG, 0, 4)      \

@@ -446,10 +446,12 @@ class _Combine(torch.autograd.Function):
         dw = torch.empty_like(weights) if need_w else None
         dy = torch.zeros_like(y) if need_y else None
         if need_w or need_y:
-            _lib.call("hi2x_moe_combine_backward", y.device, _lib.ptr(grad), _dtype(grad, "grad"),
+            ws = _lib.workspace(y.device, "hi2x_moe_combine_grad_workspace_bytes",
+                                y.shape[0] if need_y else 0)
+            _lib.call("hi2x_moe_combine_grad", y.device, _lib.ptr(grad), _dtype(grad, "grad"),
                       _lib.ptr(y), _dtype(y, "y"), y.shape[0], y.shape[1], _lib.ptr(slots),
                       _lib.ptr(weights), slots.shape[0], slots.shape[1], _lib.ptr(dw),
-                      _lib.ptr(dy))
+                      _lib.ptr(dy), _lib.ptr(ws), ws.numel())
         return dy, dw, grad.to(ctx.res[1]).view(ctx.res[0]) if need_r else None, None, None
 
 
@@ -458,8 +460,8 @@ def combine(y: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor, residua
     """``out[t] = residual[t] + sum_j weights[t, j] * y[slots[t, j]]`` over ``y [S, N]``, with
     ``slots`` (int64) and ``weights`` (float32) ``[T, k]`` of :func:`hi2_amd.moe.route`: summed
     in float32 in the order of j, rounded once to ``out_dtype`` (default: residual's, else
-    y's).  y, the weights and the residual have gradients where they require them (y's row by
-    row: no row of y may then be named twice, and :func:`hi2_amd.moe.route` names none twice)."""
+    y's).  y, the weights and the residual have gradients where they require them; a row of y
+    that several slots name takes the sum of theirs, in their order."""
     _lib.require_gpu(y, slots, weights, residual)
     _lib.refuse_tangents("combine", y, weights, residual)
     if y.dim() != 2:

@@ -661,9 +661,16 @@ int hi2x_moe_combine(const void* y, int dt_y, int64_t y_rows, int64_t n, const i
 
 /* Its gradients, from grad [t][n] contiguous: grad_weights f32 [t][top_k] (or NULL), each
  * sum over n in f32, and grad_y [y_rows][n] in y's type (or NULL), whose rows that a slot
- * names are written: weights[t][j] * grad[t] (a row that several slots name takes one of
- * theirs; hi2x_route names none twice).  A slot outside [0, y_rows) has the weight gradient
- * NaN.  The residual's gradient is grad. */
+ * names are written: the sum of weights[t][j] * grad[t] over the slots that name it, in f32
+ * in their order, rounded once.  A slot outside [0, y_rows) has the weight gradient NaN.  The
+ * residual's gradient is grad.  Workspace (with grad_y): hi2x_moe_combine_grad_workspace_bytes. */
+int hi2x_moe_combine_grad(const void* grad, int dt_grad, const void* y, int dt_y,
+                          int64_t y_rows, int64_t n, const int64_t* slots, const float* weights,
+                          int64_t t, int64_t top_k, float* grad_weights, void* grad_y, void* ws,
+                          int64_t ws_bytes, void* stream);
+int64_t hi2x_moe_combine_grad_workspace_bytes(int64_t y_rows);
+
+/* The same with a workspace from the stream's pool. */
 int hi2x_moe_combine_backward(const void* grad, int dt_grad, const void* y, int dt_y,
                               int64_t y_rows, int64_t n, const int64_t* slots,
                               const float* weights, int64_t t, int64_t top_k,

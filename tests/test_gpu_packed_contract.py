@@ -298,3 +298,41 @@ def test_residuals_of_another_shape_are_refused(dev):
     for bad in (x.view(6, 128).t(), x.reshape(-1), x[:1]):
         with pytest.raises(ValueError, match="residual"):
             moe_mlp(x, r, ex, ex, ex, residual=bad)
+
+
+def repeated(kind, t, k, rows, g):
+    """Slots that name rows several times: at random, one row only, in pairs far apart."""
+    if kind == "random":
+        return torch.randint(0, rows, (t, k), generator=g)
+    if kind == "one":
+        return torch.full((t, k), rows // 2)
+    half = torch.arange(t * k // 2)
+    return torch.cat([half, half, torch.zeros(t * k % 2, dtype=torch.int64)]).view(t, k) % rows
+
+
+@pytest.mark.parametrize("kind", ["random", "one", "pairs"])
+@pytest.mark.parametrize("t,k,rows,n", [(1, 3, 2, 5), (40, 2, 30, 260), (300, 8, 2400, 64),
+                                        (70, 3, 1, 33), (129, 4, 90, 1)])
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_rows_named_several_times_sum_their_gradients(kind, t, k, rows, n, dt, dev):
+    from hi2_amd.packed import combine
+
+    print("repeated", kind, t, k, rows, n, dt, flush=True)
+    g = torch.Generator().manual_seed(t)
+    y = torch.randn(rows, n, generator=g).to(F[dt]).to(dev).requires_grad_(True)
+    slots = repeated(kind, t, k, rows, g).to(dev)
+    w = torch.rand(t, k, generator=g).to(dev).requires_grad_(True)
+    c = torch.randn(t, n, generator=g).to(F[dt]).to(dev)
+    grads = [torch.autograd.grad(combine(y, slots, w), (y, w), c) for _ in range(2)]
+    assert all(torch.equal(a, b) for a, b in zip(*grads))
+    s, gc, wd = N(slots).astype(int), N(c), N(w)
+    want, mass = np.zeros((rows, n)), np.zeros((rows, n))
+    for j in range(k):
+        np.add.at(want, s[:, j], wd[:, j, None] * gc)
+        np.add.at(mass, s[:, j], np.abs(wd[:, j, None] * gc))
+    most = np.bincount(s.reshape(-1), minlength=rows)[:, None]  # float32 products and sums
+    unit = {"bf16": 2.0 ** -8, "f32": 2.0 ** -23}[dt]
+    assert (np.abs(N(grads[0][0]) - want) <= unit * np.abs(want) + 2 * most * 2.0 ** -24 * mass).all()
+    terms = gc[:, None] * N(y)[s]
+    lim = (n + 8) * 2.0 ** -24 * np.abs(terms).sum(-1)
+    assert (np.abs(N(grads[0][1]) - terms.sum(-1)) <= lim).all()

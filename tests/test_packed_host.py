@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from hi2_amd import _lib
-from test_packed_abi import packed
+from test_packed_abi import FAKE, packed, refused
 
 
 def test_workspace_of_slots_that_index_no_rows():
@@ -32,3 +32,17 @@ def test_tangents_are_seen_with_and_without_gradients():
             with ctx, pytest.raises(RuntimeError, match="this has no forward-mode"):
                 _lib.refuse_tangents("this", None, x, d)
     _lib.refuse_tangents("this", d)  # the level's end takes its tangents along
+
+
+def test_workspace_of_the_weighted_sums_gradient():
+    """One entry of 8 bytes for each row of y, where y has a gradient."""
+    size = _lib.lib().hi2x_moe_combine_grad_workspace_bytes
+    assert size(-1) == -1 and size(0) == 0 and size(100) >= 800
+
+    def grad(dy, ws, n):
+        return (FAKE, 0, FAKE, 0, 100, 16, FAKE, FAKE, 50, 2, FAKE, dy, ws, n, None)
+
+    refused("hi2x_moe_combine_grad", "needed", *grad(FAKE, FAKE, 256))
+    refused("hi2x_moe_combine_grad", "aligned", *grad(FAKE, FAKE + 8, 1024))
+    refused("hi2x_moe_combine_grad", "bad shape", FAKE, 0, FAKE, 0, -1, 16, FAKE, FAKE, 50, 2,
+            FAKE, FAKE, None, 0, None)
