@@ -867,11 +867,13 @@ extern "C" int hi2x_route(const void* logits, int dtype, int64_t ld, int64_t t, 
                          ? (size_t)rt * (e + groups) * 4
                          : 0;
   const dim3 grid((unsigned)nb);
+  // (each kernel's limit is its own largest, not this call's: threads share it)
 #define HI2X_ROUTE_(EPL, NT)                                                                   \
   {                                                                                            \
     if (dyn > 32768)                                                                           \
       HI2X_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(route_kernel<EPL, NT>),       \
-                                   hipFuncAttributeMaxDynamicSharedMemorySize, (int)dyn));     \
+                                   hipFuncAttributeMaxDynamicSharedMemorySize,                 \
+                                   NT / 16 * (16 * EPL + RG) * 4));                            \
     route_kernel<EPL, NT><<<grid, NT, dyn, s>>>(a);                                            \
   }
 #define HI2X_ROUTE(EPL, MOST)                       \

@@ -336,3 +336,22 @@ def test_rows_named_several_times_sum_their_gradients(kind, t, k, rows, n, dt, d
     terms = gc[:, None] * N(y)[s]
     lim = (n + 8) * 2.0 ** -24 * np.abs(terms).sum(-1)
     assert (np.abs(N(grads[0][1]) - terms.sum(-1)) <= lim).all()
+
+
+def test_threads_route_over_different_groups(dev):
+    """Two threads whose routers want different amounts of LDS of one kernel."""
+    from concurrent.futures import ThreadPoolExecutor
+
+    from hi2_amd.moe import route
+
+    def runs(e, groups):
+        with torch.cuda.device(dev), torch.cuda.stream(torch.cuda.Stream()):
+            x = torch.randn(64, e, generator=torch.Generator().manual_seed(e)).to(dev)
+            first = route(x, 4, groups=groups, top_groups=groups // 2)
+            same = [torch.equal(route(x, 4, groups=groups, top_groups=groups // 2).slots,
+                                first.slots) for _ in range(100)]
+            torch.cuda.current_stream().synchronize()
+            return all(same)
+
+    with ThreadPoolExecutor(2) as pool:
+        assert all(pool.map(runs, (256, 200), (64, 50)))
