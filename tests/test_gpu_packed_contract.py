@@ -174,6 +174,23 @@ def test_mlp_of_wide_rows(h, i, dev):
     assert off.max() < 2.0 ** -8 * np.abs(want).max()
 
 
+@pytest.mark.parametrize("t,e,h,i", [(9000, 4, 512, 256), (1500, 16, 320, 192)])
+def test_every_element_of_a_large_mlp(t, e, h, i, dev):
+    """Large and middle tiles, element by element."""
+    from hi2_amd.moe import route
+    from hi2_amd.packed import PackedExperts, moe_mlp
+
+    sides = _experts(e, i, h, 1), _experts(e, i, h, 2), _experts(e, h, i, 3)
+    plans = [PackedExperts(s[0], dev) for s in sides]
+    x = tokens(t, h, torch.bfloat16, 4, dev)
+    r = route(torch.randn(t, e, generator=torch.Generator().manual_seed(3)).to(dev), 2)
+    got, want = N(moe_mlp(x, r, *plans, residual=x)), mlp64(x, r, *sides, act="silu") + N(x)
+    assert np.isfinite(got).all()
+    # the result's rounding, and 2^-11 of each term of sums that cancel: as each row's largest
+    off = np.abs(got - want) - 2.0 ** -8 * np.abs(want)
+    assert (off <= 2.0 ** -7 * np.abs(want).max(1, keepdims=True)).all()
+
+
 def relative(got, want):
     return np.linalg.norm(N(got) - want) / np.linalg.norm(want)
 
@@ -241,6 +258,27 @@ def test_gradient_of_the_mlps_weights_keeps_the_activations_bits(dev):
         only[:, j] = 1.0
         want[:, j] = (N(c) * mlp64(x, replace(r, weights=only), *sides)).sum(1)
     assert relative(weights.grad, want) < 2.0 ** -17
+
+
+@pytest.mark.parametrize("k,t", [(192, 8), (1040, 8), (8256, 8), (17024, 8), (17024, 40),
+                                 (16384, 14), (4160, 100), (2064, 700)])
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+def test_every_column_counts_in_both_planes(k, t, dt, dev):
+    """One value a row, in the first and last columns and at the chunks' edges: the product is
+    its column times the value, bit for bit, with values that one plane cannot hold."""
+    from hi2_amd.packed import PackedLinear, packed_linear
+
+    n = 40
+    p, w = packed_tensor(n, k, [(2, 16), (4, 16), (8, 16)], 11, had=0.0)
+    edges = [k - 1, 0, k - 16, k - 2, 127, k // 128 * 128 - 1, k - 15, k - 8]
+    cols = (edges + list(range(k - 1, -1, -max(1, k // t))))[:t]
+    cols += [k - 1] * (t - len(cols))
+    # 13 bits with the weight's 11: exact in float32
+    value = 1.0 + 2.0 ** -12 if dt == "f32" else 1.0 + 2.0 ** -7
+    x = torch.zeros(t, k, dtype=F[dt], device=dev)
+    x[torch.arange(t, device=dev), torch.tensor(cols, device=dev)] = value
+    got = packed_linear(x, PackedLinear(p, dev), out_dtype=torch.float32)
+    assert np.array_equal(N(got), w.T[cols] * value)
 
 
 def dual(t):
@@ -336,6 +374,18 @@ def test_rows_named_several_times_sum_their_gradients(kind, t, k, rows, n, dt, d
     terms = gc[:, None] * N(y)[s]
     lim = (n + 8) * 2.0 ** -24 * np.abs(terms).sum(-1)
     assert (np.abs(N(grads[0][1]) - terms.sum(-1)) <= lim).all()
+
+
+def test_scanned_counts_of_64_token_workgroups(dev):
+    """Above 1024 workgroups of 64 tokens the counts are scanned by a launch of their own."""
+    from hi2_amd.moe import route, route_order
+
+    x = torch.randn(70_000, 96, generator=torch.Generator().manual_seed(1)).to(dev)
+    r = route(x, 8)
+    assert torch.equal(r.index, x.sort(dim=-1, descending=True, stable=True).indices[:, :8])
+    rows, offs = route_order(r.index, 96)
+    assert torch.equal(r.rows, rows) and torch.equal(r.offs, offs)
+    assert torch.equal(r.rows[r.slots], torch.arange(70_000, device=dev)[:, None].expand(-1, 8))
 
 
 def test_threads_route_over_different_groups(dev):
