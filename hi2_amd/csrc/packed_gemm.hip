@@ -521,13 +521,52 @@ GemmPlan plan_gemm(const hi2x_packed& w, int64_t slots, bool ranges, int npl) {
 
 }  // namespace
 
+// Rows of one launch without ranges: a grid holds 65535 tiles of them.  More go in parts.
+constexpr int64_t MOST_ROWS = 65535 * 64;
+
 int64_t packed_part_bytes(const hi2x_packed& w, int64_t slots, bool ranges, int npl) {
-  return few_rows_product(w, slots, ranges) ? 0 : plan_gemm(w, slots, ranges, npl).part_bytes();
+  if (few_rows_product(w, slots, ranges)) return 0;
+  if (!ranges && slots > MOST_ROWS) {
+    const int64_t a = packed_part_bytes(w, MOST_ROWS, ranges, npl);
+    const int64_t b = packed_part_bytes(w, (slots - 1) % MOST_ROWS + 1, ranges, npl);
+    return a > b ? a : b;
+  }
+  return plan_gemm(w, slots, ranges, npl).part_bytes();
 }
+
+namespace {
+// Rows [first, first + n) of a product without ranges.
+GemmArgs part_of(GemmArgs g, int64_t first, int64_t n) {
+  auto at = [&](const void* p, int64_t ld, int dtype) {
+    return p ? static_cast<const char*>(p) + first * ld * (dtype == 0 ? 4 : 2) : nullptr;
+  };
+  hi2x_epilogue& e = g.epi;
+  e.mul = at(e.mul, e.ld_mul, e.dt_mul);
+  e.residual = at(e.residual, e.ld_residual, e.dt_residual);
+  e.out = const_cast<char*>(at(e.out, e.ld_out, e.dt_out));
+  g.slots = n;
+  if (g.src) {
+    g.src += first;
+  } else {
+    g.x.planes += first * g.x.kp * g.x.nplanes;
+    g.x.scale += first;
+    g.x.rows -= first;
+  }
+  return g;
+}
+}  // namespace
 
 int packed_product(const GemmPair& two, int count, void* work, int64_t work_bytes,
                    hipStream_t s) {
   const GemmArgs& g = two.g[0];
+  if (!g.offs && g.slots > MOST_ROWS) {
+    for (int64_t first = 0; first < g.slots; first += MOST_ROWS) {
+      const int64_t left = g.slots - first;
+      const GemmArgs p = part_of(g, first, left < MOST_ROWS ? left : MOST_ROWS);
+      if (int rc = packed_product(GemmPair{{p, p}}, 1, work, work_bytes, s)) return rc;
+    }
+    return HI2X_OK;
+  }
   if (few_rows_product(g.w, g.slots, g.offs)) return packed_few(two, count, s);
   const GemmPlan p = plan_gemm(g.w, g.slots, g.offs, g.x.nplanes);
   if (count > 1 && p.splits > 1) {  // (their partial sums share one workspace)

@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 import torch
 
-from packed_data import act64, packed_tensor, stored
+from packed_data import act64, bound, packed_tensor, stored
 from test_gpu_packed import F, MIX, N, _experts, tokens
 
 pytestmark = pytest.mark.gpu
@@ -189,6 +189,31 @@ def test_every_element_of_a_large_mlp(t, e, h, i, dev):
     # the result's rounding, and 2^-11 of each term of sums that cancel: as each row's largest
     off = np.abs(got - want) - 2.0 ** -8 * np.abs(want)
     assert (off <= 2.0 ** -7 * np.abs(want).max(1, keepdims=True)).all()
+
+
+@pytest.mark.parametrize("rest", [5, 300])
+def test_more_rows_than_a_grid_holds(rest, dev):
+    """Rows beyond 65535 tiles of 64 go in parts, with their factor, bias and residual."""
+    from hi2_amd.packed import PackedLinear, packed_linear
+
+    n, k, part = 16, 64, 65535 * 64
+    t = part + rest
+    p, w = packed_tensor(n, k, [(4, 64)], 2)
+    x = torch.zeros(t, k, dtype=torch.bfloat16, device=dev)
+    mul = torch.zeros(t, n, dtype=torch.float16, device=dev)
+    res = torch.zeros(t, n, device=dev)
+    at = torch.tensor([0, 1, part - 1, part, part + 1, t - 1], device=dev)
+    x[at] = tokens(len(at), k, torch.bfloat16, 3, dev)
+    mul[at] = torch.randn(len(at), n, generator=torch.Generator().manual_seed(1)).half().to(dev)
+    res[at] = torch.randn(len(at), n, generator=torch.Generator().manual_seed(2)).to(dev)
+    got = packed_linear(x, PackedLinear(p, dev), mul=mul, residual=res)
+    want = stored(N(x[at]), p) @ w.T * N(mul[at]) + N(res[at])
+    xs = stored(N(x[at]), p)
+    lim = bound(want, torch.bfloat16, torch.bfloat16, xs, w, np.abs(N(mul[at]))) + \
+        2.0 ** -21 * np.abs(N(res[at]))
+    assert (np.abs(N(got[at]) - want) <= lim).all()
+    got[at] = 0
+    assert not got.any()
 
 
 def relative(got, want):
