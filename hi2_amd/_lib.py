@@ -11,6 +11,7 @@ import os
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libhi2x.so")
@@ -282,10 +283,9 @@ def require_gpu(*tensors: torch.Tensor) -> torch.device:
 def refuse_tangents(what: str, *tensors) -> None:
     """Raise where a tensor carries a forward-mode tangent: nothing here has such a derivative,
     and the kernels would drop it without a word."""
-    fwd = torch.autograd.forward_ad
-    if fwd._current_level < 0:  # outside every dual level: no tangents
+    if forward_ad._current_level < 0:  # outside every dual level: no tangents
         return
-    if any(t is not None and fwd.unpack_dual(t).tangent is not None for t in tensors):
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise RuntimeError(f"{what} has no forward-mode derivative: its inputs must carry no "
                            "tangent")
 

@@ -397,7 +397,7 @@ __device__ __forceinline__ void load16(const void* x, int64_t at, int dtype, flo
 // takes 20 us so, 23 in 64 x 64 tiles with the columns in eight shares; 28672 x 8192 30 and
 // 43).  Experts' rows take tiles: a layer of 64 experts at 64 tokens, eight each, took 315 us
 // so and 128 us in tiles.
-inline bool few_rows_product(const hi2x_packed&, int64_t slots, bool ranges) {
+inline bool few_rows_product(int64_t slots, bool ranges) {
   return !ranges && slots <= 16;
 }
 
@@ -418,12 +418,13 @@ struct RawRows {
   const int64_t* offs = nullptr;
 };
 
-// Products of `count` (1 or 2) tensors of one shape from the same activations; the epilogue's
-// arguments as for hi2x_packed_linear.
+// Products of `count` (1, or with ranges 2) tensors of one shape from the same activations; the
+// epilogue's arguments as for hi2x_packed_linear.  Ranges take no shares of the columns and need
+// no workspace.
 struct GemmPair {
   GemmArgs g[2];
 };
-int packed_few(const GemmPair& g, int count, hipStream_t s);
+int packed_few(const GemmArgs& g, hipStream_t s);
 int packed_few_raw(const GemmPair& g, int count, const RawRows& x, hipStream_t s);
 int packed_product(const GemmPair& g, int count, void* work, int64_t work_bytes, hipStream_t s);
 int64_t packed_part_bytes(const hi2x_packed& w, int64_t slots, bool ranges, int npl);
@@ -439,7 +440,7 @@ int launch_combine(const SlotRows& y, const int64_t* offs, int experts, int64_t 
 // Whether a product takes its activations as they are and transforms them inside.  Of
 // experts most have one row then: at 64 experts and 8 choices, two tokens 62 us so and 74 in
 // tiles, four 84 and 75.
-inline bool few_raw_product(const hi2x_packed&, int64_t slots, bool ranges) {
+inline bool few_raw_product(int64_t slots, bool ranges) {
   return slots <= (ranges ? FEW_RANGES : FEW_RAW);
 }
 

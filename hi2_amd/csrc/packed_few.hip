@@ -450,17 +450,17 @@ int launch_one(const FewArgs& a, int count, int64_t frags, hipStream_t s) {
 
 }  // namespace
 
-int packed_few(const GemmPair& g, int count, hipStream_t s) {
+int packed_few(const GemmArgs& g, hipStream_t s) {
   FewArgs a{};
-  a.two = g;
+  a.two = GemmPair{{g, g}};
   // More fragments a wave share their activation reads, while there are workgroups enough:
   // at 16 rows 28672 x 8192 takes 29.9 us with four, 37.6 with two and 61 with one, 8192 x
   // 8192 18.0 and 21.2, 4096 x 4096 11.6, 9.2 and 11.3, 1024 x 4096 8.4 with one and 10.4
   // with two.
-  const int64_t frags = g.g[0].w.max_frags;
-  return frags >= 512 ? launch<4, 16, GIVEN, 8>(a, count, s)
-                      : (frags >= 192 ? launch<2, 16, GIVEN, 8>(a, count, s)
-                                      : launch<1, 16, GIVEN, 8>(a, count, s));
+  const int64_t frags = g.w.max_frags;
+  return frags >= 512 ? launch<4, 16, GIVEN, 8>(a, 1, s)
+                      : (frags >= 192 ? launch<2, 16, GIVEN, 8>(a, 1, s)
+                                      : launch<1, 16, GIVEN, 8>(a, 1, s));
 }
 
 int packed_few_raw(const GemmPair& g, int count, const RawRows& x, hipStream_t s) {

@@ -443,8 +443,7 @@ __global__ __launch_bounds__(256) void packed_join_kernel(GemmArgs g, const floa
   __syncthreads();
   const int n = slot_row(g, tile, tid % (NS < 256 ? NS : 256));
   const float bias = g.epi.bias && n >= 0 ? load_as_f32(g.epi.bias, n, g.epi.dt_bias) : 0.0f;
-  store_pass<NS, PITCH, 16, NF == 4 ? 16 : (NF == 2 ? 8 : 4)>(g.epi, ep, xscale, n, bias,
-                                                              first + 16 * m, rows);
+  store_pass<NS, PITCH, 16, NF == 2 ? 8 : 4>(g.epi, ep, xscale, n, bias, first + 16 * m, rows);
 }
 
 template <int NF, int MF>
@@ -525,7 +524,7 @@ GemmPlan plan_gemm(const hi2x_packed& w, int64_t slots, bool ranges, int npl) {
 constexpr int64_t MOST_ROWS = 65535 * 64;
 
 int64_t packed_part_bytes(const hi2x_packed& w, int64_t slots, bool ranges, int npl) {
-  if (few_rows_product(w, slots, ranges)) return 0;
+  if (few_rows_product(slots, ranges)) return 0;
   if (!ranges && slots > MOST_ROWS) {
     const int64_t a = packed_part_bytes(w, MOST_ROWS, ranges, npl);
     const int64_t b = packed_part_bytes(w, (slots - 1) % MOST_ROWS + 1, ranges, npl);
@@ -567,12 +566,8 @@ int packed_product(const GemmPair& two, int count, void* work, int64_t work_byte
     }
     return HI2X_OK;
   }
-  if (few_rows_product(g.w, g.slots, g.offs)) return packed_few(two, count, s);
+  if (few_rows_product(g.slots, g.offs)) return packed_few(g, s);
   const GemmPlan p = plan_gemm(g.w, g.slots, g.offs, g.x.nplanes);
-  if (count > 1 && p.splits > 1) {  // (their partial sums share one workspace)
-    if (int rc = packed_product(two, 1, work, work_bytes, s)) return rc;
-    return packed_product(GemmPair{{two.g[1], two.g[1]}}, 1, work, work_bytes, s);
-  }
   int64_t nx = p.nx;
   if (count > 1) {
     const int64_t* m = two.g[1].w.max_tiles;
@@ -634,7 +629,7 @@ extern "C" int hi2x_packed_linear(const hi2x_packed* w, const void* x, int dtype
   const hipStream_t s = as_stream(stream);
   const RawRows raw{x, dtype, ldx, x_rows, nplanes};
   GemmArgs g{*w, hi2x_activations{}, src, offs, slots, *epi};
-  if (few_raw_product(*w, slots, offs)) return packed_few_raw(GemmPair{{g, g}}, 1, raw, s);
+  if (few_raw_product(slots, offs)) return packed_few_raw(GemmPair{{g, g}}, 1, raw, s);
   const bool each = transform_slots(*w, x_rows);
   const int64_t rows = transform_rows(*w, x_rows, src, slots);
   HI2X_REQUIRE(rows < (1ll << 31), "packed_linear: too many rows");
@@ -664,7 +659,7 @@ extern "C" int64_t hi2x_packed_workspace_bytes(const hi2x_packed* w, int64_t x_r
   if (slots == 0) return 0;
   int64_t front = 0;
   if (!given) {
-    if (few_raw_product(*w, slots, ranges)) return 0;
+    if (few_raw_product(slots, ranges)) return 0;
     const int64_t rows = transform_rows(*w, x_rows, indexed, slots);
     front = plane_bytes(*w, rows, nplanes) + align256(rows * 4);
   }
@@ -682,7 +677,7 @@ struct MlpSpace {
   int64_t in[2], in_scale[2];   // the transformed tokens: shared, or per tensor
   int64_t mid, mid_scale;       // the transformed hidden values
   int64_t in_rows[2];
-  int64_t part, bytes;
+  int64_t bytes;
 };
 
 MlpSpace mlp_space(const hi2x_packed& gate, const hi2x_packed& up, const hi2x_packed& down,
@@ -697,7 +692,7 @@ MlpSpace mlp_space(const hi2x_packed& gate, const hi2x_packed& up, const hi2x_pa
   // A bf16 result hides the rounding to fp16 (2^-11) as it hides that of one plane;
   // writing and reading the three is what the large calls are short of: 64 experts of
   // 2048 x 1024, 8 choices, 16384 tokens 2680 us in f32, 2060 so.  Short calls keep f32.
-  m.half = npl_mid == 1 && !few_raw_product(gate, slots, true);
+  m.half = npl_mid == 1 && !few_raw_product(slots, true);
   for (const hi2x_packed* p : {&gate, &up, &down})
     m.half = m.half && p->places && 16 * p->max_frags <= SLOTS16 &&
              16 * p->max_frags <= p->n + 16 * PK_SEGS;  // (as many as the readers' loads take)
@@ -707,7 +702,7 @@ MlpSpace mlp_space(const hi2x_packed& gate, const hi2x_packed& up, const hi2x_pa
   m.y = take(slots * (m.half ? 16 * down.max_frags : down.n) * size);
   const hi2x_packed* of[3] = {&gate, &up, &down};
   for (int i = 0; i < 3 && m.half; ++i) m.exps[i] = take(slots * exps_pitch(*of[i]));
-  if (!few_raw_product(gate, slots, true)) {
+  if (!few_raw_product(slots, true)) {
     for (int i = 0; i < (shared ? 1 : 2); ++i) {
       m.in_rows[i] = (i ? up : gate).per_expert ? slots : t;
       m.in[i] = take(plane_bytes(gate, m.in_rows[i], npl));
@@ -715,10 +710,6 @@ MlpSpace mlp_space(const hi2x_packed& gate, const hi2x_packed& up, const hi2x_pa
     }
     m.mid = take(plane_bytes(down, slots, npl_mid));
     m.mid_scale = take(slots * 4);
-    const int64_t a = packed_part_bytes(gate, slots, true, npl);
-    const int64_t b = packed_part_bytes(down, slots, true, npl_mid);
-    m.part = at;
-    at += a > b ? a : b;
   }
   m.bytes = at;
   return m;
@@ -764,7 +755,7 @@ extern "C" int hi2x_moe_mlp(const hi2x_packed* gate, const hi2x_packed* up,
     HI2X_REQUIRE(d >= 0 && d <= 2, "moe_mlp: dtype %d", d);
   if (t == 0) return HI2X_OK;
   HI2X_REQUIRE(rows && offs && slots && weights && out, "moe_mlp: null buffer");
-  HI2X_REQUIRE(t * gate->kp * 2 * nplanes < (1ll << 32) - 1 || few_raw_product(*gate, n, true),
+  HI2X_REQUIRE(t * gate->kp * 2 * nplanes < (1ll << 32) - 1 || few_raw_product(n, true),
                "moe_mlp: 4 GiB of activations or more cannot be taken by index");
   const hipStream_t s = as_stream(stream);
   const MlpSpace m = mlp_space(*gate, *up, *down, t, n, nplanes, nplanes_mid, shared);
@@ -786,7 +777,7 @@ extern "C" int hi2x_moe_mlp(const hi2x_packed* gate, const hi2x_packed* up,
   RawRows hidden{w.p + m.gate, 0, gate->n, n, nplanes_mid,
                  reinterpret_cast<const float*>(w.p + m.up), act};
   SlotRows results;
-  if (few_raw_product(*gate, n, true)) {
+  if (few_raw_product(n, true)) {
     if (int rc = packed_few_raw(in, 2, tokens, s)) return rc;
     if (int rc = packed_few_raw(GemmPair{{last, last}}, 1, hidden, s)) return rc;
   } else {
@@ -807,7 +798,6 @@ extern "C" int hi2x_moe_mlp(const hi2x_packed* gate, const hi2x_packed* up,
         return SlotRows{static_cast<const uint16_t*>(g.epi.out), (int)g.epi.ld_out, g.w.places,
                         g.exps, g.ep, g.x.scale, g.src, g.x.rows, g.w.n};
       };
-      hidden.x = nullptr;
       hidden.s1 = rows_of(in.g[0]);
       hidden.s2 = rows_of(in.g[1]);
       hidden.offs = offs;
@@ -815,15 +805,14 @@ extern "C" int hi2x_moe_mlp(const hi2x_packed* gate, const hi2x_packed* up,
       last.x.rows = n;
       results = rows_of(last);
     }
-    const int64_t part = m.bytes - m.part;
-    if (int rc = packed_product(in, 2, w.p + m.part, part, s)) return rc;
+    if (int rc = packed_product(in, 2, nullptr, 0, s)) return rc;
     last.x = hi2x_activations{reinterpret_cast<uint16_t*>(w.p + m.mid),
                               reinterpret_cast<float*>(w.p + m.mid_scale), n, down->kp,
                               nplanes_mid, 0};
     if (int rc = launch_activations(hidden, *down, nullptr, down->per_expert ? offs : nullptr,
                                     last.x, s))
       return rc;
-    if (int rc = packed_product(GemmPair{{last, last}}, 1, w.p + m.part, part, s)) return rc;
+    if (int rc = packed_product(GemmPair{{last, last}}, 1, nullptr, 0, s)) return rc;
   }
   if (m.half)
     return launch_combine(results, offs, (int)down->experts, n, slots, weights, t, top_k, residual,

@@ -99,7 +99,7 @@ def route(logits: torch.Tensor, top_k: int, scoring: str = "softmax", bias=None,
     ``logits`` requires a gradient they have one (the choice has none).
 
     Limits: 512 experts, 32 choices, 64 groups.  One launch for up to 64 tokens (32 above
-    256 experts), two above; the host never waits."""
+    256 experts), two above, three from 65537 (32769) on; the host never waits."""
     dev = _lib.require_gpu(logits, bias)
     _lib.refuse_tangents("route", logits, bias)
     if logits.dim() != 2:
