@@ -161,7 +161,7 @@ __device__ __forceinline__ void group_values(const RawRows& x, const f32x4v* sr,
 // in a second plane.  A thread keeps its group's values between the two where one group a thread
 // is all there is (KEEP, up to 16384 columns); rows beyond are read twice, the second time from
 // L2.  Bound by reading x and writing the planes: 16384 x 2048 in bf16 27 us, 4.9 TB/s; the hidden
-// rows of 16384 tokens and 8 of 64 experts (131072 x 1024, SlotRows) 262 us, where the way
+// rows of 16384 tokens and 8 of 64 experts (131072 x 1024, SlotRows) 255 us, where the way
 // through LDS counts (196 us with the rows in their own order).
 template <int DT, bool GLU, bool KEEP, int TPR>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void activations_kernel(

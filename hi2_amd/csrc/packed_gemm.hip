@@ -691,7 +691,7 @@ MlpSpace mlp_space(const hi2x_packed& gate, const hi2x_packed& up, const hi2x_pa
   };
   // A bf16 result hides the rounding to fp16 (2^-11) as it hides that of one plane;
   // writing and reading the three is what the large calls are short of: 64 experts of
-  // 2048 x 1024, 8 choices, 16384 tokens 2680 us in f32, 2060 so.  Short calls keep f32.
+  // 2048 x 1024, 8 choices, 16384 tokens 2680 us in f32, 2100 so.  Short calls keep f32.
   m.half = npl_mid == 1 && !few_raw_product(slots, true);
   for (const hi2x_packed* p : {&gate, &up, &down})
     m.half = m.half && p->places && 16 * p->max_frags <= SLOTS16 &&
