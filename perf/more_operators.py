@@ -75,7 +75,7 @@ def listed():
         # every expert of a layer in bfloat16 with 32-bit masters
         _adamw(192, 1024, 2048, dtype="bf16", master=True, name="adamw_192x1024x2048_bf16"),
         # many small tensors of odd sizes in half precision and 8-bit states
-        _adamw(300, 37, 129, small=3, dtype="f16", bits=8, t=0, name="adamw_300x37x129_f16_8bit"),
+        _adamw(100, 37, 129, small=3, dtype="f16", bits=8, t=0, name="adamw_100x37x129_f16_8bit"),
     ]
 
 
@@ -106,7 +106,7 @@ def draw(rng):
         return _gated(rows, width, dtype=rng.choice(["bf16", "bf16", "f16", "f32"]),
                       act=rng.choice(["silu", "silu", "gelu", "gelu_tanh", "relu"]),
                       halves=rng.random() < 0.4, grad=rng.random() < 0.6)
-    tensors = int(_log(rng, 1, 1000))
+    tensors = int(_log(rng, 1, 200))
     total = _log(rng, 3e3 * tensors, 17e7)
     width = int(_log(rng, 16, min(14336.0, total / tensors)))
     rows = max(1, int(total / tensors / width))
