@@ -74,6 +74,18 @@ SIGNATURES = {
     "hi2x_qad_weights_fwd": [_P, _P, _P, _I64, _I64, _I64, _P, _P, _P, _P],
     "hi2x_qad_weights_bwd": [_P, _P, _P, _P, _I64, _I64, _I64, _P, _P, _P, _P],
     "hi2x_qad_wht_scale": [_P, _I64, _I64, _P, _P, _I, _P],
+    "hi2x_adamw_step": [_P, _P, _P, _P, _I64, _I, _I, _P, _I64, _P, _P, _P, _P, _P, _P, _P, _P],
+    "hi2x_adamw_hold": [_P, _P, _I64, _P, _P, _P, _P, _P],
+    "hi2x_adamw_moments": [_P, _P, _P, _P, _I64, _P, _P, _P],
+    "hi2x_grouped_linear": [_P, _I, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, _I64, _P, _P, _I64,
+                            _P],
+    "hi2x_grouped_grad_x": [_P, _I, _I64, _P, _I64, _I64, _I64, _P, _I64, _P, _I64, _I64, _P, _P,
+                            _I64, _P],
+    "hi2x_grouped_grad_w": [_P, _I, _I64, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _I64, _P, _P,
+                            _I64, _P],
+    "hi2x_gated": [_P, _I64, _P, _I64, _I64, _I64, _I, _I, _P, _I64, _P],
+    "hi2x_gated_backward": [_P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I, _I, _P, _I64, _P, _I64,
+                            _P],
 }
 class Piece(ctypes.Structure):
     """hi2x_piece (include/hi2x.h): one piece of hi2x_assemble_batch."""
@@ -127,6 +139,13 @@ class Epilogue(ctypes.Structure):
                 ("dt_out", ctypes.c_int32), ("act", ctypes.c_int32), ("pad_", ctypes.c_int32)]
 
 
+class AdamwGroup(ctypes.Structure):
+    """hi2x_adamw_group (include/hi2x.h): a parameter group's options."""
+
+    _fields_ = [("lr", ctypes.c_double), ("beta1", ctypes.c_double), ("beta2", ctypes.c_double),
+                ("eps", ctypes.c_double), ("weight_decay", ctypes.c_double), ("lr_tensor", _P)]
+
+
 SIGNATURES["hi2x_packed_layout"] = [_P, _P, _P, _P, _P, _P, _P]
 SIGNATURES["hi2x_packed_activations"] = [_P, _P, _I, _I64, _I64, _P, _P, _P, _P]
 SIGNATURES["hi2x_packed_linear"] = [_P, _P, _I, _I64, _I64, _I, _P, _P, _I64, _P, _P, _I64, _P]
@@ -155,6 +174,7 @@ SIZES = {
     "hi2x_moe_mlp_workspace_bytes": [_P, _P, _P, _I64, _I64, _I, _I, _I],
     "hi2x_route_workspace_bytes": [_I64, _I64],
     "hi2x_moe_combine_grad_workspace_bytes": [_I64],
+    "hi2x_grouped_workspace_bytes": [_I, _I, _I64, _I64, _I64, _I64, _I64, _I, _I, _I],
 }
 
 

@@ -696,6 +696,97 @@ int64_t hi2x_moe_mlp_workspace_bytes(const hi2x_packed* gate, const hi2x_packed*
                                      const hi2x_packed* down, int64_t t, int64_t top_k,
                                      int nplanes, int nplanes_mid, int shared);
 
+/* ---- training weights --------------------------------------------------------------------- */
+
+/* A parameter of the AdamW step: its elements (n > 0), where its moments begin (a multiple of
+ * HI2X_ADAMW_BLOCK elements), the number of its first chunk (chunks of HI2X_ADAMW_CHUNK elements,
+ * tensor after tensor) and its group. */
+#define HI2X_ADAMW_BLOCK 256
+#define HI2X_ADAMW_CHUNK 4096
+typedef struct hi2x_adamw_tensor {
+  int64_t n;
+  int64_t start;
+  int64_t first_chunk;
+  int32_t group;
+  int32_t reserved;
+} hi2x_adamw_tensor;
+
+/* lr_tensor (device, or NULL) takes the place of lr. */
+typedef struct hi2x_adamw_group {
+  double lr, beta1, beta2, eps, weight_decay;
+  const float* lr_tensor;
+} hi2x_adamw_group;
+
+/* One AdamW step of `count` tensors of one dtype (0 f32, 1 fp16, 2 bf16), all in one launch for
+ * up to 192 tensors of up to 16 groups:
+ *   m = b1 m + (1 - b1) g, v = b2 v + (1 - b2) g^2,
+ *   p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+ * in f32, every product and sum rounded, the parameter once more to its dtype.  tensors: host
+ * array, ordered by start and by group; device_tensors: the same on the device; params and grads:
+ * host arrays of device addresses (contiguous; grads[i] NULL: the tensor is left as it is).
+ * Moments of all tensors lie in one buffer each: with bits 32 f32; with bits 8 one byte an
+ * element and f32 m_unit, v_unit an element of which serves HI2X_ADAMW_BLOCK elements: m = +-q^2
+ * unit for the byte q of either sign, v = (q^2 unit)^2; the bytes of a block whose largest is not
+ * finite stand for NaN.  Elements between a tensor's end and the next multiple of
+ * HI2X_ADAMW_BLOCK are zero and stay so.  master (or NULL): f32 parameters laid out as the
+ * moments are, which take the step in the place of fp16 or bf16 ones and are rounded to them.
+ * steps [count]: the steps each tensor has taken, counted on; done [count]: zeros, left as
+ * zeros. */
+int hi2x_adamw_step(const hi2x_adamw_tensor* tensors, const hi2x_adamw_tensor* device_tensors,
+                    void* const* params, const void* const* grads, int64_t count, int dtype,
+                    int bits, const hi2x_adamw_group* groups, int64_t n_groups, void* m, void* v,
+                    float* m_unit, float* v_unit, float* master, int64_t* steps, int32_t* done,
+                    void* stream);
+
+/* f32 moments of `blocks` x HI2X_ADAMW_BLOCK elements as bytes and units, and back. */
+int hi2x_adamw_hold(const float* m, const float* v, int64_t blocks, void* m_codes, void* v_codes,
+                    float* m_unit, float* v_unit, void* stream);
+int hi2x_adamw_moments(const void* m_codes, const void* v_codes, const float* m_unit,
+                       const float* v_unit, int64_t blocks, float* m, float* v, void* stream);
+
+/* Products grouped by expert, with ragged sizes and gradients: for the slots j of expert e's range
+ * offs[e] <= j < offs[e + 1] of `slots` slots,
+ *   out[j] = x[rows[j]] w[e]^T                                (hi2x_grouped_linear)
+ *   dx[t]  = sum over token t's slots of dy[slot] w[e]        (hi2x_grouped_grad_x)
+ *   dw[e]  = sum over expert e's slots of dy[j]^T x[rows[j]]  (hi2x_grouped_grad_w)
+ * with w [experts][n][k] contiguous and everything of one dtype (0 f32, 1 fp16, 2 bf16), summed in
+ * f32 and rounded once.  x [x_rows][k] and dy [slots][n] have rows ldx and ldy elements apart,
+ * aligned to one element; out [slots][n], dx and dw [experts][n][k] are contiguous.  rows (or
+ * NULL: slot j reads row j, x_rows = slots) and offs (experts + 1, ascending, within 0 to slots)
+ * are i64 on the device, never read by the host.  A row outside x is taken as a row of NaN.
+ * Slots outside all ranges get rows of zeros in out and in dx; an expert without slots gets zeros
+ * in dw.  hi2x_grouped_grad_x: with slots_of [t][top_k] (i64: each token's slots; one outside
+ * 0 to slots gives a row of NaN) dx is [t][k], summed in the order of top_k over what each slot
+ * has, which for fp16 and bf16 is rounded to that type first; with slots_of NULL dx is [slots][k].
+ * Workspace: hi2x_grouped_workspace_bytes of what (0 linear, 1 grad_x, 2 grad_w), tokens = x_rows
+ * (grad_x: t), indexed = rows or slots_of given, and whether x or dy (first) and w or, for
+ * grad_w, x (second) begin and continue at multiples of 16 bytes. */
+int hi2x_grouped_linear(const void* x, int dtype, int64_t ldx, int64_t x_rows, const void* w,
+                        int64_t experts, int64_t n, int64_t k, const int64_t* rows,
+                        const int64_t* offs, int64_t slots, void* out, void* ws, int64_t ws_bytes,
+                        void* stream);
+int hi2x_grouped_grad_x(const void* dy, int dtype, int64_t ldy, const void* w, int64_t experts,
+                        int64_t n, int64_t k, const int64_t* offs, int64_t slots,
+                        const int64_t* slots_of, int64_t t, int64_t top_k, void* dx, void* ws,
+                        int64_t ws_bytes, void* stream);
+int hi2x_grouped_grad_w(const void* dy, int dtype, int64_t ldy, const void* x, int64_t ldx,
+                        int64_t x_rows, int64_t experts, int64_t n, int64_t k,
+                        const int64_t* rows, const int64_t* offs, int64_t slots, void* dw,
+                        void* ws, int64_t ws_bytes, void* stream);
+int64_t hi2x_grouped_workspace_bytes(int what, int dtype, int64_t tokens, int64_t experts,
+                                     int64_t n, int64_t k, int64_t slots, int indexed,
+                                     int first_aligned, int second_aligned);
+
+/* out = act(gate) * up, [rows][n], all of one dtype with rows ld apart: act as in hi2x_epilogue.
+ * In f32, rounded once. */
+int hi2x_gated(const void* gate, int64_t ld_gate, const void* up, int64_t ld_up, int64_t rows,
+               int64_t n, int dtype, int act, void* out, int64_t ld_out, void* stream);
+
+/* Its gradients for grad [rows][n]: d_gate = grad * up * act'(gate), d_up = grad * act(gate). */
+int hi2x_gated_backward(const void* grad, int64_t ld_grad, const void* gate, int64_t ld_gate,
+                        const void* up, int64_t ld_up, int64_t rows, int64_t n, int dtype, int act,
+                        void* d_gate, int64_t ld_dgate, void* d_up, int64_t ld_dup, void* stream);
+
 /* ---- streams ---------------------------------------------------------------------------- */
 
 /* Background hint for a stream.  No counterpart in the reference (its encode runs one
