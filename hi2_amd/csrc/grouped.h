@@ -12,6 +12,7 @@ struct GroupedArgs {
   const int64_t *rows, *offs;
   int64_t ldx, ldy, x_rows, slots;
   int64_t experts, n, k;
+  uint32_t* offsets;  // of the slots' rows in x, for grad_w in tiles
 };
 
 // Expert e's slots, empty where the ranges are not as they should be.
@@ -71,5 +72,14 @@ __device__ __forceinline__ GroupedWork find_rows(const GroupedArgs& g, int tile,
   }
   return w;
 }
+
+// What a resource that offsets of 32 bits reach may span: an offset past it by this much again is
+// past it still.
+constexpr uint32_t GROUPED_SPAN = 0x7f000000u;
+
+// The product in tiles (16 bits; rows and weights at multiples of 16 bytes, n and k of 8).
+// grad_w with rows: g.offsets, room for grouped_offsets(slots) of them.
+constexpr int64_t grouped_offsets(int64_t slots) { return slots + 256; }
+int grouped_tiles(const GroupedArgs& g, int what, int dtype, hipStream_t s, const char* name);
 
 }  // namespace hi2x

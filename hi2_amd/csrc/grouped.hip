@@ -166,6 +166,25 @@ int check_grouped(const GroupedArgs& g, int dtype, const char* what) {
 
 int64_t size_of(int dtype) { return dtype == 0 ? 4 : 2; }
 
+// Whether the product goes in tiles of 16-bit values: pieces of 16 bytes are whole.
+bool in_tiles(const GroupedArgs& g, int what, int dtype) {
+  auto whole = [](const void* p, int64_t ld) { return ((uintptr_t)p & 15) == 0 && ld % 8 == 0; };
+  if (dtype == 0 || g.n % 8 || g.k % 8) return false;
+  if (what != GROUPED_GRAD_W && !whole(g.w, g.k)) return false;
+  if (what != GROUPED_LINEAR && (!whole(g.dy, g.ldy) || g.ldy >= (1 << 21))) return false;
+  if (what != GROUPED_GRAD_X &&
+      (!whole(g.x, g.ldx) || g.ldx >= (1 << 21) ||
+       (g.rows && g.x_rows * g.ldx * 2 > (int64_t)GROUPED_SPAN)))
+    return false;
+  return true;
+}
+
+template <int WHAT>
+int launch_product(const GroupedArgs& g, int dtype, hipStream_t s, const char* what) {
+  return in_tiles(g, WHAT, dtype) ? grouped_tiles(g, WHAT, dtype, s, what)
+                                  : launch_any<WHAT>(g, dtype, s, what);
+}
+
 }  // namespace
 }  // namespace hi2x
 
@@ -175,11 +194,12 @@ extern "C" int64_t hi2x_grouped_workspace_bytes(int what, int dtype, int64_t tok
                                                 int64_t experts, int64_t n, int64_t k,
                                                 int64_t slots, int indexed, int first_aligned,
                                                 int second_aligned) {
-  (void)first_aligned, (void)second_aligned;
   GroupedArgs g{};
   g.experts = experts, g.n = n, g.k = k, g.slots = slots, g.x_rows = tokens;
   if (what < 0 || what > 2 || check_grouped(g, dtype, "grouped_workspace_bytes")) return -1;
   if (what == GROUPED_GRAD_X && indexed) return align256(slots * k * size_of(dtype));
+  if (what == GROUPED_GRAD_W && indexed && dtype) return align256(grouped_offsets(slots) * 4);
+  (void)first_aligned, (void)second_aligned;
   return 0;
 }
 
@@ -197,7 +217,7 @@ extern "C" int hi2x_grouped_linear(const void* x, int dtype, int64_t ldx, int64_
   HI2X_REQUIRE(x_rows <= 1 || ldx >= k, "grouped_linear: rows of x overlap");
   if (slots == 0) return HI2X_OK;
   HI2X_REQUIRE((x || x_rows == 0) && w && offs && out, "grouped_linear: null buffer");
-  return launch_any<GROUPED_LINEAR>(g, dtype, as_stream(stream), "grouped_linear");
+  return launch_product<GROUPED_LINEAR>(g, dtype, as_stream(stream), "grouped_linear");
 }
 
 extern "C" int hi2x_grouped_grad_x(const void* dy, int dtype, int64_t ldy, const void* w,
@@ -216,13 +236,13 @@ extern "C" int hi2x_grouped_grad_x(const void* dy, int dtype, int64_t ldy, const
   if (slots_of ? t == 0 : slots == 0) return HI2X_OK;
   HI2X_REQUIRE((dy || slots == 0) && w && offs && dx, "grouped_grad_x: null buffer");
   const hipStream_t s = as_stream(stream);
-  if (!slots_of) return launch_any<GROUPED_GRAD_X>(g, dtype, s, "grouped_grad_x");
+  if (!slots_of) return launch_product<GROUPED_GRAD_X>(g, dtype, s, "grouped_grad_x");
   Workspace part;
   const size_t need = (size_t)align256(slots * k * size_of(dtype));
   if (int rc = take_workspace(part, ws, ws_bytes, need, s, "grouped_grad_x")) return rc;
   g.out = part.p;
   if (slots)
-    if (int rc = launch_any<GROUPED_GRAD_X>(g, dtype, s, "grouped_grad_x")) return rc;
+    if (int rc = launch_product<GROUPED_GRAD_X>(g, dtype, s, "grouped_grad_x")) return rc;
   if (dtype == 0)
     sum_slots_kernel<0><<<(unsigned)t, 256, 0, s>>>(part.p, slots, k, slots_of, t, (int)top_k, dx);
   else if (dtype == 1)
@@ -249,5 +269,12 @@ extern "C" int hi2x_grouped_grad_w(const void* dy, int dtype, int64_t ldy, const
                "grouped_grad_w: rows overlap");
   HI2X_REQUIRE(((x || x_rows == 0) && dy || slots == 0) && offs && dw,
                "grouped_grad_w: null buffer");
-  return launch_any<GROUPED_GRAD_W>(g, dtype, as_stream(stream), "grouped_grad_w");
+  const hipStream_t s = as_stream(stream);
+  Workspace offsets;
+  if (rows && in_tiles(g, GROUPED_GRAD_W, dtype)) {
+    const size_t need = (size_t)align256(grouped_offsets(slots) * 4);
+    if (int rc = take_workspace(offsets, ws, ws_bytes, need, s, "grouped_grad_w")) return rc;
+    g.offsets = reinterpret_cast<uint32_t*>(offsets.p);
+  }
+  return launch_product<GROUPED_GRAD_W>(g, dtype, s, "grouped_grad_w");
 }

@@ -1,0 +1,535 @@
+// Products grouped by expert in 16 bits: tiles of 256 x 256 or 128 x 128 results through LDS and
+// the matrix units.
+//
+// An operand of a tile is T rows of the contraction's values.  Where these are neighbours in
+// memory (x and w of the product, dy of the tokens' gradient) a stage of 32 of them is 64 bytes a
+// row, and a lane reads its 8 as one piece; where they are a row apart (w of the tokens'
+// gradient, dy and x of the weights') a stage is 32 rows of T values, and LDS's transposing read
+// hands a lane its column.  Both are loaded as they lie, 16 bytes a lane, straight into LDS.
+//
+// A wave holds T/2 x T/2 results in registers; a ring of four stages is in flight.
+#include "grouped.h"
+
+namespace hi2x {
+namespace {
+
+typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x16v __attribute__((ext_vector_type(16)));
+
+// Offsets past every resource: a row's, a piece's, and their sum.
+constexpr uint32_t ROW_DEAD = 0x80000000u, PIECE_DEAD = GROUPED_SPAN;
+
+// 64 lanes x 16 bytes from memory into LDS at byte `la` (+ 16 lane), in inline assembly so that the
+// compiler does not wait for it before every later LDS read.  One wait state lies between the
+// write of M0 and the load.
+__device__ __forceinline__ void lds_load16(__amdgpu_buffer_rsrc_t rs, uint32_t voff, uint32_t la) {
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :
+               : "s"(la), "v"(voff), "s"(rs)
+               : "m0");
+#pragma clang diagnostic pop
+}
+
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)v);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)((uint64_t)v >> 32));
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
+constexpr int wait_for(int vm, int lgkm) {
+  return (vm & 15) | ((vm >> 4) << 14) | (7 << 4) | (lgkm << 8);
+}
+
+// LDS accesses stay on their side.
+__device__ __forceinline__ void meet() {
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+  __builtin_amdgcn_s_barrier();
+  __atomic_signal_fence(__ATOMIC_SEQ_CST);
+}
+
+template <int DT>
+__device__ __forceinline__ f32x16v product(const s16x8& a, const s16x8& b, const f32x16v& c) {
+  if constexpr (DT == 1)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h16x8, a),
+                                                  __builtin_bit_cast(h16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b16x8, a),
+                                                   __builtin_bit_cast(b16x8, b), c, 0, 0, 0);
+}
+
+constexpr int STAGE = 32;  // of the contraction
+constexpr int RING = 4;
+
+// Neighbours of the contraction are neighbours in memory.  LDS: T rows of four 16-byte pieces,
+// piece q of row r at q ^ ((r / 4) % 4), so that the 16 rows that a read of one piece touches at
+// a time lie on different banks.
+template <int T>
+struct AlongOperand {
+  static constexpr int NC = T / 64;  // a wave's loads of a stage, 16 rows each
+  __amdgpu_buffer_rsrc_t rs;
+  uint32_t row[NC];  // this lane's rows' offsets
+  uint32_t piece;    // its piece's
+  int len;           // of the contraction
+  uint32_t at;       // LDS byte of the wave's first load
+  uint32_t read0, read1;
+  __device__ __forceinline__ void init(uint32_t lds, int wv, int half, int len_) {
+    const int lane = threadIdx.x & 63;
+    len = len_;
+    piece = 8 * ((lane & 3) ^ ((lane >> 4) & 3));
+    at = lds + NC * wv * 1024;
+    const uint32_t r = half * (T / 2) + (lane & 31);
+    const int h = lane >> 5, x = (lane >> 2) & 3;
+    read0 = r * 64 + 16 * (h ^ x);
+    read1 = r * 64 + 16 * ((2 + h) ^ x);
+  }
+  // row of load i that this lane brings
+  static __device__ __forceinline__ int row_of(int wv, int i) {
+    return 16 * (NC * wv + i) + ((threadIdx.x & 63) >> 2);
+  }
+  struct Stage {
+    uint32_t k;
+  };
+  __device__ __forceinline__ Stage begin(int st) const {
+    const uint32_t c = (uint32_t)st * STAGE + piece;
+    return Stage{c < (uint32_t)len ? 2 * c : PIECE_DEAD};
+  }
+  __device__ __forceinline__ void load(const Stage& s, int i, uint32_t buffer) const {
+    lds_load16(rs, row[i] + s.k, at + buffer + i * 1024);
+  }
+  __device__ __forceinline__ void read(s16x8 (&v)[NC], const char* from, int step) const {
+    const char* p = from + (step ? read1 : read0);
+#pragma unroll
+    for (int t = 0; t < NC; ++t) v[t] = *reinterpret_cast<const s16x8*>(p + t * 2048);
+  }
+};
+
+// Neighbours of the contraction are a row apart.  LDS: 32 rows of T / 8 pieces, piece p of row r
+// at p ^ (4 (r % 4)): a transposing read's 16 lanes take 4 rows x 32 bytes, and the four rows
+// lie on different banks.
+template <int T>
+struct AcrossOperand {
+  static constexpr int NC = T / 64, LP = T / 8, RPC = 64 / LP;  // lanes a row, rows a load
+  const char* base;
+  int64_t pitch;     // bytes
+  int64_t rows;      // of the contraction
+  uint32_t last;     // bytes of a row that count
+  uint32_t own[NC];  // this lane's offsets within a stage
+  uint32_t at;
+  uint32_t read_at[NC];
+  __device__ __forceinline__ void init(uint32_t lds, int wv, int half, int cols) {
+    const int lane = threadIdx.x & 63;
+    at = lds + NC * wv * 1024;
+    last = 2 * cols;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int r = RPC * (NC * wv + i) + lane / LP;
+      const int p = (lane % LP) ^ (4 * (r & 3));
+      own[i] = 8 * p < cols ? (uint32_t)(r * pitch) + 16 * p : PIECE_DEAD;
+    }
+    const int s = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int t = 0; t < NC; ++t)
+      read_at[t] = (8 * (g >> 1) + (s >> 2)) * (2 * T) + 8 * (s & 1) +
+                   16 * (((half * (T / 16) + 4 * t) ^ (4 * (s >> 2))) + 2 * (g & 1) +
+                         ((s & 3) >> 1));
+  }
+  struct Stage {
+    __amdgpu_buffer_rsrc_t rs;
+  };
+  __device__ __forceinline__ Stage begin(int st) const {
+    int left = (int)rows - st * STAGE;
+    left = left < STAGE ? left : STAGE;
+    const int bytes = left * (int)pitch - ((int)pitch - (int)last);
+    return Stage{__builtin_amdgcn_make_buffer_rsrc(
+        reinterpret_cast<char*>(uniform((int64_t)(base + (int64_t)st * (STAGE * pitch)))),
+        (short)0, __builtin_amdgcn_readfirstlane(bytes < 0 ? 0 : bytes), 0x00020000)};
+  }
+  __device__ __forceinline__ void load(const Stage& s, int i, uint32_t buffer) const {
+    lds_load16(s.rs, own[i], at + buffer + i * 1024);
+  }
+  __device__ __forceinline__ void read(s16x8 (&v)[NC], const char* from, int step) const {
+#pragma unroll
+    for (int t = 0; t < NC; ++t) {
+      const char* p = from + read_at[t] + step * (16 * 2 * T);
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (__attribute__((address_space(3))) s16x4*)(p));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (__attribute__((address_space(3))) s16x4*)(p + 4 * 2 * T));
+      v[t] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  }
+};
+
+// The same of rows that an index names, by their offsets in x (indexed_rows_kernel): bit 0 marks
+// a row outside.
+template <int T>
+struct IndexedOperand : AcrossOperand<T> {
+  using Base = AcrossOperand<T>;
+  using Base::LP, Base::NC, Base::RPC;
+  const __attribute__((address_space(4))) uint32_t* offsets;
+  __amdgpu_buffer_rsrc_t all;
+  int wave_row;  // the wave's first row in a stage
+  uint32_t seen;  // all offsets, or-ed
+  __device__ __forceinline__ void init(uint32_t lds, int wv, int half, int cols) {
+    this->pitch = 0;
+    Base::init(lds, wv, half, cols);
+    wave_row = RPC * NC * wv;
+    seen = 0;
+  }
+  static_assert(RPC * NC == 8, "rows of a wave's loads");
+  struct Stage {
+    u32x8 row;
+  };
+  // Rows past the end (there are offsets, of whatever) are dead: 0 x infinity would be NaN.
+  __device__ __forceinline__ Stage begin(int st) {
+    Stage s;
+    const int j0 = st * STAGE + wave_row;
+    int left = (int)this->rows - j0;
+    left = left < 0 ? 0 : (left < 8 ? left : 8);
+    const uint32_t past = 0xffu << left;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const uint32_t dead = (past << (31 - u)) & ROW_DEAD, off = offsets[j0 + u];
+      s.row[u] = off | dead;
+      seen |= dead ? 0u : off;
+    }
+    return s;
+  }
+  __device__ __forceinline__ void load(const Stage& s, int i, uint32_t buffer) const {
+    const int sub = (threadIdx.x & 63) / LP;
+    uint32_t row = s.row[RPC * i];
+#pragma unroll
+    for (int u = 1; u < RPC; ++u) row = sub == u ? s.row[RPC * i + u] : row;
+    lds_load16(all, row + this->own[i], this->at + buffer + i * 1024);
+  }
+};
+
+// acc = A B^T over `len` > 0 of the contraction.  Each accumulator has results' columns (B's rows) in
+// its registers and their rows (A's) over the lanes.
+template <int DT, int T, class A, class B>
+__device__ __forceinline__ void tile_loop(A& a, B& b, const char* lds, int len,
+                                          f32x16v (&acc)[T / 64][T / 64]) {
+  constexpr int NA = T / 64, BYTES = T * 64;  // of an operand's stage
+  constexpr int LOADS = 2 * NA;               // of a wave a stage
+  const int nst = (len + STAGE - 1) / STAGE;
+#pragma unroll
+  for (int i = 0; i < NA; ++i)
+#pragma unroll
+    for (int j = 0; j < NA; ++j)
+#pragma unroll
+      for (int u = 0; u < 16; ++u) acc[i][j][u] = 0.0f;
+  const char* la = lds;
+  const char* lb = lds + RING * BYTES;
+#pragma unroll 1
+  for (int p = 0; p < RING; ++p) {
+    const auto sa = a.begin(p);
+    const auto sb = b.begin(p);
+#pragma unroll
+    for (int i = 0; i < NA; ++i) {
+      a.load(sa, i, p * BYTES);
+      b.load(sb, i, p * BYTES);
+    }
+  }
+  __builtin_amdgcn_s_waitcnt(wait_for(3 * LOADS, 15));  // stage 0 landed
+  meet();
+  s16x8 a0[NA], b0[NA], a1[NA], b1[NA];
+  a.read(a0, la, 0);
+  b.read(b0, lb, 0);
+  int st = 0;
+  do {
+    const uint32_t cur = (uint32_t)(st % RING) * BYTES, nxt = (uint32_t)((st + 1) % RING) * BYTES;
+    a.read(a1, la + cur, 1);
+    b.read(b1, lb + cur, 1);
+    const auto sa = a.begin(st + RING);
+    const auto sb = b.begin(st + RING);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < NA; ++i)
+#pragma unroll
+      for (int j = 0; j < NA; ++j) acc[i][j] = product<DT>(b0[j], a0[i], acc[i][j]);
+    __builtin_amdgcn_sched_barrier(0);
+    // this wave has read stage st, and stage st + 1 has landed; behind the barrier nobody reads
+    // stage st any more
+    __builtin_amdgcn_s_waitcnt(wait_for(2 * LOADS, 0));
+    meet();
+    a.read(a0, la + nxt, 0);
+    b.read(b0, lb + nxt, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    // stage st + 4 takes its place, a load behind every few products (what lies past the end
+    // reads as zeros, so that every stage has the same number of loads)
+#pragma unroll
+    for (int i = 0; i < NA; ++i)
+#pragma unroll
+      for (int j = 0; j < NA; ++j) {
+        acc[i][j] = product<DT>(b1[j], a1[i], acc[i][j]);
+        const int m = i * NA + j;
+        if ((m + 1) % (NA / 2) == 0 && (m + 1) / (NA / 2) <= LOADS) {
+          const int l = (m + 1) / (NA / 2) - 1;
+          if (l & 1)
+            b.load(sb, l >> 1, cur);
+          else
+            a.load(sa, l >> 1, cur);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    __builtin_amdgcn_sched_barrier(0);
+  } while (++st < nst);
+  __builtin_amdgcn_s_waitcnt(wait_for(0, 0));
+}
+
+// The tile through LDS to rows of `out`, 16 bytes a lane where the rows allow it.  NAN_BY: rows
+// whose flag in `bad` is set become NaN (1), or all of them by the first flag (2).
+template <int DT, int T, int NAN_BY>
+__device__ __forceinline__ void store_tile(char* lds, f32x16v (&acc)[T / 64][T / 64],
+                                           uint16_t* out, int64_t cols, int rows, int width,
+                                           const uint8_t* bad) {
+  constexpr int NA = T / 64, PITCH = 2 * T + 16;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int wr = wave >> 1, wc = wave & 1;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < NA; ++i)
+#pragma unroll
+    for (int j = 0; j < NA; ++j) {
+      // (held where the matrix units write until its turn: all at once they would not fit)
+      if constexpr (T == 256) asm volatile("" : "+a"(acc[i][j]));
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        uint32_t w[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const float x = acc[i][j][4 * q + 2 * u], y = acc[i][j][4 * q + 2 * u + 1];
+          w[u] = DT == 1 ? (uint32_t)f16_bits(x) | (uint32_t)f16_bits(y) << 16
+                         : (uint32_t)bf16_bits(x) | (uint32_t)bf16_bits(y) << 16;
+        }
+        const int r = wr * (T / 2) + 32 * i + (lane & 31);
+        const int c = wc * (T / 2) + 32 * j + 8 * q + 4 * (lane >> 5);
+        *reinterpret_cast<uint2*>(lds + r * PITCH + 2 * c) = make_uint2(w[0], w[1]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  __syncthreads();
+  constexpr int LP = T / 8;
+  const uint32_t nan = DT == 1 ? 0x7e007e00u : 0x7fc07fc0u;
+  const bool wide = cols % 8 == 0 && ((uintptr_t)out & 15) == 0;
+  const int c = 8 * (tid % LP);
+  if (c >= width) return;
+#pragma unroll 4
+  for (int r = tid / LP; r < rows; r += 256 / LP) {
+    u32x4 v = *reinterpret_cast<const u32x4*>(lds + r * PITCH + 2 * c);
+    if (NAN_BY && bad[NAN_BY == 2 ? 0 : r]) v = u32x4{nan, nan, nan, nan};
+    uint16_t* to = out + r * cols + c;
+    if (wide && c + 8 <= width) {
+      *reinterpret_cast<u32x4*>(to) = v;
+    } else {
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (c + u < width) to[u] = (uint16_t)(v[u / 2] >> (16 * (u & 1)));
+    }
+  }
+}
+
+// Zeros where there is nothing to sum.
+template <int T>
+__device__ __forceinline__ void store_zeros(uint16_t* out, int64_t cols, int rows, int width) {
+  constexpr int TX = T < 256 ? T : 256;
+  const int c = threadIdx.x % TX;
+  if (c >= width) return;
+  for (int r = threadIdx.x / TX; r < rows; r += 256 / TX) out[r * cols + c] = 0;
+}
+
+template <int T>
+constexpr int LDS_BYTES = 2 * RING * T * 64 > T * (2 * T + 16) ? 2 * RING * T * 64
+                                                               : T * (2 * T + 16);
+
+// Tiles of rows of slots: workgroups go to the eight XCDs in turn, so an XCD takes all tiles of
+// four neighbouring row tiles one after the other, and rows and weights come to its L2 once.
+template <int DT, int WHAT, int T, bool INDEXED>
+__global__ __launch_bounds__(256, T == 256 ? 1 : 2) void grouped_tile_kernel(GroupedArgs g,
+                                                                              uint32_t nx,
+                                                                              uint32_t ny) {
+  constexpr int NA = T / 64, BYTES = T * 64;
+  __shared__ __attribute__((aligned(1024))) char lds[LDS_BYTES<T>];
+  __shared__ uint8_t bad[T];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wr = wv >> 1, wc = wv & 1;
+  const uint32_t base = __builtin_amdgcn_readfirstlane(
+      (uint32_t)(size_t)(__attribute__((address_space(3))) char*)lds);
+  const int n = (int)g.n, k = (int)g.k;
+  f32x16v acc[NA][NA];
+  uint16_t* const out = static_cast<uint16_t*>(g.out);
+  if constexpr (WHAT == GROUPED_GRAD_W) {
+    // An expert's tiles over all XCDs, 2 x 4 of them at a time, one to each.
+    const uint32_t xcd = blockIdx.x & 7, j = blockIdx.x >> 3;
+    const uint32_t hx = nx / 4, per = hx * (ny / 2);  // (nx, ny: rounded up to whole rounds)
+    const int e = (int)(j / per);
+    const uint32_t sub = j - e * per, my = (xcd + e) & 7;
+    const int64_t r0 = (int64_t)((sub / hx) * 2 + (my >> 2)) * T;
+    const int64_t c0 = (int64_t)((sub % hx) * 4 + (my & 3)) * T;
+    if (r0 >= n || c0 >= k) return;
+    int64_t first, end;
+    slot_range(g, e, first, end);
+    first = uniform(first);
+    end = uniform(end);
+    const int rows = (int)(n - r0 < T ? n - r0 : T), cols = (int)(k - c0 < T ? k - c0 : T);
+    uint16_t* const to = out + ((int64_t)e * n + r0) * k + c0;
+    if (first == end) {
+      store_zeros<T>(to, k, rows, cols);
+      return;
+    }
+    AcrossOperand<T> a;
+    a.base = static_cast<const char*>(g.dy) + (first * g.ldy + r0) * 2;
+    a.pitch = g.ldy * 2;
+    a.rows = end - first;
+    a.init(base, wv, wr, rows);
+    if constexpr (INDEXED) {
+      if (tid == 0) bad[0] = 0;  // (behind the loop's barriers)
+      IndexedOperand<T> b;
+      b.offsets = (const __attribute__((address_space(4))) uint32_t*)(g.offsets + first);
+      b.rows = end - first;
+      b.all = rsrc(static_cast<const char*>(g.x) + c0 * 2,
+                   g.x_rows > 0 ? ((g.x_rows - 1) * g.ldx + cols) * 2 : 0);
+      b.init(base + RING * BYTES, wv, wc, cols);
+      tile_loop<DT, T>(a, b, lds, (int)(end - first), acc);
+      if (b.seen & 1) bad[0] = 1;
+    } else {
+      AcrossOperand<T> b;
+      b.base = static_cast<const char*>(g.x) + (first * g.ldx + c0) * 2;
+      b.pitch = g.ldx * 2;
+      b.rows = end - first;
+      b.init(base + RING * BYTES, wv, wc, cols);
+      tile_loop<DT, T>(a, b, lds, (int)(end - first), acc);
+    }
+    store_tile<DT, T, INDEXED ? 2 : 0>(lds, acc, to, k, rows, cols, bad);
+  } else {
+    const uint32_t xcd = blockIdx.x & 7, j = blockIdx.x >> 3, r = j / nx, xt = j - r * nx;
+    const GroupedWork w = find_rows(g, T, ((int64_t)(r >> 2) * 8 + xcd) * 4 + (r & 3));
+    const int e = __builtin_amdgcn_readfirstlane(w.e);
+    if (e == WORK_NONE) return;
+    const int64_t first = uniform(w.first), left = uniform(w.end) - first;
+    const int live = (int)(left < T ? left : T);
+    const int64_t width = WHAT == GROUPED_LINEAR ? n : k, c0 = (int64_t)xt * T;
+    const int cols = (int)(width - c0 < T ? width - c0 : T);
+    uint16_t* const to = out + first * width + c0;
+    if (e < 0) {
+      store_zeros<T>(to, width, live, cols);
+      return;
+    }
+    AlongOperand<T> a;
+    if constexpr (WHAT == GROUPED_LINEAR) {
+      a.init(base, wv, wr, k);
+      if constexpr (INDEXED) {
+        a.rs = rsrc(g.x, g.x_rows > 0 ? ((g.x_rows - 1) * g.ldx + k) * 2 : 0);
+#pragma unroll
+        for (int i = 0; i < NA; ++i) {
+          const int t = a.row_of(wv, i);
+          int64_t s = t < live ? g.rows[first + t] : 0;
+          const bool in = s >= 0 && s < g.x_rows;
+          if ((lane & 3) == 0) bad[t] = t < live && !in;
+          a.row[i] = t < live && in ? (uint32_t)(s * g.ldx * 2) : ROW_DEAD;
+        }
+      } else {
+        a.rs = rsrc(static_cast<const char*>(g.x) + first * g.ldx * 2,
+                    ((int64_t)(live - 1) * g.ldx + k) * 2);
+#pragma unroll
+        for (int i = 0; i < NA; ++i) {
+          const int t = a.row_of(wv, i);
+          a.row[i] = t < live ? (uint32_t)(t * g.ldx * 2) : ROW_DEAD;
+        }
+      }
+      AlongOperand<T> b;
+      b.init(base + RING * BYTES, wv, wc, k);
+      b.rs = rsrc(static_cast<const char*>(g.w) + ((int64_t)e * n + c0) * k * 2,
+                  (int64_t)cols * k * 2);
+#pragma unroll
+      for (int i = 0; i < NA; ++i) {
+        const int t = b.row_of(wv, i);
+        b.row[i] = t < cols ? (uint32_t)t * (uint32_t)(k * 2) : ROW_DEAD;
+      }
+      tile_loop<DT, T>(a, b, lds, k, acc);
+    } else {
+      a.init(base, wv, wr, n);
+      a.rs = rsrc(static_cast<const char*>(g.dy) + first * g.ldy * 2,
+                  ((int64_t)(live - 1) * g.ldy + n) * 2);
+#pragma unroll
+      for (int i = 0; i < NA; ++i) {
+        const int t = a.row_of(wv, i);
+        a.row[i] = t < live ? (uint32_t)(t * g.ldy * 2) : ROW_DEAD;
+      }
+      AcrossOperand<T> b;
+      b.base = static_cast<const char*>(g.w) + ((int64_t)e * n * k + c0) * 2;
+      b.pitch = (int64_t)k * 2;
+      b.rows = n;
+      b.init(base + RING * BYTES, wv, wc, cols);
+      tile_loop<DT, T>(a, b, lds, n, acc);
+    }
+    store_tile<DT, T, INDEXED ? 1 : 0>(lds, acc, to, width, live, cols, bad);
+  }
+}
+
+// Offsets of the slots' rows in x.
+__global__ __launch_bounds__(256) void indexed_rows_kernel(const int64_t* rows, int64_t slots,
+                                                           int64_t x_rows, uint32_t pitch,
+                                                           uint32_t* offsets) {
+  const int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (j >= slots) return;
+  const uint64_t r = (uint64_t)rows[j];
+  offsets[j] = r < (uint64_t)x_rows ? (uint32_t)r * pitch : ROW_DEAD | 1;
+}
+
+template <int DT, int WHAT, int T, bool INDEXED>
+int launch_tile(const GroupedArgs& g, hipStream_t s, const char* what) {
+  const int64_t cols = WHAT == GROUPED_LINEAR ? g.n : g.k;
+  int64_t nx = (cols + T - 1) / T, ny, count;
+  if constexpr (WHAT == GROUPED_GRAD_W) {
+    nx = (nx + 3) / 4 * 4;
+    ny = ((g.n + T - 1) / T + 1) / 2 * 2;
+    count = nx * ny * g.experts;
+    if (INDEXED && g.slots)
+      indexed_rows_kernel<<<(unsigned)((g.slots + 255) / 256), 256, 0, s>>>(
+          g.rows, g.slots, g.x_rows, (uint32_t)(g.ldx * 2), g.offsets);
+  } else {
+    ny = (g.slots / T + g.experts + 2 + 31) / 32 * 32;
+    count = nx * ny;
+  }
+  HI2X_REQUIRE(count < (1ll << 31), "%s: too many results", what);
+  grouped_tile_kernel<DT, WHAT, T, INDEXED>
+      <<<(unsigned)count, 256, 0, s>>>(g, (uint32_t)nx, (uint32_t)ny);
+  return launch_status(what);
+}
+
+template <int DT, int WHAT, int T>
+int launch_indexed(const GroupedArgs& g, hipStream_t s, const char* what) {
+  if constexpr (WHAT != GROUPED_GRAD_X) {
+    if (g.rows) return launch_tile<DT, WHAT, T, true>(g, s, what);
+  }
+  return launch_tile<DT, WHAT, T, false>(g, s, what);
+}
+
+template <int DT, int WHAT>
+int launch_size(const GroupedArgs& g, hipStream_t s, const char* what) {
+  const int64_t rows = WHAT == GROUPED_GRAD_W ? g.experts * ((g.n + 255) / 256)
+                                              : g.slots / 256 + g.experts / 2;
+  const int64_t cols = ((WHAT == GROUPED_LINEAR ? g.n : g.k) + 255) / 256;
+  if (rows * cols >= 192) return launch_indexed<DT, WHAT, 256>(g, s, what);
+  return launch_indexed<DT, WHAT, 128>(g, s, what);
+}
+
+}  // namespace
+
+int grouped_tiles(const GroupedArgs& g, int what, int dtype, hipStream_t s, const char* name) {
+#define HI2X_GROUPED(WHAT) \
+  return dtype == 1 ? launch_size<1, WHAT>(g, s, name) : launch_size<2, WHAT>(g, s, name)
+  if (what == GROUPED_LINEAR) HI2X_GROUPED(GROUPED_LINEAR);
+  if (what == GROUPED_GRAD_X) HI2X_GROUPED(GROUPED_GRAD_X);
+  HI2X_GROUPED(GROUPED_GRAD_W);
+#undef HI2X_GROUPED
+}
+
+}  // namespace hi2x
