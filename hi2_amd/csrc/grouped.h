@@ -11,8 +11,8 @@ struct GroupedArgs {
   void* out;
   const int64_t *rows, *offs;
   int64_t ldx, ldy, x_rows, slots;
+  int64_t ldw;  // of w's rows; an expert's are n of them
   int64_t experts, n, k;
-  uint32_t* offsets;  // of the slots' rows in x, for grad_w in tiles
 };
 
 // Expert e's slots, empty where the ranges are not as they should be.
@@ -23,63 +23,54 @@ __device__ __forceinline__ void slot_range(const GroupedArgs& g, int e, int64_t&
   b = b < a ? a : (b > g.slots ? g.slots : b);
 }
 
-// A tile's rows: those of expert e from `first` up to its range's end, of no expert (zeros), or
-// none.
-constexpr int WORK_ZEROS = -1, WORK_NONE = -2;
-struct GroupedWork {
-  int e;
-  int64_t first, end;
+// A row tile: slots [first, first + live) of expert e, or of none (e < 0: zeros).
+struct RowTile {
+  int64_t first;
+  int32_t live, e;
+};
+struct Plan {
+  int64_t count;
+  int64_t reserved;
+  RowTile tile[1];
 };
 
-// The want-th tile of `tile` rows, expert after expert; then those of the slots behind the last
-// range and before the first.  Called by all lanes of a wave together.
-__device__ __forceinline__ GroupedWork find_rows(const GroupedArgs& g, int tile, int64_t want) {
-  GroupedWork w{WORK_NONE, 0, 0};
-  const int lane = threadIdx.x & 63;
-  const int experts = (int)g.experts;
-  int64_t before = 0;
-  for (int e0 = 0; e0 < experts + 2; e0 += 64) {
-    const int e = e0 + lane;
-    int64_t a = 0, b = 0;
-    if (e < experts) {
-      slot_range(g, e, a, b);
-    } else if (e == experts) {
-      a = g.offs[experts];
-      a = a < 0 ? 0 : (a > g.slots ? g.slots : a);
-      b = g.slots;
-    } else if (e == experts + 1) {
-      b = g.offs[0];
-      b = b < 0 ? 0 : (b > g.slots ? g.slots : b);
-    }
-    const int n = (int)((b - a + tile - 1) / tile);
-    int inc = n;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int o = __shfl_up(inc, d);
-      if (lane >= d) inc += o;
-    }
-    const int64_t upto = before + inc;
-    const unsigned long long hit = __ballot(want < upto && want >= upto - n);
-    if (hit) {
-      const int l = __builtin_ctzll(hit);
-      const int64_t base = before + __shfl(inc, l) - __shfl(n, l);
-      w.e = e0 + l < experts ? e0 + l : WORK_ZEROS;
-      w.first = __shfl(a, l) + (want - base) * tile;
-      w.end = __shfl(b, l);
-      return w;
-    }
-    before += __shfl(inc, 63);
-  }
-  return w;
+// Row tiles of T slots at most: every range's last may be partial.
+inline int64_t most_tiles(const GroupedArgs& g, int T) { return g.slots / T + g.experts + 2; }
+inline int64_t plan_bytes(const GroupedArgs& g, int T) {
+  return align256(sizeof(Plan) + most_tiles(g, T) * sizeof(RowTile));
+}
+
+// The row tiles of T slots, expert after expert, then those of the slots behind the last range and
+// before the first.
+int launch_plan(const GroupedArgs& g, int T, Plan* plan, hipStream_t s, const char* name);
+
+// The tile of a plan's row tiles x nx columns that workgroup `block` of 8 ceil(tiles / 8) takes.
+// Workgroups go to the eight XCDs in turn, and each XCD takes an eighth of the tiles, which are in
+// order of four row tiles at a time, column tile after column tile, so that rows and weights come to
+// its L2 once.
+__device__ __forceinline__ bool plan_tile(const Plan* p, uint32_t nx, uint32_t block, RowTile& w,
+                                          uint32_t& xt) {
+  const uint32_t count = (uint32_t)p->count, all = count * nx, per = (all + 7) / 8;
+  const uint32_t j = block >> 3, at = (block & 7) * per + j;
+  if (j >= per || at >= all) return false;
+  // (what comes out of a division is in a vector register, and would keep what follows there)
+  const uint32_t band = __builtin_amdgcn_readfirstlane(at / (4 * nx));
+  const uint32_t rest = at - band * (4 * nx);
+  const uint32_t deep = count - 4 * band < 4 ? count - 4 * band : 4;
+  xt = __builtin_amdgcn_readfirstlane(rest / deep);
+  w = p->tile[4 * band + rest - xt * deep];
+  return true;
 }
 
 // What a resource that offsets of 32 bits reach may span: an offset past it by this much again is
 // past it still.
 constexpr uint32_t GROUPED_SPAN = 0x7f000000u;
 
-// The product in tiles (16 bits; rows and weights at multiples of 16 bytes, n and k of 8).
-// grad_w with rows: g.offsets, room for grouped_offsets(slots) of them.
-constexpr int64_t grouped_offsets(int64_t slots) { return slots + 256; }
-int grouped_tiles(const GroupedArgs& g, int what, int dtype, hipStream_t s, const char* name);
+// The product in tiles of 16-bit operands that lie so, or of float32 ones with x within reach, and
+// the workspace that it takes for its plan.
+int64_t grouped_plan_bytes(const GroupedArgs& g, int what, int dtype);
+int grouped_tiles(const GroupedArgs& g, int what, int dtype, char* plan, hipStream_t s,
+                  const char* name);
+int grouped_f32(const GroupedArgs& g, int what, char* plan, hipStream_t s, const char* name);
 
 }  // namespace hi2x

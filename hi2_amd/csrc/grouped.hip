@@ -1,157 +1,182 @@
 // Products grouped by expert with ragged sizes, and their gradients: out = x[rows] w^T over the
-// routed slots, dx = dy w and dw = dy^T x[rows].
+// routed slots, dx = dy w and dw = dy^T x[rows].  This file: the entries, and what surrounds the
+// products (grouped_tile.hip, grouped_f32.hip).
 #include "grouped.h"
-
-#include "mfma_gemm.h"
 
 namespace hi2x {
 namespace {
 
-// ---- any type, any alignment: float32 MFMA ----------------------------------------------------
-// A workgroup's tile of 64 x 64 results, 32 of the contraction at a time through LDS, where
-// values are float32 (16-bit ones exactly); the sum of each result is a chain of FMAs.
-constexpr int FT = 64;
+int64_t size_of(int dtype) { return dtype == 0 ? 4 : 2; }
 
-template <int DT, bool ALONG>
-struct TileLoader {
-  float v[8];
-  // Element (i, c) of the operand: ALONG, neighbours in c are neighbours in memory, else in i.
-  template <class At>
-  __device__ __forceinline__ void load(At at) {
-    const int tid = threadIdx.x;
-#pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const int i = ALONG ? (tid >> 5) + 8 * u : tid & 63;
-      const int c = ALONG ? tid & 31 : (tid >> 6) + 4 * u;
-      v[u] = at(i, c);
-    }
-  }
-  __device__ __forceinline__ void store(float (*S)[MG_RP]) const {
-    const int tid = threadIdx.x;
-#pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const int i = ALONG ? (tid >> 5) + 8 * u : tid & 63;
-      const int c = ALONG ? tid & 31 : (tid >> 6) + 4 * u;
-      S[i][(c & 1) * MG_KP + (c >> 1)] = v[u];
-    }
-  }
+// Threads over rows of `pieces`: 1 << shift along a row, 256 >> shift rows a workgroup.
+struct Spread {
+  uint32_t across;  // workgroups along a row
+  int shift;
 };
-
-template <int DT, int WHAT>
-__global__ __launch_bounds__(256) void grouped_any_kernel(GroupedArgs g, uint32_t nx) {
-  __shared__ __attribute__((aligned(16))) MgSmemT<FT> sm;
-  __shared__ int64_t src[2][FT];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const uint32_t work = blockIdx.x / nx, xt = blockIdx.x - work * nx;
-  int e;
-  int64_t first, end, r0, rows_out;
-  if constexpr (WHAT == GROUPED_GRAD_W) {
-    const uint32_t ny = (uint32_t)((g.n + FT - 1) / FT);
-    e = (int)(work / ny);
-    r0 = (int64_t)(work - e * ny) * FT;
-    rows_out = g.n;
-    slot_range(g, e, first, end);
-  } else {
-    const GroupedWork w = find_rows(g, FT, work);
-    if (w.e == WORK_NONE) return;
-    e = w.e;
-    r0 = first = w.first;
-    end = rows_out = w.end;
-  }
-  const int64_t c0 = (int64_t)xt * FT;
-  const int64_t cols = WHAT == GROUPED_LINEAR ? g.n : g.k;
-  const int64_t len = WHAT == GROUPED_LINEAR ? g.k : (WHAT == GROUPED_GRAD_X ? g.n : end - first);
-  f32x16 acc[1][1];
-  mg_zero(acc);
-  // row of x of slot first + i; -1: none, -2: outside
-  auto row_of = [&](int64_t slot) -> int64_t {
-    if (slot >= end) return -1;
-    if (!g.rows) return slot;
-    const int64_t r = g.rows[slot];
-    return r >= 0 && r < g.x_rows ? r : -2;
-  };
-  auto x_at = [&](int64_t r, int64_t c) -> float {
-    if (r < 0) return r == -1 ? 0.0f : __builtin_nanf("");
-    return c < g.k ? load_as_f32(g.x, r * g.ldx + c, DT) : 0.0f;
-  };
-  auto w_at = [&](int64_t n, int64_t k) -> float {
-    return n < g.n && k < g.k ? load_as_f32(g.w, ((int64_t)e * g.n + n) * g.k + k, DT) : 0.0f;
-  };
-  auto dy_at = [&](int64_t slot, int64_t n) -> float {
-    return slot < end && n < g.n ? load_as_f32(g.dy, slot * g.ldy + n, DT) : 0.0f;
-  };
-  const int nch = e < 0 ? 0 : (int)((len + MG_KC - 1) / MG_KC);
-  if (WHAT == GROUPED_LINEAR) {
-    if (tid < FT) src[0][tid] = row_of(first + tid);
-    __syncthreads();
-  }
-  for (int ch = 0; ch < nch; ++ch) {
-    const int64_t k0 = (int64_t)ch * MG_KC;
-    if (WHAT == GROUPED_GRAD_W) {
-      if (tid < MG_KC) src[ch & 1][tid] = row_of(first + k0 + tid);
-      __syncthreads();
-    }
-    TileLoader<DT, WHAT != GROUPED_GRAD_W> a;
-    TileLoader<DT, WHAT == GROUPED_LINEAR> b;
-    if constexpr (WHAT == GROUPED_LINEAR) {
-      a.load([&](int i, int c) { return x_at(src[0][i], k0 + c); });
-      b.load([&](int i, int c) { return w_at(c0 + i, k0 + c); });
-    } else if constexpr (WHAT == GROUPED_GRAD_X) {
-      a.load([&](int i, int c) { return dy_at(r0 + i, k0 + c); });
-      b.load([&](int i, int c) { return w_at(k0 + c, c0 + i); });
-    } else {
-      a.load([&](int i, int c) { return dy_at(first + k0 + c, r0 + i); });
-      b.load([&](int i, int c) { return x_at(src[ch & 1][c], c0 + i); });
-    }
-    __syncthreads();  // the chunk before has been read
-    a.store(sm.A[0]);
-    b.store(sm.B[0]);
-    __syncthreads();
-    mg_chunk<1>(acc, sm.A[0], sm.B[0], wave >> 1, wave & 1, lane >> 5, lane & 31);
-  }
-#pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    const int64_t r = r0 + mg_row<FT>(0, j), c = c0 + mg_col<FT>(0);
-    if (r < rows_out && c < cols)
-      store_from_f32(g.out, (WHAT == GROUPED_GRAD_W ? (int64_t)e * g.n + r : r) * cols + c, DT,
-                     acc[0][0][j]);
-  }
+int64_t spread(int64_t rows, int64_t pieces, Spread& g) {
+  g.shift = 8;
+  while (g.shift > 0 && (1ll << (g.shift - 1)) >= pieces) --g.shift;
+  g.across = (uint32_t)((pieces + (1ll << g.shift) - 1) >> g.shift);
+  return g.across * ((rows + (256 >> g.shift) - 1) / (256 >> g.shift));
+}
+__device__ __forceinline__ void spread_at(const Spread& g, int64_t& row, int64_t& piece) {
+  const uint32_t band = blockIdx.x / g.across, x = blockIdx.x - band * g.across;
+  row = (int64_t)band * (256 >> g.shift) + (threadIdx.x >> g.shift);
+  piece = ((int64_t)x << g.shift) + (threadIdx.x & ((1 << g.shift) - 1));
 }
 
-// dx[t] = the sum of its slots' rows, in their order; a wave (or more) on a token.
-template <int DT>
+// ---- a token's sum over its slots -------------------------------------------------------------
+// dx[t] = the rows of t's slots added in their order, 16 bytes of a row a thread (V values; 1 where
+// rows do not begin at multiples of 16), up to four rows on their way at a time.  A slot outside
+// gives NaN.  HBM bounds it: part is read once.
+template <int DT, int V>
 __global__ __launch_bounds__(256) void sum_slots_kernel(const void* part, int64_t slots, int64_t k,
                                                         const int64_t* slots_of, int64_t t,
-                                                        int top_k, void* out) {
-  const int64_t token = blockIdx.x;
+                                                        int top_k, Spread by, void* out) {
+  int64_t token, c;
+  spread_at(by, token, c);
+  c *= V;
+  if (token >= t || c >= k) return;
   const int64_t* of = slots_of + token * top_k;
-  for (int64_t c = threadIdx.x; c < k; c += 256) {
-    float acc = 0.0f;
-    for (int j = 0; j < top_k; ++j) {
-      const int64_t s = of[j];
-      acc += s >= 0 && s < slots ? load_as_f32(part, s * k + c, DT) : __builtin_nanf("");
+  float acc[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) acc[i] = 0.0f;
+  constexpr int UN = 4;
+  for (int j0 = 0; j0 < top_k; j0 += UN) {
+    int64_t s[UN];
+    u32x4 w[UN];
+#pragma unroll
+    for (int u = 0; u < UN; ++u) s[u] = of[j0 + u < top_k ? j0 + u : top_k - 1];
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      const int64_t r = (uint64_t)s[u] < (uint64_t)slots ? s[u] : 0;
+      if constexpr (V == 1)
+        w[u][0] = DT == 0 ? static_cast<const uint32_t*>(part)[r * k + c]
+                          : (uint32_t)static_cast<const uint16_t*>(part)[r * k + c];
+      else
+        w[u] = *reinterpret_cast<const u32x4*>(static_cast<const char*>(part) +
+                                               (r * k + c) * (DT == 0 ? 4 : 2));
     }
-    store_from_f32(out, token * k + c, DT, acc);
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      if (j0 + u >= top_k) break;
+      const bool in = (uint64_t)s[u] < (uint64_t)slots;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const uint32_t h = DT == 0 ? w[u][i] : w[u][i / 2] >> (16 * (i & 1));
+        const float x = DT == 0 ? __uint_as_float(h)
+                                : (DT == 1 ? f16_from_bits((uint16_t)h)
+                                           : __uint_as_float(h << 16));
+        acc[i] += in ? x : __builtin_nanf("");
+      }
+    }
   }
+#pragma unroll
+  for (int i = 0; i < V; ++i) store_from_f32(out, token * k + c + i, DT, acc[i]);
 }
 
-template <int WHAT>
-int launch_any(const GroupedArgs& g, int dtype, hipStream_t s, const char* what) {
-  const int64_t cols = WHAT == GROUPED_LINEAR ? g.n : g.k;
-  const int64_t nx = (cols + FT - 1) / FT;
-  const int64_t ny = WHAT == GROUPED_GRAD_W ? g.experts * ((g.n + FT - 1) / FT)
-                                            : g.slots / FT + g.experts + 2;
-  HI2X_REQUIRE(nx < (1ll << 31) && ny < (1ll << 31) && nx * ny < (1ll << 31),
-               "%s: too many results", what);
-  const unsigned grid = (unsigned)(nx * ny);
-  if (dtype == 0)
-    grouped_any_kernel<0, WHAT><<<grid, 256, 0, s>>>(g, (uint32_t)nx);
-  else if (dtype == 1)
-    grouped_any_kernel<1, WHAT><<<grid, 256, 0, s>>>(g, (uint32_t)nx);
+template <int DT>
+int sum_slots(const void* part, int64_t slots, int64_t k, const int64_t* slots_of, int64_t t,
+              int64_t top_k, void* out, hipStream_t s) {
+  constexpr int WIDE = DT == 0 ? 4 : 8;
+  const bool wide = k % WIDE == 0 && ((uintptr_t)out & 15) == 0;
+  Spread by;
+  const int64_t count = spread(t, wide ? k / WIDE : k, by);
+  HI2X_REQUIRE(count < (1ll << 31), "grouped_grad_x: too many results");
+  if (wide)
+    sum_slots_kernel<DT, WIDE><<<(unsigned)count, 256, 0, s>>>(part, slots, k, slots_of, t,
+                                                              (int)top_k, by, out);
   else
-    grouped_any_kernel<2, WHAT><<<grid, 256, 0, s>>>(g, (uint32_t)nx);
+    sum_slots_kernel<DT, 1><<<(unsigned)count, 256, 0, s>>>(part, slots, k, slots_of, t,
+                                                           (int)top_k, by, out);
+  return launch_status("grouped_grad_x");
+}
+
+// ---- operands that do not lie as the tiles take them -------------------------------------------
+// Rows of `cols` 16-bit or 32-bit values copied to rows at multiples of 16 bytes, zeros behind them;
+// with `index` the rows that it names (one outside: NaN).  A thread writes 16 bytes.
+template <class W>
+__global__ __launch_bounds__(256) void copy_rows_kernel(const W* from, int64_t ld, int64_t rows,
+                                                        int64_t cols, const int64_t* index,
+                                                        int64_t from_rows, W nan, W* to,
+                                                        int64_t ld_to, Spread by) {
+  constexpr int V = 16 / sizeof(W);
+  int64_t row, c;
+  spread_at(by, row, c);
+  c *= V;
+  if (row >= rows || c >= ld_to) return;
+  const int64_t r = index ? index[row] : row;
+  const bool in = (uint64_t)r < (uint64_t)from_rows;
+  union {
+    W v[V];
+    u32x4 w;
+  };
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    v[i] = c + i < cols ? (in ? from[r * ld + c + i] : nan) : (W)0;
+  *reinterpret_cast<u32x4*>(to + row * ld_to + c) = w;
+}
+
+int copy_rows(const void* from, int64_t ld, int64_t rows, int64_t cols, const int64_t* index,
+              int64_t from_rows, int dtype, void* to, int64_t ld_to, hipStream_t s,
+              const char* what) {
+  Spread by;
+  const int64_t count = spread(rows, ld_to / (dtype == 0 ? 4 : 8), by);
+  HI2X_REQUIRE(count < (1ll << 31), "%s: too many elements", what);
+  if (count == 0) return HI2X_OK;
+  if (dtype == 0)
+    copy_rows_kernel<uint32_t><<<(unsigned)count, 256, 0, s>>>(
+        static_cast<const uint32_t*>(from), ld, rows, cols, index, from_rows, 0x7fc00000u,
+        static_cast<uint32_t*>(to), ld_to, by);
+  else
+    copy_rows_kernel<uint16_t><<<(unsigned)count, 256, 0, s>>>(
+        static_cast<const uint16_t*>(from), ld, rows, cols, index, from_rows,
+        (uint16_t)(dtype == 1 ? 0x7e00 : 0x7fc0), static_cast<uint16_t*>(to), ld_to, by);
   return launch_status(what);
 }
+
+// ---- a product's workspace ----------------------------------------------------------------------
+struct Space {
+  int64_t part = 0, x = 0, dy = 0, w = 0, plan = 0, bytes = 0;
+  bool has_part = false, has_x = false, has_dy = false, has_w = false;
+  bool gather = false;  // the copy of x is in the slots' order
+  int64_t ldx = 0, ldy = 0, ldw = 0;
+};
+
+int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
+
+// Which operands are copied, and where in the workspace what lies.  16-bit rows begin at multiples
+// of 16 bytes, and those that run along the contraction end there (or in zeros).  Of x the rows are
+// copied, or where these are beyond the reach of an index's offsets the slots'.
+Space lay_out(const GroupedArgs& g, int what, int dtype, bool summed, bool x_fits, bool dy_fits,
+              bool w_fits) {
+  Space m;
+  auto take = [&](int64_t n) {
+    const int64_t a = m.bytes;
+    m.bytes += align256(n);
+    return a;
+  };
+  const int64_t size = size_of(dtype);
+  GroupedArgs p = g;
+  if (summed) m.has_part = true, m.part = take(g.slots * g.k * size);
+  if (what != GROUPED_GRAD_X) {
+    const bool copied = dtype != 0 && (!x_fits || (what == GROUPED_LINEAR && g.k % 8));
+    m.ldx = copied ? pad8(g.k) : g.ldx;
+    m.gather = g.rows && g.x_rows * m.ldx * size > (int64_t)GROUPED_SPAN;
+    if (m.gather) m.ldx = pad8(g.k), p.rows = nullptr;
+    m.has_x = copied || m.gather;
+    if (m.has_x) m.x = take((m.gather ? g.slots : g.x_rows) * m.ldx * size);
+  }
+  if (what != GROUPED_LINEAR && dtype != 0 &&
+      (!dy_fits || (what == GROUPED_GRAD_X && g.n % 8)))
+    m.has_dy = true, m.ldy = pad8(g.n), m.dy = take(g.slots * m.ldy * size);
+  if (what != GROUPED_GRAD_W && dtype != 0 && !w_fits)
+    m.has_w = true, m.ldw = pad8(g.k), m.w = take(g.experts * g.n * m.ldw * size);
+  m.plan = take(grouped_plan_bytes(p, what, dtype));
+  return m;
+}
+
+bool lies_well(const void* p, int64_t ld) { return ((uintptr_t)p & 15) == 0 && ld % 8 == 0; }
 
 int check_grouped(const GroupedArgs& g, int dtype, const char* what) {
   HI2X_REQUIRE(dtype >= 0 && dtype <= 2, "%s: dtype %d", what, dtype);
@@ -161,28 +186,48 @@ int check_grouped(const GroupedArgs& g, int dtype, const char* what) {
                "%s: weights of %lld x %lld", what, (long long)g.n, (long long)g.k);
   HI2X_REQUIRE(g.slots >= 0 && g.slots < (1ll << 31) && g.x_rows >= 0 && g.x_rows < (1ll << 31),
                "%s: bad rows", what);
+  HI2X_REQUIRE((g.x_rows <= 1 || g.ldx < (1 << 21)) && (g.slots <= 1 || g.ldy < (1 << 21)),
+               "%s: rows more than 2^21 elements apart", what);
   return HI2X_OK;
 }
 
-int64_t size_of(int dtype) { return dtype == 0 ? 4 : 2; }
-
-// Whether the product goes in tiles of 16-bit values: pieces of 16 bytes are whole.
-bool in_tiles(const GroupedArgs& g, int what, int dtype) {
-  auto whole = [](const void* p, int64_t ld) { return ((uintptr_t)p & 15) == 0 && ld % 8 == 0; };
-  if (dtype == 0 || g.n % 8 || g.k % 8) return false;
-  if (what != GROUPED_GRAD_W && !whole(g.w, g.k)) return false;
-  if (what != GROUPED_LINEAR && (!whole(g.dy, g.ldy) || g.ldy >= (1 << 21))) return false;
-  if (what != GROUPED_GRAD_X &&
-      (!whole(g.x, g.ldx) || g.ldx >= (1 << 21) ||
-       (g.rows && g.x_rows * g.ldx * 2 > (int64_t)GROUPED_SPAN)))
-    return false;
-  return true;
-}
-
-template <int WHAT>
-int launch_product(const GroupedArgs& g, int dtype, hipStream_t s, const char* what) {
-  return in_tiles(g, WHAT, dtype) ? grouped_tiles(g, WHAT, dtype, s, what)
-                                  : launch_any<WHAT>(g, dtype, s, what);
+// The product, its operands copied first where they do not lie as it takes them.
+int run(GroupedArgs g, int what, int dtype, bool summed, void* ws, int64_t ws_bytes, Workspace& w,
+        void** part, hipStream_t s, const char* name) {
+  // workgroups of the smallest tiles, whole rounds of them
+  const int T = dtype ? 128 : 64;
+  const int64_t nx = ((what == GROUPED_LINEAR ? g.n : g.k) + T - 1) / T + 3;
+  const int64_t ny = what == GROUPED_GRAD_W ? g.experts * ((g.n + T - 1) / T + 1)
+                                            : most_tiles(g, T) + 8;
+  HI2X_REQUIRE(nx * ny < (1ll << 31), "%s: too many results", name);
+  const Space m = lay_out(g, what, dtype, summed, lies_well(g.x, g.ldx), lies_well(g.dy, g.ldy),
+                          lies_well(g.w, g.ldw));
+  if (int rc = take_workspace(w, ws, ws_bytes, (size_t)m.bytes, s, name)) return rc;
+  if (summed) g.out = *part = w.p + m.part;
+  if (m.has_x) {
+    if (int rc = copy_rows(g.x, g.ldx, m.gather ? g.slots : g.x_rows, g.k,
+                           m.gather ? g.rows : nullptr, g.x_rows, dtype, w.p + m.x, m.ldx, s, name))
+      return rc;
+    g.x = w.p + m.x;
+    g.ldx = m.ldx;
+    if (m.gather) g.rows = nullptr, g.x_rows = g.slots;
+  }
+  if (m.has_dy) {
+    if (int rc = copy_rows(g.dy, g.ldy, g.slots, g.n, nullptr, g.slots, dtype, w.p + m.dy, m.ldy,
+                           s, name))
+      return rc;
+    g.dy = w.p + m.dy;
+    g.ldy = m.ldy;
+  }
+  if (m.has_w) {
+    if (int rc = copy_rows(g.w, g.ldw, g.experts * g.n, g.k, nullptr, g.experts * g.n, dtype,
+                           w.p + m.w, m.ldw, s, name))
+      return rc;
+    g.w = w.p + m.w;
+    g.ldw = m.ldw;
+  }
+  return dtype == 0 ? grouped_f32(g, what, w.p + m.plan, s, name)
+                    : grouped_tiles(g, what, dtype, w.p + m.plan, s, name);
 }
 
 }  // namespace
@@ -190,17 +235,19 @@ int launch_product(const GroupedArgs& g, int dtype, hipStream_t s, const char* w
 
 using namespace hi2x;
 
-extern "C" int64_t hi2x_grouped_workspace_bytes(int what, int dtype, int64_t tokens,
+extern "C" int64_t hi2x_grouped_workspace_bytes(int what, int dtype, int64_t tokens, int64_t ldx,
                                                 int64_t experts, int64_t n, int64_t k,
                                                 int64_t slots, int indexed, int first_aligned,
                                                 int second_aligned) {
   GroupedArgs g{};
-  g.experts = experts, g.n = n, g.k = k, g.slots = slots, g.x_rows = tokens;
+  g.experts = experts, g.n = n, g.k = k, g.slots = slots, g.x_rows = tokens, g.ldx = ldx;
   if (what < 0 || what > 2 || check_grouped(g, dtype, "grouped_workspace_bytes")) return -1;
-  if (what == GROUPED_GRAD_X && indexed) return align256(slots * k * size_of(dtype));
-  if (what == GROUPED_GRAD_W && indexed && dtype) return align256(grouped_offsets(slots) * 4);
-  (void)first_aligned, (void)second_aligned;
-  return 0;
+  const int64_t given = 0;  // (only whether there are rows counts)
+  if (indexed && what != GROUPED_GRAD_X) g.rows = &given;
+  return lay_out(g, what, dtype, indexed && what == GROUPED_GRAD_X,
+                 what == GROUPED_LINEAR ? first_aligned : second_aligned, first_aligned,
+                 second_aligned)
+      .bytes;
 }
 
 extern "C" int hi2x_grouped_linear(const void* x, int dtype, int64_t ldx, int64_t x_rows,
@@ -209,15 +256,17 @@ extern "C" int hi2x_grouped_linear(const void* x, int dtype, int64_t ldx, int64_
                                    void* out, void* ws, int64_t ws_bytes, void* stream) {
   clear_error();
   GroupedArgs g{};
-  g.x = x, g.ldx = ldx, g.x_rows = x_rows, g.w = w, g.experts = experts, g.n = n, g.k = k;
-  g.rows = rows, g.offs = offs, g.slots = slots, g.out = out;
+  g.x = x, g.ldx = ldx, g.x_rows = x_rows, g.w = w, g.ldw = k;
+  g.experts = experts, g.n = n, g.k = k, g.rows = rows, g.offs = offs, g.slots = slots, g.out = out;
   if (int rc = check_grouped(g, dtype, "grouped_linear")) return rc;
   HI2X_REQUIRE(rows || x_rows == slots, "grouped_linear: %lld rows for %lld slots",
                (long long)x_rows, (long long)slots);
   HI2X_REQUIRE(x_rows <= 1 || ldx >= k, "grouped_linear: rows of x overlap");
   if (slots == 0) return HI2X_OK;
   HI2X_REQUIRE((x || x_rows == 0) && w && offs && out, "grouped_linear: null buffer");
-  return launch_product<GROUPED_LINEAR>(g, dtype, as_stream(stream), "grouped_linear");
+  Workspace space;
+  return run(g, GROUPED_LINEAR, dtype, false, ws, ws_bytes, space, nullptr, as_stream(stream),
+             "grouped_linear");
 }
 
 extern "C" int hi2x_grouped_grad_x(const void* dy, int dtype, int64_t ldy, const void* w,
@@ -227,7 +276,7 @@ extern "C" int hi2x_grouped_grad_x(const void* dy, int dtype, int64_t ldy, const
                                    void* stream) {
   clear_error();
   GroupedArgs g{};
-  g.dy = dy, g.ldy = ldy, g.w = w, g.experts = experts, g.n = n, g.k = k;
+  g.dy = dy, g.ldy = ldy, g.w = w, g.ldw = k, g.experts = experts, g.n = n, g.k = k;
   g.offs = offs, g.slots = slots, g.out = dx, g.x_rows = slots_of ? t : slots;
   if (int rc = check_grouped(g, dtype, "grouped_grad_x")) return rc;
   HI2X_REQUIRE(!slots_of || (t >= 0 && top_k >= 1 && top_k < (1 << 20)),
@@ -236,20 +285,16 @@ extern "C" int hi2x_grouped_grad_x(const void* dy, int dtype, int64_t ldy, const
   if (slots_of ? t == 0 : slots == 0) return HI2X_OK;
   HI2X_REQUIRE((dy || slots == 0) && w && offs && dx, "grouped_grad_x: null buffer");
   const hipStream_t s = as_stream(stream);
-  if (!slots_of) return launch_product<GROUPED_GRAD_X>(g, dtype, s, "grouped_grad_x");
-  Workspace part;
-  const size_t need = (size_t)align256(slots * k * size_of(dtype));
-  if (int rc = take_workspace(part, ws, ws_bytes, need, s, "grouped_grad_x")) return rc;
-  g.out = part.p;
+  Workspace space;
+  void* part = dx;
   if (slots)
-    if (int rc = launch_product<GROUPED_GRAD_X>(g, dtype, s, "grouped_grad_x")) return rc;
-  if (dtype == 0)
-    sum_slots_kernel<0><<<(unsigned)t, 256, 0, s>>>(part.p, slots, k, slots_of, t, (int)top_k, dx);
-  else if (dtype == 1)
-    sum_slots_kernel<1><<<(unsigned)t, 256, 0, s>>>(part.p, slots, k, slots_of, t, (int)top_k, dx);
-  else
-    sum_slots_kernel<2><<<(unsigned)t, 256, 0, s>>>(part.p, slots, k, slots_of, t, (int)top_k, dx);
-  return launch_status("grouped_grad_x");
+    if (int rc = run(g, GROUPED_GRAD_X, dtype, slots_of != nullptr, ws, ws_bytes, space, &part, s,
+                     "grouped_grad_x"))
+      return rc;
+  if (!slots_of) return HI2X_OK;
+  return dtype == 0   ? sum_slots<0>(part, slots, k, slots_of, t, top_k, dx, s)
+         : dtype == 1 ? sum_slots<1>(part, slots, k, slots_of, t, top_k, dx, s)
+                      : sum_slots<2>(part, slots, k, slots_of, t, top_k, dx, s);
 }
 
 extern "C" int hi2x_grouped_grad_w(const void* dy, int dtype, int64_t ldy, const void* x,
@@ -269,12 +314,7 @@ extern "C" int hi2x_grouped_grad_w(const void* dy, int dtype, int64_t ldy, const
                "grouped_grad_w: rows overlap");
   HI2X_REQUIRE(((x || x_rows == 0) && dy || slots == 0) && offs && dw,
                "grouped_grad_w: null buffer");
-  const hipStream_t s = as_stream(stream);
-  Workspace offsets;
-  if (rows && in_tiles(g, GROUPED_GRAD_W, dtype)) {
-    const size_t need = (size_t)align256(grouped_offsets(slots) * 4);
-    if (int rc = take_workspace(offsets, ws, ws_bytes, need, s, "grouped_grad_w")) return rc;
-    g.offsets = reinterpret_cast<uint32_t*>(offsets.p);
-  }
-  return launch_product<GROUPED_GRAD_W>(g, dtype, s, "grouped_grad_w");
+  Workspace space;
+  return run(g, GROUPED_GRAD_W, dtype, false, ws, ws_bytes, space, nullptr, as_stream(stream),
+             "grouped_grad_w");
 }

@@ -8,6 +8,8 @@
 // hands a lane its column.  Both are loaded as they lie, 16 bytes a lane, straight into LDS.
 //
 // A wave holds T/2 x T/2 results in registers; a ring of four stages is in flight.
+#include <type_traits>
+
 #include "grouped.h"
 
 namespace hi2x {
@@ -62,6 +64,10 @@ __device__ __forceinline__ f32x16v product(const s16x8& a, const s16x8& b, const
                                                    __builtin_bit_cast(b16x8, b), c, 0, 0, 0);
 }
 
+// A row's last piece counts whole: what lies in its 16 bytes behind the row is zero (along the
+// contraction) or comes out in columns that are not stored.
+__device__ __forceinline__ int whole(int n) { return (n + 7) & ~7; }
+
 constexpr int STAGE = 32;  // of the contraction
 constexpr int RING = 4;
 
@@ -70,6 +76,7 @@ constexpr int RING = 4;
 // a time lie on different banks.
 template <int T>
 struct AlongOperand {
+  static constexpr bool PAIRED = true;
   static constexpr int NC = T / 64;  // a wave's loads of a stage, 16 rows each
   __amdgpu_buffer_rsrc_t rs;
   uint32_t row[NC];  // this lane's rows' offsets
@@ -113,6 +120,7 @@ struct AlongOperand {
 // lie on different banks.
 template <int T>
 struct AcrossOperand {
+  static constexpr bool PAIRED = false;
   static constexpr int NC = T / 64, LP = T / 8, RPC = 64 / LP;  // lanes a row, rows a load
   const char* base;
   int64_t pitch;     // bytes
@@ -124,7 +132,7 @@ struct AcrossOperand {
   __device__ __forceinline__ void init(uint32_t lds, int wv, int half, int cols) {
     const int lane = threadIdx.x & 63;
     at = lds + NC * wv * 1024;
-    last = 2 * cols;
+    last = 2 * whole(cols);
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
       const int r = RPC * (NC * wv + i) + lane / LP;
@@ -142,12 +150,19 @@ struct AcrossOperand {
     __amdgpu_buffer_rsrc_t rs;
   };
   __device__ __forceinline__ Stage begin(int st) const {
-    int left = (int)rows - st * STAGE;
-    left = left < STAGE ? left : STAGE;
-    const int bytes = left * (int)pitch - ((int)pitch - (int)last);
+    // (scalar instructions by hand: the compiler clamps in a vector register, and the load would
+    // have to wait for what comes out of it)
+    int left = (int)rows - st * STAGE, bytes;
+    asm("s_min_i32 %0, %1, 32" : "=s"(left) : "s"(left) : "scc");
+    static_assert(STAGE == 32, "above");
+    bytes = __builtin_amdgcn_readfirstlane(left) * (int)pitch - ((int)pitch - (int)last);
+    asm("s_max_i32 %0, %1, 0"
+        : "=s"(bytes)
+        : "s"(__builtin_amdgcn_readfirstlane(bytes))
+        : "scc");
     return Stage{__builtin_amdgcn_make_buffer_rsrc(
         reinterpret_cast<char*>(uniform((int64_t)(base + (int64_t)st * (STAGE * pitch)))),
-        (short)0, __builtin_amdgcn_readfirstlane(bytes < 0 ? 0 : bytes), 0x00020000)};
+        (short)0, bytes, 0x00020000)};
   }
   __device__ __forceinline__ void load(const Stage& s, int i, uint32_t buffer) const {
     lds_load16(s.rs, own[i], at + buffer + i * 1024);
@@ -209,13 +224,27 @@ struct IndexedOperand : AcrossOperand<T> {
   }
 };
 
+template <bool NEEDED, class O>
+__device__ __forceinline__ auto pair_stage(O& o, int st) {
+  if constexpr (NEEDED)
+    return o.begin(st);
+  else
+    return 0;
+}
+
 // acc = A B^T over `len` > 0 of the contraction.  Each accumulator has results' columns (B's rows) in
 // its registers and their rows (A's) over the lanes.
+//
+// A ring of four stages.  The two stages of a 128-byte line of an AlongOperand are asked for one
+// right after the other, every other stage: a stage apart, the second comes when the line has left
+// the CU's cache, and every line crosses from L2 twice (16384 x 4096 x 4096: 6.7e7 requests and
+// 536 us; so: XXX).  Loads are issued behind products of the stage whose place they take, and
+// always as many (what lies past the end reads as zeros), so that "landed" is a count.
 template <int DT, int T, class A, class B>
 __device__ __forceinline__ void tile_loop(A& a, B& b, const char* lds, int len,
                                           f32x16v (&acc)[T / 64][T / 64]) {
   constexpr int NA = T / 64, BYTES = T * 64;  // of an operand's stage
-  constexpr int LOADS = 2 * NA;               // of a wave a stage
+  constexpr bool PA = A::PAIRED, PB = B::PAIRED;
   const int nst = (len + STAGE - 1) / STAGE;
 #pragma unroll
   for (int i = 0; i < NA; ++i)
@@ -225,28 +254,53 @@ __device__ __forceinline__ void tile_loop(A& a, B& b, const char* lds, int len,
       for (int u = 0; u < 16; ++u) acc[i][j][u] = 0.0f;
   const char* la = lds;
   const char* lb = lds + RING * BYTES;
-#pragma unroll 1
-  for (int p = 0; p < RING; ++p) {
-    const auto sa = a.begin(p);
-    const auto sb = b.begin(p);
+  // The loads of stages s0 (into x0) and s0 + 1 (into x1): those of paired operands, line by line,
+  // in front of the others'.
+  auto both = [&](int s0, uint32_t x0, uint32_t x1) {
+    const auto a0 = a.begin(s0);
+    const auto a1 = a.begin(s0 + 1);
+    const auto b0 = b.begin(s0);
+    const auto b1 = b.begin(s0 + 1);
+    if constexpr (PA) {
+#pragma unroll
+      for (int i = 0; i < NA; ++i) a.load(a0, i, x0), a.load(a1, i, x1);
+    }
+    if constexpr (PB) {
+#pragma unroll
+      for (int i = 0; i < NA; ++i) b.load(b0, i, x0), b.load(b1, i, x1);
+    }
 #pragma unroll
     for (int i = 0; i < NA; ++i) {
-      a.load(sa, i, p * BYTES);
-      b.load(sb, i, p * BYTES);
+      if constexpr (!PA) a.load(a0, i, x0);
+      if constexpr (!PB) b.load(b0, i, x0);
     }
-  }
-  __builtin_amdgcn_s_waitcnt(wait_for(3 * LOADS, 15));  // stage 0 landed
+#pragma unroll
+    for (int i = 0; i < NA; ++i) {
+      if constexpr (!PA) a.load(a1, i, x1);
+      if constexpr (!PB) b.load(b1, i, x1);
+    }
+  };
+  both(0, 0, BYTES);
+  both(2, 2 * BYTES, 3 * BYTES);
+  __builtin_amdgcn_s_waitcnt(wait_for(4 * NA, 15));  // stages 0 and 1 landed
   meet();
   s16x8 a0[NA], b0[NA], a1[NA], b1[NA];
   a.read(a0, la, 0);
   b.read(b0, lb, 0);
-  int st = 0;
-  do {
-    const uint32_t cur = (uint32_t)(st % RING) * BYTES, nxt = (uint32_t)((st + 1) % RING) * BYTES;
+  // Stage st in `cur`.  ODD: st is, and paired operands' stages st + 3 (into `prv`, where st - 1
+  // was) and st + 4 are asked for.
+  auto stage = [&](auto odd, int st, uint32_t prv, uint32_t cur, uint32_t nxt) {
+    constexpr bool ODD = decltype(odd)::value;
+    constexpr int PAIR = ODD ? 2 : 0;
+    constexpr int LA = NA * (PA ? PAIR : 1), LB = NA * (PB ? PAIR : 1), ALL = LA + LB;
+    // newer loads than the next stage's
+    constexpr int NEWER = NA * (!ODD ? 4 : (PA ? 0 : 2) + (PB ? 0 : 2));
     a.read(a1, la + cur, 1);
     b.read(b1, lb + cur, 1);
     const auto sa = a.begin(st + RING);
     const auto sb = b.begin(st + RING);
+    const auto pa = pair_stage<PA && ODD>(a, st + RING - 1);
+    const auto pb = pair_stage<PB && ODD>(b, st + RING - 1);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < NA; ++i)
@@ -255,30 +309,60 @@ __device__ __forceinline__ void tile_loop(A& a, B& b, const char* lds, int len,
     __builtin_amdgcn_sched_barrier(0);
     // this wave has read stage st, and stage st + 1 has landed; behind the barrier nobody reads
     // stage st any more
-    __builtin_amdgcn_s_waitcnt(wait_for(2 * LOADS, 0));
+    __builtin_amdgcn_s_waitcnt(wait_for(NEWER, 0));
     meet();
     a.read(a0, la + nxt, 0);
     b.read(b0, lb + nxt, 0);
     __builtin_amdgcn_sched_barrier(0);
-    // stage st + 4 takes its place, a load behind every few products (what lies past the end
-    // reads as zeros, so that every stage has the same number of loads)
-#pragma unroll
-    for (int i = 0; i < NA; ++i)
-#pragma unroll
-      for (int j = 0; j < NA; ++j) {
-        acc[i][j] = product<DT>(b1[j], a1[i], acc[i][j]);
-        const int m = i * NA + j;
-        if ((m + 1) % (NA / 2) == 0 && (m + 1) / (NA / 2) <= LOADS) {
-          const int l = (m + 1) / (NA / 2) - 1;
-          if (l & 1)
-            b.load(sb, l >> 1, cur);
-          else
-            a.load(sa, l >> 1, cur);
+    auto one = [&](auto number, const auto& pa, const auto& pb) {
+      constexpr int l = decltype(number)::value;
+      if constexpr (PA && l < LA) {
+        if constexpr (l & 1)
+          a.load(sa, l >> 1, cur);
+        else
+          a.load(pa, l >> 1, prv);
+      } else if constexpr (PB && l - (PA ? LA : 0) < LB) {
+        constexpr int m = l - (PA ? LA : 0);
+        if constexpr (m & 1)
+          b.load(sb, m >> 1, cur);
+        else
+          b.load(pb, m >> 1, prv);
+      } else if constexpr (PA) {
+        b.load(sb, l - LA, cur);
+      } else if constexpr (PB) {
+        a.load(sa, l - LB, cur);
+      } else {
+        if constexpr (l & 1)
+          b.load(sb, l >> 1, cur);
+        else
+          a.load(sa, l >> 1, cur);
+      }
+    };
+    auto products = [&](auto self, auto number, auto done) {
+      constexpr int m = decltype(number)::value, d = decltype(done)::value;
+      if constexpr (m < NA * NA) {
+        acc[m / NA][m % NA] = product<DT>(b1[m % NA], a1[m / NA], acc[m / NA][m % NA]);
+        constexpr int upto = ALL * (m + 1) / (NA * NA);
+        if constexpr (upto > d) {
+          one(std::integral_constant<int, d>{}, pa, pb);
+          if constexpr (upto > d + 1) one(std::integral_constant<int, d + 1>{}, pa, pb);
           __builtin_amdgcn_sched_barrier(0);
         }
+        self(self, std::integral_constant<int, m + 1>{}, std::integral_constant<int, upto>{});
       }
+    };
+    products(products, std::integral_constant<int, 0>{}, std::integral_constant<int, 0>{});
     __builtin_amdgcn_sched_barrier(0);
-  } while (++st < nst);
+  };
+  int st = 0;
+  uint32_t cur = 0;
+  do {
+    const uint32_t other = cur ^ (2 * BYTES);
+    stage(std::false_type{}, st, 0, cur, cur + BYTES);
+    stage(std::true_type{}, st + 1, cur, cur + BYTES, other);
+    cur = other;
+    st += 2;
+  } while (st < nst);
   __builtin_amdgcn_s_waitcnt(wait_for(0, 0));
 }
 
@@ -347,12 +431,76 @@ template <int T>
 constexpr int LDS_BYTES = 2 * RING * T * 64 > T * (2 * T + 16) ? 2 * RING * T * 64
                                                                : T * (2 * T + 16);
 
-// Tiles of rows of slots: workgroups go to the eight XCDs in turn, so an XCD takes all tiles of
-// four neighbouring row tiles one after the other, and rows and weights come to its L2 once.
+// The plan's row tiles.  One workgroup: the ranges' first tiles by a scan, then a thread to a tile.
+// (Found by every workgroup for itself, a tile's expert cost 2 us, and nobody knew how many tiles
+// there are.)
+constexpr int MOST_EXPERTS = 7000;
+__global__ __launch_bounds__(1024) void grouped_plan_kernel(GroupedArgs g, int T, Plan* plan,
+                                                            int64_t most) {
+  __shared__ int first_tile[MOST_EXPERTS + 3];
+  __shared__ int sums[16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int experts = (int)g.experts, ranges = experts + 2;
+  auto range = [&](int e, int64_t& a, int64_t& b) {
+    auto clamp = [&](int64_t v) { return v < 0 ? 0 : (v > g.slots ? g.slots : v); };
+    if (e < experts) {
+      slot_range(g, e, a, b);
+    } else {
+      a = e == experts ? clamp(g.offs[experts]) : 0;
+      b = e == experts ? g.slots : clamp(g.offs[0]);
+    }
+  };
+  int before = 0;
+  for (int e0 = 0; e0 < ranges; e0 += 1024) {
+    const int e = e0 + tid;
+    int64_t a = 0, b = 0;
+    if (e < ranges) range(e, a, b);
+    const int n = (int)((b - a + T - 1) / T);
+    int inc = n;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int o = __shfl_up(inc, d);
+      if (lane >= d) inc += o;
+    }
+    if (lane == 63) sums[wave] = inc;
+    __syncthreads();
+    int base = before, all = 0;
+    for (int w = 0; w < 16; ++w) {
+      if (w < wave) base += sums[w];
+      all += sums[w];
+    }
+    if (e < ranges) first_tile[e] = base + inc - n;
+    before += all;
+    __syncthreads();
+  }
+  // (ranges that overlap, as they should not, could make more tiles than there is room for)
+  const int count = before < most ? before : (int)most;
+  if (tid == 0) {
+    first_tile[ranges] = before;
+    plan->count = count;
+  }
+  __syncthreads();
+  for (int y = tid; y < count; y += 1024) {
+    int lo = 0, hi = ranges - 1;  // the last range whose first tile is y or before
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (first_tile[mid] <= y)
+        lo = mid;
+      else
+        hi = mid - 1;
+    }
+    int64_t a, b;
+    range(lo, a, b);
+    const int64_t at = a + (int64_t)(y - first_tile[lo]) * T, left = b - at;
+    plan->tile[y] = RowTile{at, (int32_t)(left < T ? left : T), lo < experts ? lo : -1};
+  }
+}
+
 template <int DT, int WHAT, int T, bool INDEXED>
 __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void grouped_tile_kernel(GroupedArgs g,
                                                                               uint32_t nx,
-                                                                              uint32_t ny) {
+                                                                              uint32_t ny,
+                                                                              const void* plan) {
   constexpr int NA = T / 64, BYTES = T * 64;
   __shared__ __attribute__((aligned(1024))) char lds[LDS_BYTES<T>];
   __shared__ uint8_t bad[T];
@@ -368,10 +516,12 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void grouped_tile_kernel(Gro
     // An expert's tiles over all XCDs, 2 x 4 of them at a time, one to each.
     const uint32_t xcd = blockIdx.x & 7, j = blockIdx.x >> 3;
     const uint32_t hx = nx / 4, per = hx * (ny / 2);  // (nx, ny: rounded up to whole rounds)
-    const int e = (int)(j / per);
+    // (what comes out of a division is in a vector register, and would keep what follows there)
+    const int e = __builtin_amdgcn_readfirstlane(j / per);
     const uint32_t sub = j - e * per, my = (xcd + e) & 7;
-    const int64_t r0 = (int64_t)((sub / hx) * 2 + (my >> 2)) * T;
-    const int64_t c0 = (int64_t)((sub % hx) * 4 + (my & 3)) * T;
+    const uint32_t sy = __builtin_amdgcn_readfirstlane(sub / hx), sx = sub - sy * hx;
+    const int64_t r0 = (int64_t)(sy * 2 + (my >> 2)) * T;
+    const int64_t c0 = (int64_t)(sx * 4 + (my & 3)) * T;
     if (r0 >= n || c0 >= k) return;
     int64_t first, end;
     slot_range(g, e, first, end);
@@ -391,10 +541,11 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void grouped_tile_kernel(Gro
     if constexpr (INDEXED) {
       if (tid == 0) bad[0] = 0;  // (behind the loop's barriers)
       IndexedOperand<T> b;
-      b.offsets = (const __attribute__((address_space(4))) uint32_t*)(g.offsets + first);
+      b.offsets = (const __attribute__((address_space(4))) uint32_t*)(
+          static_cast<const uint32_t*>(plan) + first);
       b.rows = end - first;
       b.all = rsrc(static_cast<const char*>(g.x) + c0 * 2,
-                   g.x_rows > 0 ? ((g.x_rows - 1) * g.ldx + cols) * 2 : 0);
+                   g.x_rows > 0 ? ((g.x_rows - 1) * g.ldx + whole(cols)) * 2 : 0);
       b.init(base + RING * BYTES, wv, wc, cols);
       tile_loop<DT, T>(a, b, lds, (int)(end - first), acc);
       if (b.seen & 1) bad[0] = 1;
@@ -408,12 +559,12 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void grouped_tile_kernel(Gro
     }
     store_tile<DT, T, INDEXED ? 2 : 0>(lds, acc, to, k, rows, cols, bad);
   } else {
-    const uint32_t xcd = blockIdx.x & 7, j = blockIdx.x >> 3, r = j / nx, xt = j - r * nx;
-    const GroupedWork w = find_rows(g, T, ((int64_t)(r >> 2) * 8 + xcd) * 4 + (r & 3));
+    RowTile w;
+    uint32_t xt;
+    if (!plan_tile(static_cast<const Plan*>(plan), nx, blockIdx.x, w, xt)) return;
     const int e = __builtin_amdgcn_readfirstlane(w.e);
-    if (e == WORK_NONE) return;
-    const int64_t first = uniform(w.first), left = uniform(w.end) - first;
-    const int live = (int)(left < T ? left : T);
+    const int live = __builtin_amdgcn_readfirstlane(w.live);
+    const int64_t first = uniform(w.first);
     const int64_t width = WHAT == GROUPED_LINEAR ? n : k, c0 = (int64_t)xt * T;
     const int cols = (int)(width - c0 < T ? width - c0 : T);
     uint16_t* const to = out + first * width + c0;
@@ -425,7 +576,7 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void grouped_tile_kernel(Gro
     if constexpr (WHAT == GROUPED_LINEAR) {
       a.init(base, wv, wr, k);
       if constexpr (INDEXED) {
-        a.rs = rsrc(g.x, g.x_rows > 0 ? ((g.x_rows - 1) * g.ldx + k) * 2 : 0);
+        a.rs = rsrc(g.x, g.x_rows > 0 ? ((g.x_rows - 1) * g.ldx + whole(k)) * 2 : 0);
 #pragma unroll
         for (int i = 0; i < NA; ++i) {
           const int t = a.row_of(wv, i);
@@ -436,7 +587,7 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void grouped_tile_kernel(Gro
         }
       } else {
         a.rs = rsrc(static_cast<const char*>(g.x) + first * g.ldx * 2,
-                    ((int64_t)(live - 1) * g.ldx + k) * 2);
+                    ((int64_t)(live - 1) * g.ldx + whole(k)) * 2);
 #pragma unroll
         for (int i = 0; i < NA; ++i) {
           const int t = a.row_of(wv, i);
@@ -445,26 +596,26 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void grouped_tile_kernel(Gro
       }
       AlongOperand<T> b;
       b.init(base + RING * BYTES, wv, wc, k);
-      b.rs = rsrc(static_cast<const char*>(g.w) + ((int64_t)e * n + c0) * k * 2,
-                  (int64_t)cols * k * 2);
+      b.rs = rsrc(static_cast<const char*>(g.w) + ((int64_t)e * n + c0) * g.ldw * 2,
+                  ((int64_t)(cols - 1) * g.ldw + whole(k)) * 2);
 #pragma unroll
       for (int i = 0; i < NA; ++i) {
         const int t = b.row_of(wv, i);
-        b.row[i] = t < cols ? (uint32_t)t * (uint32_t)(k * 2) : ROW_DEAD;
+        b.row[i] = t < cols ? (uint32_t)(t * g.ldw * 2) : ROW_DEAD;
       }
       tile_loop<DT, T>(a, b, lds, k, acc);
     } else {
       a.init(base, wv, wr, n);
       a.rs = rsrc(static_cast<const char*>(g.dy) + first * g.ldy * 2,
-                  ((int64_t)(live - 1) * g.ldy + n) * 2);
+                  ((int64_t)(live - 1) * g.ldy + whole(n)) * 2);
 #pragma unroll
       for (int i = 0; i < NA; ++i) {
         const int t = a.row_of(wv, i);
         a.row[i] = t < live ? (uint32_t)(t * g.ldy * 2) : ROW_DEAD;
       }
       AcrossOperand<T> b;
-      b.base = static_cast<const char*>(g.w) + ((int64_t)e * n * k + c0) * 2;
-      b.pitch = (int64_t)k * 2;
+      b.base = static_cast<const char*>(g.w) + ((int64_t)e * n * g.ldw + c0) * 2;
+      b.pitch = g.ldw * 2;
       b.rows = n;
       b.init(base + RING * BYTES, wv, wc, cols);
       tile_loop<DT, T>(a, b, lds, n, acc);
@@ -484,48 +635,61 @@ __global__ __launch_bounds__(256) void indexed_rows_kernel(const int64_t* rows, 
 }
 
 template <int DT, int WHAT, int T, bool INDEXED>
-int launch_tile(const GroupedArgs& g, hipStream_t s, const char* what) {
+int launch_tile(const GroupedArgs& g, char* plan, hipStream_t s, const char* what) {
   const int64_t cols = WHAT == GROUPED_LINEAR ? g.n : g.k;
-  int64_t nx = (cols + T - 1) / T, ny, count;
+  int64_t nx = (cols + T - 1) / T, ny;
   if constexpr (WHAT == GROUPED_GRAD_W) {
     nx = (nx + 3) / 4 * 4;
     ny = ((g.n + T - 1) / T + 1) / 2 * 2;
-    count = nx * ny * g.experts;
     if (INDEXED && g.slots)
       indexed_rows_kernel<<<(unsigned)((g.slots + 255) / 256), 256, 0, s>>>(
-          g.rows, g.slots, g.x_rows, (uint32_t)(g.ldx * 2), g.offsets);
+          g.rows, g.slots, g.x_rows, (uint32_t)(g.ldx * 2), reinterpret_cast<uint32_t*>(plan));
+    ny *= g.experts;
   } else {
-    ny = (g.slots / T + g.experts + 2 + 31) / 32 * 32;
-    count = nx * ny;
+    ny = most_tiles(g, T);
+    if (int rc = launch_plan(g, T, reinterpret_cast<Plan*>(plan), s, what)) return rc;
   }
-  HI2X_REQUIRE(count < (1ll << 31), "%s: too many results", what);
-  grouped_tile_kernel<DT, WHAT, T, INDEXED>
-      <<<(unsigned)count, 256, 0, s>>>(g, (uint32_t)nx, (uint32_t)ny);
+  const int64_t count = (nx * ny + 7) / 8 * 8;
+  grouped_tile_kernel<DT, WHAT, T, INDEXED><<<(unsigned)count, 256, 0, s>>>(
+      g, (uint32_t)nx, (uint32_t)(ny / (WHAT == GROUPED_GRAD_W ? g.experts : 1)), plan);
   return launch_status(what);
 }
 
 template <int DT, int WHAT, int T>
-int launch_indexed(const GroupedArgs& g, hipStream_t s, const char* what) {
+int launch_indexed(const GroupedArgs& g, char* plan, hipStream_t s, const char* what) {
   if constexpr (WHAT != GROUPED_GRAD_X) {
-    if (g.rows) return launch_tile<DT, WHAT, T, true>(g, s, what);
+    if (g.rows) return launch_tile<DT, WHAT, T, true>(g, plan, s, what);
   }
-  return launch_tile<DT, WHAT, T, false>(g, s, what);
+  return launch_tile<DT, WHAT, T, false>(g, plan, s, what);
 }
 
 template <int DT, int WHAT>
-int launch_size(const GroupedArgs& g, hipStream_t s, const char* what) {
+int launch_size(const GroupedArgs& g, char* plan, hipStream_t s, const char* what) {
   const int64_t rows = WHAT == GROUPED_GRAD_W ? g.experts * ((g.n + 255) / 256)
                                               : g.slots / 256 + g.experts / 2;
   const int64_t cols = ((WHAT == GROUPED_LINEAR ? g.n : g.k) + 255) / 256;
-  if (rows * cols >= 192) return launch_indexed<DT, WHAT, 256>(g, s, what);
-  return launch_indexed<DT, WHAT, 128>(g, s, what);
+  if (rows * cols >= 192) return launch_indexed<DT, WHAT, 256>(g, plan, s, what);
+  return launch_indexed<DT, WHAT, 128>(g, plan, s, what);
 }
 
 }  // namespace
 
-int grouped_tiles(const GroupedArgs& g, int what, int dtype, hipStream_t s, const char* name) {
-#define HI2X_GROUPED(WHAT) \
-  return dtype == 1 ? launch_size<1, WHAT>(g, s, name) : launch_size<2, WHAT>(g, s, name)
+int launch_plan(const GroupedArgs& g, int T, Plan* plan, hipStream_t s, const char* name) {
+  grouped_plan_kernel<<<1, 1024, 0, s>>>(g, T, plan, most_tiles(g, T));
+  return launch_status(name);
+}
+
+int64_t grouped_plan_bytes(const GroupedArgs& g, int what, int dtype) {
+  // (offsets past a range's end are read, and not used)
+  if (what == GROUPED_GRAD_W) return g.rows && dtype ? align256((g.slots + 256) * 4) : 0;
+  return plan_bytes(g, dtype ? 128 : 64);
+}
+
+int grouped_tiles(const GroupedArgs& g, int what, int dtype, char* plan, hipStream_t s,
+                  const char* name) {
+#define HI2X_GROUPED(WHAT)                                     \
+  return dtype == 1 ? launch_size<1, WHAT>(g, plan, s, name) : \
+                      launch_size<2, WHAT>(g, plan, s, name)
   if (what == GROUPED_LINEAR) HI2X_GROUPED(GROUPED_LINEAR);
   if (what == GROUPED_GRAD_X) HI2X_GROUPED(GROUPED_GRAD_X);
   HI2X_GROUPED(GROUPED_GRAD_W);

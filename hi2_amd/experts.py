@@ -65,8 +65,8 @@ def _linear(x, w, offs, rows, slots):
     dt = DTYPES[x.dtype]
     out = torch.empty(slots, n, dtype=x.dtype, device=x.device)
     if slots and n:
-        ws, size = _workspace(x.device, _LINEAR, dt, x.shape[0], e, n, k, slots, rows is not None,
-                              _aligned(x), k * x.element_size() % 16 == 0)
+        ws, size = _workspace(x.device, _LINEAR, dt, x.shape[0], _pitch(x), e, n, k, slots,
+                              rows is not None, _aligned(x), _aligned(w.view(e * n, k)))
         _lib.call("hi2x_grouped_linear", x.device, x.data_ptr(), dt, _pitch(x), x.shape[0],
                   w.data_ptr(), e, n, k, _lib.ptr(rows), offs.data_ptr(), slots, out.data_ptr(),
                   _lib.ptr(ws), size)
@@ -96,16 +96,16 @@ class _Grouped(torch.autograd.Function):
             dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
             top_k = 0 if slots_of is None else slots_of.shape[1]
             if x.shape[0]:
-                ws, size = _workspace(dev, _GRAD_X, dt, x.shape[0], e, n, k, slots,
+                ws, size = _workspace(dev, _GRAD_X, dt, x.shape[0], k, e, n, k, slots,
                                       slots_of is not None, _aligned(grad),
-                                      k * x.element_size() % 16 == 0)
+                                      _aligned(w.view(e * n, k)))
                 _lib.call("hi2x_grouped_grad_x", dev, grad.data_ptr(), dt, _pitch(grad),
                           w.data_ptr(), e, n, k, offs.data_ptr(), slots, _lib.ptr(slots_of),
                           x.shape[0], top_k, dx.data_ptr(), _lib.ptr(ws), size)
         if ctx.needs_input_grad[1]:
             dw = torch.empty(e, n, k, dtype=w.dtype, device=dev)
-            ws, size = _workspace(dev, _GRAD_W, dt, x.shape[0], e, n, k, slots, rows is not None,
-                                  _aligned(grad), _aligned(x))
+            ws, size = _workspace(dev, _GRAD_W, dt, x.shape[0], _pitch(x), e, n, k, slots,
+                                  rows is not None, _aligned(grad), _aligned(x))
             _lib.call("hi2x_grouped_grad_w", dev, grad.data_ptr(), dt, _pitch(grad), x.data_ptr(),
                       _pitch(x), x.shape[0], e, n, k, _lib.ptr(rows), offs.data_ptr(), slots,
                       dw.data_ptr(), _lib.ptr(ws), size)

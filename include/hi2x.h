@@ -759,8 +759,9 @@ int hi2x_adamw_moments(const void* m_codes, const void* v_codes, const float* m_
  * 0 to slots gives a row of NaN) dx is [t][k], summed in the order of top_k over what each slot
  * has, which for fp16 and bf16 is rounded to that type first; with slots_of NULL dx is [slots][k].
  * Workspace: hi2x_grouped_workspace_bytes of what (0 linear, 1 grad_x, 2 grad_w), tokens = x_rows
- * (grad_x: t), indexed = rows or slots_of given, and whether x or dy (first) and w or, for
- * grad_w, x (second) begin and continue at multiples of 16 bytes. */
+ * (grad_x: t) and ldx (grad_x: any), indexed = rows or slots_of given, and whether the first operand
+ * (x; for the gradients dy) and the second (w; for grad_w x) begin and continue at multiples of 16
+ * bytes (those that do not are copied there). */
 int hi2x_grouped_linear(const void* x, int dtype, int64_t ldx, int64_t x_rows, const void* w,
                         int64_t experts, int64_t n, int64_t k, const int64_t* rows,
                         const int64_t* offs, int64_t slots, void* out, void* ws, int64_t ws_bytes,
@@ -773,9 +774,9 @@ int hi2x_grouped_grad_w(const void* dy, int dtype, int64_t ldy, const void* x, i
                         int64_t x_rows, int64_t experts, int64_t n, int64_t k,
                         const int64_t* rows, const int64_t* offs, int64_t slots, void* dw,
                         void* ws, int64_t ws_bytes, void* stream);
-int64_t hi2x_grouped_workspace_bytes(int what, int dtype, int64_t tokens, int64_t experts,
-                                     int64_t n, int64_t k, int64_t slots, int indexed,
-                                     int first_aligned, int second_aligned);
+int64_t hi2x_grouped_workspace_bytes(int what, int dtype, int64_t tokens, int64_t ldx,
+                                     int64_t experts, int64_t n, int64_t k, int64_t slots,
+                                     int indexed, int first_aligned, int second_aligned);
 
 /* out = act(gate) * up, [rows][n], all of one dtype with rows ld apart: act as in hi2x_epilogue.
  * In f32, rounded once. */

@@ -32,6 +32,7 @@ def linear(x=FAKE, dtype=2, ldx=64, x_rows=8, w=FAKE, experts=2, n=32, k=64, row
     ("bad rows", dict(slots=1 << 31)),
     ("8 rows for 9 slots", dict(rows=None, slots=9)),
     ("overlap", dict(ldx=63)),
+    ("2^21 elements apart", dict(ldx=1 << 21)),
     ("null buffer", dict(x=None)),
     ("null buffer", dict(w=None)),
     ("null buffer", dict(offs=None)),
@@ -79,10 +80,16 @@ def test_grouped_grad_w_refuses(match, args):
 
 def test_workspace_query_refuses():
     size = _lib.lib().hi2x_grouped_workspace_bytes
-    assert size(3, 0, 1, 1, 1, 1, 1, 0, 1, 1) == -1
-    assert size(0, 5, 1, 1, 1, 1, 1, 0, 1, 1) == -1
-    assert size(1, 0, 1, 0, 1, 1, 1, 0, 1, 1) == -1
-    assert size(1, 2, 100, 4, 64, 128, 200, 1, 1, 1) >= 200 * 128 * 2
+    assert size(3, 0, 1, 1, 1, 1, 1, 1, 0, 1, 1) == -1
+    assert size(0, 5, 1, 1, 1, 1, 1, 1, 0, 1, 1) == -1
+    assert size(1, 0, 1, 1, 0, 1, 1, 1, 0, 1, 1) == -1
+    assert size(1, 2, 100, 128, 4, 64, 128, 200, 1, 1, 1) >= 200 * 128 * 2
+    # copies: of unaligned operands, and of rows beyond an index's reach
+    plain = size(0, 2, 100, 128, 4, 64, 128, 200, 1, 1, 1)
+    assert plain < 1 << 20
+    assert size(0, 2, 100, 128, 4, 64, 128, 200, 1, 0, 1) >= plain + 100 * 128 * 2
+    assert size(0, 2, 100, 128, 4, 64, 127, 200, 1, 1, 0) >= plain + 4 * 64 * 128 * 2
+    assert size(0, 2, 1 << 20, 1 << 12, 4, 64, 4096, 300, 1, 1, 1) >= 300 * 4096 * 2
 
 
 def gated(gate=FAKE, ldg=64, up=FAKE, ldu=64, rows=4, n=64, dtype=2, act=2, out=FAKE, ldo=64):
