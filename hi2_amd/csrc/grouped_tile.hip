@@ -7,7 +7,7 @@
 // gradient, dy and x of the weights') a stage is 32 rows of T values, and LDS's transposing read
 // hands a lane its column.  Both are loaded as they lie, 16 bytes a lane, straight into LDS.
 //
-// A wave holds T/2 x T/2 results in registers; a ring of four stages is in flight.
+// A wave holds T/2 x T/2 results in registers; a ring of four stages (or two) is in flight.
 #include <type_traits>
 
 #include "grouped.h"
@@ -69,7 +69,6 @@ __device__ __forceinline__ f32x16v product(const s16x8& a, const s16x8& b, const
 __device__ __forceinline__ int whole(int n) { return (n + 7) & ~7; }
 
 constexpr int STAGE = 32;  // of the contraction
-constexpr int RING = 4;
 
 // Neighbours of the contraction are neighbours in memory.  LDS: T rows of four 16-byte pieces,
 // piece q of row r at q ^ ((r / 4) % 4), so that the 16 rows that a read of one piece touches at
@@ -180,47 +179,30 @@ struct AcrossOperand {
   }
 };
 
-// The same of rows that an index names, by their offsets in x (indexed_rows_kernel): bit 0 marks
-// a row outside.
+// The same of rows that an index names: their offsets in x lie in LDS, dead ones behind the last.
 template <int T>
 struct IndexedOperand : AcrossOperand<T> {
   using Base = AcrossOperand<T>;
   using Base::LP, Base::NC, Base::RPC;
-  const __attribute__((address_space(4))) uint32_t* offsets;
+  const uint32_t* table;  // in LDS
   __amdgpu_buffer_rsrc_t all;
-  int wave_row;  // the wave's first row in a stage
-  uint32_t seen;  // all offsets, or-ed
+  int lane_row;  // of the wave's first load
   __device__ __forceinline__ void init(uint32_t lds, int wv, int half, int cols) {
     this->pitch = 0;
     Base::init(lds, wv, half, cols);
-    wave_row = RPC * NC * wv;
-    seen = 0;
+    lane_row = RPC * NC * wv + (threadIdx.x & 63) / LP;
   }
-  static_assert(RPC * NC == 8, "rows of a wave's loads");
   struct Stage {
-    u32x8 row;
+    uint32_t row[NC];
   };
-  // Rows past the end (there are offsets, of whatever) are dead: 0 x infinity would be NaN.
-  __device__ __forceinline__ Stage begin(int st) {
+  __device__ __forceinline__ Stage begin(int st) const {
     Stage s;
-    const int j0 = st * STAGE + wave_row;
-    int left = (int)this->rows - j0;
-    left = left < 0 ? 0 : (left < 8 ? left : 8);
-    const uint32_t past = 0xffu << left;
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const uint32_t dead = (past << (31 - u)) & ROW_DEAD, off = offsets[j0 + u];
-      s.row[u] = off | dead;
-      seen |= dead ? 0u : off;
-    }
+    for (int i = 0; i < NC; ++i) s.row[i] = table[st * STAGE + lane_row + RPC * i];
     return s;
   }
   __device__ __forceinline__ void load(const Stage& s, int i, uint32_t buffer) const {
-    const int sub = (threadIdx.x & 63) / LP;
-    uint32_t row = s.row[RPC * i];
-#pragma unroll
-    for (int u = 1; u < RPC; ++u) row = sub == u ? s.row[RPC * i + u] : row;
-    lds_load16(all, row + this->own[i], this->at + buffer + i * 1024);
+    lds_load16(all, s.row[i] + this->own[i], this->at + buffer + i * 1024);
   }
 };
 
@@ -232,26 +214,21 @@ __device__ __forceinline__ auto pair_stage(O& o, int st) {
     return 0;
 }
 
-// acc = A B^T over `len` > 0 of the contraction.  Each accumulator has results' columns (B's rows) in
-// its registers and their rows (A's) over the lanes.
+// acc += A B^T over `len` > 0 of the contraction.  Each accumulator has results' columns (B's rows)
+// in its registers and their rows (A's) over the lanes.
 //
-// A ring of four stages.  The two stages of a 128-byte line of an AlongOperand are asked for one
+// A ring of four stages, or of two where more workgroups to a CU hide what it does not.  The two stages of a 128-byte line of an AlongOperand are asked for one
 // right after the other, every other stage: a stage apart, the second comes when the line has left
 // the CU's cache, and every line crosses from L2 twice (16384 x 4096 x 4096: 6.7e7 requests and
 // 536 us; so: XXX).  Loads are issued behind products of the stage whose place they take, and
 // always as many (what lies past the end reads as zeros), so that "landed" is a count.
-template <int DT, int T, class A, class B>
+template <int DT, int T, int RING, class A, class B>
 __device__ __forceinline__ void tile_loop(A& a, B& b, const char* lds, int len,
                                           f32x16v (&acc)[T / 64][T / 64]) {
   constexpr int NA = T / 64, BYTES = T * 64;  // of an operand's stage
   constexpr bool PA = A::PAIRED, PB = B::PAIRED;
+  static_assert(RING == 4 || (RING == 2 && !PA && !PB), "pairs need four stages");
   const int nst = (len + STAGE - 1) / STAGE;
-#pragma unroll
-  for (int i = 0; i < NA; ++i)
-#pragma unroll
-    for (int j = 0; j < NA; ++j)
-#pragma unroll
-      for (int u = 0; u < 16; ++u) acc[i][j][u] = 0.0f;
   const char* la = lds;
   const char* lb = lds + RING * BYTES;
   // The loads of stages s0 (into x0) and s0 + 1 (into x1): those of paired operands, line by line,
@@ -281,8 +258,9 @@ __device__ __forceinline__ void tile_loop(A& a, B& b, const char* lds, int len,
     }
   };
   both(0, 0, BYTES);
-  both(2, 2 * BYTES, 3 * BYTES);
-  __builtin_amdgcn_s_waitcnt(wait_for(4 * NA, 15));  // stages 0 and 1 landed
+  if constexpr (RING == 4) both(2, 2 * BYTES, 3 * BYTES);
+  // stage 0 landed, and with a ring of four stage 1
+  __builtin_amdgcn_s_waitcnt(wait_for(RING == 4 ? 4 * NA : 2 * NA, 15));
   meet();
   s16x8 a0[NA], b0[NA], a1[NA], b1[NA];
   a.read(a0, la, 0);
@@ -294,7 +272,7 @@ __device__ __forceinline__ void tile_loop(A& a, B& b, const char* lds, int len,
     constexpr int PAIR = ODD ? 2 : 0;
     constexpr int LA = NA * (PA ? PAIR : 1), LB = NA * (PB ? PAIR : 1), ALL = LA + LB;
     // newer loads than the next stage's
-    constexpr int NEWER = NA * (!ODD ? 4 : (PA ? 0 : 2) + (PB ? 0 : 2));
+    constexpr int NEWER = RING == 2 ? 0 : NA * (!ODD ? 4 : (PA ? 0 : 2) + (PB ? 0 : 2));
     a.read(a1, la + cur, 1);
     b.read(b1, lb + cur, 1);
     const auto sa = a.begin(st + RING);
@@ -357,7 +335,7 @@ __device__ __forceinline__ void tile_loop(A& a, B& b, const char* lds, int len,
   int st = 0;
   uint32_t cur = 0;
   do {
-    const uint32_t other = cur ^ (2 * BYTES);
+    const uint32_t other = RING == 2 ? 0 : cur ^ (2 * BYTES);
     stage(std::false_type{}, st, 0, cur, cur + BYTES);
     stage(std::true_type{}, st + 1, cur, cur + BYTES, other);
     cur = other;
@@ -427,9 +405,14 @@ __device__ __forceinline__ void store_zeros(uint16_t* out, int64_t cols, int row
   for (int r = threadIdx.x / TX; r < rows; r += 256 / TX) out[r * cols + c] = 0;
 }
 
-template <int T>
+template <int T, int RING>
 constexpr int LDS_BYTES = 2 * RING * T * 64 > T * (2 * T + 16) ? 2 * RING * T * 64
                                                                : T * (2 * T + 16);
+
+// Slots whose rows' offsets are in LDS at a time, and offsets behind them that the ring reads.
+template <int T, int RING>
+constexpr int SEGMENT = T == 256 ? 4096 : (RING == 4 ? 2048 : 1024);
+constexpr int BEHIND = 224;
 
 // The plan's row tiles.  One workgroup: the ranges' first tiles by a scan, then a thread to a tile.
 // (Found by every workgroup for itself, a tile's expert cost 2 us, and nobody knew how many tiles
@@ -496,14 +479,16 @@ __global__ __launch_bounds__(1024) void grouped_plan_kernel(GroupedArgs g, int T
   }
 }
 
-template <int DT, int WHAT, int T, bool INDEXED>
-__global__ __launch_bounds__(256, T == 256 ? 1 : 2) void grouped_tile_kernel(GroupedArgs g,
+template <int DT, int WHAT, int T, int RING, bool INDEXED>
+__global__ __launch_bounds__(256, T == 256 ? 1 : 8 / RING) void grouped_tile_kernel(GroupedArgs g,
                                                                               uint32_t nx,
                                                                               uint32_t ny,
                                                                               const void* plan) {
   constexpr int NA = T / 64, BYTES = T * 64;
-  __shared__ __attribute__((aligned(1024))) char lds[LDS_BYTES<T>];
+  __shared__ __attribute__((aligned(1024))) char lds[LDS_BYTES<T, RING>];
   __shared__ uint8_t bad[T];
+  constexpr bool TABLE = WHAT == GROUPED_GRAD_W && INDEXED;
+  __shared__ uint32_t table[TABLE ? SEGMENT<T, RING> + BEHIND : 1];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wr = wv >> 1, wc = wv & 1;
@@ -511,6 +496,12 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void grouped_tile_kernel(Gro
       (uint32_t)(size_t)(__attribute__((address_space(3))) char*)lds);
   const int n = (int)g.n, k = (int)g.k;
   f32x16v acc[NA][NA];
+#pragma unroll
+  for (int i = 0; i < NA; ++i)
+#pragma unroll
+    for (int j = 0; j < NA; ++j)
+#pragma unroll
+      for (int u = 0; u < 16; ++u) acc[i][j][u] = 0.0f;
   uint16_t* const out = static_cast<uint16_t*>(g.out);
   if constexpr (WHAT == GROUPED_GRAD_W) {
     // An expert's tiles over all XCDs, 2 x 4 of them at a time, one to each.
@@ -539,23 +530,42 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void grouped_tile_kernel(Gro
     a.rows = end - first;
     a.init(base, wv, wr, rows);
     if constexpr (INDEXED) {
-      if (tid == 0) bad[0] = 0;  // (behind the loop's barriers)
+      if (tid == 0) bad[0] = 0;
       IndexedOperand<T> b;
-      b.offsets = (const __attribute__((address_space(4))) uint32_t*)(
-          static_cast<const uint32_t*>(plan) + first);
-      b.rows = end - first;
+      b.table = table;
       b.all = rsrc(static_cast<const char*>(g.x) + c0 * 2,
                    g.x_rows > 0 ? ((g.x_rows - 1) * g.ldx + whole(cols)) * 2 : 0);
       b.init(base + RING * BYTES, wv, wc, cols);
-      tile_loop<DT, T>(a, b, lds, (int)(end - first), acc);
-      if (b.seen & 1) bad[0] = 1;
+      constexpr int SEG = SEGMENT<T, RING>;
+      const int all = (int)(end - first);
+      const int64_t* const index = g.rows + first;
+      for (int at = 0; at < all; at += SEG) {
+        const int len = all - at < SEG ? all - at : SEG;
+        __syncthreads();  // the segment before has been read
+        for (int u = tid; u < SEG + BEHIND; u += 256) {
+          uint32_t off = ROW_DEAD;
+          if (u < len) {
+            const uint64_t r = (uint64_t)index[at + u];
+            if (r < (uint64_t)g.x_rows)
+              off = (uint32_t)r * (uint32_t)(g.ldx * 2);
+            else
+              bad[0] = 1;
+          }
+          table[u] = off;
+          if (u >= len + BEHIND) break;
+        }
+        __syncthreads();
+        a.base = static_cast<const char*>(g.dy) + ((first + at) * g.ldy + r0) * 2;
+        a.rows = len;
+        tile_loop<DT, T, RING>(a, b, lds, len, acc);
+      }
     } else {
       AcrossOperand<T> b;
       b.base = static_cast<const char*>(g.x) + (first * g.ldx + c0) * 2;
       b.pitch = g.ldx * 2;
       b.rows = end - first;
       b.init(base + RING * BYTES, wv, wc, cols);
-      tile_loop<DT, T>(a, b, lds, (int)(end - first), acc);
+      tile_loop<DT, T, RING>(a, b, lds, (int)(end - first), acc);
     }
     store_tile<DT, T, INDEXED ? 2 : 0>(lds, acc, to, k, rows, cols, bad);
   } else {
@@ -603,7 +613,7 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void grouped_tile_kernel(Gro
         const int t = b.row_of(wv, i);
         b.row[i] = t < cols ? (uint32_t)(t * g.ldw * 2) : ROW_DEAD;
       }
-      tile_loop<DT, T>(a, b, lds, k, acc);
+      tile_loop<DT, T, RING>(a, b, lds, k, acc);
     } else {
       a.init(base, wv, wr, n);
       a.rs = rsrc(static_cast<const char*>(g.dy) + first * g.ldy * 2,
@@ -618,58 +628,70 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 2) void grouped_tile_kernel(Gro
       b.pitch = g.ldw * 2;
       b.rows = n;
       b.init(base + RING * BYTES, wv, wc, cols);
-      tile_loop<DT, T>(a, b, lds, n, acc);
+      tile_loop<DT, T, RING>(a, b, lds, n, acc);
     }
     store_tile<DT, T, INDEXED ? 1 : 0>(lds, acc, to, width, live, cols, bad);
   }
 }
 
-// Offsets of the slots' rows in x.
-__global__ __launch_bounds__(256) void indexed_rows_kernel(const int64_t* rows, int64_t slots,
-                                                           int64_t x_rows, uint32_t pitch,
-                                                           uint32_t* offsets) {
-  const int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (j >= slots) return;
-  const uint64_t r = (uint64_t)rows[j];
-  offsets[j] = r < (uint64_t)x_rows ? (uint32_t)r * pitch : ROW_DEAD | 1;
-}
-
-template <int DT, int WHAT, int T, bool INDEXED>
+template <int DT, int WHAT, int T, int RING, bool INDEXED>
 int launch_tile(const GroupedArgs& g, char* plan, hipStream_t s, const char* what) {
   const int64_t cols = WHAT == GROUPED_LINEAR ? g.n : g.k;
-  int64_t nx = (cols + T - 1) / T, ny;
+  int64_t nx = (cols + T - 1) / T, ny, count;
   if constexpr (WHAT == GROUPED_GRAD_W) {
     nx = (nx + 3) / 4 * 4;
     ny = ((g.n + T - 1) / T + 1) / 2 * 2;
-    if (INDEXED && g.slots)
-      indexed_rows_kernel<<<(unsigned)((g.slots + 255) / 256), 256, 0, s>>>(
-          g.rows, g.slots, g.x_rows, (uint32_t)(g.ldx * 2), reinterpret_cast<uint32_t*>(plan));
-    ny *= g.experts;
+    count = nx * ny * g.experts;
   } else {
     ny = most_tiles(g, T);
+    count = (nx * ny + 7) / 8 * 8;
     if (int rc = launch_plan(g, T, reinterpret_cast<Plan*>(plan), s, what)) return rc;
   }
-  const int64_t count = (nx * ny + 7) / 8 * 8;
-  grouped_tile_kernel<DT, WHAT, T, INDEXED><<<(unsigned)count, 256, 0, s>>>(
-      g, (uint32_t)nx, (uint32_t)(ny / (WHAT == GROUPED_GRAD_W ? g.experts : 1)), plan);
+  grouped_tile_kernel<DT, WHAT, T, RING, INDEXED>
+      <<<(unsigned)count, 256, 0, s>>>(g, (uint32_t)nx, (uint32_t)ny, plan);
   return launch_status(what);
 }
 
-template <int DT, int WHAT, int T>
+template <int DT, int WHAT, int T, int RING>
 int launch_indexed(const GroupedArgs& g, char* plan, hipStream_t s, const char* what) {
   if constexpr (WHAT != GROUPED_GRAD_X) {
-    if (g.rows) return launch_tile<DT, WHAT, T, true>(g, plan, s, what);
+    if (g.rows) return launch_tile<DT, WHAT, T, RING, true>(g, plan, s, what);
   }
-  return launch_tile<DT, WHAT, T, false>(g, plan, s, what);
+  return launch_tile<DT, WHAT, T, RING, false>(g, plan, s, what);
 }
 
+// What `tiles` tiles of `stages` stages take, in us: rounds of `cap` of them, a + b for each stage,
+// and where a last round leaves half the places empty b2.
+double rounds(double tiles, double cap, double a, double stages, double b, double b2) {
+  const double whole = __builtin_floor(tiles / cap), rest = tiles - whole * cap;
+  return whole * (a + b * stages) +
+         (rest <= 0 ? 0 : a + stages * (2 * rest <= cap ? b2 : b));
+}
+
+// 256-tiles, one workgroup to a CU, read LDS half as often for a product; 128-tiles, two to a CU,
+// fill the chip with fewer results and leave less of a range's last tile empty.  Measured (us a
+// stage, at full and half chips): 0.87 for 256-tiles, 0.55 and 0.35 for 128-tiles; 8 experts of 14336
+// x 4096 in ranges of 128 slots 236 and 212 us, of 1024 819 and 1034.
 template <int DT, int WHAT>
 int launch_size(const GroupedArgs& g, char* plan, hipStream_t s, const char* what) {
-  const int64_t rows = WHAT == GROUPED_GRAD_W ? g.experts * ((g.n + 255) / 256)
-                                              : g.slots / 256 + g.experts / 2;
-  const int64_t cols = ((WHAT == GROUPED_LINEAR ? g.n : g.k) + 255) / 256;
-  if (rows * cols >= 192) return launch_indexed<DT, WHAT, 256>(g, plan, s, what);
-  return launch_indexed<DT, WHAT, 128>(g, plan, s, what);
+  if constexpr (WHAT == GROUPED_GRAD_W) {
+    const int64_t tiles = g.experts * ((g.n + 255) / 256) * ((g.k + 255) / 256);
+    if (tiles >= 192 && g.slots >= 1024 * g.experts)
+      return launch_indexed<DT, WHAT, 256, 4>(g, plan, s, what);
+    return launch_indexed<DT, WHAT, 128, 2>(g, plan, s, what);
+  } else {
+    const double cols = WHAT == GROUPED_LINEAR ? g.n : g.k;
+    const double stages = ((WHAT == GROUPED_LINEAR ? g.k : g.n) + STAGE - 1) / STAGE;
+    // a live expert's last row tile is half full on average
+    const double part = 0.5 * (g.slots < g.experts ? g.slots : g.experts);
+    auto tiles = [&](int T) {
+      return __builtin_ceil(cols / T) * ((double)g.slots / T + part);
+    };
+    if (rounds(tiles(256), 256, 5, stages, 0.87, 0.87) <
+        rounds(tiles(128), 512, 3, stages, 0.55, 0.35))
+      return launch_indexed<DT, WHAT, 256, 4>(g, plan, s, what);
+    return launch_indexed<DT, WHAT, 128, 4>(g, plan, s, what);
+  }
 }
 
 }  // namespace
@@ -680,9 +702,7 @@ int launch_plan(const GroupedArgs& g, int T, Plan* plan, hipStream_t s, const ch
 }
 
 int64_t grouped_plan_bytes(const GroupedArgs& g, int what, int dtype) {
-  // (offsets past a range's end are read, and not used)
-  if (what == GROUPED_GRAD_W) return g.rows && dtype ? align256((g.slots + 256) * 4) : 0;
-  return plan_bytes(g, dtype ? 128 : 64);
+  return what == GROUPED_GRAD_W ? 0 : plan_bytes(g, dtype ? 128 : 64);
 }
 
 int grouped_tiles(const GroupedArgs& g, int what, int dtype, char* plan, hipStream_t s,
