@@ -1,4 +1,5 @@
-"""Build ``libhi2x.so`` (the gfx950 HIP library behind the C ABI in include/hi2x.h).
+"""Build ``libhi2x.so`` (the gfx950 HIP library behind the C ABI in include/hi2x.h) and
+``_tensors.so`` (host code: the addresses of many torch tensors in one call).
 
     python -m hi2_amd.build          # or hi2_amd.build.build()
 
@@ -19,6 +20,7 @@ SOURCES = ["api.hip", "gptq.hip", "ladder.hip", "format.hip", "hessian.hip", "ch
            "refine.hip", "stats.hip", "qad.hip", "packed.hip", "packed_few.hip",
            "packed_gemm.hip", "route.hip", "adamw.hip", "gated.hip", "grouped.hip",
            "grouped_tile.hip", "grouped_f32.hip"]
+TENSORS = os.path.join(HERE, "_tensors.so")
 ARCH = "gfx950"
 
 OBJDIR = os.path.join(os.path.dirname(HERE), "_build")
@@ -49,13 +51,30 @@ def _run(cmd: list[str]) -> tuple[int, str]:
     return r.returncode, out
 
 
+def tensors_command(out: str) -> list[str]:
+    """The host compiler's command for ``csrc/tensors.cpp`` against torch's headers."""
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I" + sysconfig.get_paths()["include"], *("-I" + p for p in include_paths()),
+           os.path.join(CSRC, "tensors.cpp"), "-o", out]
+    for p in library_paths():
+        cmd += ["-L" + p, "-Wl,-rpath," + p]
+    return cmd + ["-ltorch_python", "-ltorch_cpu", "-lc10"]
+
+
 def build(verbose: bool = False, jobs: int | None = None) -> str:
     """Compile every HIP source into ``hi2_amd/libhi2x.so`` (always recompiles): one
-    object per source, compiled in parallel under ``_build/``, then one link."""
+    object per source, compiled in parallel under ``_build/``, then one link; and beside it
+    ``hi2_amd/_tensors.so``."""
     os.makedirs(OBJDIR, exist_ok=True)
     objs = [os.path.join(OBJDIR, os.path.splitext(s)[0] + ".o") for s in SOURCES]
     cmds = [[hipcc(), *FLAGS, "-c", os.path.join(CSRC, s), "-o", o]
-            for s, o in zip(SOURCES, objs)]
+            for s, o in zip(SOURCES, objs)] + [tensors_command(TENSORS + ".tmp")]
     jobs = jobs or min(len(cmds), max(1, min(os.cpu_count() or 1, 16)))
     with ThreadPoolExecutor(jobs) as pool:
         results = list(pool.map(_run, cmds))
@@ -65,7 +84,8 @@ def build(verbose: bool = False, jobs: int | None = None) -> str:
             if out.strip():
                 print(out)
         if rc != 0:
-            raise RuntimeError(f"hipcc failed ({rc}) on {cmd[-3]}:\n{out}")
+            raise RuntimeError(f"{os.path.basename(cmd[0])} failed ({rc}): {' '.join(cmd)}\n{out}")
+    os.replace(TENSORS + ".tmp", TENSORS)
     tmp = LIB + ".tmp"
     rc, out = _run([hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", *objs, "-o", tmp])
     if rc != 0:

@@ -7,8 +7,6 @@ host never waiting."""
 
 from __future__ import annotations
 
-from operator import attrgetter
-
 import numpy as np
 import torch
 
@@ -22,7 +20,16 @@ DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 _TENSOR = np.dtype([("n", "<i8"), ("start", "<i8"), ("first_chunk", "<i8"), ("group", "<i4"),
                     ("reserved", "<i4")])
-_grad, _dtype, _nbytes = attrgetter("grad"), attrgetter("dtype"), attrgetter("nbytes")
+
+
+def _tensors():
+    """The host extension; raises where it is not built."""
+    try:
+        from . import _tensors as module
+    except ImportError as e:
+        raise RuntimeError(f"hi2_amd/_tensors.so is not built or does not load ({e}): run "
+                           "`python -m hi2_amd.build`") from e
+    return module
 
 
 class _Set:
@@ -31,8 +38,8 @@ class _Set:
     def __init__(self, dtype, entries, dev):
         self.dtype = dtype
         self.params = [p for p, _, _ in entries]
-        self.dtypes = [dtype] * len(entries)
-        self.sizes = [p.nbytes for p in self.params]
+        self.sizes = np.array([p.numel() for p in self.params], dtype=np.int64)
+        self.addresses = np.zeros((2, len(entries)), dtype=np.uint64)  # written in every step
         table = np.zeros(len(entries), dtype=_TENSOR)
         chunk = 0
         for i, (p, start, group) in enumerate(entries):
@@ -141,30 +148,14 @@ class AdamW(torch.optim.Optimizer):
         at = 0
         for s in self._sets:
             n = len(s.params)
-            grads = list(map(_grad, s.params))
-            skipped = any(g is None for g in grads)
-            live = [g for g in grads if g is not None] if skipped else grads
-            # (attributes through map: tens of nanoseconds a tensor, and there may be thousands)
-            if list(map(_dtype, s.params)) != s.dtypes or list(map(_nbytes, s.params)) != s.sizes:
-                raise RuntimeError("AdamW: a parameter's type or size changed after construction")
-            if not all(map(torch.Tensor.is_contiguous, s.params)):
-                raise RuntimeError("AdamW: a parameter is no longer contiguous")
-            if not all(map(torch.Tensor.is_contiguous, live)):
-                grads = [None if g is None else g.contiguous() for g in grads]
-                live = [g for g in grads if g is not None]
-            if skipped:
-                sizes = [z for z, g in zip(s.sizes, grads) if g is not None]
-                pointers = [0 if g is None else g.data_ptr() for g in grads]
-            else:
-                sizes, pointers = s.sizes, list(map(torch.Tensor.data_ptr, grads))
-            if list(map(_nbytes, live)) != sizes or any(g.device != self.device for g in live[:1]):
-                raise RuntimeError("AdamW: a gradient has not its parameter's type and size")
-            addresses = np.array([list(map(torch.Tensor.data_ptr, s.params)), pointers],
-                                 dtype=np.uint64)
+            at_p, at_g = s.addresses[0].ctypes.data, s.addresses[1].ctypes.data
+            odd = {i: s.params[i].grad.contiguous() for i in _tensors().addresses(
+                s.params, s.sizes.ctypes.data, DTYPES[s.dtype], self.device.index, at_p, at_g)}
+            for i, g in odd.items():
+                s.addresses[1, i] = g.data_ptr()
             units = self._units
             _lib.call("hi2x_adamw_step", self.device, s.table.ctypes.data,
-                      s.device_table.data_ptr(), addresses[0].ctypes.data,
-                      addresses[1].ctypes.data, n, DTYPES[s.dtype], self.state_bits, groups,
+                      s.device_table.data_ptr(), at_p, at_g, n, DTYPES[s.dtype], self.state_bits, groups,
                       len(groups), self._m.data_ptr(), self._v.data_ptr(),
                       None if units is None else units[0].data_ptr(),
                       None if units is None else units[1].data_ptr(),

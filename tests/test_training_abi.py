@@ -5,6 +5,7 @@ import ctypes
 
 import numpy as np
 import pytest
+import torch
 
 from hi2_amd import _lib
 from hi2_amd.optim import _TENSOR
@@ -154,3 +155,18 @@ def test_adamw_conversions_refuse():
     refused("hi2x_adamw_hold", "null", FAKE, FAKE, 4, FAKE, FAKE, None, FAKE, None)
     refused("hi2x_adamw_hold", "aligned", FAKE + 4, FAKE, 4, FAKE, FAKE, FAKE, FAKE, None)
     refused("hi2x_adamw_moments", "blocks", FAKE, FAKE, FAKE, FAKE, -1, FAKE, FAKE, None)
+
+
+def test_addresses_of_tensors_are_checked():
+    from hi2_amd import _tensors
+
+    sizes, out = np.array([4], dtype=np.int64), np.zeros((2, 1), dtype=np.uint64)
+    more = sizes.ctypes.data, 0, 0, out[0].ctypes.data, out[1].ctypes.data
+    assert _tensors.addresses([], *more) == []
+    for bad in ([torch.zeros(4)], [torch.zeros(5)], [torch.zeros(4, dtype=torch.float64)], [3]):
+        with pytest.raises(RuntimeError, match="AdamW"):
+            _tensors.addresses(bad, *more)
+    with pytest.raises(TypeError):
+        _tensors.addresses((), *more)
+    with pytest.raises(ValueError, match="dtype 3"):
+        _tensors.addresses([], sizes.ctypes.data, 3, 0, 0, 0)
