@@ -19,7 +19,8 @@ LIB = os.path.join(HERE, "libhi2x.so")
 SOURCES = ["api.hip", "gptq.hip", "ladder.hip", "format.hip", "hessian.hip", "chol.hip",
            "refine.hip", "stats.hip", "qad.hip", "packed.hip", "packed_few.hip",
            "packed_gemm.hip", "route.hip", "adamw.hip", "gated.hip", "grouped.hip",
-           "grouped_tile.hip", "grouped_f32.hip"]
+           "grouped_tile.hip", "grouped_f32.hip",
+           "grouped_few.hip"]
 TENSORS = os.path.join(HERE, "_tensors.so")
 ARCH = "gfx950"
 

@@ -71,6 +71,15 @@ constexpr uint32_t GROUPED_SPAN = 0x7f000000u;
 int64_t grouped_plan_bytes(const GroupedArgs& g, int what, int dtype);
 int grouped_tiles(const GroupedArgs& g, int what, int dtype, char* plan, hipStream_t s,
                   const char* name);
+
+// The product of a few slots of 16 bits, whatever its operands' alignment, without a workspace.  Up
+// to 32 slots (8 experts of 1024 x 2048, a slot each: 7.7 us, in tiles 23.5; 64 slots of 64 of them
+// 62 us and 45), and more where the weights would have to be copied for the tiles.
+inline bool few_slots(const GroupedArgs& g, int dtype, bool w_fits) {
+  return dtype != 0 && g.experts <= 512 && g.slots <= (w_fits ? 32 : 256);
+}
+int grouped_few(const GroupedArgs& g, int dtype, hipStream_t s, const char* name);
+
 int grouped_f32(const GroupedArgs& g, int what, char* plan, hipStream_t s, const char* name);
 
 }  // namespace hi2x

@@ -151,6 +151,7 @@ int64_t pad8(int64_t n) { return (n + 7) / 8 * 8; }
 Space lay_out(const GroupedArgs& g, int what, int dtype, bool summed, bool x_fits, bool dy_fits,
               bool w_fits) {
   Space m;
+  if (what == GROUPED_LINEAR && few_slots(g, dtype, w_fits)) return m;
   auto take = [&](int64_t n) {
     const int64_t a = m.bytes;
     m.bytes += align256(n);
@@ -200,6 +201,8 @@ int run(GroupedArgs g, int what, int dtype, bool summed, void* ws, int64_t ws_by
   const int64_t ny = what == GROUPED_GRAD_W ? g.experts * ((g.n + T - 1) / T + 1)
                                             : most_tiles(g, T) + 8;
   HI2X_REQUIRE(nx * ny < (1ll << 31), "%s: too many results", name);
+  if (what == GROUPED_LINEAR && few_slots(g, dtype, lies_well(g.w, g.ldw)))
+    return grouped_few(g, dtype, s, name);
   const Space m = lay_out(g, what, dtype, summed, lies_well(g.x, g.ldx), lies_well(g.dy, g.ldy),
                           lies_well(g.w, g.ldw));
   if (int rc = take_workspace(w, ws, ws_bytes, (size_t)m.bytes, s, name)) return rc;

@@ -127,6 +127,35 @@ def test_products_and_gradients(dev, dtype, case):
     run_case(TYPES[dtype], *case)
 
 
+FEW = [
+    # (experts, n, k, counts, tokens, top_k, gather): a few slots, odd sizes, more slots of odd ones
+    (64, 128, 256, [1 if i % 8 == 3 else 0 for i in range(64)], 1, 8, True),
+    (3, 40, 2048, [0, 17, 0], 17, 1, True),
+    (2, 17, 1000, [16, 15], 31, 1, False),
+    (130, 24, 72, [1 if i > 120 else 0 for i in range(130)], 9, 1, True),
+    (4, 100, 1003, [33, 0, 100, 1], 67, 2, True),
+    (2, 999, 77, [3, 29], 8, 4, True),
+    (600, 24, 40, [1 if i % 100 == 7 else 0 for i in range(600)], 6, 1, True),
+]
+
+
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("case", FEW, ids=lambda c: f"{c[0]}x{c[1]}x{c[2]}_{c[4]}t{c[5]}")
+def test_few_slots(dev, dtype, case):
+    run_case(TYPES[dtype], *case, seed=3)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("n,k,counts", [
+    (1024, 4096, [3, 60, 5, 0]), (2048, 512, [130, 600, 2]), (512, 256, [5000, 0, 9100, 17]),
+    (257, 2050, [700, 40]), (4096, 96, [1, 300, 64, 1000]),
+])
+def test_every_tile_form(dev, dtype, n, k, counts):
+    """Shapes that take 256-tiles, 128-tiles and, for the weights' gradient, several segments of
+    rows' offsets."""
+    run_case(TYPES[dtype], len(counts), n, k, counts, sum(counts), 1, True, seed=9)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 def test_large_ragged(dev, dtype):
     counts = [1500, 0, 700, 3, 1, 890, 257, 745]

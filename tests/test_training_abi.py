@@ -89,7 +89,8 @@ def test_workspace_query_refuses():
     plain = size(0, 2, 100, 128, 4, 64, 128, 200, 1, 1, 1)
     assert plain < 1 << 20
     assert size(0, 2, 100, 128, 4, 64, 128, 200, 1, 0, 1) >= plain + 100 * 128 * 2
-    assert size(0, 2, 100, 128, 4, 64, 127, 200, 1, 1, 0) >= plain + 4 * 64 * 128 * 2
+    assert size(0, 2, 100, 128, 4, 64, 127, 300, 1, 1, 0) >= plain + 4 * 64 * 128 * 2
+    assert size(0, 2, 100, 128, 4, 64, 127, 200, 1, 1, 0) == 0  # (a few slots take them as they are)
     assert size(0, 2, 1 << 20, 1 << 12, 4, 64, 4096, 300, 1, 1, 1) >= 300 * 4096 * 2
 
 
