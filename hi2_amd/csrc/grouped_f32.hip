@@ -1,63 +1,63 @@
 // Products grouped by expert in float32: tiles of 64 x 64 on the float32 matrix unit.
 #include "grouped.h"
-#include "mfma_gemm.h"
 
 namespace hi2x {
 namespace {
 
 // A workgroup's tile of 64 x 64 results, 32 of the contraction at a time through two LDS buffers:
-// while one is multiplied the next chunk is on its way into registers.  A result is one chain of
-// FMAs.  Lanes take neighbours in memory, along the contraction or across it, one value each, so
-// rows may begin anywhere.  Offsets are 32 bits from a chunk's or a tile's first row.
-constexpr int FT = 64;
+// while one is multiplied the next two chunks are on their way into registers.  A wave has 16 rows and
+// two fragments of 16 columns, and leaves out fragments and steps in which nothing lives, so that short
+// ranges and odd sizes cost what they hold (60 experts of 520 x 1001, 3108 slots: XXX).  Lanes take
+// neighbours in memory, along the contraction or across it, one value each, so rows may begin
+// anywhere.  Offsets are 32 bits from a chunk's or a tile's first row.
+constexpr int FT = 64, KC = 32;
+constexpr int THREADS = 512, EACH = FT * KC / THREADS;  // values of an operand's chunk a thread
+constexpr int PITCH = KC + 4;  // floats of a row in LDS
+struct Buffers {
+  float a[2][FT][PITCH], b[2][FT][PITCH];
+};
 constexpr uint32_t DEAD = 0x80000000u, SPAN = GROUPED_SPAN;
 
 __device__ __forceinline__ float load_f32(__amdgpu_buffer_rsrc_t rs, uint32_t off) {
   return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, (int)off, 0, 0));
 }
 
-// Neighbours along the contraction: lane c = tid % 32 of rows tid / 32 + 8 u.
+// Neighbours along the contraction: lane c = tid % 32 of rows tid / 32 + 16 u.
 struct AlongLoader {
   __amdgpu_buffer_rsrc_t rs;
-  uint32_t row[8];
+  uint32_t row[EACH];
   int len;
-  float v[8];
-  static __device__ __forceinline__ int row_of(int u) { return (threadIdx.x >> 5) + 8 * u; }
-  __device__ __forceinline__ void load(int k0) {
+  static __device__ __forceinline__ int row_of(int u) { return (threadIdx.x >> 5) + 16 * u; }
+  __device__ __forceinline__ void load(int k0, float (&v)[EACH]) const {
     const uint32_t c = k0 + (threadIdx.x & 31);
     const uint32_t at = c < (uint32_t)len ? 4 * c : SPAN;
 #pragma unroll
-    for (int u = 0; u < 8; ++u) v[u] = load_f32(rs, row[u] + at);
+    for (int u = 0; u < EACH; ++u) v[u] = load_f32(rs, row[u] + at);
   }
-  __device__ __forceinline__ void store(float (*S)[MG_RP]) const {
-    const int c = threadIdx.x & 31;
+  static __device__ __forceinline__ void store(float (*S)[PITCH], const float (&v)[EACH]) {
 #pragma unroll
-    for (int u = 0; u < 8; ++u) S[row_of(u)][(c & 1) * MG_KP + (c >> 1)] = v[u];
+    for (int u = 0; u < EACH; ++u) S[row_of(u)][threadIdx.x & 31] = v[u];
   }
 };
 
-// Neighbours across it: lane i = tid % 64 of the contraction's rows tid / 64 + 4 u.
+// Neighbours across it: lane i = tid % 64 of the contraction's rows tid / 64 + 8 u.
 struct AcrossLoader {
   const char* base;  // of the tile's columns
   int64_t pitch;     // bytes
   int len;
   uint32_t col;      // this lane's column, dead past the last
-  float v[8];
-  static __device__ __forceinline__ int row_of(int u) { return (threadIdx.x >> 6) + 4 * u; }
-  __device__ __forceinline__ void load(int k0) {
-    const int left = len - k0 < MG_KC ? len - k0 : MG_KC;
+  static __device__ __forceinline__ int row_of(int u) { return (threadIdx.x >> 6) + 8 * u; }
+  __device__ __forceinline__ void load(int k0, float (&v)[EACH]) const {
+    const int left = len - k0 < KC ? len - k0 : KC;
     const __amdgpu_buffer_rsrc_t rs =
         rsrc(base + (int64_t)k0 * pitch, (left - 1) * pitch + FT * 4);
 #pragma unroll
-    for (int u = 0; u < 8; ++u)
+    for (int u = 0; u < EACH; ++u)
       v[u] = load_f32(rs, row_of(u) < left ? (uint32_t)(row_of(u) * pitch) + col : DEAD);
   }
-  __device__ __forceinline__ void store(float (*S)[MG_RP]) const {
+  static __device__ __forceinline__ void store(float (*S)[PITCH], const float (&v)[EACH]) {
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const int c = row_of(u);
-      S[threadIdx.x & 63][(c & 1) * MG_KP + (c >> 1)] = v[u];
-    }
+    for (int u = 0; u < EACH; ++u) S[threadIdx.x & 63][row_of(u)] = v[u];
   }
 };
 
@@ -66,15 +66,15 @@ struct IndexedLoader : AcrossLoader {
   const int64_t* index;
   __amdgpu_buffer_rsrc_t all;
   int64_t x_rows;
-  __device__ __forceinline__ void load(int k0) {
-    int64_t r[8];
+  __device__ __forceinline__ void load(int k0, float (&v)[EACH]) const {
+    int64_t r[EACH];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
+    for (int u = 0; u < EACH; ++u) {
       const int j = k0 + row_of(u);
       r[u] = index[j < len ? j : len - 1];
     }
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
+    for (int u = 0; u < EACH; ++u) {
       const bool live = k0 + row_of(u) < len, in = (uint64_t)r[u] < (uint64_t)x_rows;
       v[u] = load_f32(all, live && in ? (uint32_t)(r[u] * pitch) + col : DEAD);
       if (live && !in) v[u] = __builtin_nanf("");
@@ -82,44 +82,91 @@ struct IndexedLoader : AcrossLoader {
   }
 };
 
+// A chunk's products for F fragments of columns: all operands are read before the first product, and
+// neighbouring products are of different sums.
+template <int F>
+__device__ __forceinline__ void chunk_products(f32x4v (&acc)[2], const float* xs, const float* ys,
+                                               int left) {
+  f32x4v x[KC / 16], y[KC / 16][F];
+#pragma unroll
+  for (int h = 0; h < KC / 16; ++h) {
+    x[h] = *reinterpret_cast<const f32x4v*>(xs + 16 * h);
+#pragma unroll
+    for (int f = 0; f < F; ++f)
+      y[h][f] = *reinterpret_cast<const f32x4v*>(ys + 16 * f * PITCH + 16 * h);
+  }
+#pragma unroll
+  for (int h = 0; h < KC / 16; ++h) {
+    if (16 * h >= left) break;
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int f = 0; f < F; ++f)
+        acc[f] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[h][s], y[h][f][s], acc[f], 0, 0, 0);
+  }
+}
+
+// acc += A B^T over `len` of the contraction, for `rows` x `cols` results that live.  Of 16 values of
+// the contraction lane group q = lane / 16 has 4 q .. 4 q + 3, one to each of four steps.
 template <class A, class B>
-__device__ __forceinline__ void f32_loop(f32x16 (&acc)[1][1], MgSmemT<FT>& sm, A& a, B& b,
-                                         int len) {
+__device__ __forceinline__ void f32_loop(f32x4v (&acc)[2], Buffers& sm, A& a, B& b, int len,
+                                         int rows, int cols) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int nch = (len + MG_KC - 1) / MG_KC;
-  a.load(0);
-  b.load(0);
-  a.store(sm.A[0]);
-  b.store(sm.B[0]);
+  const int i = lane & 15, q = lane >> 4;
+  const int nch = (len + KC - 1) / KC;
+  const int wr = 16 * (wave & 3), wc = 32 * (wave >> 2);
+  const int frags = wr < rows ? (cols - wc + 15) / 16 : 0;
+  float va[2][EACH], vb[2][EACH];
+  a.load(0, va[0]);
+  b.load(0, vb[0]);
+  if (nch > 1) {
+    a.load(KC, va[1]);
+    b.load(KC, vb[1]);
+  }
+  a.store(sm.a[0], va[0]);
+  b.store(sm.b[0], vb[0]);
   __syncthreads();
-  for (int ch = 0; ch < nch; ++ch) {
-    const int buf = ch & 1;
-    const bool more = ch + 1 < nch;
-    if (more) {
-      a.load((ch + 1) * MG_KC);
-      b.load((ch + 1) * MG_KC);
+  // chunk ch in its buffer, the next in the other set of registers, the one behind it asked for
+  auto chunk = [&](int ch, int buf, float (&fa)[EACH], float (&fb)[EACH],
+                   const float (&na)[EACH], const float (&nb)[EACH]) {
+    if (ch + 2 < nch) {
+      a.load((ch + 2) * KC, fa);
+      b.load((ch + 2) * KC, fb);
     }
-    mg_chunk<1>(acc, sm.A[buf], sm.B[buf], wave >> 1, wave & 1, lane >> 5, lane & 31);
+    const int left = len - ch * KC;
+    const float* xs = &sm.a[buf][wr + i][4 * q];
+    const float* ys = &sm.b[buf][wc + i][4 * q];
+    if (frags >= 2)
+      chunk_products<2>(acc, xs, ys, left);
+    else if (frags == 1)
+      chunk_products<1>(acc, xs, ys, left);
     __builtin_amdgcn_sched_barrier(0);
-    if (more) {  // (the other buffer was last read before the barrier)
-      a.store(sm.A[buf ^ 1]);
-      b.store(sm.B[buf ^ 1]);
+    if (ch + 1 < nch) {  // (the other buffer was last read before the barrier)
+      a.store(sm.a[buf ^ 1], na);
+      b.store(sm.b[buf ^ 1], nb);
     }
     __syncthreads();
+  };
+  for (int ch = 0; ch < nch; ch += 2) {
+    chunk(ch, 0, va[0], vb[0], va[1], vb[1]);
+    if (ch + 1 < nch) chunk(ch + 1, 1, va[1], vb[1], va[0], vb[0]);
   }
 }
 
 template <int WHAT, bool INDEXED>
-__global__ __launch_bounds__(256) void grouped_f32_kernel(GroupedArgs g, uint32_t nx,
+__global__ __launch_bounds__(THREADS) void grouped_f32_kernel(GroupedArgs g, uint32_t nx,
                                                           uint32_t ny, const Plan* plan) {
-  __shared__ __attribute__((aligned(16))) MgSmemT<FT> sm;
+  __shared__ __attribute__((aligned(16))) Buffers sm;
   const int n = (int)g.n, k = (int)g.k;
   float* const out = static_cast<float*>(g.out);
-  f32x16 acc[1][1];
-  mg_zero(acc);
+  f32x4v acc[2];
+#pragma unroll
+  for (int f = 0; f < 2; ++f) acc[f] = f32x4v{0.0f, 0.0f, 0.0f, 0.0f};
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int row0 = 16 * (wave & 3) + 4 * (lane >> 4), col0 = 32 * (wave >> 2) + (lane & 15);
   int64_t to;  // of the tile's first result
   int rows, cols, width;
-  uint32_t bad = 0;  // rows of NaN, by accumulator register
+  uint32_t bad = 0;  // rows of NaN among this lane's four
   if constexpr (WHAT == GROUPED_GRAD_W) {
     const uint32_t tiles = nx * ny;
     const int e = (int)(blockIdx.x / tiles), t = (int)(blockIdx.x - e * tiles);
@@ -142,7 +189,7 @@ __global__ __launch_bounds__(256) void grouped_f32_kernel(GroupedArgs g, uint32_
         b.pitch = g.ldx * 4;
         b.len = len;
         b.col = i < cols ? 4 * i : DEAD;
-        f32_loop(acc, sm, a, b, len);
+        f32_loop(acc, sm, a, b, len, rows, cols);
       };
       if constexpr (INDEXED) {
         IndexedLoader b;
@@ -178,10 +225,10 @@ __global__ __launch_bounds__(256) void grouped_f32_kernel(GroupedArgs g, uint32_
         };
         bool in;
 #pragma unroll
-        for (int u = 0; u < 8; ++u) a.row[u] = row(a.row_of(u), in);
+        for (int u = 0; u < EACH; ++u) a.row[u] = row(a.row_of(u), in);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          row(mg_row<FT>(0, j), in);
+        for (int j = 0; j < 4; ++j) {
+          row(row0 + j, in);
           bad |= in ? 0u : 1u << j;
         }
       } else {
@@ -190,7 +237,7 @@ __global__ __launch_bounds__(256) void grouped_f32_kernel(GroupedArgs g, uint32_
                         w.first * ld * 4,
                     ((w.live - 1) * ld + a.len) * 4);
 #pragma unroll
-        for (int u = 0; u < 8; ++u)
+        for (int u = 0; u < EACH; ++u)
           a.row[u] = a.row_of(u) < w.live ? (uint32_t)(a.row_of(u) * ld * 4) : DEAD;
       }
       const char* we = static_cast<const char*>(g.w) + (int64_t)w.e * n * g.ldw * 4;
@@ -199,25 +246,27 @@ __global__ __launch_bounds__(256) void grouped_f32_kernel(GroupedArgs g, uint32_
         b.len = k;
         b.rs = rsrc(we + c0 * g.ldw * 4, ((cols - 1) * g.ldw + k) * 4);
 #pragma unroll
-        for (int u = 0; u < 8; ++u)
+        for (int u = 0; u < EACH; ++u)
           b.row[u] = b.row_of(u) < cols ? (uint32_t)(b.row_of(u) * g.ldw * 4) : DEAD;
-        f32_loop(acc, sm, a, b, k);
+        f32_loop(acc, sm, a, b, k, rows, cols);
       } else {
         AcrossLoader b;
         b.base = we + c0 * 4;
         b.pitch = g.ldw * 4;
         b.len = n;
         b.col = (int)(threadIdx.x & 63) < cols ? 4 * (threadIdx.x & 63) : DEAD;
-        f32_loop(acc, sm, a, b, n);
+        f32_loop(acc, sm, a, b, n, rows, cols);
       }
     }
   }
 #pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    const int r = mg_row<FT>(0, j), c = mg_col<FT>(0);
-    if (r < rows && c < cols)
-      out[to + (int64_t)r * width + c] = bad >> j & 1 ? __builtin_nanf("") : acc[0][0][j];
-  }
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int f = 0; f < 2; ++f) {
+      const int r = row0 + j, c = col0 + 16 * f;
+      if (r < rows && c < cols)
+        out[to + (int64_t)r * width + c] = bad >> j & 1 ? __builtin_nanf("") : acc[f][j];
+    }
 }
 
 template <int WHAT, bool INDEXED>
@@ -230,7 +279,7 @@ int launch(const GroupedArgs& g, char* plan, hipStream_t s, const char* name) {
     if (int rc = launch_plan(g, FT, p, s, name)) return rc;
   }
   grouped_f32_kernel<WHAT, INDEXED>
-      <<<(unsigned)count, 256, 0, s>>>(g, (uint32_t)nx, (uint32_t)ny, p);
+      <<<(unsigned)count, THREADS, 0, s>>>(g, (uint32_t)nx, (uint32_t)ny, p);
   return launch_status(name);
 }
 
