@@ -94,43 +94,63 @@ int sum_slots(const void* part, int64_t slots, int64_t k, const int64_t* slots_o
 
 // ---- operands that do not lie as the tiles take them -------------------------------------------
 // Rows of `cols` 16-bit or 32-bit values copied to rows at multiples of 16 bytes, zeros behind them;
-// with `index` the rows that it names (one outside: NaN).  A thread writes 16 bytes.
+// with `index` the rows that it names (one outside: NaN), with `offs` those of experts that have
+// slots, `per` rows each.  A thread writes 16 bytes, which it reads as words of 4: of 16-bit rows
+// that begin between two words five of them, shifted.  (The fifth ends no further than the word
+// that the row's last value is in.)
+typedef uint32_t u32x4w __attribute__((ext_vector_type(4), aligned(4)));
 template <class W>
 __global__ __launch_bounds__(256) void copy_rows_kernel(const W* from, int64_t ld, int64_t rows,
                                                         int64_t cols, const int64_t* index,
-                                                        int64_t from_rows, W nan, W* to,
-                                                        int64_t ld_to, Spread by) {
+                                                        int64_t from_rows, const int64_t* offs,
+                                                        int64_t per, W nan, W* to, int64_t ld_to,
+                                                        Spread by) {
   constexpr int V = 16 / sizeof(W);
   int64_t row, c;
   spread_at(by, row, c);
   c *= V;
   if (row >= rows || c >= ld_to) return;
+  if (offs) {
+    const int64_t e = row / per;
+    if (offs[e + 1] <= offs[e]) return;
+  }
   const int64_t r = index ? index[row] : row;
   const bool in = (uint64_t)r < (uint64_t)from_rows;
+  const W* const at = from + r * ld + c;
   union {
     W v[V];
     u32x4 w;
   };
+  if (in && c + V <= cols) {
+    const uint32_t odd = sizeof(W) == 2 ? (uint32_t)((uintptr_t)at & 2) : 0;
+    const char* base = reinterpret_cast<const char*>(at) - odd;
+    w = *reinterpret_cast<const u32x4w*>(base);
+    if (odd) {
+      const uint32_t last = *reinterpret_cast<const uint32_t*>(base + 16);
 #pragma unroll
-  for (int i = 0; i < V; ++i)
-    v[i] = c + i < cols ? (in ? from[r * ld + c + i] : nan) : (W)0;
+      for (int i = 0; i < 4; ++i) w[i] = w[i] >> 16 | (i < 3 ? w[i + 1] : last) << 16;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = c + i < cols ? (in ? at[i] : nan) : (W)0;
+  }
   *reinterpret_cast<u32x4*>(to + row * ld_to + c) = w;
 }
 
 int copy_rows(const void* from, int64_t ld, int64_t rows, int64_t cols, const int64_t* index,
-              int64_t from_rows, int dtype, void* to, int64_t ld_to, hipStream_t s,
-              const char* what) {
+              int64_t from_rows, const int64_t* offs, int64_t per, int dtype, void* to,
+              int64_t ld_to, hipStream_t s, const char* what) {
   Spread by;
   const int64_t count = spread(rows, ld_to / (dtype == 0 ? 4 : 8), by);
   HI2X_REQUIRE(count < (1ll << 31), "%s: too many elements", what);
   if (count == 0) return HI2X_OK;
   if (dtype == 0)
     copy_rows_kernel<uint32_t><<<(unsigned)count, 256, 0, s>>>(
-        static_cast<const uint32_t*>(from), ld, rows, cols, index, from_rows, 0x7fc00000u,
-        static_cast<uint32_t*>(to), ld_to, by);
+        static_cast<const uint32_t*>(from), ld, rows, cols, index, from_rows, offs, per,
+        0x7fc00000u, static_cast<uint32_t*>(to), ld_to, by);
   else
     copy_rows_kernel<uint16_t><<<(unsigned)count, 256, 0, s>>>(
-        static_cast<const uint16_t*>(from), ld, rows, cols, index, from_rows,
+        static_cast<const uint16_t*>(from), ld, rows, cols, index, from_rows, offs, per,
         (uint16_t)(dtype == 1 ? 0x7e00 : 0x7fc0), static_cast<uint16_t*>(to), ld_to, by);
   return launch_status(what);
 }
@@ -209,22 +229,23 @@ int run(GroupedArgs g, int what, int dtype, bool summed, void* ws, int64_t ws_by
   if (summed) g.out = *part = w.p + m.part;
   if (m.has_x) {
     if (int rc = copy_rows(g.x, g.ldx, m.gather ? g.slots : g.x_rows, g.k,
-                           m.gather ? g.rows : nullptr, g.x_rows, dtype, w.p + m.x, m.ldx, s, name))
+                           m.gather ? g.rows : nullptr, g.x_rows, nullptr, 0, dtype, w.p + m.x,
+                           m.ldx, s, name))
       return rc;
     g.x = w.p + m.x;
     g.ldx = m.ldx;
     if (m.gather) g.rows = nullptr, g.x_rows = g.slots;
   }
   if (m.has_dy) {
-    if (int rc = copy_rows(g.dy, g.ldy, g.slots, g.n, nullptr, g.slots, dtype, w.p + m.dy, m.ldy,
-                           s, name))
+    if (int rc = copy_rows(g.dy, g.ldy, g.slots, g.n, nullptr, g.slots, nullptr, 0, dtype,
+                           w.p + m.dy, m.ldy, s, name))
       return rc;
     g.dy = w.p + m.dy;
     g.ldy = m.ldy;
   }
   if (m.has_w) {
-    if (int rc = copy_rows(g.w, g.ldw, g.experts * g.n, g.k, nullptr, g.experts * g.n, dtype,
-                           w.p + m.w, m.ldw, s, name))
+    if (int rc = copy_rows(g.w, g.ldw, g.experts * g.n, g.k, nullptr, g.experts * g.n, g.offs, g.n,
+                           dtype, w.p + m.w, m.ldw, s, name))
       return rc;
     g.w = w.p + m.w;
     g.ldw = m.ldw;
