@@ -35,7 +35,9 @@ struct Plan {
 };
 
 // Row tiles of T slots at most: every range's last may be partial.
-inline int64_t most_tiles(const GroupedArgs& g, int T) { return g.slots / T + g.experts + 2; }
+inline int64_t most_tiles(const GroupedArgs& g, int T) {
+  return g.slots / T + (g.slots < g.experts ? g.slots : g.experts) + 2;
+}
 inline int64_t plan_bytes(const GroupedArgs& g, int T) {
   return align256(sizeof(Plan) + most_tiles(g, T) * sizeof(RowTile));
 }
@@ -44,12 +46,12 @@ inline int64_t plan_bytes(const GroupedArgs& g, int T) {
 // before the first.
 int launch_plan(const GroupedArgs& g, int T, Plan* plan, hipStream_t s, const char* name);
 
-// The tile of a plan's row tiles x nx columns that workgroup `block` of 8 ceil(tiles / 8) takes.
+// The tile of a plan's row tiles (y) x nx columns (xt) that workgroup `block` of 8 ceil(tiles / 8) takes.
 // Workgroups go to the eight XCDs in turn, and each XCD takes an eighth of the tiles, which are in
 // order of four row tiles at a time, column tile after column tile, so that rows and weights come to
 // its L2 once.
 __device__ __forceinline__ bool plan_tile(const Plan* p, uint32_t nx, uint32_t block, RowTile& w,
-                                          uint32_t& xt) {
+                                          uint32_t& xt, uint32_t& y) {
   const uint32_t count = (uint32_t)p->count, all = count * nx, per = (all + 7) / 8;
   const uint32_t j = block >> 3, at = (block & 7) * per + j;
   if (j >= per || at >= all) return false;
@@ -58,7 +60,8 @@ __device__ __forceinline__ bool plan_tile(const Plan* p, uint32_t nx, uint32_t b
   const uint32_t rest = at - band * (4 * nx);
   const uint32_t deep = count - 4 * band < 4 ? count - 4 * band : 4;
   xt = __builtin_amdgcn_readfirstlane(rest / deep);
-  w = p->tile[4 * band + rest - xt * deep];
+  y = 4 * band + rest - xt * deep;
+  w = p->tile[y];
   return true;
 }
 

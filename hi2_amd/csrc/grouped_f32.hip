@@ -206,8 +206,8 @@ __global__ __launch_bounds__(THREADS) void grouped_f32_kernel(GroupedArgs g, uin
     }
   } else {
     RowTile w;
-    uint32_t xt;
-    if (!plan_tile(plan, nx, blockIdx.x, w, xt)) return;
+    uint32_t xt, y;
+    if (!plan_tile(plan, nx, blockIdx.x, w, xt, y)) return;
     width = WHAT == GROUPED_LINEAR ? n : k;
     const int c0 = (int)xt * FT;
     rows = w.live;

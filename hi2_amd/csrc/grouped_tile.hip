@@ -79,14 +79,14 @@ struct AlongOperand {
   static constexpr int NC = T / 64;  // a wave's loads of a stage, 16 rows each
   __amdgpu_buffer_rsrc_t rs;
   uint32_t row[NC];  // this lane's rows' offsets
-  uint32_t piece;    // its piece's
-  int len;           // of the contraction
+  uint32_t piece;    // its piece's, behind `from`
+  int len;           // end of the contraction
   uint32_t at;       // LDS byte of the wave's first load
   uint32_t read0, read1;
-  __device__ __forceinline__ void init(uint32_t lds, int wv, int half, int len_) {
+  __device__ __forceinline__ void init(uint32_t lds, int wv, int half, int from, int end) {
     const int lane = threadIdx.x & 63;
-    len = len_;
-    piece = 8 * ((lane & 3) ^ ((lane >> 4) & 3));
+    len = end;
+    piece = from + 8 * ((lane & 3) ^ ((lane >> 4) & 3));
     at = lds + NC * wv * 1024;
     const uint32_t r = half * (T / 2) + (lane & 31);
     const int h = lane >> 5, x = (lane >> 2) & 3;
@@ -433,7 +433,7 @@ __global__ __launch_bounds__(1024) void grouped_plan_kernel(GroupedArgs g, int T
       b = e == experts ? g.slots : clamp(g.offs[0]);
     }
   };
-  int before = 0;
+  int64_t before = 0;  // (ranges that overlap, as they should not, can make very many)
   for (int e0 = 0; e0 < ranges; e0 += 1024) {
     const int e = e0 + tid;
     int64_t a = 0, b = 0;
@@ -447,19 +447,19 @@ __global__ __launch_bounds__(1024) void grouped_plan_kernel(GroupedArgs g, int T
     }
     if (lane == 63) sums[wave] = inc;
     __syncthreads();
-    int base = before, all = 0;
+    int64_t base = before, all = 0;
     for (int w = 0; w < 16; ++w) {
       if (w < wave) base += sums[w];
       all += sums[w];
     }
-    if (e < ranges) first_tile[e] = base + inc - n;
+    base += inc - n;
+    if (e < ranges) first_tile[e] = base < most ? (int)base : (int)most;
     before += all;
     __syncthreads();
   }
-  // (ranges that overlap, as they should not, could make more tiles than there is room for)
-  const int count = before < most ? before : (int)most;
+  const int count = (int)(before < most ? before : most);
   if (tid == 0) {
-    first_tile[ranges] = before;
+    first_tile[ranges] = count;
     plan->count = count;
   }
   __syncthreads();
@@ -479,11 +479,27 @@ __global__ __launch_bounds__(1024) void grouped_plan_kernel(GroupedArgs g, int T
   }
 }
 
-template <int DT, int WHAT, int T, int RING, bool INDEXED>
-__global__ __launch_bounds__(256, T == 256 ? 1 : 8 / RING) void grouped_tile_kernel(GroupedArgs g,
-                                                                              uint32_t nx,
-                                                                              uint32_t ny,
-                                                                              const void* plan) {
+// A tile's sums (+ add) to `part`, a tile after a tile, as the accumulators hold them.
+template <int T>
+__device__ __forceinline__ void store_part(float* part, uint64_t tile,
+                                           const f32x16v (&acc)[T / 64][T / 64], float add) {
+  f32x4v* to = reinterpret_cast<f32x4v*>(part) + tile * (T * T / 4) + (threadIdx.x >> 6) * (T * T / 16) +
+               (threadIdx.x & 63);
+#pragma unroll
+  for (int i = 0; i < T / 64; ++i)
+#pragma unroll
+    for (int j = 0; j < T / 64; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q, to += 64)
+        *to = f32x4v{acc[i][j][4 * q] + add, acc[i][j][4 * q + 1] + add,
+                     acc[i][j][4 * q + 2] + add, acc[i][j][4 * q + 3] + add};
+}
+
+// SPLIT: a tile's contraction is cut into `splits` ranges, of `per` stages (of the
+// weights' gradient: of as many as its expert's slots need), and grouped_join_kernel adds their sums.
+template <int DT, int WHAT, int T, int RING, bool INDEXED, bool SPLIT>
+__global__ __launch_bounds__(256, T == 256 ? 1 : 8 / RING) void grouped_tile_kernel(
+    GroupedArgs g, uint32_t nx, uint32_t ny, const void* plan, float* part, int splits, int per) {
   constexpr int NA = T / 64, BYTES = T * 64;
   __shared__ __attribute__((aligned(1024))) char lds[LDS_BYTES<T, RING>];
   __shared__ uint8_t bad[T];
@@ -506,10 +522,11 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 8 / RING) void grouped_tile_ker
   if constexpr (WHAT == GROUPED_GRAD_W) {
     // An expert's tiles over all XCDs, 2 x 4 of them at a time, one to each.
     const uint32_t xcd = blockIdx.x & 7, j = blockIdx.x >> 3;
-    const uint32_t hx = nx / 4, per = hx * (ny / 2);  // (nx, ny: rounded up to whole rounds)
+    const uint32_t hx = nx / 4, tiles = hx * (ny / 2);  // (nx, ny: rounded up to whole rounds)
     // (what comes out of a division is in a vector register, and would keep what follows there)
-    const int e = __builtin_amdgcn_readfirstlane(j / per);
-    const uint32_t sub = j - e * per, my = (xcd + e) & 7;
+    const uint32_t ez = __builtin_amdgcn_readfirstlane(j / tiles);
+    const int e = SPLIT ? __builtin_amdgcn_readfirstlane(ez / splits) : ez;
+    const uint32_t sub = j - ez * tiles, my = (xcd + ez) & 7;
     const uint32_t sy = __builtin_amdgcn_readfirstlane(sub / hx), sx = sub - sy * hx;
     const int64_t r0 = (int64_t)(sy * 2 + (my >> 2)) * T;
     const int64_t c0 = (int64_t)(sx * 4 + (my & 3)) * T;
@@ -520,9 +537,18 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 8 / RING) void grouped_tile_ker
     end = uniform(end);
     const int rows = (int)(n - r0 < T ? n - r0 : T), cols = (int)(k - c0 < T ? k - c0 : T);
     uint16_t* const to = out + ((int64_t)e * n + r0) * k + c0;
+    const uint32_t z = SPLIT ? ez - e * splits : 0;
     if (first == end) {
-      store_zeros<T>(to, k, rows, cols);
+      if (z == 0) store_zeros<T>(to, k, rows, cols);
       return;
+    }
+    if (SPLIT) {  // a range of whole stages, which may hold nothing
+      const uint32_t len = (uint32_t)(end - first);
+      const int64_t by = __builtin_amdgcn_readfirstlane((len + splits - 1) / splits + STAGE - 1) &
+                         ~(STAGE - 1);
+      const int64_t at = first + z * by;
+      first = at < end ? at : end;
+      end = at + by < end ? at + by : end;
     }
     AcrossOperand<T> a;
     a.base = static_cast<const char*>(g.dy) + (first * g.ldy + r0) * 2;
@@ -565,13 +591,22 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 8 / RING) void grouped_tile_ker
       b.pitch = g.ldx * 2;
       b.rows = end - first;
       b.init(base + RING * BYTES, wv, wc, cols);
-      tile_loop<DT, T, RING>(a, b, lds, (int)(end - first), acc);
+      if (!SPLIT || first < end) tile_loop<DT, T, RING>(a, b, lds, (int)(end - first), acc);
     }
-    store_tile<DT, T, INDEXED ? 2 : 0>(lds, acc, to, k, rows, cols, bad);
+    if constexpr (SPLIT) {
+      // (all of the tile is NaN then, by any of its ranges)
+      const float add = INDEXED && first < end && bad[0] ? __builtin_nanf("") : 0.0f;
+      const uint32_t y = e * ((n + T - 1) / T) + (uint32_t)(r0 / T), across = (k + T - 1) / T;
+      store_part<T>(part, ((uint64_t)y * across + c0 / T) * splits + z, acc, add);
+    } else {
+      store_tile<DT, T, INDEXED ? 2 : 0>(lds, acc, to, k, rows, cols, bad);
+    }
   } else {
     RowTile w;
-    uint32_t xt;
-    if (!plan_tile(static_cast<const Plan*>(plan), nx, blockIdx.x, w, xt)) return;
+    uint32_t xt, y;
+    if (!plan_tile(static_cast<const Plan*>(plan), nx * splits, blockIdx.x, w, xt, y)) return;
+    const uint32_t z = SPLIT ? xt % splits : 0;
+    if (SPLIT) xt = __builtin_amdgcn_readfirstlane(xt / splits);
     const int e = __builtin_amdgcn_readfirstlane(w.e);
     const int live = __builtin_amdgcn_readfirstlane(w.live);
     const int64_t first = uniform(w.first);
@@ -579,12 +614,15 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 8 / RING) void grouped_tile_ker
     const int cols = (int)(width - c0 < T ? width - c0 : T);
     uint16_t* const to = out + first * width + c0;
     if (e < 0) {
-      store_zeros<T>(to, width, live, cols);
+      if (z == 0) store_zeros<T>(to, width, live, cols);
       return;
     }
+    const int all = WHAT == GROUPED_LINEAR ? k : n;  // of the contraction
+    const int from = SPLIT ? __builtin_amdgcn_readfirstlane(z * per * STAGE) : 0;
+    const int end = SPLIT && from + per * STAGE < all ? from + per * STAGE : all;
     AlongOperand<T> a;
     if constexpr (WHAT == GROUPED_LINEAR) {
-      a.init(base, wv, wr, k);
+      a.init(base, wv, wr, from, end);
       if constexpr (INDEXED) {
         a.rs = rsrc(g.x, g.x_rows > 0 ? ((g.x_rows - 1) * g.ldx + whole(k)) * 2 : 0);
 #pragma unroll
@@ -605,7 +643,7 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 8 / RING) void grouped_tile_ker
         }
       }
       AlongOperand<T> b;
-      b.init(base + RING * BYTES, wv, wc, k);
+      b.init(base + RING * BYTES, wv, wc, from, end);
       b.rs = rsrc(static_cast<const char*>(g.w) + ((int64_t)e * n + c0) * g.ldw * 2,
                   ((int64_t)(cols - 1) * g.ldw + whole(k)) * 2);
 #pragma unroll
@@ -613,9 +651,9 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 8 / RING) void grouped_tile_ker
         const int t = b.row_of(wv, i);
         b.row[i] = t < cols ? (uint32_t)(t * g.ldw * 2) : ROW_DEAD;
       }
-      tile_loop<DT, T, RING>(a, b, lds, k, acc);
+      tile_loop<DT, T, RING>(a, b, lds, end - from, acc);
     } else {
-      a.init(base, wv, wr, n);
+      a.init(base, wv, wr, from, end);
       a.rs = rsrc(static_cast<const char*>(g.dy) + first * g.ldy * 2,
                   ((int64_t)(live - 1) * g.ldy + whole(n)) * 2);
 #pragma unroll
@@ -624,40 +662,109 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 8 / RING) void grouped_tile_ker
         a.row[i] = t < live ? (uint32_t)(t * g.ldy * 2) : ROW_DEAD;
       }
       AcrossOperand<T> b;
-      b.base = static_cast<const char*>(g.w) + ((int64_t)e * n * g.ldw + c0) * 2;
+      b.base = static_cast<const char*>(g.w) + (((int64_t)e * n + from) * g.ldw + c0) * 2;
       b.pitch = g.ldw * 2;
-      b.rows = n;
+      b.rows = end - from;
       b.init(base + RING * BYTES, wv, wc, cols);
-      tile_loop<DT, T, RING>(a, b, lds, n, acc);
+      tile_loop<DT, T, RING>(a, b, lds, end - from, acc);
     }
-    store_tile<DT, T, INDEXED ? 1 : 0>(lds, acc, to, width, live, cols, bad);
+    if constexpr (SPLIT)
+      store_part<T>(part, ((uint64_t)y * nx + xt) * splits + z, acc, 0.0f);
+    else
+      store_tile<DT, T, INDEXED ? 1 : 0>(lds, acc, to, width, live, cols, bad);
   }
 }
 
+// The sums of a tile's ranges, added in their order; a workgroup to the quarter that one wave of the
+// product held, a wave to 32 x 32 of its results.
+template <int DT, int WHAT, bool INDEXED>
+__global__ __launch_bounds__(256) void grouped_join_kernel(GroupedArgs g, int width, uint32_t nx,
+                                                           uint32_t ny, const Plan* plan,
+                                                           const float* part, int splits) {
+  constexpr int T = 128;
+  const uint32_t tile = blockIdx.x / 4, quarter = blockIdx.x & 3, y = tile / nx, xt = tile - y * nx;
+  RowTile w;
+  if constexpr (WHAT == GROUPED_GRAD_W) {
+    const int e = y / ny, r0 = (y - e * ny) * T;
+    int64_t first, end;
+    slot_range(g, e, first, end);
+    if (first == end) return;
+    w = RowTile{e * g.n + r0, (int32_t)(g.n - r0), e};
+  } else {
+    if (y >= (uint32_t)plan->count) return;
+    w = plan->tile[y];
+    if (w.e < 0) return;
+  }
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const f32x4v* from = reinterpret_cast<const f32x4v*>(part) + (int64_t)tile * splits * (T * T / 4) +
+                       quarter * (T * T / 16) + wave * 256 + lane;
+  f32x4v sum[4] = {};
+  for (int z = 0; z < splits; ++z)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) sum[q] += from[(int64_t)z * (T * T / 4) + q * 64];
+  const int r = (quarter >> 1) * 64 + (wave >> 1) * 32 + (lane & 31);
+  if (r >= w.live) return;
+  if constexpr (INDEXED && WHAT == GROUPED_LINEAR) {
+    if ((uint64_t)g.rows[w.first + r] >= (uint64_t)g.x_rows)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) sum[q] = sum[q] + __builtin_nanf("");
+  }
+  uint16_t* const to = static_cast<uint16_t*>(g.out) + (w.first + r) * width;
+  const int c0 = (int)xt * T + (quarter & 1) * 64 + (wave & 1) * 32 + 4 * (lane >> 5);
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int c = c0 + 8 * q + u;
+      if (c < width) store_from_f32(to, c, DT, sum[q][u]);
+    }
+}
+
+// How a product goes: in tiles of T, its contraction cut into `splits` ranges of `per` stages.
+struct Cut {
+  int T, splits, per;
+};
+
 template <int DT, int WHAT, int T, int RING, bool INDEXED>
-int launch_tile(const GroupedArgs& g, char* plan, hipStream_t s, const char* what) {
+int launch_tile(const GroupedArgs& g, const Cut& cut, char* plan, hipStream_t s,
+                const char* what) {
   const int64_t cols = WHAT == GROUPED_LINEAR ? g.n : g.k;
-  int64_t nx = (cols + T - 1) / T, ny, count;
+  int64_t nx = (cols + T - 1) / T, ny = (g.n + T - 1) / T, count;
+  const int64_t tiles = nx * (WHAT == GROUPED_GRAD_W ? ny * g.experts : most_tiles(g, T));
+  const uint32_t across = (uint32_t)nx, down = (uint32_t)ny;
   if constexpr (WHAT == GROUPED_GRAD_W) {
     nx = (nx + 3) / 4 * 4;
-    ny = ((g.n + T - 1) / T + 1) / 2 * 2;
-    count = nx * ny * g.experts;
+    ny = (ny + 1) / 2 * 2;
+    count = nx * ny * g.experts * cut.splits;
   } else {
     ny = most_tiles(g, T);
-    count = (nx * ny + 7) / 8 * 8;
+    count = (nx * cut.splits * ny + 7) / 8 * 8;
     if (int rc = launch_plan(g, T, reinterpret_cast<Plan*>(plan), s, what)) return rc;
   }
-  grouped_tile_kernel<DT, WHAT, T, RING, INDEXED>
-      <<<(unsigned)count, 256, 0, s>>>(g, (uint32_t)nx, (uint32_t)ny, plan);
+  if constexpr (T == 128) {
+    if (cut.splits > 1) {
+      const Plan* p = reinterpret_cast<const Plan*>(plan);
+      float* part = reinterpret_cast<float*>(
+          plan + (WHAT == GROUPED_GRAD_W ? 0 : plan_bytes(g, T)));
+      grouped_tile_kernel<DT, WHAT, T, RING, INDEXED, true><<<(unsigned)count, 256, 0, s>>>(
+          g, (uint32_t)nx, (uint32_t)ny, p, part, cut.splits, cut.per);
+      grouped_join_kernel<DT, WHAT, INDEXED><<<(unsigned)(tiles * 4), 256, 0, s>>>(
+          g, (int)cols, across, down, p, part, cut.splits);
+      return launch_status(what);
+    }
+  }
+  grouped_tile_kernel<DT, WHAT, T, RING, INDEXED, false>
+      <<<(unsigned)count, 256, 0, s>>>(g, (uint32_t)nx, (uint32_t)ny, plan, nullptr, 1, 0);
   return launch_status(what);
 }
 
 template <int DT, int WHAT, int T, int RING>
-int launch_indexed(const GroupedArgs& g, char* plan, hipStream_t s, const char* what) {
+int launch_indexed(const GroupedArgs& g, const Cut& cut, char* plan, hipStream_t s,
+                   const char* what) {
   if constexpr (WHAT != GROUPED_GRAD_X) {
-    if (g.rows) return launch_tile<DT, WHAT, T, RING, true>(g, plan, s, what);
+    if (g.rows) return launch_tile<DT, WHAT, T, RING, true>(g, cut, plan, s, what);
   }
-  return launch_tile<DT, WHAT, T, RING, false>(g, plan, s, what);
+  return launch_tile<DT, WHAT, T, RING, false>(g, cut, plan, s, what);
 }
 
 // What `tiles` tiles of `stages` stages take, in us: rounds of `cap` of them, a + b for each stage,
@@ -671,27 +778,52 @@ double rounds(double tiles, double cap, double a, double stages, double b, doubl
 // 256-tiles, one workgroup to a CU, read LDS half as often for a product; 128-tiles, two to a CU,
 // fill the chip with fewer results and leave less of a range's last tile empty.  Measured (us a
 // stage, at full and half chips): 0.87 for 256-tiles, 0.55 and 0.35 for 128-tiles; 8 experts of 14336
-// x 4096 in ranges of 128 slots 236 and 212 us, of 1024 819 and 1034.
+// x 4096 in ranges of 128 slots 236 and 212 us, of 1024 819 and 1034.  The weights' gradient takes
+// 0.75 a stage in 256-tiles, and in 128-tiles of a two-stage ring, four to a CU, hides the stores of
+// short sums behind others: ranges of 64 slots 72 us and 62, of 512 585 and 619.
+// Tiles that leave half the chip empty split their contraction where that saves more than the join
+// costs, 4 us and 0.025 for each range that a tile is cut into: 512 slots of 8 experts of 1024 x 4096
+// 44 us and 27, 300 of one of 1024 x 14336 133 and 33; 256 of 8 of 2048 x 1024 17 and, split, 22; the
+// gradient of 8 of 512 x 512 from 65536 slots 121 and 71, of one of 1024 x 1024 from 131072 2560 and
+// 373.
+Cut cut_of(const GroupedArgs& g, int what) {
+  const bool grad_w = what == GROUPED_GRAD_W;
+  const double cols = what == GROUPED_LINEAR ? g.n : g.k;
+  const int stages = (int)(((what == GROUPED_LINEAR ? g.k : grad_w ? g.slots / g.experts : g.n) +
+                            STAGE - 1) / STAGE);
+  // a live expert's last row tile is half full on average
+  const double live = g.slots < g.experts ? g.slots : g.experts;
+  auto tiles = [&](int T) {
+    const double rows = (double)g.slots / T + 0.5 * live;
+    return __builtin_ceil(cols / T) * (grad_w        ? g.experts * __builtin_ceil((double)g.n / T)
+                                       : rows > live ? rows
+                                                     : live);
+  };
+  if (grad_w ? tiles(256) >= 192 && g.slots >= 384 * g.experts
+             : rounds(tiles(256), 256, 5, stages, 0.87, 0.87) <
+                   rounds(tiles(128), 512, 3, stages, 0.55, 0.35))
+    return Cut{256, 1, 0};
+  Cut c{128, 1, stages};
+  const double all = tiles(128);
+  double best = stages * 0.35;
+  for (int splits = 2; splits <= 16 && all >= 1 && all * splits <= 512; ++splits) {
+    int per = (stages + splits - 1) / splits;
+    per += per & 1;  // (whole lines of 128 bytes)
+    const double us = per * (all * splits > 256 ? 0.55 : 0.35) + 4 + 0.025 * all * splits;
+    if (us < best) {
+      best = us;
+      c.per = per;
+      c.splits = (stages + per - 1) / per;
+    }
+  }
+  return c;
+}
+
 template <int DT, int WHAT>
 int launch_size(const GroupedArgs& g, char* plan, hipStream_t s, const char* what) {
-  if constexpr (WHAT == GROUPED_GRAD_W) {
-    const int64_t tiles = g.experts * ((g.n + 255) / 256) * ((g.k + 255) / 256);
-    if (tiles >= 192 && g.slots >= 1024 * g.experts)
-      return launch_indexed<DT, WHAT, 256, 4>(g, plan, s, what);
-    return launch_indexed<DT, WHAT, 128, 2>(g, plan, s, what);
-  } else {
-    const double cols = WHAT == GROUPED_LINEAR ? g.n : g.k;
-    const double stages = ((WHAT == GROUPED_LINEAR ? g.k : g.n) + STAGE - 1) / STAGE;
-    // a live expert's last row tile is half full on average
-    const double part = 0.5 * (g.slots < g.experts ? g.slots : g.experts);
-    auto tiles = [&](int T) {
-      return __builtin_ceil(cols / T) * ((double)g.slots / T + part);
-    };
-    if (rounds(tiles(256), 256, 5, stages, 0.87, 0.87) <
-        rounds(tiles(128), 512, 3, stages, 0.55, 0.35))
-      return launch_indexed<DT, WHAT, 256, 4>(g, plan, s, what);
-    return launch_indexed<DT, WHAT, 128, 4>(g, plan, s, what);
-  }
+  const Cut cut = cut_of(g, WHAT);
+  if (cut.T == 256) return launch_indexed<DT, WHAT, 256, 4>(g, cut, plan, s, what);
+  return launch_indexed<DT, WHAT, 128, WHAT == GROUPED_GRAD_W ? 2 : 4>(g, cut, plan, s, what);
 }
 
 }  // namespace
@@ -702,7 +834,13 @@ int launch_plan(const GroupedArgs& g, int T, Plan* plan, hipStream_t s, const ch
 }
 
 int64_t grouped_plan_bytes(const GroupedArgs& g, int what, int dtype) {
-  return what == GROUPED_GRAD_W ? 0 : plan_bytes(g, dtype ? 128 : 64);
+  const bool grad_w = what == GROUPED_GRAD_W;
+  if (dtype == 0) return grad_w ? 0 : plan_bytes(g, 64);
+  const Cut cut = cut_of(g, what);
+  const int64_t nx = ((what == GROUPED_LINEAR ? g.n : g.k) + cut.T - 1) / cut.T;
+  const int64_t tiles = nx * (grad_w ? g.experts * ((g.n + cut.T - 1) / cut.T) : most_tiles(g, cut.T));
+  return (grad_w ? 0 : plan_bytes(g, cut.T)) +
+         (cut.splits > 1 ? tiles * cut.splits * cut.T * cut.T * 4 : 0);
 }
 
 int grouped_tiles(const GroupedArgs& g, int what, int dtype, char* plan, hipStream_t s,

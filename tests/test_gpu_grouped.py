@@ -162,6 +162,75 @@ def test_large_ragged(dev, dtype):
     run_case(TYPES[dtype], 8, 768, 1024, counts, sum(counts) // 4, 4, True, seed=5)
 
 
+LONG = [
+    # (experts, n, k, counts, tokens, top_k, gather): few tiles, a long contraction of the product,
+    # of the input's gradient or of the weights'
+    (1, 256, 8192, [100], 50, 2, True),
+    (3, 136, 5000, [130, 0, 1], 131, 1, True),
+    (4, 130, 4100, [64, 1, 0, 63], 128, 1, False),
+    (2, 9000, 200, [33, 97], 65, 2, True),
+    (4, 128, 264, [9000, 0, 33, 3167], 6100, 2, True),
+    (2, 70, 130, [7001, 8], 7009, 1, False),
+]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("case", LONG, ids=lambda c: f"{c[0]}x{c[1]}x{c[2]}_{c[4]}t{c[5]}")
+def test_long_contractions_of_few_tiles(dev, dtype, case):
+    run_case(TYPES[dtype], *case, seed=13)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_long_contractions_with_gaps_and_bad_rows(dev, dtype):
+    """Slots of no expert, rows outside and experts without slots where contractions are split, and
+    the same bits each time."""
+    t = TYPES[dtype]
+    n, k = 160, 4096
+    offs = torch.tensor([7, 47, 47, 6047, 6048]).cuda()
+    g = torch.Generator().manual_seed(2)
+    rows = torch.randint(0, 500, (6100,), generator=g).cuda()
+    x, w = values((500, k), t, 1, 0.1), values((4, n, k), t, 2, 0.1)
+    dy = values((6100, n), t, 3, 0.1)
+    dy[:7] = float("nan")
+    dy[6048:] = float("inf")
+    rows[:7] = -5
+    few = torch.tensor([7, 27, 27, 126, 127]).cuda()
+    for at, slots in ((offs, 6100), (few, 140)):
+        for bad in (None, 20):
+            r = rows[:slots].clone()
+            if bad is not None:
+                r[bad] = 500
+            wr = w.clone().requires_grad_(True)
+            y = grouped_linear(x, wr, at, r)
+            dw, = torch.autograd.grad(y, wr, dy[:slots])
+            o = at.tolist()
+            assert not y[:o[0]].any() and not y[o[-1]:].any() and not dw[1].any()
+            nan = torch.isnan(y).any(1)
+            assert nan.nonzero().flatten().tolist() == ([] if bad is None else [bad])
+            assert bool(torch.isnan(dw[0]).all()) == (bad is not None)
+            assert torch.isfinite(dw[2:]).all()
+            keep = ~nan
+            # (the oracle without the slots that no expert has)
+            inner, d = r.clamp(0, 499)[o[0]:o[-1]], dy[o[0]:o[-1]]
+            y0, ym, _, _, dw0, dwm = oracle(x, w, at - o[0], inner, None, d)
+            pick = keep[o[0]:o[-1]]
+            check(y[o[0]:o[-1]][pick], y0[pick], rounded(y0, sums(ym, k), t)[pick])
+            check(dw[2:], dw0[2:], rounded(dw0, sums(dwm, 6000), t)[2:])
+            again = grouped_linear(x, wr, at, r)
+            assert torch.equal(again[keep], y[keep])
+            assert torch.equal(torch.autograd.grad(again, wr, dy[:slots])[0][2:], dw[2:])
+    # the input's gradient over a long contraction, with gaps
+    w2 = values((4, k, n), t, 4, 0.1)
+    xr = values((140, n), t, 5).requires_grad_(True)
+    d = values((140, k), t, 6, 0.1)
+    d[:7] = float("nan")
+    d[127:] = float("nan")
+    dx, = torch.autograd.grad(grouped_linear(xr, w2, few), xr, d)
+    assert not dx[:7].any() and not dx[127:].any()
+    _, _, d0, dm, _, _ = oracle(xr.detach()[7:127], w2, few - 7, None, None, d[7:127])
+    check(dx[7:127], d0, rounded(d0, sums(dm, k), t))
+
+
 @pytest.mark.parametrize("dtype", list(TYPES))
 def test_strides_and_alignment(dev, dtype):
     """Rows that begin anywhere give what contiguous ones do, bit for bit."""
