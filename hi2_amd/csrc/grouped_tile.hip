@@ -83,12 +83,12 @@ struct AlongOperand {
   int len;           // end of the contraction
   uint32_t at;       // LDS byte of the wave's first load
   uint32_t read0, read1;
-  __device__ __forceinline__ void init(uint32_t lds, int wv, int half, int from, int end) {
+  __device__ __forceinline__ void init(uint32_t lds, int wv, int first, int from, int end) {
     const int lane = threadIdx.x & 63;
     len = end;
     piece = from + 8 * ((lane & 3) ^ ((lane >> 4) & 3));
     at = lds + NC * wv * 1024;
-    const uint32_t r = half * (T / 2) + (lane & 31);
+    const uint32_t r = first + (lane & 31);
     const int h = lane >> 5, x = (lane >> 2) & 3;
     read0 = r * 64 + 16 * (h ^ x);
     read1 = r * 64 + 16 * ((2 + h) ^ x);
@@ -107,10 +107,11 @@ struct AlongOperand {
   __device__ __forceinline__ void load(const Stage& s, int i, uint32_t buffer) const {
     lds_load16(rs, row[i] + s.k, at + buffer + i * 1024);
   }
-  __device__ __forceinline__ void read(s16x8 (&v)[NC], const char* from, int step) const {
+  template <int M>
+  __device__ __forceinline__ void read(s16x8 (&v)[M], const char* from, int step) const {
     const char* p = from + (step ? read1 : read0);
 #pragma unroll
-    for (int t = 0; t < NC; ++t) v[t] = *reinterpret_cast<const s16x8*>(p + t * 2048);
+    for (int t = 0; t < M; ++t) v[t] = *reinterpret_cast<const s16x8*>(p + t * 2048);
   }
 };
 
@@ -128,7 +129,7 @@ struct AcrossOperand {
   uint32_t own[NC];  // this lane's offsets within a stage
   uint32_t at;
   uint32_t read_at[NC];
-  __device__ __forceinline__ void init(uint32_t lds, int wv, int half, int cols) {
+  __device__ __forceinline__ void init(uint32_t lds, int wv, int first, int cols) {
     const int lane = threadIdx.x & 63;
     at = lds + NC * wv * 1024;
     last = 2 * whole(cols);
@@ -142,7 +143,7 @@ struct AcrossOperand {
 #pragma unroll
     for (int t = 0; t < NC; ++t)
       read_at[t] = (8 * (g >> 1) + (s >> 2)) * (2 * T) + 8 * (s & 1) +
-                   16 * (((half * (T / 16) + 4 * t) ^ (4 * (s >> 2))) + 2 * (g & 1) +
+                   16 * (((first / 8 + 4 * t) ^ (4 * (s >> 2))) + 2 * (g & 1) +
                          ((s & 3) >> 1));
   }
   struct Stage {
@@ -166,9 +167,10 @@ struct AcrossOperand {
   __device__ __forceinline__ void load(const Stage& s, int i, uint32_t buffer) const {
     lds_load16(s.rs, own[i], at + buffer + i * 1024);
   }
-  __device__ __forceinline__ void read(s16x8 (&v)[NC], const char* from, int step) const {
+  template <int M>
+  __device__ __forceinline__ void read(s16x8 (&v)[M], const char* from, int step) const {
 #pragma unroll
-    for (int t = 0; t < NC; ++t) {
+    for (int t = 0; t < M; ++t) {
       const char* p = from + read_at[t] + step * (16 * 2 * T);
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
           (__attribute__((address_space(3))) s16x4*)(p));
@@ -187,9 +189,9 @@ struct IndexedOperand : AcrossOperand<T> {
   const uint32_t* table;  // in LDS
   __amdgpu_buffer_rsrc_t all;
   int lane_row;  // of the wave's first load
-  __device__ __forceinline__ void init(uint32_t lds, int wv, int half, int cols) {
+  __device__ __forceinline__ void init(uint32_t lds, int wv, int first, int cols) {
     this->pitch = 0;
-    Base::init(lds, wv, half, cols);
+    Base::init(lds, wv, first, cols);
     lane_row = RPC * NC * wv + (threadIdx.x & 63) / LP;
   }
   struct Stage {
@@ -217,12 +219,12 @@ __device__ __forceinline__ auto pair_stage(O& o, int st) {
 // acc += A B^T over `len` > 0 of the contraction.  Each accumulator has results' columns (B's rows)
 // in its registers and their rows (A's) over the lanes.
 //
-// A ring of four stages, or of two where more workgroups to a CU hide what it does not.  The two stages of a 128-byte line of an AlongOperand are asked for one
-// right after the other, every other stage: a stage apart, the second comes when the line has left
-// the CU's cache, and every line crosses from L2 twice (16384 x 4096 x 4096: 6.7e7 requests and
-// 536 us; so: XXX).  Loads are issued behind products of the stage whose place they take, and
+// A ring of four stages, or of two where more workgroups to a CU hide what it does not.  The two
+// stages of a 128-byte line of an AlongOperand are asked for one right after the other, every other
+// stage: a stage apart, the second comes when the line has left the CU's cache, and every line
+// crosses from L2 twice (16384 x 4096 x 4096: 6.7e7 requests and 536 us; so half as many, and 461 us).  Loads are issued behind products of the stage whose place they take, and
 // always as many (what lies past the end reads as zeros), so that "landed" is a count.
-template <int DT, int T, int RING, class A, class B>
+template <int DT, int T, int RING, int MA, int MB, class A, class B>
 __device__ __forceinline__ void tile_loop(A& a, B& b, const char* lds, int len,
                                           f32x16v (&acc)[T / 64][T / 64]) {
   constexpr int NA = T / 64, BYTES = T * 64;  // of an operand's stage
@@ -262,7 +264,7 @@ __device__ __forceinline__ void tile_loop(A& a, B& b, const char* lds, int len,
   // stage 0 landed, and with a ring of four stage 1
   __builtin_amdgcn_s_waitcnt(wait_for(RING == 4 ? 4 * NA : 2 * NA, 15));
   meet();
-  s16x8 a0[NA], b0[NA], a1[NA], b1[NA];
+  s16x8 a0[MA], b0[MB], a1[MA], b1[MB];
   a.read(a0, la, 0);
   b.read(b0, lb, 0);
   // Stage st in `cur`.  ODD: st is, and paired operands' stages st + 3 (into `prv`, where st - 1
@@ -281,9 +283,9 @@ __device__ __forceinline__ void tile_loop(A& a, B& b, const char* lds, int len,
     const auto pb = pair_stage<PB && ODD>(b, st + RING - 1);
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int i = 0; i < NA; ++i)
+    for (int i = 0; i < MA; ++i)
 #pragma unroll
-      for (int j = 0; j < NA; ++j) acc[i][j] = product<DT>(b0[j], a0[i], acc[i][j]);
+      for (int j = 0; j < MB; ++j) acc[i][j] = product<DT>(b0[j], a0[i], acc[i][j]);
     __builtin_amdgcn_sched_barrier(0);
     // this wave has read stage st, and stage st + 1 has landed; behind the barrier nobody reads
     // stage st any more
@@ -318,9 +320,9 @@ __device__ __forceinline__ void tile_loop(A& a, B& b, const char* lds, int len,
     };
     auto products = [&](auto self, auto number, auto done) {
       constexpr int m = decltype(number)::value, d = decltype(done)::value;
-      if constexpr (m < NA * NA) {
-        acc[m / NA][m % NA] = product<DT>(b1[m % NA], a1[m / NA], acc[m / NA][m % NA]);
-        constexpr int upto = ALL * (m + 1) / (NA * NA);
+      if constexpr (m < MA * MB) {
+        acc[m / MB][m % MB] = product<DT>(b1[m % MB], a1[m / MB], acc[m / MB][m % MB]);
+        constexpr int upto = ALL * (m + 1) / (MA * MB);
         if constexpr (upto > d) {
           one(std::integral_constant<int, d>{}, pa, pb);
           if constexpr (upto > d + 1) one(std::integral_constant<int, d + 1>{}, pa, pb);
@@ -346,7 +348,7 @@ __device__ __forceinline__ void tile_loop(A& a, B& b, const char* lds, int len,
 
 // The tile through LDS to rows of `out`, 16 bytes a lane where the rows allow it.  NAN_BY: rows
 // whose flag in `bad` is set become NaN (1), or all of them by the first flag (2).
-template <int DT, int T, int NAN_BY>
+template <int DT, int T, int NAN_BY, int MB = T / 64>
 __device__ __forceinline__ void store_tile(char* lds, f32x16v (&acc)[T / 64][T / 64],
                                            uint16_t* out, int64_t cols, int rows, int width,
                                            const uint8_t* bad) {
@@ -357,7 +359,7 @@ __device__ __forceinline__ void store_tile(char* lds, f32x16v (&acc)[T / 64][T /
 #pragma unroll
   for (int i = 0; i < NA; ++i)
 #pragma unroll
-    for (int j = 0; j < NA; ++j) {
+    for (int j = 0; j < MB; ++j) {
       // (held where the matrix units write until its turn: all at once they would not fit)
       if constexpr (T == 256) asm volatile("" : "+a"(acc[i][j]));
 #pragma unroll
@@ -369,8 +371,8 @@ __device__ __forceinline__ void store_tile(char* lds, f32x16v (&acc)[T / 64][T /
           w[u] = DT == 1 ? (uint32_t)f16_bits(x) | (uint32_t)f16_bits(y) << 16
                          : (uint32_t)bf16_bits(x) | (uint32_t)bf16_bits(y) << 16;
         }
-        const int r = wr * (T / 2) + 32 * i + (lane & 31);
-        const int c = wc * (T / 2) + 32 * j + 8 * q + 4 * (lane >> 5);
+        const int r = (MB == NA ? wr * (T / 2) : 0) + 32 * i + (lane & 31);
+        const int c = (MB == NA ? wc * (T / 2) : wave * (T / 4)) + 32 * j + 8 * q + 4 * (lane >> 5);
         *reinterpret_cast<uint2*>(lds + r * PITCH + 2 * c) = make_uint2(w[0], w[1]);
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -554,14 +556,14 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 8 / RING) void grouped_tile_ker
     a.base = static_cast<const char*>(g.dy) + (first * g.ldy + r0) * 2;
     a.pitch = g.ldy * 2;
     a.rows = end - first;
-    a.init(base, wv, wr, rows);
+    a.init(base, wv, wr * (T / 2), rows);
     if constexpr (INDEXED) {
       if (tid == 0) bad[0] = 0;
       IndexedOperand<T> b;
       b.table = table;
       b.all = rsrc(static_cast<const char*>(g.x) + c0 * 2,
                    g.x_rows > 0 ? ((g.x_rows - 1) * g.ldx + whole(cols)) * 2 : 0);
-      b.init(base + RING * BYTES, wv, wc, cols);
+      b.init(base + RING * BYTES, wv, wc * (T / 2), cols);
       constexpr int SEG = SEGMENT<T, RING>;
       const int all = (int)(end - first);
       const int64_t* const index = g.rows + first;
@@ -583,15 +585,15 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 8 / RING) void grouped_tile_ker
         __syncthreads();
         a.base = static_cast<const char*>(g.dy) + ((first + at) * g.ldy + r0) * 2;
         a.rows = len;
-        tile_loop<DT, T, RING>(a, b, lds, len, acc);
+        tile_loop<DT, T, RING, NA, NA>(a, b, lds, len, acc);
       }
     } else {
       AcrossOperand<T> b;
       b.base = static_cast<const char*>(g.x) + (first * g.ldx + c0) * 2;
       b.pitch = g.ldx * 2;
       b.rows = end - first;
-      b.init(base + RING * BYTES, wv, wc, cols);
-      if (!SPLIT || first < end) tile_loop<DT, T, RING>(a, b, lds, (int)(end - first), acc);
+      b.init(base + RING * BYTES, wv, wc * (T / 2), cols);
+      if (!SPLIT || first < end) tile_loop<DT, T, RING, NA, NA>(a, b, lds, (int)(end - first), acc);
     }
     if constexpr (SPLIT) {
       // (all of the tile is NaN then, by any of its ranges)
@@ -620,9 +622,25 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 8 / RING) void grouped_tile_ker
     const int all = WHAT == GROUPED_LINEAR ? k : n;  // of the contraction
     const int from = SPLIT ? __builtin_amdgcn_readfirstlane(z * per * STAGE) : 0;
     const int end = SPLIT && from + per * STAGE < all ? from + per * STAGE : all;
+    // Of 256 x 256 with half the rows at most a wave takes 128 x 64, half as many products (64 experts
+    // of 1024 x 2048 with 64 slots each 78 us, so 66).
+    const bool half = T == 256 && live <= T / 2;
+    auto finish = [&](auto& a, auto& b) {
+      if constexpr (T == 256)
+        if (half) {
+        tile_loop<DT, T, RING, NA, NA / 2>(a, b, lds, end - from, acc);
+        store_tile<DT, T, INDEXED ? 1 : 0, NA / 2>(lds, acc, to, width, live, cols, bad);
+        return;
+      }
+      tile_loop<DT, T, RING, NA, NA>(a, b, lds, end - from, acc);
+      if constexpr (SPLIT)
+        store_part<T>(part, ((uint64_t)y * nx + xt) * splits + z, acc, 0.0f);
+      else
+        store_tile<DT, T, INDEXED ? 1 : 0>(lds, acc, to, width, live, cols, bad);
+    };
     AlongOperand<T> a;
     if constexpr (WHAT == GROUPED_LINEAR) {
-      a.init(base, wv, wr, from, end);
+      a.init(base, wv, half ? 0 : wr * (T / 2), from, end);
       if constexpr (INDEXED) {
         a.rs = rsrc(g.x, g.x_rows > 0 ? ((g.x_rows - 1) * g.ldx + whole(k)) * 2 : 0);
 #pragma unroll
@@ -643,7 +661,7 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 8 / RING) void grouped_tile_ker
         }
       }
       AlongOperand<T> b;
-      b.init(base + RING * BYTES, wv, wc, from, end);
+      b.init(base + RING * BYTES, wv, half ? wv * (T / 4) : wc * (T / 2), from, end);
       b.rs = rsrc(static_cast<const char*>(g.w) + ((int64_t)e * n + c0) * g.ldw * 2,
                   ((int64_t)(cols - 1) * g.ldw + whole(k)) * 2);
 #pragma unroll
@@ -651,9 +669,9 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 8 / RING) void grouped_tile_ker
         const int t = b.row_of(wv, i);
         b.row[i] = t < cols ? (uint32_t)(t * g.ldw * 2) : ROW_DEAD;
       }
-      tile_loop<DT, T, RING>(a, b, lds, end - from, acc);
+      finish(a, b);
     } else {
-      a.init(base, wv, wr, from, end);
+      a.init(base, wv, half ? 0 : wr * (T / 2), from, end);
       a.rs = rsrc(static_cast<const char*>(g.dy) + first * g.ldy * 2,
                   ((int64_t)(live - 1) * g.ldy + whole(n)) * 2);
 #pragma unroll
@@ -665,13 +683,9 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 8 / RING) void grouped_tile_ker
       b.base = static_cast<const char*>(g.w) + (((int64_t)e * n + from) * g.ldw + c0) * 2;
       b.pitch = g.ldw * 2;
       b.rows = end - from;
-      b.init(base + RING * BYTES, wv, wc, cols);
-      tile_loop<DT, T, RING>(a, b, lds, end - from, acc);
+      b.init(base + RING * BYTES, wv, half ? wv * (T / 4) : wc * (T / 2), cols);
+      finish(a, b);
     }
-    if constexpr (SPLIT)
-      store_part<T>(part, ((uint64_t)y * nx + xt) * splits + z, acc, 0.0f);
-    else
-      store_tile<DT, T, INDEXED ? 1 : 0>(lds, acc, to, width, live, cols, bad);
   }
 }
 
@@ -776,11 +790,14 @@ double rounds(double tiles, double cap, double a, double stages, double b, doubl
 }
 
 // 256-tiles, one workgroup to a CU, read LDS half as often for a product; 128-tiles, two to a CU,
-// fill the chip with fewer results and leave less of a range's last tile empty.  Measured (us a
-// stage, at full and half chips): 0.87 for 256-tiles, 0.55 and 0.35 for 128-tiles; 8 experts of 14336
-// x 4096 in ranges of 128 slots 236 and 212 us, of 1024 819 and 1034.  The weights' gradient takes
-// 0.75 a stage in 256-tiles, and in 128-tiles of a two-stage ring, four to a CU, hides the stores of
-// short sums behind others: ranges of 64 slots 72 us and 62, of 512 585 and 619.
+// fill the chip with fewer results and leave less of a range's last tile empty.  The rule counts
+// rounds of the chip with what was measured a stage (us, at full and half chips): 0.87 for 256-tiles,
+// 0.55 and 0.35 for 128-tiles.  Over 80 products of ragged ranges, 32 to 1024 slots an expert, what
+// it takes is 1.3% slower than the better on average and 21% at most (always 128: 3%, always 256:
+// 13%); 8 experts of 14336 x 4096 with 256 slots each 380 us and 465, of 2048 x 4096 with 384 220 and 152.
+// The weights' gradient takes 0.75 a stage in 256-tiles, and in 128-tiles of a two-stage ring, four
+// to a CU, hides the stores of short sums behind others: ranges of 64 slots 72 us and 62, of 512 585
+// and 619.
 // Tiles that leave half the chip empty split their contraction where that saves more than the join
 // costs, 4 us and 0.025 for each range that a tile is cut into: 512 slots of 8 experts of 1024 x 4096
 // 44 us and 27, 300 of one of 1024 x 14336 133 and 33; 256 of 8 of 2048 x 1024 17 and, split, 22; the
@@ -793,23 +810,26 @@ Cut cut_of(const GroupedArgs& g, int what) {
                             STAGE - 1) / STAGE);
   // a live expert's last row tile is half full on average
   const double live = g.slots < g.experts ? g.slots : g.experts;
-  auto tiles = [&](int T) {
-    const double rows = (double)g.slots / T + 0.5 * live;
-    return __builtin_ceil(cols / T) * (grad_w        ? g.experts * __builtin_ceil((double)g.n / T)
-                                       : rows > live ? rows
-                                                     : live);
+  auto tiles = [&](int T, double part) {
+    const double rows = (double)g.slots / T + part * live, least = T == 256 ? part * live : live;
+    return __builtin_ceil(cols / T) * (grad_w         ? g.experts * __builtin_ceil((double)g.n / T)
+                                       : rows > least ? rows
+                                                      : least);
   };
-  if (grad_w ? tiles(256) >= 192 && g.slots >= 384 * g.experts
-             : rounds(tiles(256), 256, 5, stages, 0.87, 0.87) <
-                   rounds(tiles(128), 512, 3, stages, 0.55, 0.35))
+  const double all = tiles(128, 0.5);
+  if (grad_w ? tiles(256, 0) >= 192 && g.slots >= 384 * g.experts
+             : 0.9 * rounds(tiles(256, 0.6), 256, 5, stages, 0.87, 0.87) <
+                   rounds(all, 512, 3, stages, 0.55, 0.35))
     return Cut{256, 1, 0};
   Cut c{128, 1, stages};
-  const double all = tiles(128);
-  double best = stages * 0.35;
+  // (the weights come from memory at 4.5e6 bytes a us whatever the cut)
+  const double read = grad_w ? 0 : live * g.n * g.k * 2 / 4.5e6;
+  double best = 0.8 * (stages * 0.35 > read ? stages * 0.35 : read);
   for (int splits = 2; splits <= 16 && all >= 1 && all * splits <= 512; ++splits) {
     int per = (stages + splits - 1) / splits;
     per += per & 1;  // (whole lines of 128 bytes)
-    const double us = per * (all * splits > 256 ? 0.55 : 0.35) + 4 + 0.025 * all * splits;
+    const double work = per * (all * splits > 256 ? 0.55 : 0.35);
+    const double us = (work > read ? work : read) + 4 + 0.025 * all * splits;
     if (us < best) {
       best = us;
       c.per = per;
