@@ -222,8 +222,9 @@ __device__ __forceinline__ auto pair_stage(O& o, int st) {
 // A ring of four stages, or of two where more workgroups to a CU hide what it does not.  The two
 // stages of a 128-byte line of an AlongOperand are asked for one right after the other, every other
 // stage: a stage apart, the second comes when the line has left the CU's cache, and every line
-// crosses from L2 twice (16384 x 4096 x 4096: 6.7e7 requests and 536 us; so half as many, and 461 us).  Loads are issued behind products of the stage whose place they take, and
-// always as many (what lies past the end reads as zeros), so that "landed" is a count.
+// crosses from L2 twice (16384 x 4096 x 4096: 6.7e7 requests and 536 us; so half as many, and 461 us).
+// Loads are issued behind products of the stage whose place they take, and always as many (what lies
+// past the end reads as zeros), so that "landed" is a count.
 template <int DT, int T, int RING, int MA, int MB, class A, class B>
 __device__ __forceinline__ void tile_loop(A& a, B& b, const char* lds, int len,
                                           f32x16v (&acc)[T / 64][T / 64]) {
