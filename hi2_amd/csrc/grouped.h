@@ -13,6 +13,7 @@ struct GroupedArgs {
   int64_t ldx, ldy, x_rows, slots;
   int64_t ldw;  // of w's rows; an expert's are n of them
   int64_t experts, n, k;
+  bool past = false;  // results go past the caches
 };
 
 // Expert e's slots, empty where the ranges are not as they should be.
@@ -46,8 +47,8 @@ inline int64_t plan_bytes(const GroupedArgs& g, int T) {
 // before the first.
 int launch_plan(const GroupedArgs& g, int T, Plan* plan, hipStream_t s, const char* name);
 
-// The tile of a plan's row tiles (y) x nx columns (xt) that workgroup `block` of 8 ceil(tiles / 8) takes.
-// Workgroups go to the eight XCDs in turn, and each XCD takes an eighth of the tiles, which are in
+// The tile of a plan's row tiles (y) x nx columns (xt) that workgroup `block` of 8 ceil(tiles / 8)
+// takes.  Workgroups go to the eight XCDs in turn, and each XCD takes an eighth of the tiles, which are in
 // order of four row tiles at a time, column tile after column tile, so that rows and weights come to
 // its L2 once.
 __device__ __forceinline__ bool plan_tile(const Plan* p, uint32_t nx, uint32_t block, RowTile& w,

@@ -71,8 +71,17 @@ __global__ __launch_bounds__(256) void sum_slots_kernel(const void* part, int64_
       }
     }
   }
+  if constexpr (V == 8) {
+    u32x4 w;
 #pragma unroll
-  for (int i = 0; i < V; ++i) store_from_f32(out, token * k + c + i, DT, acc[i]);
+    for (int i = 0; i < 4; ++i)
+      w[i] = DT == 1 ? (uint32_t)f16_bits(acc[2 * i]) | (uint32_t)f16_bits(acc[2 * i + 1]) << 16
+                     : (uint32_t)bf16_bits(acc[2 * i]) | (uint32_t)bf16_bits(acc[2 * i + 1]) << 16;
+    *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(out) + token * k + c) = w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) store_from_f32(out, token * k + c + i, DT, acc[i]);
+  }
 }
 
 template <int DT>

@@ -352,7 +352,7 @@ __device__ __forceinline__ void tile_loop(A& a, B& b, const char* lds, int len,
 template <int DT, int T, int NAN_BY, int MB = T / 64>
 __device__ __forceinline__ void store_tile(char* lds, f32x16v (&acc)[T / 64][T / 64],
                                            uint16_t* out, int64_t cols, int rows, int width,
-                                           const uint8_t* bad) {
+                                           const uint8_t* bad, bool past) {
   constexpr int NA = T / 64, PITCH = 2 * T + 16;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int wr = wave >> 1, wc = wave & 1;
@@ -384,19 +384,29 @@ __device__ __forceinline__ void store_tile(char* lds, f32x16v (&acc)[T / 64][T /
   const bool wide = cols % 8 == 0 && ((uintptr_t)out & 15) == 0;
   const int c = 8 * (tid % LP);
   if (c >= width) return;
+  // (two loops: of two stores at one place the compiler makes one, which is not past the caches)
+  auto store = [&](auto stream) {
 #pragma unroll 4
-  for (int r = tid / LP; r < rows; r += 256 / LP) {
-    u32x4 v = *reinterpret_cast<const u32x4*>(lds + r * PITCH + 2 * c);
-    if (NAN_BY && bad[NAN_BY == 2 ? 0 : r]) v = u32x4{nan, nan, nan, nan};
-    uint16_t* to = out + r * cols + c;
-    if (wide && c + 8 <= width) {
-      *reinterpret_cast<u32x4*>(to) = v;
-    } else {
+    for (int r = tid / LP; r < rows; r += 256 / LP) {
+      u32x4 v = *reinterpret_cast<const u32x4*>(lds + r * PITCH + 2 * c);
+      if (NAN_BY && bad[NAN_BY == 2 ? 0 : r]) v = u32x4{nan, nan, nan, nan};
+      uint16_t* to = out + r * cols + c;
+      if (wide && c + 8 <= width) {
+        if constexpr (decltype(stream)::value)
+          __builtin_nontemporal_store(v, reinterpret_cast<u32x4*>(to));
+        else
+          *reinterpret_cast<u32x4*>(to) = v;
+      } else {
 #pragma unroll
-      for (int u = 0; u < 8; ++u)
-        if (c + u < width) to[u] = (uint16_t)(v[u / 2] >> (16 * (u & 1)));
+        for (int u = 0; u < 8; ++u)
+          if (c + u < width) to[u] = (uint16_t)(v[u / 2] >> (16 * (u & 1)));
+      }
     }
-  }
+  };
+  if (past)
+    store(std::true_type{});
+  else
+    store(std::false_type{});
 }
 
 // Zeros where there is nothing to sum.
@@ -602,7 +612,7 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 8 / RING) void grouped_tile_ker
       const uint32_t y = e * ((n + T - 1) / T) + (uint32_t)(r0 / T), across = (k + T - 1) / T;
       store_part<T>(part, ((uint64_t)y * across + c0 / T) * splits + z, acc, add);
     } else {
-      store_tile<DT, T, INDEXED ? 2 : 0>(lds, acc, to, k, rows, cols, bad);
+      store_tile<DT, T, INDEXED ? 2 : 0>(lds, acc, to, k, rows, cols, bad, g.past);
     }
   } else {
     RowTile w;
@@ -630,14 +640,14 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 8 / RING) void grouped_tile_ker
       if constexpr (T == 256)
         if (half) {
         tile_loop<DT, T, RING, NA, NA / 2>(a, b, lds, end - from, acc);
-        store_tile<DT, T, INDEXED ? 1 : 0, NA / 2>(lds, acc, to, width, live, cols, bad);
+        store_tile<DT, T, INDEXED ? 1 : 0, NA / 2>(lds, acc, to, width, live, cols, bad, g.past);
         return;
       }
       tile_loop<DT, T, RING, NA, NA>(a, b, lds, end - from, acc);
       if constexpr (SPLIT)
         store_part<T>(part, ((uint64_t)y * nx + xt) * splits + z, acc, 0.0f);
       else
-        store_tile<DT, T, INDEXED ? 1 : 0>(lds, acc, to, width, live, cols, bad);
+        store_tile<DT, T, INDEXED ? 1 : 0>(lds, acc, to, width, live, cols, bad, g.past);
     };
     AlongOperand<T> a;
     if constexpr (WHAT == GROUPED_LINEAR) {
@@ -795,7 +805,8 @@ double rounds(double tiles, double cap, double a, double stages, double b, doubl
 // rounds of the chip with what was measured a stage (us, at full and half chips): 0.87 for 256-tiles,
 // 0.55 and 0.35 for 128-tiles.  Over 80 products of ragged ranges, 32 to 1024 slots an expert, what
 // it takes is 1.3% slower than the better on average and 21% at most (always 128: 3%, always 256:
-// 13%); 8 experts of 14336 x 4096 with 256 slots each 380 us and 465, of 2048 x 4096 with 384 220 and 152.
+// 13%); 8 experts of 14336 x 4096 with 256 slots each 380 us and 465, 16 of 2048 x 4096 with 384 each
+// 220 and 152.
 // The weights' gradient takes 0.75 a stage in 256-tiles, and in 128-tiles of a two-stage ring, four
 // to a CU, hides the stores of short sums behind others: ranges of 64 slots 72 us and 62, of 512 585
 // and 619.
@@ -864,8 +875,16 @@ int64_t grouped_plan_bytes(const GroupedArgs& g, int what, int dtype) {
          (cut.splits > 1 ? tiles * cut.splits * cut.T * cut.T * 4 : 0);
 }
 
-int grouped_tiles(const GroupedArgs& g, int what, int dtype, char* plan, hipStream_t s,
+int grouped_tiles(const GroupedArgs& args, int what, int dtype, char* plan, hipStream_t s,
                   const char* name) {
+  GroupedArgs g = args;
+  // Results that fill half of the last cache (256 MB) would only push the operands out (the weights'
+  // gradient of 8 experts of 14336 x 4096 from 2048 slots 411 us, so 363; of 64 of 1024 x 2048 from
+  // 16384 131 and 109).
+  const int64_t results = what == GROUPED_GRAD_W   ? g.experts * g.n * g.k
+                          : what == GROUPED_LINEAR ? g.slots * g.n
+                                                   : g.slots * g.k;
+  g.past = results * 2 > 128ll << 20;
 #define HI2X_GROUPED(WHAT)                                     \
   return dtype == 1 ? launch_size<1, WHAT>(g, plan, s, name) : \
                       launch_size<2, WHAT>(g, plan, s, name)

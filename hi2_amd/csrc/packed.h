@@ -9,6 +9,7 @@ typedef _Float16 h16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4v __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 // The columns are walked in chunks of 128.  MFMA step s (0..3) of a chunk multiplies the
 // 32 columns 128 c + 32 q + 8 s + j (q = lane / 16, j < 8): the sum does not depend on the
