@@ -43,12 +43,38 @@ static_assert(sizeof(Launch) <= 4096 - 64, "kernel arguments");
 // it would be there for the next.  192 tensors of 1024 x 2048 in bfloat16 with masters 2135 us,
 // so 2049; 1024 x 4096 in float32, 29, would take 33.
 constexpr int64_t STREAM_BYTES = 512ll << 20;
-template <bool STREAM, class T>
-__device__ __forceinline__ T get(const T* p) {
+template <bool STREAM>
+__device__ __forceinline__ float4 get(const float4* p) {
+  if constexpr (!STREAM) return *p;
+  const f32x4v f = __builtin_nontemporal_load(reinterpret_cast<const f32x4v*>(p));
+  return make_float4(f.x, f.y, f.z, f.w);
+}
+template <bool STREAM>
+__device__ __forceinline__ uint2 get(const uint2* p) {
+  if constexpr (!STREAM) return *p;
+  const u32x2 h = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(p));
+  return make_uint2(h.x, h.y);
+}
+template <bool STREAM>
+__device__ __forceinline__ uint32_t get(const uint32_t* p) {
   return STREAM ? __builtin_nontemporal_load(p) : *p;
 }
-template <bool STREAM, class T>
-__device__ __forceinline__ void put(T* p, T v) {
+template <bool STREAM>
+__device__ __forceinline__ void put(float4* p, float4 v) {
+  if constexpr (STREAM)
+    __builtin_nontemporal_store(f32x4v{v.x, v.y, v.z, v.w}, reinterpret_cast<f32x4v*>(p));
+  else
+    *p = v;
+}
+template <bool STREAM>
+__device__ __forceinline__ void put(uint2* p, uint2 v) {
+  if constexpr (STREAM)
+    __builtin_nontemporal_store(u32x2{v.x, v.y}, reinterpret_cast<u32x2*>(p));
+  else
+    *p = v;
+}
+template <bool STREAM>
+__device__ __forceinline__ void put(uint32_t* p, uint32_t v) {
   if constexpr (STREAM)
     __builtin_nontemporal_store(v, p);
   else
@@ -60,12 +86,12 @@ __device__ __forceinline__ void load4(const void* p, int64_t i, int64_t n, bool 
                                       float (&x)[4]) {
   if (vec) {
     if constexpr (DT == 0) {
-      const f32x4v f =
-          get<STREAM>(reinterpret_cast<const f32x4v*>(static_cast<const float*>(p) + i));
+      const float4 f =
+          get<STREAM>(reinterpret_cast<const float4*>(static_cast<const float*>(p) + i));
       x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
     } else {
-      const u32x2 h =
-          get<STREAM>(reinterpret_cast<const u32x2*>(static_cast<const uint16_t*>(p) + i));
+      const uint2 h =
+          get<STREAM>(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + i));
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const uint16_t b = (uint16_t)((j < 2 ? h.x : h.y) >> (16 * (j & 1)));
@@ -83,8 +109,8 @@ __device__ __forceinline__ void store4(void* p, int64_t i, int64_t n, bool vec,
                                        const float (&x)[4]) {
   if (vec) {
     if constexpr (DT == 0) {
-      put<STREAM>(reinterpret_cast<f32x4v*>(static_cast<float*>(p) + i),
-                  f32x4v{x[0], x[1], x[2], x[3]});
+      put<STREAM>(reinterpret_cast<float4*>(static_cast<float*>(p) + i),
+                  make_float4(x[0], x[1], x[2], x[3]));
     } else {
       uint32_t w[2];
 #pragma unroll
@@ -93,7 +119,7 @@ __device__ __forceinline__ void store4(void* p, int64_t i, int64_t n, bool vec,
         const uint32_t b = DT == 1 ? f16_bits(x[2 * j + 1]) : bf16_bits(x[2 * j + 1]);
         w[j] = a | b << 16;
       }
-      put<STREAM>(reinterpret_cast<u32x2*>(static_cast<uint16_t*>(p) + i), u32x2{w[0], w[1]});
+      put<STREAM>(reinterpret_cast<uint2*>(static_cast<uint16_t*>(p) + i), make_uint2(w[0], w[1]));
     }
   } else {
 #pragma unroll
