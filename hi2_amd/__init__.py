@@ -11,6 +11,9 @@ and run every arithmetic step in the HIP kernels of ``libhi2x.so`` (C ABI:
 
 ``hi2_amd.packed`` and ``hi2_amd.moe.route`` run what was encoded: products by packed tensors
 and experts, and the router in front of them.
+
+``hi2_amd.experts`` and ``hi2_amd.optim`` train: products grouped by expert with their gradients, the
+gated activation, the MLP of experts, and AdamW over many tensors with moments in 32 or 8 bits.
 """
 
 __version__ = "0.1.0"

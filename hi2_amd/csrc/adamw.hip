@@ -4,7 +4,8 @@
 //   p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //
 // in float32, each product and sum rounded by itself.  Nothing is reused, so HBM bounds it: 28
-// bytes of a float32 weight with 32-bit moments, 16 with 8-bit ones.
+// bytes of a float32 weight with 32-bit moments, 16 with 8-bit ones.  192 tensors of 1024 x 2048 in
+// bfloat16 with masters 2049 us (5.9 TB/s), 3 of 14336 x 4096 in float32 with 8-bit moments 600 (4.7).
 //
 // 8-bit moments: blocks of 256 elements (one wave's 64 lanes x 4) hold m = +-q^2 d with |q| <=
 // 127, and the root of v as q^2 d with q <= 255, d the block's largest over 127^2 or 255^2.  The

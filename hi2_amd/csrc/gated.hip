@@ -1,7 +1,8 @@
 // The gated activation between the products of an MLP, out = act(gate) * up, and its gradients
 //   d_gate = grad * up * act'(gate),  d_up = grad * act(gate),
 // in float32 from one pass over the operands, each result rounded once.  HBM bounds both (3 and 5
-// elements moved for one of the result).
+// elements moved for one of the result): 131072 x 1024 in bfloat16 178 us (4.5 TB/s) and 251 (5.3),
+// where a large copy has 4.9.
 #include <type_traits>
 
 #include "packed.h"

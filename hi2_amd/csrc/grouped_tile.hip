@@ -7,7 +7,9 @@
 // gradient, dy and x of the weights') a stage is 32 rows of T values, and LDS's transposing read
 // hands a lane its column.  Both are loaded as they lie, 16 bytes a lane, straight into LDS.
 //
-// A wave holds T/2 x T/2 results in registers; a ring of four stages (or two) is in flight.
+// A wave holds T/2 x T/2 results in registers; a ring of four stages (or two) is in flight.  64 experts
+// of 1024 x 2048, 2048 slots each in bfloat16: 576 us (955 TFLOP/s), the tokens' gradient 611 (900),
+// the weights' 516 (1066); one library product of the size reaches 1298, 1080 and 625.
 #include <type_traits>
 
 #include "grouped.h"
