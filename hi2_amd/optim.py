@@ -95,6 +95,10 @@ class AdamW(torch.optim.Optimizer):
             if p.numel():
                 by_type.setdefault(p.dtype, []).append((p, at, gi))
             at += -(-p.numel() // BLOCK) * BLOCK
+        spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size())
+                       for p, _ in every if p.numel())
+        if any(b < end for (_, end), (b, _) in zip(spans, spans[1:])):
+            raise ValueError("two parameters share memory, or one is there twice")
         #: the first element of each parameter in the buffers
         self.starts = starts
         self._params = [p for p, _ in every]
@@ -145,17 +149,20 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         groups = (_lib.AdamwGroup * len(self.param_groups))(
             *(_lib.AdamwGroup(*self._options(g)) for g in self.param_groups))
+        odd = []  # gradients made contiguous, alive until they are read
+        for s in self._sets:  # (all of them before the first launch: a step is taken whole or not)
+            at_p, at_g = s.addresses[0].ctypes.data, s.addresses[1].ctypes.data
+            for i in _tensors().addresses(s.params, s.sizes.ctypes.data, DTYPES[s.dtype],
+                                          self.device.index, at_p, at_g):
+                odd.append(s.params[i].grad.contiguous())
+                s.addresses[1, i] = odd[-1].data_ptr()
         at = 0
+        units = self._units
         for s in self._sets:
             n = len(s.params)
-            at_p, at_g = s.addresses[0].ctypes.data, s.addresses[1].ctypes.data
-            odd = {i: s.params[i].grad.contiguous() for i in _tensors().addresses(
-                s.params, s.sizes.ctypes.data, DTYPES[s.dtype], self.device.index, at_p, at_g)}
-            for i, g in odd.items():
-                s.addresses[1, i] = g.data_ptr()
-            units = self._units
             _lib.call("hi2x_adamw_step", self.device, s.table.ctypes.data,
-                      s.device_table.data_ptr(), at_p, at_g, n, DTYPES[s.dtype], self.state_bits, groups,
+                      s.device_table.data_ptr(), s.addresses[0].ctypes.data,
+                      s.addresses[1].ctypes.data, n, DTYPES[s.dtype], self.state_bits, groups,
                       len(groups), self._m.data_ptr(), self._v.data_ptr(),
                       None if units is None else units[0].data_ptr(),
                       None if units is None else units[1].data_ptr(),
@@ -224,7 +231,8 @@ class AdamW(torch.optim.Optimizer):
     @torch.no_grad()
     def load_state_dict(self, state_dict: dict) -> None:
         """Take over a :meth:`state_dict` of an optimizer over the same parameters and of the same
-        ``state_bits`` and ``master``."""
+        ``state_bits`` and ``master``.  A learning rate that is a tensor here stays that tensor and
+        takes the value."""
         given = state_dict["state"]
         mine = self.state_dict()["state"]
         if given["state_bits"] != self.state_bits or list(given["starts"]) != self.starts:
@@ -237,9 +245,17 @@ class AdamW(torch.optim.Optimizer):
             if (a is None) != (b is None) or a is not None and (a.shape != b.shape or
                                                                 a.dtype != b.dtype):
                 raise ValueError(f"load_state_dict: {name} does not fit")
+        taken = []
         for g, h in zip(self.param_groups, state_dict["param_groups"]):
             options = {k: v for k, v in h.items() if k != "params"}
+            if isinstance(options.get("lr"), torch.Tensor):
+                options["lr"] = options["lr"].to(self.device, copy=True)
             self._options({**g, **options})
+            taken.append(options)
+        for g, options in zip(self.param_groups, taken):
+            if isinstance(g["lr"], torch.Tensor) and "lr" in options:
+                lr = options.pop("lr")  # (the tensor stays: captured steps read it)
+                g["lr"].copy_(lr) if isinstance(lr, torch.Tensor) else g["lr"].fill_(lr)
             g.update(options)
         for name in ("m", "v", "units", "steps", "master"):
             if mine[name] is not None:

@@ -200,3 +200,60 @@ def test_weights_past_32_bits_of_offsets(dev, slots):
                 (dw[i], d.T @ a, d.abs().T @ a.abs(), slots)):
             bound = 2.0 ** -8 * want.abs() + (length + 8) * 2.0 ** -23 * 1.01 * size + 1e-38
             assert bool(((got.detach().double() - want).abs() <= bound).all())
+
+
+def test_a_step_is_taken_whole_or_not(dev):
+    """A parameter that no longer fits refuses the step before any other has taken it."""
+    a = torch.ones(300, device=dev, requires_grad=True)
+    b = torch.ones(70, dtype=torch.bfloat16, device=dev, requires_grad=True)
+    opt = AdamW([a, b], lr=0.1)
+    a.grad, b.grad = torch.ones_like(a), torch.ones_like(b)
+    b.data = torch.ones(71, dtype=torch.bfloat16, device=dev)
+    with pytest.raises(RuntimeError, match="changed after construction"):
+        opt.step()
+    assert bool((a == 1).all()) and not opt.moments()[0].any()
+
+
+def test_parameters_that_share_memory_are_refused(dev):
+    base = torch.zeros(100, device=dev)
+    a, b = base[:60].requires_grad_(True), base[59:].requires_grad_(True)
+    with pytest.raises(ValueError, match="share memory"):
+        AdamW([a, b])
+    with pytest.raises(ValueError, match="share memory|some parameters appear in more"):
+        AdamW([dict(params=[a]), dict(params=[base[:60].requires_grad_(True)])])
+    AdamW([a, base[60:].requires_grad_(True)])
+
+
+def test_a_state_is_taken_over_whole_or_not(dev):
+    def make(lr):
+        ps = [torch.ones(5, device=dev, requires_grad=True) for _ in range(2)]
+        return AdamW([dict(params=[ps[0]], lr=lr), dict(params=[ps[1]])])
+
+    tensor = torch.full((1,), 0.25, device=dev)
+    opt, other = make(tensor), make(torch.full((1,), 0.5, device=dev))
+    bad = other.state_dict()
+    bad["param_groups"][1]["eps"] = -1.0
+    with pytest.raises(ValueError, match="eps"):
+        opt.load_state_dict(bad)
+    assert float(tensor) == 0.25 and opt.param_groups[1]["eps"] == 1e-8
+    good = other.state_dict()
+    good["param_groups"][0]["lr"] = good["param_groups"][0]["lr"].cpu()
+    opt.load_state_dict(good)
+    assert opt.param_groups[0]["lr"] is tensor and float(tensor) == 0.5
+
+
+@pytest.mark.parametrize("tokens", [0, 1])
+def test_few_or_no_tokens(dev, tokens):
+    g = torch.Generator().manual_seed(8)
+    gate, up, down = ((torch.randn(s, generator=g) * 0.1).bfloat16().to(dev).requires_grad_(True)
+                      for s in ((3, 32, 64), (3, 32, 64), (3, 64, 32)))
+    x = torch.randn(tokens, 64, generator=g).bfloat16().to(dev).requires_grad_(True)
+    r = route(torch.randn(tokens, 3, generator=g).to(dev), 2)
+    y = experts_mlp(x, r, gate, up, down)
+    grads = torch.autograd.grad(y, (x, gate, up, down), torch.ones_like(y))
+    assert y.shape == x.shape and grads[0].shape == x.shape
+    used = [False] * 3
+    for e in r.index.flatten().tolist():
+        used[e] = True
+    for v in grads[1:]:
+        assert [bool(v[e].any()) for e in range(3)] == used and torch.isfinite(v).all()
