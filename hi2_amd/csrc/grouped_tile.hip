@@ -8,8 +8,8 @@
 // hands a lane its column.  Both are loaded as they lie, 16 bytes a lane, straight into LDS.
 //
 // A wave holds T/2 x T/2 results in registers; a ring of four stages (or two) is in flight.  64 experts
-// of 1024 x 2048, 2048 slots each in bfloat16: 576 us (955 TFLOP/s), the tokens' gradient 611 (900),
-// the weights' 516 (1066); one library product of the size reaches 1298, 1080 and 625.
+// of 1024 x 2048, 2048 slots each in bfloat16: 533 us (1032 TFLOP/s), the tokens' gradient 574 (958),
+// the weights' 485 (1134); one library product of the size reaches 1298, 1080 and 625.
 #include <type_traits>
 
 #include "grouped.h"
@@ -109,11 +109,9 @@ struct AlongOperand {
   __device__ __forceinline__ void load(const Stage& s, int i, uint32_t buffer) const {
     lds_load16(rs, row[i] + s.k, at + buffer + i * 1024);
   }
-  template <int M>
-  __device__ __forceinline__ void read(s16x8 (&v)[M], const char* from, int step) const {
-    const char* p = from + (step ? read1 : read0);
-#pragma unroll
-    for (int t = 0; t < M; ++t) v[t] = *reinterpret_cast<const s16x8*>(p + t * 2048);
+  // fragment t of 16 of the stage's 32
+  __device__ __forceinline__ s16x8 read(const char* from, int step, int t) const {
+    return *reinterpret_cast<const s16x8*>(from + (step ? read1 : read0) + t * 2048);
   }
 };
 
@@ -169,17 +167,13 @@ struct AcrossOperand {
   __device__ __forceinline__ void load(const Stage& s, int i, uint32_t buffer) const {
     lds_load16(s.rs, own[i], at + buffer + i * 1024);
   }
-  template <int M>
-  __device__ __forceinline__ void read(s16x8 (&v)[M], const char* from, int step) const {
-#pragma unroll
-    for (int t = 0; t < M; ++t) {
-      const char* p = from + read_at[t] + step * (16 * 2 * T);
-      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          (__attribute__((address_space(3))) s16x4*)(p));
-      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          (__attribute__((address_space(3))) s16x4*)(p + 4 * 2 * T));
-      v[t] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-    }
+  __device__ __forceinline__ s16x8 read(const char* from, int step, int t) const {
+    const char* p = from + read_at[t] + step * (16 * 2 * T);
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (__attribute__((address_space(3))) s16x4*)(p));
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (__attribute__((address_space(3))) s16x4*)(p + 4 * 2 * T));
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
   }
 };
 
@@ -224,7 +218,8 @@ __device__ __forceinline__ auto pair_stage(O& o, int st) {
 // A ring of four stages, or of two where more workgroups to a CU hide what it does not.  The two
 // stages of a 128-byte line of an AlongOperand are asked for one right after the other, every other
 // stage: a stage apart, the second comes when the line has left the CU's cache, and every line
-// crosses from L2 twice (16384 x 4096 x 4096: 6.7e7 requests and 536 us; so half as many, and 461 us).
+// crosses from L2 twice (16384 x 4096 x 4096: 6.7e7 requests and 536 us; so half as many and 461, by
+// now 440).
 // Loads are issued behind products of the stage whose place they take, and always as many (what lies
 // past the end reads as zeros), so that "landed" is a count.
 template <int DT, int T, int RING, int MA, int MB, class A, class B>
@@ -268,8 +263,22 @@ __device__ __forceinline__ void tile_loop(A& a, B& b, const char* lds, int len,
   __builtin_amdgcn_s_waitcnt(wait_for(RING == 4 ? 4 * NA : 2 * NA, 15));
   meet();
   s16x8 a0[MA], b0[MB], a1[MA], b1[MB];
-  a.read(a0, la, 0);
-  b.read(b0, lb, 0);
+  // Read r of a step's fragments, those of B first.
+  auto fragment = [&](auto number, s16x8(&av)[MA], s16x8(&bv)[MB], uint32_t buffer, int step) {
+    constexpr int r = decltype(number)::value;
+    if constexpr (r < MB)
+      bv[r] = b.read(lb + buffer, step, r);
+    else if constexpr (r < MA + MB)
+      av[r - MB] = a.read(la + buffer, step, r - MB);
+  };
+  auto fragments = [&](auto self, auto number) {
+    constexpr int r = decltype(number)::value;
+    if constexpr (r < MA + MB) {
+      fragment(number, a0, b0, 0, 0);
+      self(self, std::integral_constant<int, r + 1>{});
+    }
+  };
+  fragments(fragments, std::integral_constant<int, 0>{});
   // Stage st in `cur`.  ODD: st is, and paired operands' stages st + 3 (into `prv`, where st - 1
   // was) and st + 4 are asked for.
   auto stage = [&](auto odd, int st, uint32_t prv, uint32_t cur, uint32_t nxt) {
@@ -278,25 +287,28 @@ __device__ __forceinline__ void tile_loop(A& a, B& b, const char* lds, int len,
     constexpr int LA = NA * (PA ? PAIR : 1), LB = NA * (PB ? PAIR : 1), ALL = LA + LB;
     // newer loads than the next stage's
     constexpr int NEWER = RING == 2 ? 0 : NA * (!ODD ? 4 : (PA ? 0 : 2) + (PB ? 0 : 2));
-    a.read(a1, la + cur, 1);
-    b.read(b1, lb + cur, 1);
     const auto sa = a.begin(st + RING);
     const auto sb = b.begin(st + RING);
     const auto pa = pair_stage<PA && ODD>(a, st + RING - 1);
     const auto pb = pair_stage<PB && ODD>(b, st + RING - 1);
     __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int i = 0; i < MA; ++i)
-#pragma unroll
-      for (int j = 0; j < MB; ++j) acc[i][j] = product<DT>(b0[j], a0[i], acc[i][j]);
-    __builtin_amdgcn_sched_barrier(0);
+    // (a read behind each product: the matrix unit would wait for eight in a row; 131072 slots of 64
+    // experts of 1024 x 2048 550 us, so 533, the weights' gradient 517 and 485)
+    auto first = [&](auto self, auto number) {
+      constexpr int m = decltype(number)::value;
+      if constexpr (m < MA * MB) {
+        acc[m / MB][m % MB] = product<DT>(b0[m % MB], a0[m / MB], acc[m / MB][m % MB]);
+        static_assert(MA + MB <= MA * MB, "a product to each read");
+        fragment(number, a1, b1, cur, 1);
+        __builtin_amdgcn_sched_barrier(0);
+        self(self, std::integral_constant<int, m + 1>{});
+      }
+    };
+    first(first, std::integral_constant<int, 0>{});
     // this wave has read stage st, and stage st + 1 has landed; behind the barrier nobody reads
     // stage st any more
     __builtin_amdgcn_s_waitcnt(wait_for(NEWER, 0));
     meet();
-    a.read(a0, la + nxt, 0);
-    b.read(b0, lb + nxt, 0);
-    __builtin_amdgcn_sched_barrier(0);
     auto one = [&](auto number, const auto& pa, const auto& pb) {
       constexpr int l = decltype(number)::value;
       if constexpr (PA && l < LA) {
@@ -325,6 +337,8 @@ __device__ __forceinline__ void tile_loop(A& a, B& b, const char* lds, int len,
       constexpr int m = decltype(number)::value, d = decltype(done)::value;
       if constexpr (m < MA * MB) {
         acc[m / MB][m % MB] = product<DT>(b1[m % MB], a1[m / MB], acc[m / MB][m % MB]);
+        fragment(number, a0, b0, nxt, 0);
+        __builtin_amdgcn_sched_barrier(0);
         constexpr int upto = ALL * (m + 1) / (MA * MB);
         if constexpr (upto > d) {
           one(std::integral_constant<int, d>{}, pa, pb);
