@@ -61,11 +61,12 @@ def tensors_command(out: str) -> list[str]:
 
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-I" + os.path.join(os.path.dirname(os.path.dirname(hipcc())), "include"),
            "-I" + sysconfig.get_paths()["include"], *("-I" + p for p in include_paths()),
            os.path.join(CSRC, "tensors.cpp"), "-o", out]
     for p in library_paths():
         cmd += ["-L" + p, "-Wl,-rpath," + p]
-    return cmd + ["-ltorch_python", "-ltorch_cpu", "-lc10"]
+    return cmd + ["-ltorch_python", "-ltorch_cpu", "-lc10_hip", "-lc10"]
 
 
 def build(verbose: bool = False, jobs: int | None = None) -> str:

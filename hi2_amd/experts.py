@@ -16,9 +16,12 @@ inputs' type."""
 
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from . import _lib
+from .optim import _tensors
 from .packed import ACTIVATIONS, DTYPES, combine
 
 __all__ = ["grouped_linear", "gated", "experts_mlp"]
@@ -161,31 +164,17 @@ def grouped_linear(x: torch.Tensor, w: torch.Tensor, offs: torch.Tensor,
     return _linear(_rows(x), w.contiguous(), offs, rows, count)
 
 
-class _Gated(torch.autograd.Function):
-    """The gated activation with both gradients."""
+_gated_graph = None
 
-    @staticmethod
-    def forward(ctx, gate, up, act):
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(gate, up)
-        ctx.act = act
-        return _gated(gate, up, act)
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad):
-        if grad is None:
-            return None, None, None
-        gate, up = ctx.saved_tensors
-        rows, n = gate.shape
-        both = torch.empty(2, rows, n, dtype=gate.dtype, device=gate.device)
-        d_gate, d_up = both[0], both[1]
-        grad = _rows(grad)
-        if rows and n:
-            _lib.call("hi2x_gated_backward", gate.device, grad.data_ptr(), _pitch(grad),
-                      gate.data_ptr(), _pitch(gate), up.data_ptr(), _pitch(up), rows, n,
-                      DTYPES[gate.dtype], ctx.act, d_gate.data_ptr(), n, d_up.data_ptr(), n)
-        return d_gate, d_up, None
+def _bind():
+    """The host extension's activation with its gradients, on the library's entries."""
+    global _gated_graph
+    module, lib = _tensors(), _lib.lib()
+    module.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
+        lib.hi2x_gated, lib.hi2x_gated_backward, lib.hi2x_last_error)))
+    _gated_graph = module.gated
+    return _gated_graph
 
 
 def _gated(gate, up, act):
@@ -217,7 +206,7 @@ def gated(gate: torch.Tensor, up: torch.Tensor, activation: str = "silu") -> tor
         gate, up = gate.reshape(rows, shape[-1]), up.reshape(rows, shape[-1])
     gate, up = _rows(gate), _rows(up)
     if torch.is_grad_enabled() and (gate.requires_grad or up.requires_grad):
-        out = _Gated.apply(gate, up, act)
+        out = (_gated_graph or _bind())(gate, up, act)
     else:
         out = _gated(gate, up, act)
     return out if len(shape) == 2 else out.view(shape)

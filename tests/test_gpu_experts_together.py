@@ -257,3 +257,42 @@ def test_few_or_no_tokens(dev, tokens):
         used[e] = True
     for v in grads[1:]:
         assert [bool(v[e].any()) for e in range(3)] == used and torch.isfinite(v).all()
+
+
+def test_gated_in_the_graph(dev):
+    """One input with a gradient, none used, an expanded gradient, a graph kept, second derivatives
+    refused, an input changed in between, another stream."""
+    g = torch.Generator().manual_seed(9)
+    a, b = (torch.randn(40, 24, generator=g).to(dev) for _ in range(2))
+    ar, br = a.clone().requires_grad_(True), b.clone().requires_grad_(True)
+    both = torch.autograd.grad(gated(ar, br).sum(), (ar, br))
+    want = torch.autograd.grad(gated(ar, br), (ar, br), torch.ones_like(a))
+    assert all(torch.equal(x, y) for x, y in zip(both, want))
+    only, = torch.autograd.grad(gated(ar, b).sum(), ar)
+    other, = torch.autograd.grad(gated(a, br).sum(), br)
+    assert torch.equal(only, both[0]) and torch.equal(other, both[1])
+    y = gated(ar, br)
+    first = torch.autograd.grad(y.sum(), ar, retain_graph=True)[0]
+    assert torch.equal(first, torch.autograd.grad(y.sum(), ar)[0])
+    with pytest.raises(RuntimeError, match="second time|freed"):
+        torch.autograd.grad(y.sum(), ar)
+    d, = torch.autograd.grad(gated(ar, br).sum(), ar, create_graph=True)
+    assert torch.equal(d, both[0])
+    with pytest.raises(RuntimeError, match="twice"):
+        d.sum().backward()
+    y = gated(ar, br)
+    with torch.no_grad():
+        ar.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.sum().backward()
+    del y
+    three = torch.randn(2, 3, 5, generator=g).half().to(dev).requires_grad_(True)
+    z = gated(three, three * 2, "relu")
+    assert z.shape == three.shape and torch.autograd.grad(z.sum(), three)[0].shape == three.shape
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        ys = torch.autograd.grad(gated(ar, br), (ar, br), torch.ones_like(a))
+    torch.cuda.current_stream().wait_stream(side)
+    now = torch.autograd.grad(gated(ar, br), (ar, br), torch.ones_like(a))
+    assert all(torch.equal(x, y) for x, y in zip(ys, now))
