@@ -14,6 +14,7 @@ struct GroupedArgs {
   int64_t ldw;  // of w's rows; an expert's are n of them
   int64_t experts, n, k;
   bool past = false;  // results go past the caches
+  bool f32_out = false;  // of 16-bit operands (the tokens' gradient of each slot, to be added up)
 };
 
 // Expert e's slots, empty where the ranges are not as they should be.

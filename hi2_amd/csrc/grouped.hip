@@ -26,11 +26,12 @@ __device__ __forceinline__ void spread_at(const Spread& g, int64_t& row, int64_t
 }
 
 // ---- a token's sum over its slots -------------------------------------------------------------
-// dx[t] = the rows of t's slots added in their order, 16 bytes of a row a thread (V values; 1 where
-// rows do not begin at multiples of 16), up to four rows on their way at a time.  A slot outside
-// gives NaN.  HBM bounds it: part is read once.
+// dx[t] = the rows of t's slots added in their order, V values a thread (4, 16 bytes of a row; 1 where rows
+// do not begin at multiples of 16 bytes), up to four rows on their way at a time.  A slot outside gives
+// NaN.  Rows are float32 whatever dx's type: rounded to 16 bits before they are added they would cost
+// half the traffic and 1.4 times the error.  HBM bounds it: part is read once.
 template <int DT, int V>
-__global__ __launch_bounds__(256) void sum_slots_kernel(const void* part, int64_t slots, int64_t k,
+__global__ __launch_bounds__(256) void sum_slots_kernel(const float* part, int64_t slots, int64_t k,
                                                         const int64_t* slots_of, int64_t t,
                                                         int top_k, Spread by, void* out) {
   int64_t token, c;
@@ -44,40 +45,34 @@ __global__ __launch_bounds__(256) void sum_slots_kernel(const void* part, int64_
   constexpr int UN = 4;
   for (int j0 = 0; j0 < top_k; j0 += UN) {
     int64_t s[UN];
-    u32x4 w[UN];
+    f32x4v w[UN];
 #pragma unroll
     for (int u = 0; u < UN; ++u) s[u] = of[j0 + u < top_k ? j0 + u : top_k - 1];
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
       const int64_t r = (uint64_t)s[u] < (uint64_t)slots ? s[u] : 0;
+      w[u] = f32x4v{0.0f, 0.0f, 0.0f, 0.0f};
+      if (slots == 0) continue;  // (no row to read in the place of one outside)
       if constexpr (V == 1)
-        w[u][0] = DT == 0 ? static_cast<const uint32_t*>(part)[r * k + c]
-                          : (uint32_t)static_cast<const uint16_t*>(part)[r * k + c];
+        w[u][0] = part[r * k + c];
       else
-        w[u] = *reinterpret_cast<const u32x4*>(static_cast<const char*>(part) +
-                                               (r * k + c) * (DT == 0 ? 4 : 2));
+        w[u] = *reinterpret_cast<const f32x4v*>(part + r * k + c);
     }
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
       if (j0 + u >= top_k) break;
       const bool in = (uint64_t)s[u] < (uint64_t)slots;
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const uint32_t h = DT == 0 ? w[u][i] : w[u][i / 2] >> (16 * (i & 1));
-        const float x = DT == 0 ? __uint_as_float(h)
-                                : (DT == 1 ? f16_from_bits((uint16_t)h)
-                                           : __uint_as_float(h << 16));
-        acc[i] += in ? x : __builtin_nanf("");
-      }
+      for (int i = 0; i < V; ++i) acc[i] += in ? w[u][i] : __builtin_nanf("");
     }
   }
-  if constexpr (V == 8) {
-    u32x4 w;
+  if constexpr (V == 4 && DT != 0) {
+    u32x2 w;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 2; ++i)
       w[i] = DT == 1 ? (uint32_t)f16_bits(acc[2 * i]) | (uint32_t)f16_bits(acc[2 * i + 1]) << 16
                      : (uint32_t)bf16_bits(acc[2 * i]) | (uint32_t)bf16_bits(acc[2 * i + 1]) << 16;
-    *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(out) + token * k + c) = w;
+    *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(out) + token * k + c) = w;
   } else {
 #pragma unroll
     for (int i = 0; i < V; ++i) store_from_f32(out, token * k + c + i, DT, acc[i]);
@@ -87,17 +82,17 @@ __global__ __launch_bounds__(256) void sum_slots_kernel(const void* part, int64_
 template <int DT>
 int sum_slots(const void* part, int64_t slots, int64_t k, const int64_t* slots_of, int64_t t,
               int64_t top_k, void* out, hipStream_t s) {
-  constexpr int WIDE = DT == 0 ? 4 : 8;
-  const bool wide = k % WIDE == 0 && ((uintptr_t)out & 15) == 0;
+  const bool wide = k % 4 == 0 && ((uintptr_t)out & 15) == 0;
+  const float* p = static_cast<const float*>(part);
   Spread by;
-  const int64_t count = spread(t, wide ? k / WIDE : k, by);
+  const int64_t count = spread(t, wide ? k / 4 : k, by);
   HI2X_REQUIRE(count < (1ll << 31), "grouped_grad_x: too many results");
   if (wide)
-    sum_slots_kernel<DT, WIDE><<<(unsigned)count, 256, 0, s>>>(part, slots, k, slots_of, t,
-                                                              (int)top_k, by, out);
+    sum_slots_kernel<DT, 4><<<(unsigned)count, 256, 0, s>>>(p, slots, k, slots_of, t, (int)top_k, by,
+                                                            out);
   else
-    sum_slots_kernel<DT, 1><<<(unsigned)count, 256, 0, s>>>(part, slots, k, slots_of, t,
-                                                           (int)top_k, by, out);
+    sum_slots_kernel<DT, 1><<<(unsigned)count, 256, 0, s>>>(p, slots, k, slots_of, t, (int)top_k, by,
+                                                            out);
   return launch_status("grouped_grad_x");
 }
 
@@ -188,7 +183,7 @@ Space lay_out(const GroupedArgs& g, int what, int dtype, bool summed, bool x_fit
   };
   const int64_t size = size_of(dtype);
   GroupedArgs p = g;
-  if (summed) m.has_part = true, m.part = take(g.slots * g.k * size);
+  if (summed) m.has_part = true, m.part = take(g.slots * g.k * 4);
   if (what != GROUPED_GRAD_X) {
     const bool copied = dtype != 0 && (!x_fits || (what == GROUPED_LINEAR && g.k % 8));
     m.ldx = copied ? pad8(g.k) : g.ldx;
@@ -235,7 +230,7 @@ int run(GroupedArgs g, int what, int dtype, bool summed, void* ws, int64_t ws_by
   const Space m = lay_out(g, what, dtype, summed, lies_well(g.x, g.ldx), lies_well(g.dy, g.ldy),
                           lies_well(g.w, g.ldw));
   if (int rc = take_workspace(w, ws, ws_bytes, (size_t)m.bytes, s, name)) return rc;
-  if (summed) g.out = *part = w.p + m.part;
+  if (summed) g.out = *part = w.p + m.part, g.f32_out = true;
   if (m.has_x) {
     if (int rc = copy_rows(g.x, g.ldx, m.gather ? g.slots : g.x_rows, g.k,
                            m.gather ? g.rows : nullptr, g.x_rows, nullptr, 0, dtype, w.p + m.x,

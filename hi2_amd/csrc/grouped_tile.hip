@@ -425,9 +425,66 @@ __device__ __forceinline__ void store_tile(char* lds, f32x16v (&acc)[T / 64][T /
     store(std::false_type{});
 }
 
+// The tile's sums as they are, to float32 rows of `out`, half of its rows through LDS at a time; 16 bytes a
+// lane where the rows allow it.
+template <int T, int MB = T / 64>
+__device__ __forceinline__ void store_sums(char* lds, f32x16v (&acc)[T / 64][T / 64], float* out,
+                                           int64_t cols, int rows, int width, bool past) {
+  constexpr int NA = T / 64, PITCH = 4 * T + 16, LP = T / 4;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int wr = wave >> 1, wc = wave & 1;
+  const bool wide = cols % 4 == 0 && ((uintptr_t)out & 15) == 0;
+  const int c = 4 * (tid % LP);
+  for (int half = 0; half < (MB == NA ? 2 : 1); ++half) {
+    __syncthreads();  // what was in LDS has been read
+    if (MB != NA || wr == half) {
+#pragma unroll
+      for (int i = 0; i < NA; ++i)
+#pragma unroll
+        for (int j = 0; j < MB; ++j) {
+          if constexpr (T == 256) asm volatile("" : "+a"(acc[i][j]));  // (as in store_tile)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int r = 32 * i + (lane & 31);
+            const int at = (MB == NA ? wc * (T / 2) : wave * (T / 4)) + 32 * j + 8 * q +
+                           4 * (lane >> 5);
+            *reinterpret_cast<f32x4v*>(lds + r * PITCH + 4 * at) =
+                f32x4v{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2],
+                       acc[i][j][4 * q + 3]};
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        }
+    }
+    __syncthreads();
+    const int live = rows - half * (T / 2) < T / 2 ? rows - half * (T / 2) : T / 2;
+    if (c >= width) continue;
+    auto store = [&](auto stream) {
+#pragma unroll 4
+      for (int r = tid / LP; r < live; r += 256 / LP) {
+        const f32x4v v = *reinterpret_cast<const f32x4v*>(lds + r * PITCH + 4 * c);
+        float* to = out + (half * (T / 2) + r) * cols + c;
+        if (wide && c + 4 <= width) {
+          if constexpr (decltype(stream)::value)
+            __builtin_nontemporal_store(v, reinterpret_cast<f32x4v*>(to));
+          else
+            *reinterpret_cast<f32x4v*>(to) = v;
+        } else {
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            if (c + u < width) to[u] = v[u];
+        }
+      }
+    };
+    if (past)
+      store(std::true_type{});
+    else
+      store(std::false_type{});
+  }
+}
+
 // Zeros where there is nothing to sum.
-template <int T>
-__device__ __forceinline__ void store_zeros(uint16_t* out, int64_t cols, int rows, int width) {
+template <int T, class V>
+__device__ __forceinline__ void store_zeros(V* out, int64_t cols, int rows, int width) {
   constexpr int TX = T < 256 ? T : 256;
   const int c = threadIdx.x % TX;
   if (c >= width) return;
@@ -642,8 +699,14 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 8 / RING) void grouped_tile_ker
     const int64_t width = WHAT == GROUPED_LINEAR ? n : k, c0 = (int64_t)xt * T;
     const int cols = (int)(width - c0 < T ? width - c0 : T);
     uint16_t* const to = out + first * width + c0;
+    const bool sums = WHAT == GROUPED_GRAD_X && g.f32_out;
+    static_assert(T / 2 * (4 * T + 16) <= LDS_BYTES<T, 4>, "store_sums");
+    float* const to_sums = static_cast<float*>(g.out) + first * width + c0;
     if (e < 0) {
-      if (z == 0) store_zeros<T>(to, width, live, cols);
+      if (z == 0 && sums)
+        store_zeros<T>(to_sums, width, live, cols);
+      else if (z == 0)
+        store_zeros<T>(to, width, live, cols);
       return;
     }
     const int all = WHAT == GROUPED_LINEAR ? k : n;  // of the contraction
@@ -653,15 +716,21 @@ __global__ __launch_bounds__(256, T == 256 ? 1 : 8 / RING) void grouped_tile_ker
     // of 1024 x 2048 with 64 slots each 78 us, so 66).
     const bool half = T == 256 && live <= T / 2;
     auto finish = [&](auto& a, auto& b) {
-      if constexpr (T == 256)
+      if constexpr (T == 256) {
         if (half) {
-        tile_loop<DT, T, RING, NA, NA / 2>(a, b, lds, end - from, acc);
-        store_tile<DT, T, INDEXED ? 1 : 0, NA / 2>(lds, acc, to, width, live, cols, bad, g.past);
-        return;
+          tile_loop<DT, T, RING, NA, NA / 2>(a, b, lds, end - from, acc);
+          if (sums)
+            store_sums<T, NA / 2>(lds, acc, to_sums, width, live, cols, g.past);
+          else
+            store_tile<DT, T, INDEXED ? 1 : 0, NA / 2>(lds, acc, to, width, live, cols, bad, g.past);
+          return;
+        }
       }
       tile_loop<DT, T, RING, NA, NA>(a, b, lds, end - from, acc);
       if constexpr (SPLIT)
         store_part<T>(part, ((uint64_t)y * nx + xt) * splits + z, acc, 0.0f);
+      else if (sums)
+        store_sums<T>(lds, acc, to_sums, width, live, cols, g.past);
       else
         store_tile<DT, T, INDEXED ? 1 : 0>(lds, acc, to, width, live, cols, bad, g.past);
     };
@@ -750,14 +819,15 @@ __global__ __launch_bounds__(256) void grouped_join_kernel(GroupedArgs g, int wi
 #pragma unroll
       for (int q = 0; q < 4; ++q) sum[q] = sum[q] + __builtin_nanf("");
   }
-  uint16_t* const to = static_cast<uint16_t*>(g.out) + (w.first + r) * width;
+  const int dt = WHAT == GROUPED_GRAD_X && g.f32_out ? 0 : DT;
+  char* const to = static_cast<char*>(g.out) + (w.first + r) * width * (dt == 0 ? 4 : 2);
   const int c0 = (int)xt * T + (quarter & 1) * 64 + (wave & 1) * 32 + 4 * (lane >> 5);
 #pragma unroll
   for (int q = 0; q < 4; ++q)
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int c = c0 + 8 * q + u;
-      if (c < width) store_from_f32(to, c, DT, sum[q][u]);
+      if (c < width) store_from_f32(to, c, dt, sum[q][u]);
     }
 }
 
@@ -900,7 +970,7 @@ int grouped_tiles(const GroupedArgs& args, int what, int dtype, char* plan, hipS
   const int64_t results = what == GROUPED_GRAD_W   ? g.experts * g.n * g.k
                           : what == GROUPED_LINEAR ? g.slots * g.n
                                                    : g.slots * g.k;
-  g.past = results * 2 > 128ll << 20;
+  g.past = results * (g.f32_out ? 4 : 2) > 128ll << 20;
 #define HI2X_GROUPED(WHAT)                                     \
   return dtype == 1 ? launch_size<1, WHAT>(g, plan, s, name) : \
                       launch_size<2, WHAT>(g, plan, s, name)

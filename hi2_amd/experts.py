@@ -134,10 +134,9 @@ def grouped_linear(x: torch.Tensor, w: torch.Tensor, offs: torch.Tensor,
     behind its last range.
 
     x and w have gradients where they require them: an expert without slots gets zeros.  With
-    ``rows``, x's takes ``slots``, the slots of each token, and is the sum over them, in their order,
-    of what each slot has (16-bit types: rounded to the type first, which adds an error of the size
-    of the result's own rounding).  Everything is of one type; 1 to 7000 experts, N and K below 2^20,
-    S and T below 2^31."""
+    ``rows``, x's takes ``slots``, the slots of each token, and is the float32 sum over them, in
+    their order, of what each slot has.  Everything is of one type; 1 to 7000 experts, N and K below
+    2^20, S and T below 2^31."""
     if x.dim() != 2 or w.dim() != 3 or w.shape[2] != x.shape[1]:
         raise ValueError(f"grouped_linear: x {tuple(x.shape)} and w {tuple(w.shape)}, expected "
                          "[T, K] and [E, N, K]")

@@ -757,7 +757,7 @@ int hi2x_adamw_moments(const void* m_codes, const void* v_codes, const float* m_
  * Slots outside all ranges get rows of zeros in out and in dx; an expert without slots gets zeros
  * in dw.  hi2x_grouped_grad_x: with slots_of [t][top_k] (i64: each token's slots; one outside
  * 0 to slots gives a row of NaN) dx is [t][k], summed in the order of top_k over what each slot
- * has, which for fp16 and bf16 is rounded to that type first; with slots_of NULL dx is [slots][k].
+ * has, in f32; with slots_of NULL dx is [slots][k].
  * Workspace: hi2x_grouped_workspace_bytes of what (0 linear, 1 grad_x, 2 grad_w), tokens = x_rows
  * (grad_x: t) and ldx (grad_x: any), indexed = rows or slots_of given, and whether the first operand
  * (x; for the gradients dy) and the second (w; for grad_w x) begin and continue at multiples of 16
