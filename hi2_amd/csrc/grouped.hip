@@ -269,6 +269,7 @@ extern "C" int64_t hi2x_grouped_workspace_bytes(int what, int dtype, int64_t tok
                                                 int second_aligned) {
   GroupedArgs g{};
   g.experts = experts, g.n = n, g.k = k, g.slots = slots, g.x_rows = tokens, g.ldx = ldx;
+  if (what == GROUPED_GRAD_W && slots == 0) g.x_rows = 0;  // (as in the call)
   if (what < 0 || what > 2 || check_grouped(g, dtype, "grouped_workspace_bytes")) return -1;
   const int64_t given = 0;  // (only whether there are rows counts)
   if (indexed && what != GROUPED_GRAD_X) g.rows = &given;
@@ -287,7 +288,7 @@ extern "C" int hi2x_grouped_linear(const void* x, int dtype, int64_t ldx, int64_
   g.x = x, g.ldx = ldx, g.x_rows = x_rows, g.w = w, g.ldw = k;
   g.experts = experts, g.n = n, g.k = k, g.rows = rows, g.offs = offs, g.slots = slots, g.out = out;
   if (int rc = check_grouped(g, dtype, "grouped_linear")) return rc;
-  HI2X_REQUIRE(rows || x_rows == slots, "grouped_linear: %lld rows for %lld slots",
+  HI2X_REQUIRE(rows || x_rows == slots || slots == 0, "grouped_linear: %lld rows for %lld slots",
                (long long)x_rows, (long long)slots);
   HI2X_REQUIRE(x_rows <= 1 || ldx >= k, "grouped_linear: rows of x overlap");
   if (slots == 0) return HI2X_OK;
@@ -336,12 +337,14 @@ extern "C" int hi2x_grouped_grad_w(const void* dy, int dtype, int64_t ldy, const
   g.experts = experts, g.n = n, g.k = k, g.rows = rows, g.offs = offs, g.slots = slots;
   g.out = dw;
   if (int rc = check_grouped(g, dtype, "grouped_grad_w")) return rc;
-  HI2X_REQUIRE(rows || x_rows == slots, "grouped_grad_w: %lld rows for %lld slots",
+  // (where there are no slots, rows may be NULL as the address of an empty array is)
+  HI2X_REQUIRE(rows || x_rows == slots || slots == 0, "grouped_grad_w: %lld rows for %lld slots",
                (long long)x_rows, (long long)slots);
   HI2X_REQUIRE((x_rows <= 1 || ldx >= k) && (slots <= 1 || ldy >= n),
                "grouped_grad_w: rows overlap");
   HI2X_REQUIRE(((x || x_rows == 0) && dy || slots == 0) && offs && dw,
                "grouped_grad_w: null buffer");
+  if (slots == 0) g.x_rows = 0, g.rows = nullptr;  // no row of x is read
   Workspace space;
   return run(g, GROUPED_GRAD_W, dtype, false, ws, ws_bytes, space, nullptr, as_stream(stream),
              "grouped_grad_w");
