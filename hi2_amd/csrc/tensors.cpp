@@ -77,6 +77,28 @@ PyObject* addresses(PyObject*, PyObject* args) {
   return odd;
 }
 
+// stepped(params, grads): autograd's version counters of the parameters whose gradients' addresses in
+// `grads` (of uint64 elements, one a parameter) are not 0 count the write that a step was to them.
+PyObject* stepped(PyObject*, PyObject* args) {
+  PyObject* params;
+  unsigned long long grads;
+  if (!PyArg_ParseTuple(args, "O!K", &PyList_Type, &params, &grads)) return nullptr;
+  const uint64_t* g = reinterpret_cast<const uint64_t*>(grads);
+  HANDLE_TH_ERRORS
+  const Py_ssize_t count = PyList_GET_SIZE(params);
+  for (Py_ssize_t i = 0; i < count; ++i) {
+    PyObject* o = PyList_GET_ITEM(params, i);
+    if (!THPVariable_Check(o)) {
+      PyErr_Format(PyExc_RuntimeError, "AdamW: not a tensor (parameter %zd)", i);
+      return nullptr;
+    }
+    const at::Tensor& p = THPVariable_Unpack(o);
+    if (g[i] && !p.is_inference()) p.unsafeGetTensorImpl()->bump_version();
+  }
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
 // The entries of libhi2x.so, by address (the library is loaded by Python, once).
 decltype(&hi2x_gated) gated_entry;
 decltype(&hi2x_gated_backward) gated_backward_entry;
@@ -176,6 +198,7 @@ PyObject* gated(PyObject*, PyObject* args) {
 }
 
 PyMethodDef methods[] = {{"addresses", addresses, METH_VARARGS, "Tensors' addresses."},
+                         {"stepped", stepped, METH_VARARGS, "Count a step's writes."},
                          {"bind", bind, METH_VARARGS, "The library's entries."},
                          {"gated", gated, METH_VARARGS, "The gated activation, differentiable."},
                          {nullptr, nullptr, 0, nullptr}};

@@ -142,7 +142,8 @@ class AdamW(torch.optim.Optimizer):
 
     @torch.no_grad()
     def step(self, closure=None):
-        """One step with the gradients in ``p.grad``, enqueued on the current stream."""
+        """One step with the gradients in ``p.grad``, enqueued on the current stream.  To autograd it
+        is a write in place: a backward that still needs the old parameters raises."""
         loss = None
         if closure is not None:
             with torch.enable_grad():
@@ -169,6 +170,7 @@ class AdamW(torch.optim.Optimizer):
                       None if self.master is None or s.dtype == torch.float32
                       else self.master.data_ptr(),
                       self._steps[at:].data_ptr(), self._done[at:].data_ptr())
+            _tensors().stepped(s.params, s.addresses[1].ctypes.data)
             at += n
         return loss
 
