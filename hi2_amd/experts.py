@@ -37,6 +37,14 @@ def _rows(x: torch.Tensor) -> torch.Tensor:
     return x
 
 
+def _near_rows(x: torch.Tensor) -> torch.Tensor:
+    """The same for the grouped products, whose rows are less than 2^21 elements apart (as those of
+    ``h[:, -1]`` of long sequences are not: they are copied)."""
+    if x.shape[0] > 1 and x.stride(0) >= 1 << 21:
+        return x.contiguous()
+    return _rows(x)
+
+
 def _pitch(x: torch.Tensor) -> int:
     return x.stride(0) if x.shape[0] > 1 else x.shape[1]
 
@@ -93,7 +101,7 @@ class _Grouped(torch.autograd.Function):
         x, w, offs, rows, slots_of = ctx.saved_tensors
         e, n, k = w.shape
         dev, dt, slots = x.device, DTYPES[x.dtype], grad.shape[0]
-        grad = _rows(grad)
+        grad = _near_rows(grad)
         dx = dw = None
         if ctx.needs_input_grad[0]:
             dx = torch.empty(x.shape, dtype=x.dtype, device=dev)
@@ -159,8 +167,8 @@ def grouped_linear(x: torch.Tensor, w: torch.Tensor, offs: torch.Tensor,
     if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad):
         if x.requires_grad and rows is not None and slots is None:
             raise ValueError("grouped_linear: with rows, the gradient of x takes slots")
-        return _Grouped.apply(_rows(x), w.contiguous(), offs, rows, slots, count)
-    return _linear(_rows(x), w.contiguous(), offs, rows, count)
+        return _Grouped.apply(_near_rows(x), w.contiguous(), offs, rows, slots, count)
+    return _linear(_near_rows(x), w.contiguous(), offs, rows, count)
 
 
 _gated_graph = None

@@ -750,10 +750,10 @@ int hi2x_adamw_moments(const void* m_codes, const void* v_codes, const float* m_
  *   dx[t]  = sum over token t's slots of dy[slot] w[e]        (hi2x_grouped_grad_x)
  *   dw[e]  = sum over expert e's slots of dy[j]^T x[rows[j]]  (hi2x_grouped_grad_w)
  * with w [experts][n][k] contiguous and everything of one dtype (0 f32, 1 fp16, 2 bf16), summed in
- * f32 and rounded once.  x [x_rows][k] and dy [slots][n] have rows ldx and ldy elements apart,
- * aligned to one element; out [slots][n], dx and dw [experts][n][k] are contiguous.  rows (or
- * NULL: slot j reads row j, x_rows = slots; or there are no slots) and offs (experts + 1,
- * ascending, within 0 to slots)
+ * f32 and rounded once.  x [x_rows][k] and dy [slots][n] have rows ldx and ldy elements apart
+ * (less than 2^21; of one row it does not count), aligned to one element; out [slots][n], dx and
+ * dw [experts][n][k] are contiguous.  rows (or NULL: slot j reads row j, x_rows = slots; or there
+ * are no slots) and offs (experts + 1, ascending, within 0 to slots)
  * are i64 on the device, never read by the host.  A row outside x is taken as a row of NaN.
  * Slots outside all ranges get rows of zeros in out and in dx; an expert without slots gets zeros
  * in dw.  hi2x_grouped_grad_x: with slots_of [t][top_k] (i64: each token's slots; one outside
