@@ -201,6 +201,12 @@ Space lay_out(const GroupedArgs& g, int what, int dtype, bool summed, bool x_fit
   return m;
 }
 
+// How far the next row is does not count where there is one, but the tiles find by it where the rows end.
+void one_row(GroupedArgs& g) {
+  if (g.x_rows <= 1) g.ldx = g.k;
+  if (g.slots <= 1) g.ldy = g.n;
+}
+
 bool lies_well(const void* p, int64_t ld) { return ((uintptr_t)p & 15) == 0 && ld % 8 == 0; }
 
 int check_grouped(const GroupedArgs& g, int dtype, const char* what) {
@@ -219,6 +225,7 @@ int check_grouped(const GroupedArgs& g, int dtype, const char* what) {
 // The product, its operands copied first where they do not lie as it takes them.
 int run(GroupedArgs g, int what, int dtype, bool summed, void* ws, int64_t ws_bytes, Workspace& w,
         void** part, hipStream_t s, const char* name) {
+  one_row(g);
   // workgroups of the smallest tiles, whole rounds of them
   const int T = dtype ? 128 : 64;
   const int64_t nx = ((what == GROUPED_LINEAR ? g.n : g.k) + T - 1) / T + 3;
@@ -273,8 +280,10 @@ extern "C" int64_t hi2x_grouped_workspace_bytes(int what, int dtype, int64_t tok
   if (what < 0 || what > 2 || check_grouped(g, dtype, "grouped_workspace_bytes")) return -1;
   const int64_t given = 0;  // (only whether there are rows counts)
   if (indexed && what != GROUPED_GRAD_X) g.rows = &given;
+  one_row(g);
+  const int x_aligned = what == GROUPED_LINEAR ? first_aligned : second_aligned;
   return lay_out(g, what, dtype, indexed && what == GROUPED_GRAD_X,
-                 what == GROUPED_LINEAR ? first_aligned : second_aligned, first_aligned,
+                 x_aligned && (tokens > 1 || k % 8 == 0), first_aligned && (slots > 1 || n % 8 == 0),
                  second_aligned)
       .bytes;
 }
