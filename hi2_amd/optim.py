@@ -109,6 +109,8 @@ class AdamW(torch.optim.Optimizer):
         self._units = torch.zeros(2, self._blocks, dtype=torch.float32, device=dev) \
             if state_bits == 8 else None
         self._sets = [_Set(d, entries, dev) for d, entries in by_type.items()]
+        self._types = [str(p.dtype) for p in self._params]
+        self._numels = [p.numel() for p in self._params]
         count = sum(len(s.params) for s in self._sets)
         self._steps = torch.zeros(count, dtype=torch.int64, device=dev)
         self._done = torch.zeros(count, dtype=torch.int32, device=dev)
@@ -120,6 +122,13 @@ class AdamW(torch.optim.Optimizer):
         self._laid_out = True
         for g in self.param_groups:
             self._options(g)
+
+    @staticmethod
+    def _counted(types, numels) -> list:
+        """The parameters in the order of their counts of steps: type after type, the empty ones
+        left out."""
+        live = [i for i, n in enumerate(numels) if n]
+        return [i for t in dict.fromkeys(types[i] for i in live) for i in live if types[i] == t]
 
     def add_param_group(self, param_group):
         if self._laid_out:
@@ -226,18 +235,20 @@ class AdamW(torch.optim.Optimizer):
     def state_dict(self) -> dict:
         """The options and the state: the buffers themselves, not copies of them."""
         out = super().state_dict()
-        out["state"] = dict(state_bits=self.state_bits, starts=list(self.starts), m=self._m,
+        out["state"] = dict(state_bits=self.state_bits, starts=list(self.starts),
+                            sizes=list(self._numels), types=list(self._types), m=self._m,
                             v=self._v, units=self._units, steps=self._steps, master=self.master)
         return out
 
     @torch.no_grad()
     def load_state_dict(self, state_dict: dict) -> None:
         """Take over a :meth:`state_dict` of an optimizer over the same parameters and of the same
-        ``state_bits`` and ``master``.  A learning rate that is a tensor here stays that tensor and
-        takes the value."""
+        ``state_bits`` and ``master``; the parameters' types may be others.  A learning rate that is
+        a tensor here stays that tensor and takes the value."""
         given = state_dict["state"]
         mine = self.state_dict()["state"]
-        if given["state_bits"] != self.state_bits or list(given["starts"]) != self.starts:
+        if given["state_bits"] != self.state_bits or list(given["starts"]) != self.starts or \
+                list(given.get("sizes", self._numels)) != self._numels:
             raise ValueError("load_state_dict: the state is of other parameters or another width")
         if [(len(g["params"])) for g in state_dict["param_groups"]] != \
                 [len(g["params"]) for g in self.param_groups]:
@@ -247,6 +258,12 @@ class AdamW(torch.optim.Optimizer):
             if (a is None) != (b is None) or a is not None and (a.shape != b.shape or
                                                                 a.dtype != b.dtype):
                 raise ValueError(f"load_state_dict: {name} does not fit")
+        steps = given["steps"]
+        theirs = self._counted(given.get("types", self._types), self._numels)
+        ours = self._counted(self._types, self._numels)
+        if theirs != ours:  # counts lie type after type
+            at = {p: i for i, p in enumerate(theirs)}
+            steps = steps[torch.tensor([at[p] for p in ours], device=steps.device)]
         taken = []
         for g, h in zip(self.param_groups, state_dict["param_groups"]):
             options = {k: v for k, v in h.items() if k != "params"}
@@ -259,6 +276,7 @@ class AdamW(torch.optim.Optimizer):
                 lr = options.pop("lr")  # (the tensor stays: captured steps read it)
                 g["lr"].copy_(lr) if isinstance(lr, torch.Tensor) else g["lr"].fill_(lr)
             g.update(options)
-        for name in ("m", "v", "units", "steps", "master"):
+        self._steps.copy_(steps)
+        for name in ("m", "v", "units", "master"):
             if mine[name] is not None:
                 mine[name].copy_(given[name])
