@@ -72,7 +72,10 @@ class AdamW(torch.optim.Optimizer):
 
     Moments (and masters) of all parameters lie in one buffer each, in the order of the groups,
     every parameter from a multiple of 256 elements on (:attr:`starts`).  Parameters cannot be
-    added, and their types and sizes not changed, after construction."""
+    added, and their types and sizes not changed, after construction.  Options of other AdamW
+    variants (``amsgrad``, ``maximize``, ``differentiable``, ``decoupled_weight_decay=False``) are
+    refused in a group or a state; what else a group holds (names, what a scheduler keeps there)
+    stays there."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 1e-2, state_bits: int = 32, master: bool = False):
@@ -138,6 +141,10 @@ class AdamW(torch.optim.Optimizer):
     def _options(self, g) -> tuple:
         """A group's options as ``hi2x_adamw_group``, checked."""
         lr, (b1, b2), eps, wd = g["lr"], g["betas"], g["eps"], g["weight_decay"]
+        for name, given in (("amsgrad", False), ("maximize", False), ("differentiable", False),
+                            ("decoupled_weight_decay", True)):
+            if bool(g.get(name, given)) is not given:
+                raise ValueError(f"AdamW has no {name}={g[name]}")
         tensor = None
         if isinstance(lr, torch.Tensor):
             if lr.device != self.device or lr.dtype != torch.float32 or lr.numel() != 1:
