@@ -291,7 +291,8 @@ __global__ __launch_bounds__(256) void adamw_kernel(Launch a) {
       p[j] = p[j] * f.decay - (m[j] / (s[j] * f.root + f.eps)) * f.step;
     }
     store4<DT, STREAM>(pp, e, t.n, vec, p);
-    if constexpr (MASTER) store4<0, STREAM>(a.master, at, at + 4, true, p);
+    // (past the tensor's end p may be 0 / 0, where eps is 0: the masters stay zero there)
+    if constexpr (MASTER) store4<0, STREAM>(a.master + t.start, e, t.n, e + 4 <= t.n, p);
     if constexpr (BITS == 32) {
       store4<0, STREAM>(a.m, at, at + 4, true, m);
       store4<0, STREAM>(a.v, at, at + 4, true, v);

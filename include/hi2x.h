@@ -727,9 +727,9 @@ typedef struct hi2x_adamw_group {
  * Moments of all tensors lie in one buffer each: with bits 32 f32; with bits 8 one byte an
  * element and f32 m_unit, v_unit an element of which serves HI2X_ADAMW_BLOCK elements: m = +-q^2
  * unit for the byte q of either sign, v = (q^2 unit)^2; the bytes of a block whose largest is not
- * finite stand for NaN.  Elements between a tensor's end and the next multiple of
- * HI2X_ADAMW_BLOCK are zero and stay so.  master (or NULL): f32 parameters laid out as the
- * moments are, which take the step in the place of fp16 or bf16 ones and are rounded to them.
+ * finite stand for NaN.  master (or NULL): f32 parameters laid out as the moments are, which take
+ * the step in the place of fp16 or bf16 ones and are rounded to them.  Elements between a tensor's
+ * end and the next multiple of HI2X_ADAMW_BLOCK are zero, of moments and masters, and stay so.
  * steps [count]: the steps each tensor has taken, counted on; done [count]: zeros, left as
  * zeros. */
 int hi2x_adamw_step(const hi2x_adamw_tensor* tensors, const hi2x_adamw_tensor* device_tensors,

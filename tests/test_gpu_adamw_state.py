@@ -83,3 +83,21 @@ def test_empty_parameters_have_no_count(dev):
     qs, other = make((F32, F32, BF16), (1, 2, 3), (0, 70, 5))
     other.load_state_dict(opt.state_dict())
     assert other.state_dict()["state"]["steps"].tolist() == [1, 1]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_between_parameters_there_are_zeros(dev, dtype, bits):
+    """Also in the masters, and where eps is 0."""
+    ps = [torch.nn.Parameter(torch.ones(n, dtype=dtype).cuda()) for n in (301, 255, 4097, 6, 512)]
+    opt = AdamW(ps, lr=0.5, eps=0.0, state_bits=bits, master=True)
+    for i in range(2):
+        for p in ps:
+            p.grad = torch.full_like(p, 0.5 - i)
+        opt.step()
+    between = torch.ones(opt.master.numel(), dtype=torch.bool, device="cuda")
+    for p, a in zip(ps, opt.starts):
+        between[a:a + p.numel()] = False
+        assert torch.isfinite(p).all() and torch.equal(opt.master[a:a + p.numel()].to(dtype), p)
+    for buffer in (opt.master, *opt.moments()):
+        assert not buffer[between].any()
