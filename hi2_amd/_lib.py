@@ -175,6 +175,7 @@ SIZES = {
     "hi2x_route_workspace_bytes": [_I64, _I64],
     "hi2x_moe_combine_grad_workspace_bytes": [_I64],
     "hi2x_grouped_workspace_bytes": [_I, _I, _I64, _I64, _I64, _I64, _I64, _I64, _I, _I, _I],
+    "hi2x_grouped_form": [_I, _I, _I64, _I64, _I64, _I64, _P],
 }
 
 

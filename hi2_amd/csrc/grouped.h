@@ -77,6 +77,9 @@ int64_t grouped_plan_bytes(const GroupedArgs& g, int what, int dtype);
 int grouped_tiles(const GroupedArgs& g, int what, int dtype, char* plan, hipStream_t s,
                   const char* name);
 
+// The side of the tiles that 16-bit operands take, and the ranges that their contraction is cut into.
+int grouped_tile_side(const GroupedArgs& g, int what, int64_t& splits);
+
 // The product of a few slots of 16 bits, whatever its operands' alignment, without a workspace.  Up
 // to 32 slots (8 experts of 1024 x 2048, a slot each: 7.7 us, in tiles 23.5; 64 slots of 64 of them
 // 62 us and 45), and more where the weights would have to be copied for the tiles.

@@ -288,6 +288,20 @@ extern "C" int64_t hi2x_grouped_workspace_bytes(int what, int dtype, int64_t tok
       .bytes;
 }
 
+extern "C" int64_t hi2x_grouped_form(int what, int dtype, int64_t experts, int64_t n, int64_t k,
+                                     int64_t slots, int64_t* splits) {
+  GroupedArgs g{};
+  g.experts = experts, g.n = n, g.k = k, g.slots = slots, g.x_rows = slots;
+  if (what < 0 || what > 2 || check_grouped(g, dtype, "grouped_form")) return -1;
+  int64_t ranges = 1, side = 64;
+  if (what == GROUPED_LINEAR && few_slots(g, dtype, k % 8 == 0))
+    side = 16;
+  else if (dtype != 0)
+    side = grouped_tile_side(g, what, ranges);
+  if (splits) *splits = ranges;
+  return side;
+}
+
 extern "C" int hi2x_grouped_linear(const void* x, int dtype, int64_t ldx, int64_t x_rows,
                                    const void* w, int64_t experts, int64_t n, int64_t k,
                                    const int64_t* rows, const int64_t* offs, int64_t slots,

@@ -961,6 +961,12 @@ int64_t grouped_plan_bytes(const GroupedArgs& g, int what, int dtype) {
          (cut.splits > 1 ? tiles * cut.splits * cut.T * cut.T * 4 : 0);
 }
 
+int grouped_tile_side(const GroupedArgs& g, int what, int64_t& splits) {
+  const Cut cut = cut_of(g, what);
+  splits = cut.splits;
+  return cut.T;
+}
+
 int grouped_tiles(const GroupedArgs& args, int what, int dtype, char* plan, hipStream_t s,
                   const char* name) {
   GroupedArgs g = args;

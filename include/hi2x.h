@@ -779,6 +779,12 @@ int64_t hi2x_grouped_workspace_bytes(int what, int dtype, int64_t tokens, int64_
                                      int64_t experts, int64_t n, int64_t k, int64_t slots,
                                      int indexed, int first_aligned, int second_aligned);
 
+/* Which form a product (what as above) takes: the side of its tiles (256 or 128; f32: 64; 16 where it goes
+ * without tiles, a few slots), -1 for bad sizes, and in *splits (or NULL) the ranges that a tile's
+ * contraction is cut into.  It goes by sizes alone, with w aligned to 16 bytes. */
+int64_t hi2x_grouped_form(int what, int dtype, int64_t experts, int64_t n, int64_t k,
+                          int64_t slots, int64_t* splits);
+
 /* out = act(gate) * up, [rows][n], all of one dtype with rows ld apart: act as in hi2x_epilogue.
  * In f32, rounded once. */
 int hi2x_gated(const void* gate, int64_t ld_gate, const void* up, int64_t ld_up, int64_t rows,
