@@ -81,8 +81,8 @@ int grouped_tiles(const GroupedArgs& g, int what, int dtype, char* plan, hipStre
 int grouped_tile_side(const GroupedArgs& g, int what, int64_t& splits);
 
 // The product of a few slots of 16 bits, whatever its operands' alignment, without a workspace.  Up
-// to 32 slots (8 experts of 1024 x 2048, a slot each: 7.7 us, in tiles 23.5; 64 slots of 64 of them
-// 62 us and 45), and more where the weights would have to be copied for the tiles.
+// to 32 slots (8 experts of 1024 x 2048, a slot each, weights in the last cache: 7.7 us, in tiles 23.5; 64
+// slots of 64 of them 62 us and 45), and more where the weights would have to be copied for the tiles.
 inline bool few_slots(const GroupedArgs& g, int dtype, bool w_fits) {
   return dtype != 0 && g.experts <= 512 && g.slots <= (w_fits ? 32 : 256);
 }

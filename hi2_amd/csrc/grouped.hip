@@ -29,7 +29,8 @@ __device__ __forceinline__ void spread_at(const Spread& g, int64_t& row, int64_t
 // dx[t] = the rows of t's slots added in their order, V values a thread (4, 16 bytes of a row; 1 where rows
 // do not begin at multiples of 16 bytes), up to four rows on their way at a time.  A slot outside gives
 // NaN.  Rows are float32 whatever dx's type: rounded to 16 bits before they are added they would cost
-// half the traffic and 1.4 times the error.  HBM bounds it: part is read once.
+// half the traffic and 1.4 times the error.  HBM bounds it: part is read once (16384 tokens of eight slots
+// of 2048 208 us, 5.5 TB/s).
 template <int DT, int V>
 __global__ __launch_bounds__(256) void sum_slots_kernel(const float* part, int64_t slots, int64_t k,
                                                         const int64_t* slots_of, int64_t t,

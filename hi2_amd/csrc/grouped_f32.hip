@@ -7,10 +7,10 @@ namespace {
 // A workgroup's tile of 64 x 64 results, 32 of the contraction at a time through two LDS buffers:
 // while one is multiplied the next two chunks are on their way into registers.  A wave has 16 rows and
 // two fragments of 16 columns, and leaves out fragments and steps in which nothing lives, so that short
-// ranges and odd sizes cost what they hold (60 experts of 520 x 1001, 3108 slots: 64 us, and 212 with
-// both gradients, where 256 threads a tile and one chunk ahead took 229).  Lanes take neighbours in
-// memory, along the contraction or across it, one value each, so rows may begin anywhere.  Offsets are
-// 32 bits from a chunk's or a tile's first row.
+// ranges and odd sizes cost what they hold (60 experts of 520 x 1001, 3108 slots: 63 us, and 209 to 218
+// with both gradients; 256 threads a tile and one chunk ahead took 229 where this took 212).  Lanes take
+// neighbours in memory, along the contraction or across it, one value each, so rows may begin anywhere.
+// Offsets are 32 bits from a chunk's or a tile's first row.
 constexpr int FT = 64, KC = 32;
 constexpr int THREADS = 512, EACH = FT * KC / THREADS;  // values of an operand's chunk a thread
 constexpr int PITCH = KC + 4;  // floats of a row in LDS

@@ -8,8 +8,9 @@
 // hands a lane its column.  Both are loaded as they lie, 16 bytes a lane, straight into LDS.
 //
 // A wave holds T/2 x T/2 results in registers; a ring of four stages (or two) is in flight.  64 experts
-// of 1024 x 2048, 2048 slots each in bfloat16: 533 us (1032 TFLOP/s), the tokens' gradient 574 (958),
-// the weights' 485 (1134); one library product of the size reaches 1298, 1080 and 625.
+// of 1024 x 2048, 2048 slots each in bfloat16: 533 us (1032 TFLOP/s), the tokens' gradient 570 (965;
+// of tokens with eight slots each 825 with its float32 rows and their sums), the weights' 478 (1150); one
+// library product of the size reaches 1298, 1080 and 625.
 #include <type_traits>
 
 #include "grouped.h"
@@ -426,7 +427,8 @@ __device__ __forceinline__ void store_tile(char* lds, f32x16v (&acc)[T / 64][T /
 }
 
 // The tile's sums as they are, to float32 rows of `out`, half of its rows through LDS at a time; 16 bytes a
-// lane where the rows allow it.
+// lane where the rows allow it.  Twice the bytes of store_tile's (131072 slots of 64 experts of 1024 x 2048
+// 617 us for 570).
 template <int T, int MB = T / 64>
 __device__ __forceinline__ void store_sums(char* lds, f32x16v (&acc)[T / 64][T / 64], float* out,
                                            int64_t cols, int rows, int width, bool past) {
@@ -892,7 +894,9 @@ double rounds(double tiles, double cap, double a, double stages, double b, doubl
 // 0.55 and 0.35 for 128-tiles.  Over 80 products of ragged ranges, 32 to 1024 slots an expert, what
 // it takes is 1.3% slower than the better on average and 21% at most (always 128: 3%, always 256:
 // 13%); 8 experts of 14336 x 4096 with 256 slots each 380 us and 465, 16 of 2048 x 4096 with 384 each
-// 220 and 152.
+// 220 and 152.  It goes by the mean range, as the ranges are on the device: where one of 64 experts of
+// 1024 x 2048 has nine tenths of 131072 slots, its 32 tiles of the weights' gradient run alone, 1872 us
+// for 552 of even ranges.
 // The weights' gradient takes 0.75 a stage in 256-tiles, and in 128-tiles of a two-stage ring, four
 // to a CU, hides the stores of short sums behind others: ranges of 64 slots 72 us and 62, of 512 585
 // and 619.
