@@ -153,7 +153,8 @@ struct Gated : torch::autograd::Function<Gated> {
     {
       const at::AutoGradMode off(false);
       const variable_list saved = ctx->get_saved_variables();
-      const at::Tensor &gate = saved[0], &up = saved[1], grad = rows_of(grads[0]);
+      // (saved tensors' hooks may give them back in other strides than they were saved with)
+      const at::Tensor gate = rows_of(saved[0]), up = rows_of(saved[1]), grad = rows_of(grads[0]);
       const c10::DeviceGuard guard(gate.device());
       for (at::Tensor& d : both) d = at::empty({gate.size(0), gate.size(1)}, gate.options());
       if (both[0].numel())

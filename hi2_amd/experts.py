@@ -98,7 +98,10 @@ class _Grouped(torch.autograd.Function):
     def backward(ctx, grad):
         if grad is None:
             return (None,) * 6
+        # (saved tensors' hooks may give them back in other strides than they were saved with)
         x, w, offs, rows, slots_of = ctx.saved_tensors
+        x, w, offs = _near_rows(x), w.contiguous(), offs.contiguous()
+        rows, slots_of = (v if v is None else v.contiguous() for v in (rows, slots_of))
         e, n, k = w.shape
         dev, dt, slots = x.device, DTYPES[x.dtype], grad.shape[0]
         grad = _near_rows(grad)
