@@ -69,6 +69,11 @@ class _Weights(torch.autograd.Function):
         if grad is None:
             return None, None, None
         logits, index = ctx.saved_tensors
+        # (saved tensors' hooks may give them back in other strides than they were saved with)
+        index = index.contiguous()
+        if logits.shape[1] > 1 and logits.stride(1) != 1 or \
+                logits.shape[0] > 1 and logits.stride(0) < logits.shape[1]:
+            logits = logits.contiguous()
         scoring, renormalise, scale = ctx.args
         t, e = logits.shape
         d = torch.empty(t, e, dtype=logits.dtype, device=logits.device)

@@ -440,7 +440,8 @@ class _Combine(torch.autograd.Function):
     def backward(ctx, grad):
         if grad is None:
             return (None,) * 5
-        y, weights, slots = ctx.saved_tensors
+        # (saved tensors' hooks may give them back in other strides than they were saved with)
+        y, weights, slots = (v.contiguous() for v in ctx.saved_tensors)
         need_y, need_w, need_r = ctx.needs_input_grad[:3]
         grad = grad.contiguous()
         dw = torch.empty_like(weights) if need_w else None

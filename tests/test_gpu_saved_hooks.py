@@ -5,6 +5,7 @@ import torch
 
 from hi2_amd.experts import experts_mlp, gated, grouped_linear
 from hi2_amd.moe import route
+from hi2_amd.packed import combine
 
 pytestmark = pytest.mark.gpu
 
@@ -55,3 +56,22 @@ def test_saved_on_the_host(dev):
     with torch.autograd.graph.save_on_cpu():
         y = experts_mlp(x, r, gate, up, down)
     assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y.sum(), leaves), want))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("hook", [swapped, thinned])
+def test_router_and_weighted_sum(dev, dtype, hook):
+    g = torch.Generator().manual_seed(2)
+    logits = torch.zeros(40, 8) + torch.arange(8.0)  # (rows alike)
+    y = torch.full((80, 24), 0.5, dtype=dtype, device=dev)
+    dy = torch.randn(40, 24, generator=g).to(dtype).to(dev)
+    for constant in (False, True):
+        lo = (torch.zeros(40, 8) if constant else logits + torch.randn(40, 8, generator=g)).to(dev)
+        out = []
+        for pack in (lambda v: v, hook):
+            lr, yr = lo.clone().requires_grad_(True), y.clone().requires_grad_(True)
+            with torch.autograd.graph.saved_tensors_hooks(pack, lambda v: v):
+                r = route(lr, 2)
+                z = combine(yr, r.slots, r.weights, None, dtype)
+            out.append(torch.autograd.grad(z, (lr, yr), dy))
+        assert all(torch.equal(a, b) for a, b in zip(*out))
