@@ -138,6 +138,10 @@ class AdamW(torch.optim.Optimizer):
             raise RuntimeError("AdamW: parameters cannot be added after construction")
         super().add_param_group(param_group)
 
+    def __getstate__(self):
+        raise TypeError("AdamW is not copied or pickled, which would leave its moments behind: take "
+                        "its state_dict")
+
     def _options(self, g) -> tuple:
         """A group's options as ``hi2x_adamw_group``, checked."""
         lr, (b1, b2), eps, wd = g["lr"], g["betas"], g["eps"], g["weight_decay"]

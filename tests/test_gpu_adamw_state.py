@@ -101,3 +101,14 @@ def test_between_parameters_there_are_zeros(dev, dtype, bits):
         assert torch.isfinite(p).all() and torch.equal(opt.master[a:a + p.numel()].to(dtype), p)
     for buffer in (opt.master, *opt.moments()):
         assert not buffer[between].any()
+
+
+def test_no_copy_without_the_moments(dev):
+    """A pickle held the options alone, and what was read back had no state to step with."""
+    import pickle
+
+    _, opt = make((F32, F32, F32), (1, 2, 3))
+    for take in (copy.copy, copy.deepcopy, pickle.dumps):
+        with pytest.raises(TypeError, match="state_dict"):
+            take(opt)
+    assert "lr" in repr(opt)
